@@ -16,6 +16,7 @@
 #include <sstream>
 
 #include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime_api.h>
 #include <nvtx3/nvToolsExt.h>
@@ -43,7 +44,8 @@ constexpr auto F32 = at::kFloat;
   X(sb_rmsnorm_bwd) X(sb_glu_fwd) X(sb_glu_bwd) X(sb_ce_fwd) X(sb_ce_bwd) X(sb_dwconv_fwd) X(sb_dwconv_fwd_taps) X(sb_dwconv_bwd) \
   X(sb_se_fwd) X(sb_se_fwd_taps) X(sb_se_bwd) X(sb_mr_fwd) X(sb_mr_bwd) X(sb_mr_tc_fwd) X(sb_mr_tc_bwd) X(sb_mr_umma_fwd) X(sb_mr_umma_bwd) \
   X(sb_li_fwd_tiled) \
-  X(sb_li_bwd_tiled_chunk) X(sb_li_bwd_tiled) X(sb_attn_fwd) X(sb_attn_bwd) X(sb_attn_rope)
+  X(sb_li_bwd_tiled_chunk) X(sb_li_bwd_tiled) X(sb_attn_fwd) X(sb_attn_bwd) X(sb_attn_rope) \
+  X(sb_layernorm_fwd) X(sb_layernorm_bwd_blocks) X(sb_layernorm_bwd) X(sb_act8_quantize) X(sb_act8_dequantize)
 
 struct {
 #define SB_DECLARE(name) decltype(&::name) name = nullptr;
@@ -337,6 +339,39 @@ struct RmsNormResidual : Function<RmsNormResidual> {
     const variable_list s = ctx->get_saved_variables();
     auto d = saved_norm_bwd(ctx, s[0], s[1], s[2], g[0], g[1]);
     return {d.first, d.second, Tensor(), Tensor()};
+  }
+};
+
+// ------------------------------------------------------------------------------------ layer norm
+int type_code(at::ScalarType t) { return t == BF16 ? 0 : t == at::kHalf ? 1 : 2; }
+
+// Layer norm; with `residual` the second output carries x down the residual branch and the gradient arriving there is added inside the
+// backward kernel.
+struct LayerNorm : Function<LayerNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& b, double eps, bool residual, bool train) {
+    Tensor x2 = rows_contiguous(x), wc = contiguous(w), bc = contiguous(b), y = alloc_like(x2), st;
+    const int64_t T = x2.size(0), D = x2.size(1);
+    if (train) st = alloc({T, 2}, F32, x.device());
+    SB_CALL(sb_layernorm_fwd, 1, ptr(x2), ptr(wc), ptr(bc), out(y), f32o(st), (int)T, (int)D, (float)eps, type_code(x.scalar_type()), stream());
+    ctx->save_for_backward({x2, wc, st});
+    ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->set_materialize_grads(false);
+    if (residual) return {y.view(x.sizes()), x.view_as(x)};
+    return {y.view(x.sizes())};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const Tensor gres = g.size() > 1 ? g[1] : Tensor();
+    if (!g[0].defined()) return {gres, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &x2 = s[0], &w = s[1], &st = s[2];
+    const int64_t T = x2.size(0), D = x2.size(1);
+    const int type = type_code(x2.scalar_type());
+    Tensor g2 = contiguous(g[0].reshape({T, D})), r2 = gres.defined() ? contiguous(gres.reshape({T, D})) : Tensor();
+    Tensor dx = alloc_like(x2), dw = alloc({D}, x2.scalar_type(), x2.device()), db = alloc_like(dw),
+           partial = alloc({(int64_t)L.sb_layernorm_bwd_blocks(T, D, type) * 2 * D}, F32, x2.device());
+    SB_CALL(sb_layernorm_bwd, T > 0 ? 2 : 1, ptr(x2), ptr(w), ptr(g2), f32(st), ptr(r2), out(dx), out(dw), out(db), f32o(partial), (int)T, (int)D,
+            type, stream());
+    return {dx.view(ctx->saved_data["shape"].toIntVector()), dw, db, Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -708,6 +743,36 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     no_transforms();
     variable_list r = RmsNormResidual::apply(x, w, eps, form);
     return std::make_tuple(r[0], r[1]);
+  });
+  m.def("layernorm", [](const Tensor& x, const Tensor& w, const Tensor& b, double eps) {
+    no_transforms();
+    const c10::cuda::CUDAGuard device(x.device());
+    return LayerNorm::apply(x, w, b, eps, false, wants_grad({&x, &w, &b}))[0];
+  });
+  m.def("layernorm_residual", [](const Tensor& x, const Tensor& w, const Tensor& b, double eps) {
+    no_transforms();
+    const c10::cuda::CUDAGuard device(x.device());
+    variable_list r = LayerNorm::apply(x, w, b, eps, true, wants_grad({&x, &w, &b}));
+    return std::make_tuple(r[0], r[1]);
+  });
+  m.def("act_quantize", [](const Tensor& x) {
+    no_transforms();
+    const c10::cuda::CUDAGuard device(x.device());
+    const Tensor xc = contiguous(x.detach());
+    const int64_t D = xc.size(-1), T = D ? xc.numel() / D : 0;
+    Tensor q = alloc(xc.sizes(), at::kChar, xc.device()), s = alloc(with_last(xc.sizes(), (D + 127) / 128), F32, xc.device());
+    SB_CALL(sb_act8_quantize, T > 0, ptr(xc), out(q), f32o(s), (long long)T, (int)D, type_code(xc.scalar_type()), stream());
+    return std::make_tuple(q, s);
+  });
+  m.def("act_dequantize", [](const Tensor& q, const Tensor& scale, int64_t type) {
+    no_transforms();
+    const c10::cuda::CUDAGuard device(q.device());
+    const Tensor qc = contiguous(q), sc = contiguous(scale);
+    const at::ScalarType t = type == 0 ? BF16 : type == 1 ? at::kHalf : F32;
+    const int64_t D = qc.size(-1), T = D ? qc.numel() / D : 0;
+    Tensor x = alloc(qc.sizes(), t, qc.device());
+    SB_CALL(sb_act8_dequantize, T > 0, ptr(qc), f32(sc), out(x), (long long)T, (int)D, (int)type, stream());
+    return x;
   });
   m.def("norm_linear", [](const Tensor& x, const Tensor& wn, double eps, int64_t form, const py::object& w, const OptTensor& bias) {
     no_transforms();

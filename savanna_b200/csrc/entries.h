@@ -55,6 +55,14 @@ int sb_li_bwd_tiled_chunk();
 int sb_li_bwd_tiled(const void* feat, const void* dz, const float* modal, const float* bias, const float* state_in, const float* dstate_out,
                     float* S, float* A, float* dRp, float* dBp, void* dfeat, float* dR, float* dll, float* db, float* dstate_in, int B,
                     int L, int D, int O, cudaStream_t st);
+// layernorm.cu
+int sb_layernorm_fwd(const void* x, const void* w, const void* b, void* y, float* stats, int rows, int D, float eps, int type, cudaStream_t st);
+int sb_layernorm_bwd_blocks(int rows, int D, int type);
+int sb_layernorm_bwd(const void* x, const void* w, const void* dy, const float* stats, const void* gres, void* dx, void* dw, void* db,
+                     float* partial, int rows, int D, int type, cudaStream_t st);
+// act8.cu
+int sb_act8_quantize(const void* x, void* q, float* scale, long long rows, int D, int type, cudaStream_t st);
+int sb_act8_dequantize(const void* q, const float* scale, void* x, long long rows, int D, int type, cudaStream_t st);
 // attn_sm100.cu
 int sb_attn_fwd(const void* q, const void* k, const void* v, void* out, float* lse, int B, int H, int Lq, int Lk, const long long* q_str,
                 const long long* k_str, const long long* v_str, const long long* o_str, int causal, float scale, unsigned int* status,

@@ -1,0 +1,567 @@
+// Layer norm over the last dimension, forward and backward, of bf16, fp16 or fp32 rows (statistics and sums in fp32).
+//
+//   y = (x - mean) rstd w + b,   rstd = 1 / sqrt(mean((x - mean)^2) + eps)
+//   g = dy w,  xh = (x - mean) rstd:   dx = rstd (g - mean(g) - xh mean(g xh)) (+ gres),   dw = sum over rows of dy xh,   db = sum of dy
+//
+// The variance is that of the differences from the mean, never the difference of two large sums: a warp takes it around its own mean, and
+// warps are joined by  M2 = sum_w M2_w + n_w (mean_w - mean)^2.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "device_info.h"
+#include "entries.h"
+#include "pdl.cuh"
+
+namespace sb {
+namespace ln {
+
+typedef __nv_bfloat16 bf16;
+
+// What 16 bytes of a type hold, and single values of it.
+template <class T> struct Of;
+template <> struct Of<bf16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void get(const uint4& v, float (&f)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+  }
+  static __device__ __forceinline__ uint32_t two(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ uint4 put(const float (&f)[8]) {
+    return make_uint4(two(f[0], f[1]), two(f[2], f[3]), two(f[4], f[5]), two(f[6], f[7]));
+  }
+  static __device__ __forceinline__ float one(bf16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ bf16 from(float v) { return __float2bfloat16_rn(v); }
+};
+template <> struct Of<__half> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void get(const uint4& v, float (&f)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = t.x; f[2 * i + 1] = t.y;
+    }
+  }
+  static __device__ __forceinline__ uint32_t two(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ uint4 put(const float (&f)[8]) {
+    return make_uint4(two(f[0], f[1]), two(f[2], f[3]), two(f[4], f[5]), two(f[6], f[7]));
+  }
+  static __device__ __forceinline__ float one(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ __half from(float v) { return __float2half_rn(v); }
+};
+template <> struct Of<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void get(const uint4& v, float (&f)[4]) {
+    f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
+  }
+  static __device__ __forceinline__ uint4 put(const float (&f)[4]) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+  static __device__ __forceinline__ float one(float v) { return v; }
+  static __device__ __forceinline__ float from(float v) { return v; }
+};
+
+// Vector or value i of a row: VEC is Of<T>::N (16-byte accesses) or 1 (any width, any alignment).
+template <class T, int VEC> __device__ __forceinline__ void load(const T* p, size_t i, float (&f)[VEC]) {
+  if constexpr (VEC == 1) f[0] = Of<T>::one(p[i]);
+  else Of<T>::get(reinterpret_cast<const uint4*>(p)[i], f);
+}
+template <class T, int VEC> __device__ __forceinline__ void store(T* p, size_t i, const float (&f)[VEC]) {
+  if constexpr (VEC == 1) p[i] = Of<T>::from(f[0]);
+  else reinterpret_cast<uint4*>(p)[i] = Of<T>::put(f);
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// ------------------------------------------------------------------------------------ forward
+// W warps take a row, V vectors a lane, all loaded before the first sum.
+__host__ __device__ constexpr int fwd_rows(int W) { return W == 1 ? 4 : 1; }
+
+template <class T, int VEC, int V, int W>
+__global__ void __launch_bounds__(32 * W * fwd_rows(W))
+fwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict__ b, T* __restrict__ y, float2* __restrict__ stats, int rows,
+           int D, float eps) {
+  __shared__ float2 red[W];
+  const int lane = threadIdx.x & 31, warp = W > 1 ? threadIdx.x >> 5 : 0, i0 = warp * 32 + lane, nv = D / VEC;
+  const size_t row = (size_t)blockIdx.x * fwd_rows(W) + threadIdx.x / (32 * W);
+  if (row >= (size_t)rows) return;                       // a whole warp of W == 1, never part of a row
+  const T* src = x + row * D;
+  float f[V][VEC];
+  int n = 0;                                             // values of this warp
+  float s = 0.f;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int i = i0 + 32 * W * v;
+    n += min(max(nv - (warp * 32 + 32 * W * v), 0), 32) * VEC;
+    if (i < nv) load<T, VEC>(src, i, f[v]);
+    else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f[v][j] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) s += f[v][j];
+  s = warp_sum(s);
+  float mean = n ? s / n : 0.f, m2 = 0.f;
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    if (i0 + 32 * W * v < nv) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) { const float d = f[v][j] - mean; m2 = fmaf(d, d, m2); }
+    }
+  m2 = warp_sum(m2);
+  if (W > 1) {
+    if (lane == 0) red[warp] = make_float2(s, m2);
+    __syncthreads();
+    float tot = 0.f;
+#pragma unroll
+    for (int k = 0; k < W; ++k) tot += red[k].x;
+    mean = tot / D;
+    m2 = 0.f;
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      int nk = 0;
+#pragma unroll
+      for (int v = 0; v < V; ++v) nk += min(max(nv - (k * 32 + 32 * W * v), 0), 32) * VEC;
+      const float d = nk ? red[k].x / nk - mean : 0.f;
+      m2 += fmaf(nk * d, d, red[k].y);
+    }
+  }
+  const float rstd = rsqrtf(m2 / D + eps);
+  if (stats && i0 == 0) stats[row] = make_float2(mean, rstd);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int i = i0 + 32 * W * v;
+    if (i < nv) {
+      float g[VEC], c[VEC];
+      load<T, VEC>(w, i, g);
+      load<T, VEC>(b, i, c);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f[v][j] = fmaf((f[v][j] - mean) * rstd, g[j], c[j]);
+      store<T, VEC>(y + row * D, i, f[v]);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------ backward
+// A thread owns V vectors of columns and keeps their dw and db sums in registers; W warps share a row, a block holds several such groups
+// and walks over the rows.  partial[block] = [dw | db] of the block's rows, added up by reduce_kernel in a fixed order.
+//
+// The rows come through a ring in shared memory, R rows at a time and S of those ahead: a thread copies the 16 bytes of each row and
+// tensor that it owns, nobody else reads them, so there is no barrier for them, only the thread's own wait.
+constexpr int BWD_THREADS = 512;
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ uint4 take(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+
+// Sums of 2 R values over the W warps of a group, the same in all of its threads; `red` [W][2 R] floats of its own for every other call.
+template <int R>
+__device__ __forceinline__ void group_sums(float (&s)[2 * R], float* red, int W, int bar, int wid, int lane) {
+  constexpr int P = 2 * R;
+  // halves of the values change lanes in the first steps: lane l ends with the warp's sum of value l / (32 / P)
+  int o = 16;
+#pragma unroll
+  for (int n = P / 2; n; n >>= 1, o >>= 1) {
+    const bool upper = lane & o;
+#pragma unroll
+    for (int k = 0; k < n; ++k) {
+      const float got = __shfl_xor_sync(0xffffffffu, upper ? s[k] : s[k + n], o);
+      s[k] = (upper ? s[k + n] : s[k]) + got;
+    }
+  }
+  for (; o; o >>= 1) s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
+  float t = s[0];
+  if (W > 1) {
+    constexpr int Q = 32 / P;                            // lanes per value
+    if (lane % Q == 0) red[wid * P + lane / Q] = t;
+    asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(32 * W) : "memory");
+    t = 0.f;
+    for (int k = lane % Q; k < W; k += Q) t += red[k * P + lane / Q];
+#pragma unroll
+    for (int d = Q / 2; d; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
+  }
+#pragma unroll
+  for (int k = 0; k < P; ++k) s[k] = __shfl_sync(0xffffffffu, t, k * (32 / P));
+}
+
+template <class T, int V, int R, int S, bool RES>
+__global__ void __launch_bounds__(BWD_THREADS, V == 1 ? 2 : 1)
+bwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict__ dy, const float2* __restrict__ stats,
+           const T* __restrict__ gres, T* __restrict__ dx, float* __restrict__ partial, int rows, int D, int W) {
+  constexpr int N = Of<T>::N, NT = RES ? 3 : 2;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float red_all[2][16][2 * R];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, grp = warp / W, wid = warp - grp * W, gl = wid * 32 + lane;
+  const int nv = D / N, G = (blockDim.x >> 5) / W, units = (rows + R - 1) / R;
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + threadIdx.x * 16, part = blockDim.x * 16;
+  auto slot = [&](int s, int r, int t, int v) { return ring + (((s * R + r) * NT + t) * V + v) * part; };
+  auto fetch = [&](int u, int s) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int row = u * R + r;
+      if (u < units && row < rows) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const int i = gl + 32 * W * v;
+          if (i < nv) {
+            const size_t o = (size_t)row * D + (size_t)i * N;
+            copy16(slot(s, r, 0, v), x + o);
+            copy16(slot(s, r, 1, v), dy + o);
+            if (RES) copy16(slot(s, r, 2, v), gres + o);
+          }
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  float wf[V][N], dwa[V][N], dba[V][N];
+  const int step = gridDim.x * G;
+  int u = blockIdx.x * G + grp;
+#pragma unroll
+  for (int s = 0; s < S; ++s) fetch(u + s * step, s);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int i = gl + 32 * W * v;
+    if (i < nv) Of<T>::get(reinterpret_cast<const uint4*>(w)[i], wf[v]);
+#pragma unroll
+    for (int j = 0; j < N; ++j) { if (i >= nv) wf[v][j] = 0.f; dwa[v][j] = 0.f; dba[v][j] = 0.f; }
+  }
+  auto row_stats = [&](int un, float2 (&st)[R]) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) st[r] = un < units && un * R + r < rows ? stats[un * R + r] : make_float2(0.f, 0.f);
+  };
+  float2 next[R];                                        // of the next rows: as far away as they are
+  row_stats(u, next);
+  const float inv = 1.f / D;
+  int s = 0;
+  for (int it = 0; u < units; u += step, ++it) {
+    float2 st[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) st[r] = next[r];
+    row_stats(u + step, next);
+    asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
+    uint4 xc[R][V], gc[R][V];
+    float sums[2 * R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const bool live = u * R + r < rows;
+      float a = 0.f, c = 0.f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const bool have = live && gl + 32 * W * v < nv;
+        xc[r][v] = have ? take(slot(s, r, 0, v)) : make_uint4(0, 0, 0, 0);
+        gc[r][v] = have ? take(slot(s, r, 1, v)) : make_uint4(0, 0, 0, 0);
+        float xf[N], gf[N];
+        Of<T>::get(xc[r][v], xf); Of<T>::get(gc[r][v], gf);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const float xh = (xf[j] - st[r].x) * st[r].y, g = gf[j] * wf[v][j];
+          dwa[v][j] = fmaf(gf[j], xh, dwa[v][j]);
+          dba[v][j] += gf[j];
+          a += g;
+          c = fmaf(g, xh, c);
+        }
+      }
+      sums[2 * r] = a; sums[2 * r + 1] = c;
+    }
+    group_sums<R>(sums, &red_all[it & 1][grp * W][0], W, 1 + grp, wid, lane);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (u * R + r >= rows) break;
+      const float c1 = sums[2 * r] * inv, c2 = sums[2 * r + 1] * inv;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int i = gl + 32 * W * v;
+        if (i < nv) {
+          float xf[N], gf[N], o[N];
+          Of<T>::get(xc[r][v], xf); Of<T>::get(gc[r][v], gf);
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            const float xh = (xf[j] - st[r].x) * st[r].y;
+            o[j] = st[r].y * (gf[j] * wf[v][j] - c1 - xh * c2);
+          }
+          if (RES) {
+            float rf[N];
+            Of<T>::get(take(slot(s, r, 2, v)), rf);
+#pragma unroll
+            for (int j = 0; j < N; ++j) o[j] += rf[j];
+          }
+          reinterpret_cast<uint4*>(dx + (size_t)(u * R + r) * D)[i] = Of<T>::put(o);
+        }
+      }
+    }
+    fetch(u + S * step, s);                              // this thread has read the slot that it fills again
+    if (++s == S) s = 0;
+  }
+  // the groups of a block in their order, through the ring, which nothing is copied into any more
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  float* out = partial + (size_t)blockIdx.x * 2 * D;
+  if (G == 1) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int i = gl + 32 * W * v;
+      if (i < nv) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) { out[i * N + j] = dwa[v][j]; out[D + i * N + j] = dba[v][j]; }
+      }
+    }
+    return;
+  }
+  __syncthreads();
+  float* sh = reinterpret_cast<float*>(smem);
+  if (grp < G) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int i = gl + 32 * W * v;
+      if (i < nv) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) { sh[(size_t)grp * 2 * D + i * N + j] = dwa[v][j]; sh[(size_t)grp * 2 * D + D + i * N + j] = dba[v][j]; }
+      }
+    }
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < 2 * D; c += blockDim.x) {
+    float t = 0.f;
+    for (int g = 0; g < G; ++g) t += sh[(size_t)g * 2 * D + c];
+    out[c] = t;
+  }
+}
+
+// Widths that 16-byte vectors do not divide, and rows off a 16-byte boundary: a block per row, V single values a thread, the next row's on
+// their way while this one is summed.
+template <class T, int V>
+__global__ void __launch_bounds__(V > 8 ? 1024 : 256)
+bwd_any_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict__ dy, const float2* __restrict__ stats,
+               const T* __restrict__ gres, T* __restrict__ dx, float* __restrict__ partial, int rows, int D) {
+  __shared__ float red[2][32][2];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  float wf[V], dwa[V], dba[V];
+  T xn[V], gn[V], rn[V];
+  auto fetch = [&](int row) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int i = threadIdx.x + v * blockDim.x;
+      if (row < rows && i < D) {
+        xn[v] = x[(size_t)row * D + i];
+        gn[v] = dy[(size_t)row * D + i];
+        if (gres) rn[v] = gres[(size_t)row * D + i];
+      }
+    }
+  };
+  int row = blockIdx.x;
+  fetch(row);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int i = threadIdx.x + v * blockDim.x;
+    wf[v] = i < D ? Of<T>::one(w[i]) : 0.f;
+    dwa[v] = dba[v] = 0.f;
+  }
+  const float inv = 1.f / D;
+  for (int it = 0; row < rows; row += gridDim.x, ++it) {
+    const float2 st = stats[row];
+    float xh[V], g[V], r[V], a = 0.f, c = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const bool have = (int)(threadIdx.x + v * blockDim.x) < D;
+      const float gf = have ? Of<T>::one(gn[v]) : 0.f;
+      xh[v] = have ? (Of<T>::one(xn[v]) - st.x) * st.y : 0.f;
+      r[v] = have && gres ? Of<T>::one(rn[v]) : 0.f;
+      g[v] = gf * wf[v];
+      dwa[v] = fmaf(gf, xh[v], dwa[v]);
+      dba[v] += gf;
+      a += g[v];
+      c = fmaf(g[v], xh[v], c);
+    }
+    fetch(row + gridDim.x);
+    a = warp_sum(a); c = warp_sum(c);
+    if (lane == 0) { red[it & 1][wid][0] = a; red[it & 1][wid][1] = c; }
+    __syncthreads();
+    a = warp_sum(lane < nw ? red[it & 1][lane][0] : 0.f) * inv;
+    c = warp_sum(lane < nw ? red[it & 1][lane][1] : 0.f) * inv;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int i = threadIdx.x + v * blockDim.x;
+      if (i < D) dx[(size_t)row * D + i] = Of<T>::from(st.y * (g[v] - a - xh[v] * c) + r[v]);
+    }
+  }
+  float* out = partial + (size_t)blockIdx.x * 2 * D;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int i = threadIdx.x + v * blockDim.x;
+    if (i < D) { out[i] = dwa[v]; out[D + i] = dba[v]; }
+  }
+}
+
+// dw, db = sum over the blocks of partial [nblk][2][D]: a block takes 32 columns, its 32 thread rows split the partial rows.
+template <class T>
+__global__ void __launch_bounds__(1024)
+reduce_kernel(const float* partial, T* dw, T* db, int nblk, int D) {
+  __shared__ float sh[32][33];
+  const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5, c = blockIdx.x * 32 + cx;
+  wait_for_previous();
+  float s = 0.f;
+  if (c < 2 * D) {
+#pragma unroll 4
+    for (int k = ry; k < nblk; k += 32) s += partial[(size_t)k * 2 * D + c];
+  }
+  sh[ry][cx] = s;
+  __syncthreads();
+  const float t = warp_sum(sh[cx][ry]);                  // column ry of this block, its 32 parts over the lanes
+  const int o = blockIdx.x * 32 + ry;
+  if (cx == 0 && o < 2 * D) (o < D ? dw[o] : db[o - D]) = Of<T>::from(t);
+}
+
+// ------------------------------------------------------------------------------------ launchers
+constexpr int MAX_D = 16384;
+
+template <class T, int VEC, int V, int W>
+static int launch_fwd(const void* x, const void* w, const void* b, void* y, float* stats, int rows, int D, float eps, cudaStream_t st) {
+  const int per = fwd_rows(W);
+  fwd_kernel<T, VEC, V, W><<<(rows + per - 1) / per, 32 * W * per, 0, st>>>((const T*)x, (const T*)w, (const T*)b, (T*)y, (float2*)stats, rows, D, eps);
+  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+}
+
+template <class T, int VEC>
+static int forward(const void* x, const void* w, const void* b, void* y, float* stats, int rows, int D, float eps, cudaStream_t st) {
+  const int nv = D / VEC, lanes = (nv + 31) / 32;        // warps that hold a row with one vector a lane
+#define LN_FWD(V, W) return launch_fwd<T, VEC, V, W>(x, w, b, y, stats, rows, D, eps, st)
+  if (lanes <= 1) LN_FWD(1, 1);
+  if (lanes <= 2) LN_FWD(2, 1);
+  if (lanes <= 4) LN_FWD(4, 1);
+  if (lanes <= 8) LN_FWD(2, 4);
+  if (lanes <= 16) LN_FWD(4, 4);
+  if (lanes <= 32) LN_FWD(4, 8);
+  if (lanes <= 64) LN_FWD(4, 16);
+  if (lanes <= 128) LN_FWD(8, 16);
+  if constexpr (VEC == 1) {
+    if (lanes <= 256) LN_FWD(8, 32);
+    LN_FWD(16, 32);
+  }
+#undef LN_FWD
+  return -3;
+}
+
+struct Plan { int W, V, threads, grid; };
+// Backward by vectors: `n` values a vector
+static Plan plan_vec(int rows, int D, int n) {
+  const int lanes = (D / n + 31) / 32;                   // 1 .. 128
+  Plan p;
+  p.V = lanes <= 16 ? 1 : lanes <= 32 ? 2 : lanes <= 64 ? 4 : 8;
+  p.W = p.V == 1 ? lanes : 16;
+  const int G = p.V == 1 ? 16 / p.W : 1, R = p.V <= 2 ? 2 : 1;
+  p.threads = 32 * p.W * G;
+  const int units = (rows + R - 1) / R, blocks = (units + G - 1) / G, most = (p.V == 1 ? 2 : 1) * num_sms();
+  p.grid = blocks < most ? blocks : most;
+  return p;
+}
+static Plan plan_any(int rows, int D) {
+  Plan p;
+  p.threads = D <= 2048 ? 256 : 1024;
+  const int v = (D + p.threads - 1) / p.threads;
+  p.V = p.threads == 256 ? (v <= 2 ? 2 : v <= 4 ? 4 : 8) : 16;
+  p.W = p.threads / 32;
+  const int most = (p.threads == 256 ? 4 : 1) * num_sms();
+  p.grid = rows < most ? rows : most;
+  return p;
+}
+
+template <class T, int V, int R, int S, bool RES>
+static int launch_bwd(const Plan& p, const void* x, const void* w, const void* dy, const float* stats, const void* gres, void* dx, float* partial,
+                      int rows, int D, cudaStream_t st) {
+  const int ring = S * R * (RES ? 3 : 2) * V * p.threads * 16;
+  if (ring > 40 * 1024 && cudaFuncSetAttribute(bwd_kernel<T, V, R, S, RES>, cudaFuncAttributeMaxDynamicSharedMemorySize, ring) != cudaSuccess) return -2;
+  bwd_kernel<T, V, R, S, RES><<<p.grid, p.threads, ring, st>>>((const T*)x, (const T*)w, (const T*)dy, (const float2*)stats, (const T*)gres, (T*)dx,
+                                                               partial, rows, D, p.W);
+  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+}
+
+template <class T>
+static int backward(const void* x, const void* w, const void* dy, const float* stats, const void* gres, void* dx, void* dw, void* db, float* partial,
+                    int rows, int D, bool vec, cudaStream_t st) {
+  const Plan p = vec ? plan_vec(rows, D, Of<T>::N) : plan_any(rows, D);
+  int rc = 0;
+#define LN_BWD(V, R, S) rc = gres ? launch_bwd<T, V, R, S, true>(p, x, w, dy, stats, gres, dx, partial, rows, D, st) \
+                                  : launch_bwd<T, V, R, S, false>(p, x, w, dy, stats, gres, dx, partial, rows, D, st)
+#define LN_ANY(V) bwd_any_kernel<T, V><<<p.grid, p.threads, 0, st>>>((const T*)x, (const T*)w, (const T*)dy, (const float2*)stats, (const T*)gres, \
+                                                                     (T*)dx, partial, rows, D)
+  if (rows > 0) {
+    if (vec) {
+      if (p.V == 1) LN_BWD(1, 2, 2);
+      else if (p.V == 2) LN_BWD(2, 2, 2);
+      else if (p.V == 4) LN_BWD(4, 1, 2);
+      else if constexpr (Of<T>::N == 4) LN_BWD(8, 1, 1);
+      else rc = -3;
+      if (rc) return rc;
+    } else {
+      if (p.V == 2) LN_ANY(2);
+      else if (p.V == 4) LN_ANY(4);
+      else if (p.V == 8) LN_ANY(8);
+      else LN_ANY(16);
+      if (cudaGetLastError() != cudaSuccess) return -2;
+    }
+  }
+#undef LN_BWD
+#undef LN_ANY
+  return launch_chained(false, reduce_kernel<T>, dim3((2 * D + 31) / 32), 1024, 0, st, (const float*)partial, (T*)dw, (T*)db, rows > 0 ? p.grid : 0, D);
+}
+
+static bool on16(std::initializer_list<const void*> ps) {
+  uintptr_t a = 0;
+  for (const void* p : ps) a |= reinterpret_cast<uintptr_t>(p);
+  return (a & 15) == 0;
+}
+
+}  // namespace ln
+}  // namespace sb
+
+using namespace sb::ln;
+
+// x, y [rows, D], w and b [D] of one type (0: bf16, 1: fp16, 2: fp32); stats [rows, 2] fp32 (mean, rstd) for the backward, or null.
+extern "C" int sb_layernorm_fwd(const void* x, const void* w, const void* b, void* y, float* stats, int rows, int D, float eps, int type,
+                                cudaStream_t st) {
+  if (D < 1 || D > MAX_D || rows < 0 || type < 0 || type > 2) return -1;
+  if (rows == 0) return 0;
+  const bool vec = D % (type == 2 ? 4 : 8) == 0 && on16({x, w, b, y});
+  if (type == 0) return vec ? forward<bf16, 8>(x, w, b, y, stats, rows, D, eps, st) : forward<bf16, 1>(x, w, b, y, stats, rows, D, eps, st);
+  if (type == 1) return vec ? forward<__half, 8>(x, w, b, y, stats, rows, D, eps, st) : forward<__half, 1>(x, w, b, y, stats, rows, D, eps, st);
+  return vec ? forward<float, 4>(x, w, b, y, stats, rows, D, eps, st) : forward<float, 1>(x, w, b, y, stats, rows, D, eps, st);
+}
+
+// Rows of 2 D floats that sb_layernorm_bwd needs as scratch.
+extern "C" int sb_layernorm_bwd_blocks(int rows, int D, int type) {
+  if (rows <= 0 || D < 1) return 1;
+  const int n = type == 2 ? 4 : 8, any = plan_any(rows, D).grid;
+  const int vec = D % n == 0 ? plan_vec(rows, D, n).grid : 0;
+  return vec > any ? vec : any;
+}
+
+// dx [rows, D] (gres, the gradient that came along the residual branch, added; may be null), dw and db [D], written.  Two launches.
+extern "C" int sb_layernorm_bwd(const void* x, const void* w, const void* dy, const float* stats, const void* gres, void* dx, void* dw, void* db,
+                                float* partial, int rows, int D, int type, cudaStream_t st) {
+  if (D < 1 || D > MAX_D || rows < 0 || type < 0 || type > 2) return -1;
+  const bool vec = D % (type == 2 ? 4 : 8) == 0 && on16({x, w, dy, gres, dx});
+  if (type == 0) return backward<bf16>(x, w, dy, stats, gres, dx, dw, db, partial, rows, D, vec, st);
+  if (type == 1) return backward<__half>(x, w, dy, stats, gres, dx, dw, db, partial, rows, D, vec, st);
+  return backward<float>(x, w, dy, stats, gres, dx, dw, db, partial, rows, D, vec, st);
+}

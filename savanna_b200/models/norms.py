@@ -49,10 +49,19 @@ class ScaleNorm(nn.Module):
 
 
 class LayerNorm(nn.LayerNorm):
+    """`torch.nn.LayerNorm`'s parameters; CUDA tensors run the layer norm kernels (ops.layernorm)."""
+
     def __init__(self, dim, eps=1e-5, dtype=None, device=None):
         super().__init__(dim, eps=eps, dtype=dtype, device=device)
         self.weight.is_norm_param = True
         self.bias.is_norm_param = True
+
+    def forward(self, x):
+        return ops.layernorm(x, self.weight, self.bias, self.eps) if ops._k(x) else super().forward(x)
+
+    def forward_with_residual(self, x):
+        """(norm(x), x for the residual branch)."""
+        return ops.layernorm_residual(x, self.weight, self.bias, self.eps) if ops._k(x) else (super().forward(x), x)
 
 
 def get_norm(cfg, dtype=None, device=None) -> nn.Module:

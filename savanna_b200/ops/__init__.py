@@ -96,6 +96,29 @@ def rmsnorm_residual(x, weight, eps: float, form: str = "te"):
     return ref.rmsnorm(x, weight, eps, form), x
 
 
+def _check_layernorm(x, weight, bias):
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"layernorm takes [..., D] with D >= 1, got {tuple(x.shape)}")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if tuple(t.shape) != (x.shape[-1],):
+            raise ValueError(f"layernorm {name} {tuple(t.shape)} for rows of {x.shape[-1]} values")
+
+
+def layernorm(x, weight, bias, eps: float):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension.  CUDA: bf16, fp16 or fp32 (x, weight and bias alike), rows of
+    up to 16384 values of any width, statistics and the gradients' sums over the rows in fp32."""
+    _check_layernorm(x, weight, bias)
+    return _co().layernorm(x, weight, bias, eps) if _k(x) else ref.layernorm(x, weight, bias, eps)
+
+
+def layernorm_residual(x, weight, bias, eps: float):
+    """(layernorm(x), x): as `rmsnorm_residual`."""
+    _check_layernorm(x, weight, bias)
+    if _k(x):
+        return _co().layernorm_residual(x, weight, bias, eps)
+    return ref.layernorm(x, weight, bias, eps), x
+
+
 def linear(x, w, bias=None, fp8: bool = False, residual=None):
     """x w^T (+ bias) (+ residual).  On CUDA bias and residual are added in the GEMM epilogue."""
     if _k(x):
@@ -201,6 +224,28 @@ def attention_packed(qkv, cos, sin, causal=True):
     if cos is not None and (cos.shape[-1] % 16 or cos.shape[-1] > 128 or cos.shape[0] != qkv.shape[1]):
         return None
     return flash_sm100.attention_packed(qkv, cos, sin, causal)
+
+
+# ----------------------------------------------------------------------------- activation checkpoints
+
+
+def act_quantize(x):
+    """x [..., D] (bf16, fp16 or fp32) -> (q int8 of x's shape, scale fp32 [..., ceil(D / 128)]): 128 consecutive values of a row share
+    a scale of amax / 127, so that a value comes back within amax / 254 of itself and a rounding to its type.  A block that holds an infinity
+    or NaN comes back as NaN.  Not differentiated: the form in which a checkpointed activation waits for its recomputation."""
+    if x.dim() < 1 or x.shape[-1] < 1 or x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError(f"act_quantize takes bf16, fp16 or fp32 [..., D] with D >= 1, got {x.dtype} {tuple(x.shape)}")
+    return _co().act_quantize(x) if _k(x) else ref.act_quantize(x)
+
+
+def act_dequantize(q, scale, dtype=torch.bfloat16):
+    """q * scale as `dtype`: what `act_quantize` kept."""
+    if dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError(f"act_dequantize gives bf16, fp16 or fp32, not {dtype}")
+    if q.dtype != torch.int8 or q.dim() < 1 or q.shape[-1] < 1 or scale.dtype != torch.float32 or scale.device != q.device \
+            or tuple(scale.shape) != tuple(q.shape[:-1]) + (-(-q.shape[-1] // ref.ACT_BLOCK),):
+        raise ValueError(f"act_dequantize takes what act_quantize returned, got q {q.dtype} {tuple(q.shape)}, scale {scale.dtype} {tuple(scale.shape)}")
+    return _co().act_dequantize(q, scale, dtype) if _k(q) else ref.act_dequantize(q, scale, dtype)
 
 
 # ----------------------------------------------------------------------------- loss / optimizer

@@ -1052,6 +1052,38 @@ def rmsnorm(x, weight, eps, form="te"):
     return _native("rmsnorm", x, weight, float(eps), 0 if form == "te" else 1)
 
 
+# ----------------------------------------------------------------------------- layer norm, activations in 8 bits
+
+_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}       # type codes of csrc/layernorm.cu and csrc/act8.cu
+
+
+def _layernorm_covers(x, weight, bias) -> bool:
+    """One type, rows of up to 16384 values that 32 bits count; anything else runs PyTorch's layer norm."""
+    return (x.dtype in _TYPES and weight.dtype == x.dtype and bias is not None and bias.dtype == x.dtype and 1 <= x.shape[-1] <= 16384
+            and x.numel() // max(1, x.shape[-1]) < 2 ** 31 and weight.device == x.device and bias.device == x.device)
+
+
+def layernorm(x, weight, bias, eps):
+    if not _layernorm_covers(x, weight, bias):
+        return torch.nn.functional.layer_norm(x, (x.shape[-1],), weight, bias, eps)
+    return _native("layernorm", x, weight, bias, float(eps))
+
+
+def layernorm_residual(x, weight, bias, eps):
+    """(layernorm(x), x) with the two gradients combined in one backward kernel."""
+    if not _layernorm_covers(x, weight, bias):
+        return torch.nn.functional.layer_norm(x, (x.shape[-1],), weight, bias, eps), x
+    return _native("layernorm_residual", x, weight, bias, float(eps))
+
+
+def act_quantize(x):
+    return _N.act_quantize(x)
+
+
+def act_dequantize(q, scale, dtype):
+    return _N.act_dequantize(q, scale, _TYPES[dtype])
+
+
 # ----------------------------------------------------------------------------- gated activation
 
 

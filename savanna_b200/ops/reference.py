@@ -38,6 +38,27 @@ def layernorm(x, weight, bias, eps):
     return F.layer_norm(x.float(), (x.shape[-1],), weight.float(), None if bias is None else bias.float(), eps).to(x.dtype)
 
 
+# ----------------------------------------------------------------------------- activations in 8 bits
+
+ACT_BLOCK = 128          # consecutive values of a row that share a scale
+
+
+def act_quantize(x):
+    """(q int8, scale fp32 [..., ceil(D / 128)]): scale = amax / 127 of each block, q = round(x * (127 / amax))."""
+    D = x.shape[-1]
+    n = -(-D // ACT_BLOCK)
+    xf = F.pad(x.detach().float(), (0, n * ACT_BLOCK - D)).view(*x.shape[:-1], n, ACT_BLOCK)
+    amax = xf.abs().amax(-1, keepdim=True)
+    q = torch.round(xf * (127.0 / amax.clamp(min=1e-30))).nan_to_num(0.0, 127.0, -127.0).clamp(-127, 127).to(torch.int8)
+    return q.view(*x.shape[:-1], n * ACT_BLOCK)[..., :D].contiguous(), (amax / 127.0).squeeze(-1)
+
+
+def act_dequantize(q, scale, dtype):
+    D, n = q.shape[-1], scale.shape[-1]
+    qf = F.pad(q.float(), (0, n * ACT_BLOCK - D)).view(*q.shape[:-1], n, ACT_BLOCK)
+    return (qf * scale.unsqueeze(-1)).view(*q.shape[:-1], n * ACT_BLOCK)[..., :D].to(dtype)
+
+
 # ----------------------------------------------------------------------------- linear
 
 
