@@ -3,7 +3,7 @@
 //   scale = amax / 127 over 128 consecutive values of a row (its last block may be shorter),  q = rint(x * (127 / amax)),  x' = q * scale
 //
 // |x - x'| is at most amax / 254 and a rounding to x's own type.  The largest magnitude is taken over the bit patterns, where NaN lies above
-// infinity: a block that holds one of them gets such a scale and comes back as NaN, so that an overflow stays visible.  A block below 1e-30
+// infinity: a block that holds one of them has a scale of NaN and comes back as NaN, so that an overflow stays visible.  A block below 1e-30
 // comes back as nearly zero.
 //
 // Bound by memory: 2 + 1 bytes a value for 16-bit types, one pass; a lane has four 16-byte loads on their way.
@@ -32,128 +32,191 @@ template <class T, int N> struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16
 
 __device__ __forceinline__ uint32_t magnitude(float f) { return __float_as_uint(f) & 0x7fffffffu; }
 __device__ __forceinline__ float inverse(float amax) { return 127.f / (amax < TINY ? TINY : amax); }     // NaN stays NaN
-__device__ __forceinline__ int8_t code(float x, float inv) {
-  const float r = rintf(x * inv);
-  return (int8_t)(r >= 127.f ? 127 : r <= -127.f ? -127 : r == r ? (int)r : 0);
+// rint(x * inv), whose magnitude is at most 127, in the low byte: a product of up to 2^22 added to 1.5 * 2^23 is rounded to an integer, half
+// to even.  (A conversion instruction for each value ran at a quarter of the rate.)
+__device__ __forceinline__ uint32_t code(float x, float inv) { return __float_as_uint(fmaf(x, inv, 12582912.f)); }
+__device__ __forceinline__ uint32_t four(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+// The scale of a block whose largest magnitude has the bits m: NaN for infinity and NaN.
+__device__ __forceinline__ float step_of(uint32_t m) { return m < 0x7f800000u ? __uint_as_float(m) / 127.f : __uint_as_float(0x7fffffffu); }
+// The four codes of a word as floats: 2^23 + (q + 128) by its bits, from which 2^23 + 128 is taken.
+__device__ __forceinline__ void uncode(uint32_t w, float (&f)[4]) {
+  w ^= 0x80808080u;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f[j] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + j)) - 8388736.f;
+}
+
+// The values that a lane loads at once, their largest magnitude (as fp32 bits) and one by one.
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
+template <class T> struct Eight { uint4 v; };
+template <> struct Eight<float> { uint4 v, w; };
+__device__ __forceinline__ uint32_t top(const uint4& v) {            // both halves of each word: magnitudes of 16-bit types order as integers
+  const uint32_t k = 0x7fff7fffu, m = max_u16x2(max_u16x2(v.x & k, v.y & k), max_u16x2(v.z & k, v.w & k));
+  return max(m & 0xffffu, m >> 16);
+}
+__device__ __forceinline__ uint32_t top(const Eight<bf16>& e) { return top(e.v) << 16; }
+__device__ __forceinline__ uint32_t top(const Eight<__half>& e) { return __float_as_uint(__half2float(__ushort_as_half((unsigned short)top(e.v)))); }
+__device__ __forceinline__ uint32_t top(const Eight<float>& e) {
+  const uint32_t k = 0x7fffffffu;
+  return max(max(max(e.v.x & k, e.v.y & k), max(e.v.z & k, e.v.w & k)), max(max(e.w.x & k, e.w.y & k), max(e.w.z & k, e.w.w & k)));
+}
+__device__ __forceinline__ void values(const Eight<bf16>& e, float (&f)[8]) {
+  const uint32_t w[4] = {e.v.x, e.v.y, e.v.z, e.v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+__device__ __forceinline__ void values(const Eight<__half>& e, float (&f)[8]) {
+  const uint32_t w[4] = {e.v.x, e.v.y, e.v.z, e.v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    f[2 * i] = t.x; f[2 * i + 1] = t.y;
+  }
+}
+__device__ __forceinline__ void values(const Eight<float>& e, float (&f)[8]) {
+  const uint32_t w[8] = {e.v.x, e.v.y, e.v.z, e.v.w, e.w.x, e.w.y, e.w.z, e.w.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
+}
+
+// First value of 128-block b, and how many of the block there are.  WHOLE: D % 128 == 0, the blocks lie one behind the other.
+struct Rows { uint32_t per_row, D; };
+template <bool WHOLE>
+__device__ __forceinline__ long long place(long long b, const Rows& r, int& n) {
+  n = BLOCK;
+  if (WHOLE) return b * BLOCK;
+  const long long row = b < 0x80000000LL ? (long long)((uint32_t)b / r.per_row) : b / r.per_row;
+  const uint32_t c = uint32_t(b - row * r.per_row) * BLOCK;
+  n = min((uint32_t)BLOCK, r.D - c);
+  return row * r.D + c;
 }
 
 // Eight values a lane, 16 lanes a block, D % 8 == 0 and 16-byte boundaries; U blocks a half-warp, all loaded before the first is used.
-template <class T, int U>
+template <class T, int U, bool WHOLE>
 __global__ void __launch_bounds__(256)
-quantize_vec_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scale, long long blocks, int per_row, int D) {
+quantize_vec_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scale, long long blocks, Rows r) {
   const long long first = ((long long)blockIdx.x * 16 + (threadIdx.x >> 4)) * U;
   const int l = threadIdx.x & 15;
-  Pack<T, 8> in[U];
+  Eight<T> in[U];
   long long at[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const long long b = first + u, row = b / per_row;
-    const int c = int(b - row * per_row) * BLOCK + l * 8;
-    at[u] = b < blocks && c < D ? row * D + c : -1;
-    if (at[u] >= 0) in[u] = *reinterpret_cast<const Pack<T, 8>*>(x + at[u]);
+    int n;
+    at[u] = place<WHOLE>(first + u, r, n) + l * 8;
+    if (first + u >= blocks || l * 8 >= n) at[u] = -1;
+    in[u] = Eight<T>{};
+    if (at[u] >= 0) in[u] = *reinterpret_cast<const Eight<T>*>(x + at[u]);
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    float f[8];
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) { f[j] = at[u] >= 0 ? up(in[u].v[j]) : 0.f; m = max(m, magnitude(f[j])); }
+    uint32_t m = top(in[u]);
 #pragma unroll
     for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float amax = __uint_as_float(m), inv = inverse(amax);
-    Pack<int8_t, 8> out;
+    const float inv = inverse(__uint_as_float(m));
+    float f[8];
+    values(in[u], f);
+    uint32_t c[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) out.v[j] = code(f[j], inv);
-    if (at[u] >= 0) *reinterpret_cast<Pack<int8_t, 8>*>(q + at[u]) = out;
-    if (l == 0 && first + u < blocks) scale[first + u] = amax / 127.f;
+    for (int j = 0; j < 8; ++j) c[j] = code(f[j], inv);
+    if (at[u] >= 0) *reinterpret_cast<uint2*>(q + at[u]) = make_uint2(four(c[0], c[1], c[2], c[3]), four(c[4], c[5], c[6], c[7]));
+    if (l == 0 && at[u] >= 0) scale[first + u] = step_of(m);
   }
 }
 
 // Any width and alignment: a warp a block, four values a lane.
 template <class T>
 __global__ void __launch_bounds__(256)
-quantize_any_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scale, long long blocks, int per_row, int D) {
+quantize_any_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scale, long long blocks, Rows r) {
   const long long b = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (b >= blocks) return;
   const int l = threadIdx.x & 31;
-  const long long row = b / per_row;
-  const int c0 = int(b - row * per_row) * BLOCK;
+  int n;
+  const long long at = place<false>(b, r, n);
   float f[4];
   uint32_t m = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int c = c0 + l + 32 * j;
-    f[j] = c < D ? up(x[row * D + c]) : 0.f;
+    f[j] = l + 32 * j < n ? up(x[at + l + 32 * j]) : 0.f;
     m = max(m, magnitude(f[j]));
   }
   m = __reduce_max_sync(0xffffffffu, m);
-  const float amax = __uint_as_float(m), inv = inverse(amax);
+  const float inv = inverse(__uint_as_float(m));
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int c = c0 + l + 32 * j;
-    if (c < D) q[row * D + c] = code(f[j], inv);
-  }
-  if (l == 0) scale[b] = amax / 127.f;
+  for (int j = 0; j < 4; ++j)
+    if (l + 32 * j < n) q[at + l + 32 * j] = (int8_t)(uint8_t)code(f[j], inv);
+  if (l == 0) scale[b] = step_of(m);
 }
 
-template <class T, int U>
+// 16 values a lane, eight lanes a block, where the blocks are whole and q lies on a 16-byte boundary, else eight values and 16 lanes.
+template <class T, int U, bool WHOLE, int N>
 __global__ void __launch_bounds__(256)
-dequantize_vec_kernel(const int8_t* __restrict__ q, const float* __restrict__ scale, T* __restrict__ x, long long blocks, int per_row, int D) {
-  const long long first = ((long long)blockIdx.x * 16 + (threadIdx.x >> 4)) * U;
-  const int l = threadIdx.x & 15;
-  Pack<int8_t, 8> in[U];
+dequantize_vec_kernel(const int8_t* __restrict__ q, const float* __restrict__ scale, T* __restrict__ x, long long blocks, Rows r) {
+  constexpr int LANES = BLOCK / N;
+  const long long first = ((long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES) * U;
+  const int l = threadIdx.x % LANES;
+  Pack<uint32_t, N / 4> in[U];
   float s[U];
   long long at[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const long long b = first + u, row = b / per_row;
-    const int c = int(b - row * per_row) * BLOCK + l * 8;
-    at[u] = b < blocks && c < D ? row * D + c : -1;
-    if (at[u] >= 0) { in[u] = *reinterpret_cast<const Pack<int8_t, 8>*>(q + at[u]); s[u] = scale[b]; }
+    int n;
+    at[u] = place<WHOLE>(first + u, r, n) + l * N;
+    if (first + u >= blocks || l * N >= n) at[u] = -1;
+    if (at[u] >= 0) { in[u] = *reinterpret_cast<const Pack<uint32_t, N / 4>*>(q + at[u]); s[u] = scale[first + u]; }
   }
 #pragma unroll
   for (int u = 0; u < U; ++u)
     if (at[u] >= 0) {
-      Pack<T, 8> out;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) down((float)in[u].v[j] * s[u], out.v[j]);
-      *reinterpret_cast<Pack<T, 8>*>(x + at[u]) = out;
+      for (int h = 0; h < N / 8; ++h) {
+        float f[8];
+        uncode(in[u].v[2 * h], reinterpret_cast<float(&)[4]>(f[0]));
+        uncode(in[u].v[2 * h + 1], reinterpret_cast<float(&)[4]>(f[4]));
+        Pack<T, 8> out;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) down(f[j] * s[u], out.v[j]);
+        *reinterpret_cast<Pack<T, 8>*>(x + at[u] + 8 * h) = out;
+      }
     }
 }
 
 template <class T>
 __global__ void __launch_bounds__(256)
-dequantize_any_kernel(const int8_t* __restrict__ q, const float* __restrict__ scale, T* __restrict__ x, long long blocks, int per_row, int D) {
+dequantize_any_kernel(const int8_t* __restrict__ q, const float* __restrict__ scale, T* __restrict__ x, long long blocks, Rows r) {
   const long long b = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (b >= blocks) return;
-  const long long row = b / per_row;
-  const int c0 = int(b - row * per_row) * BLOCK;
+  int n;
+  const long long at = place<false>(b, r, n);
   const float s = scale[b];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int c = c0 + (threadIdx.x & 31) + 32 * j;
-    if (c < D) down((float)q[row * D + c] * s, x[row * D + c]);
+    const int c = (threadIdx.x & 31) + 32 * j;
+    if (c < n) down((float)q[at + c] * s, x[at + c]);
   }
 }
 
-constexpr int U = 4;
-
 template <class T>
 static int quantize(const void* x, void* q, float* scale, long long rows, int D, bool vec, cudaStream_t st) {
-  const int per = (D + BLOCK - 1) / BLOCK;
-  const long long blocks = rows * per, grid = vec ? (blocks + 16 * U - 1) / (16 * U) : (blocks + 7) / 8;
+  constexpr int U = sizeof(T) == 4 ? 2 : 4;
+  const Rows r{(uint32_t)((D + BLOCK - 1) / BLOCK), (uint32_t)D};
+  const long long blocks = rows * r.per_row, per = vec ? 16 * U : 8, grid = (blocks + per - 1) / per;
   if (grid > 0x7fffffffLL) return -1;
-  if (vec) quantize_vec_kernel<T, U><<<(unsigned)grid, 256, 0, st>>>((const T*)x, (int8_t*)q, scale, blocks, per, D);
-  else quantize_any_kernel<T><<<(unsigned)grid, 256, 0, st>>>((const T*)x, (int8_t*)q, scale, blocks, per, D);
+  if (!vec) quantize_any_kernel<T><<<(unsigned)grid, 256, 0, st>>>((const T*)x, (int8_t*)q, scale, blocks, r);
+  else if (D % BLOCK == 0) quantize_vec_kernel<T, U, true><<<(unsigned)grid, 256, 0, st>>>((const T*)x, (int8_t*)q, scale, blocks, r);
+  else quantize_vec_kernel<T, U, false><<<(unsigned)grid, 256, 0, st>>>((const T*)x, (int8_t*)q, scale, blocks, r);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 template <class T>
 static int dequantize(const void* q, const float* scale, void* x, long long rows, int D, bool vec, cudaStream_t st) {
-  const int per = (D + BLOCK - 1) / BLOCK;
-  const long long blocks = rows * per, grid = vec ? (blocks + 16 * U - 1) / (16 * U) : (blocks + 7) / 8;
+  constexpr int U = 4;
+  const Rows r{(uint32_t)((D + BLOCK - 1) / BLOCK), (uint32_t)D};
+  const bool wide = vec && D % BLOCK == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+  const long long blocks = rows * r.per_row, per = wide ? 32 * U : vec ? 16 * U : 8, grid = (blocks + per - 1) / per;
   if (grid > 0x7fffffffLL) return -1;
-  if (vec) dequantize_vec_kernel<T, U><<<(unsigned)grid, 256, 0, st>>>((const int8_t*)q, scale, (T*)x, blocks, per, D);
-  else dequantize_any_kernel<T><<<(unsigned)grid, 256, 0, st>>>((const int8_t*)q, scale, (T*)x, blocks, per, D);
+  if (wide) dequantize_vec_kernel<T, U, true, 16><<<(unsigned)grid, 256, 0, st>>>((const int8_t*)q, scale, (T*)x, blocks, r);
+  else if (vec) dequantize_vec_kernel<T, U, false, 8><<<(unsigned)grid, 256, 0, st>>>((const int8_t*)q, scale, (T*)x, blocks, r);
+  else dequantize_any_kernel<T><<<(unsigned)grid, 256, 0, st>>>((const int8_t*)q, scale, (T*)x, blocks, r);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 static bool by_vector(const void* x, const void* q, int D) {

@@ -12,6 +12,7 @@
 
 #include "device_info.h"
 #include "entries.h"
+#include "f32x2.cuh"
 #include "pdl.cuh"
 
 namespace sb {
@@ -70,6 +71,20 @@ template <> struct Of<float> {
   static __device__ __forceinline__ float from(float v) { return v; }
 };
 
+// The same as pairs (f32x2.cuh)
+template <class T> __device__ __forceinline__ void get2(const uint4& v, f2 (&f)[Of<T>::N / 2]) {
+  float t[Of<T>::N];
+  Of<T>::get(v, t);
+#pragma unroll
+  for (int i = 0; i < Of<T>::N / 2; ++i) f[i] = f2_pack(t[2 * i], t[2 * i + 1]);
+}
+template <class T> __device__ __forceinline__ uint4 put2(const f2 (&f)[Of<T>::N / 2]) {
+  float t[Of<T>::N];
+#pragma unroll
+  for (int i = 0; i < Of<T>::N / 2; ++i) { const float2 p = f2_unpack(f[i]); t[2 * i] = p.x; t[2 * i + 1] = p.y; }
+  return Of<T>::put(t);
+}
+
 // Vector or value i of a row: VEC is Of<T>::N (16-byte accesses) or 1 (any width, any alignment).
 template <class T, int VEC> __device__ __forceinline__ void load(const T* p, size_t i, float (&f)[VEC]) {
   if constexpr (VEC == 1) f[0] = Of<T>::one(p[i]);
@@ -87,19 +102,22 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 // ------------------------------------------------------------------------------------ forward
-// W warps take a row, V vectors a lane, all loaded before the first sum.
+// W warps take a row, V vectors a lane, all loaded before the first sum.  Bound by memory with many rows: 8192 x 4096 bf16 25.1 us (a copy
+// takes 22.2); a few rows take the chain load, two sums, barrier, store.
 __host__ __device__ constexpr int fwd_rows(int W) { return W == 1 ? 4 : 1; }
 
 template <class T, int VEC, int V, int W>
 __global__ void __launch_bounds__(32 * W * fwd_rows(W))
 fwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict__ b, T* __restrict__ y, float2* __restrict__ stats, int rows,
            int D, float eps) {
-  __shared__ float2 red[W];
+  __shared__ float4 red[W];
   const int lane = threadIdx.x & 31, warp = W > 1 ? threadIdx.x >> 5 : 0, i0 = warp * 32 + lane, nv = D / VEC;
   const size_t row = (size_t)blockIdx.x * fwd_rows(W) + threadIdx.x / (32 * W);
   if (row >= (size_t)rows) return;                       // a whole warp of W == 1, never part of a row
   const T* src = x + row * D;
-  float f[V][VEC];
+  // the weights as well where a lane has few of them: a row alone on its SM then waits once
+  constexpr bool AHEAD = V * VEC <= 16;
+  float f[V][VEC], g[AHEAD ? V : 1][VEC], c[AHEAD ? V : 1][VEC];
   int n = 0;                                             // values of this warp
   float s = 0.f;
 #pragma unroll
@@ -112,12 +130,17 @@ fwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict
       for (int j = 0; j < VEC; ++j) f[v][j] = 0.f;
     }
   }
+  if (AHEAD) {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (i0 + 32 * W * v < nv) { load<T, VEC>(w, i0 + 32 * W * v, g[AHEAD ? v : 0]); load<T, VEC>(b, i0 + 32 * W * v, c[AHEAD ? v : 0]); }
+  }
 #pragma unroll
   for (int v = 0; v < V; ++v)
 #pragma unroll
     for (int j = 0; j < VEC; ++j) s += f[v][j];
   s = warp_sum(s);
-  float mean = n ? s / n : 0.f, m2 = 0.f;
+  float mean = n ? __fdividef(s, (float)n) : 0.f, m2 = 0.f;
 #pragma unroll
   for (int v = 0; v < V; ++v)
     if (i0 + 32 * W * v < nv) {
@@ -125,34 +148,29 @@ fwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict
       for (int j = 0; j < VEC; ++j) { const float d = f[v][j] - mean; m2 = fmaf(d, d, m2); }
     }
   m2 = warp_sum(m2);
-  if (W > 1) {
-    if (lane == 0) red[warp] = make_float2(s, m2);
+  if (W > 1) {                                           // the warps' results, one a lane: the same sums in every warp
+    if (lane == 0) red[warp] = make_float4(s, m2, mean, (float)n);
     __syncthreads();
-    float tot = 0.f;
+    const float4 k = red[lane % W];
+    mean = k.x;
 #pragma unroll
-    for (int k = 0; k < W; ++k) tot += red[k].x;
-    mean = tot / D;
-    m2 = 0.f;
+    for (int o = W / 2; o; o >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, o);
+    mean = __fdividef(mean, (float)D);
+    const float d = k.z - mean;
+    m2 = fmaf(k.w * d, d, k.y);
 #pragma unroll
-    for (int k = 0; k < W; ++k) {
-      int nk = 0;
-#pragma unroll
-      for (int v = 0; v < V; ++v) nk += min(max(nv - (k * 32 + 32 * W * v), 0), 32) * VEC;
-      const float d = nk ? red[k].x / nk - mean : 0.f;
-      m2 += fmaf(nk * d, d, red[k].y);
-    }
+    for (int o = W / 2; o; o >>= 1) m2 += __shfl_xor_sync(0xffffffffu, m2, o);
   }
-  const float rstd = rsqrtf(m2 / D + eps);
+  const float rstd = rsqrtf(__fdividef(m2, (float)D) + eps);
   if (stats && i0 == 0) stats[row] = make_float2(mean, rstd);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int i = i0 + 32 * W * v;
     if (i < nv) {
-      float g[VEC], c[VEC];
-      load<T, VEC>(w, i, g);
-      load<T, VEC>(b, i, c);
+      const int k = AHEAD ? v : 0;
+      if (!AHEAD) { load<T, VEC>(w, i, g[k]); load<T, VEC>(b, i, c[k]); }
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) f[v][j] = fmaf((f[v][j] - mean) * rstd, g[j], c[j]);
+      for (int j = 0; j < VEC; ++j) f[v][j] = fmaf((f[v][j] - mean) * rstd, g[k][j], c[k][j]);
       store<T, VEC>(y + row * D, i, f[v]);
     }
   }
@@ -163,7 +181,9 @@ fwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict
 // and walks over the rows.  partial[block] = [dw | db] of the block's rows, added up by reduce_kernel in a fixed order.
 //
 // The rows come through a ring in shared memory, R rows at a time and S of those ahead: a thread copies the 16 bytes of each row and
-// tensor that it owns, nobody else reads them, so there is no barrier for them, only the thread's own wait.
+// tensor that it owns, nobody else reads them, so there is no barrier for them, only the thread's own wait.  8192 x 4096 bf16 with residual:
+// 47.2 us with two rows at a time and two of those ahead (a copy of as many bytes takes 42.5), 48.7 with one row, 50.3 with four and none
+// ahead; with scalar arithmetic, and x and dy kept in registers over the barrier (which spilled), 79.  Without residual 42.3 (32.3).
 constexpr int BWD_THREADS = 512;
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
@@ -176,8 +196,9 @@ __device__ __forceinline__ uint4 take(uint32_t a) {
 }
 
 // Sums of 2 R values over the W warps of a group, the same in all of its threads; `red` [W][2 R] floats of its own for every other call.
-template <int R>
-__device__ __forceinline__ void group_sums(float (&s)[2 * R], float* red, int W, int bar, int wid, int lane) {
+template <int R, int W16>
+__device__ __forceinline__ void group_sums(float (&s)[2 * R], float* red, int warps, int bar, int wid, int lane) {
+  const int W = W16 ? 16 : warps;
   constexpr int P = 2 * R;
   // halves of the values change lanes in the first steps: lane l ends with the warp's sum of value l / (32 / P)
   int o = 16;
@@ -197,7 +218,11 @@ __device__ __forceinline__ void group_sums(float (&s)[2 * R], float* red, int W,
     if (lane % Q == 0) red[wid * P + lane / Q] = t;
     asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(32 * W) : "memory");
     t = 0.f;
-    for (int k = lane % Q; k < W; k += Q) t += red[k * P + lane / Q];
+#pragma unroll
+    for (int k = 0; k < 16; k += Q) {
+      const int at = k + lane % Q;
+      if (W16 || at < W) t += red[at * P + lane / Q];
+    }
 #pragma unroll
     for (int d = Q / 2; d; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
   }
@@ -205,10 +230,11 @@ __device__ __forceinline__ void group_sums(float (&s)[2 * R], float* red, int W,
   for (int k = 0; k < P; ++k) s[k] = __shfl_sync(0xffffffffu, t, k * (32 / P));
 }
 
-template <class T, int V, int R, int S, bool RES>
+template <class T, int V, int R, int S, bool RES, bool W16>
 __global__ void __launch_bounds__(BWD_THREADS, V == 1 ? 2 : 1)
 bwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict__ dy, const float2* __restrict__ stats,
-           const T* __restrict__ gres, T* __restrict__ dx, float* __restrict__ partial, int rows, int D, int W) {
+           const T* __restrict__ gres, T* __restrict__ dx, float* __restrict__ partial, int rows, int D, int warps) {
+  const int W = W16 ? 16 : warps;
   constexpr int N = Of<T>::N, NT = RES ? 3 : 2;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float red_all[2][16][2 * R];
@@ -223,9 +249,8 @@ bwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict
       if (u < units && row < rows) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const int i = gl + 32 * W * v;
-          if (i < nv) {
-            const size_t o = (size_t)row * D + (size_t)i * N;
+          if (gl + 32 * W * v < nv) {
+            const size_t o = (size_t)row * D + (gl + 32 * W * v) * N;
             copy16(slot(s, r, 0, v), x + o);
             copy16(slot(s, r, 1, v), dy + o);
             if (RES) copy16(slot(s, r, 2, v), gres + o);
@@ -235,7 +260,8 @@ bwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  float wf[V][N], dwa[V][N], dba[V][N];
+  constexpr int M = N / 2;
+  f2 wf[V][M], dwa[V][M], dba[V][M];
   const int step = gridDim.x * G;
   int u = blockIdx.x * G + grp;
 #pragma unroll
@@ -243,9 +269,9 @@ bwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int i = gl + 32 * W * v;
-    if (i < nv) Of<T>::get(reinterpret_cast<const uint4*>(w)[i], wf[v]);
+    get2<T>(i < nv ? reinterpret_cast<const uint4*>(w)[i] : make_uint4(0, 0, 0, 0), wf[v]);
 #pragma unroll
-    for (int j = 0; j < N; ++j) { if (i >= nv) wf[v][j] = 0.f; dwa[v][j] = 0.f; dba[v][j] = 0.f; }
+    for (int j = 0; j < M; ++j) dwa[v][j] = dba[v][j] = 0;
   }
   auto row_stats = [&](int un, float2 (&st)[R]) {
 #pragma unroll
@@ -256,58 +282,60 @@ bwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict
   const float inv = 1.f / D;
   int s = 0;
   for (int it = 0; u < units; u += step, ++it) {
-    float2 st[R];
+    f2 rs[R], off[R];                                    // xh = x rstd - mean rstd
+    float rstd[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) st[r] = next[r];
+    for (int r = 0; r < R; ++r) {
+      const float m = -next[r].x * next[r].y;
+      rstd[r] = next[r].y;
+      rs[r] = f2_pack(rstd[r], rstd[r]); off[r] = f2_pack(m, m);
+    }
     row_stats(u + step, next);
     asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
-    uint4 xc[R][V], gc[R][V];
     float sums[2 * R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const bool live = u * R + r < rows;
-      float a = 0.f, c = 0.f;
+      f2 a = 0, c = 0;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const bool have = live && gl + 32 * W * v < nv;
-        xc[r][v] = have ? take(slot(s, r, 0, v)) : make_uint4(0, 0, 0, 0);
-        gc[r][v] = have ? take(slot(s, r, 1, v)) : make_uint4(0, 0, 0, 0);
-        float xf[N], gf[N];
-        Of<T>::get(xc[r][v], xf); Of<T>::get(gc[r][v], gf);
+        if (live && gl + 32 * W * v < nv) {
+          f2 xf[M], gf[M];
+          get2<T>(take(slot(s, r, 0, v)), xf); get2<T>(take(slot(s, r, 1, v)), gf);
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const float xh = (xf[j] - st[r].x) * st[r].y, g = gf[j] * wf[v][j];
-          dwa[v][j] = fmaf(gf[j], xh, dwa[v][j]);
-          dba[v][j] += gf[j];
-          a += g;
-          c = fmaf(g, xh, c);
+          for (int j = 0; j < M; ++j) {
+            const f2 xh = f2_fma(xf[j], rs[r], off[r]), g = f2_mul(gf[j], wf[v][j]);
+            dwa[v][j] = f2_fma(gf[j], xh, dwa[v][j]);
+            dba[v][j] = f2_add(dba[v][j], gf[j]);
+            a = f2_add(a, g);
+            c = f2_fma(g, xh, c);
+          }
         }
       }
-      sums[2 * r] = a; sums[2 * r + 1] = c;
+      const float2 ta = f2_unpack(a), tc = f2_unpack(c);
+      sums[2 * r] = ta.x + ta.y; sums[2 * r + 1] = tc.x + tc.y;
     }
-    group_sums<R>(sums, &red_all[it & 1][grp * W][0], W, 1 + grp, wid, lane);
+    group_sums<R, W16>(sums, &red_all[it & 1][grp * W][0], W, 1 + grp, wid, lane);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       if (u * R + r >= rows) break;
-      const float c1 = sums[2 * r] * inv, c2 = sums[2 * r + 1] * inv;
+      const float k1 = -rstd[r] * (sums[2 * r] * inv), k2 = -rstd[r] * (sums[2 * r + 1] * inv);
+      const f2 c1 = f2_pack(k1, k1), c2 = f2_pack(k2, k2);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const int i = gl + 32 * W * v;
         if (i < nv) {
-          float xf[N], gf[N], o[N];
-          Of<T>::get(xc[r][v], xf); Of<T>::get(gc[r][v], gf);
+          f2 xf[M], gf[M];
+          get2<T>(take(slot(s, r, 0, v)), xf); get2<T>(take(slot(s, r, 1, v)), gf);
 #pragma unroll
-          for (int j = 0; j < N; ++j) {
-            const float xh = (xf[j] - st[r].x) * st[r].y;
-            o[j] = st[r].y * (gf[j] * wf[v][j] - c1 - xh * c2);
-          }
+          for (int j = 0; j < M; ++j)
+            xf[j] = f2_fma(f2_fma(xf[j], rs[r], off[r]), c2, f2_fma(f2_mul(gf[j], wf[v][j]), rs[r], c1));
           if (RES) {
-            float rf[N];
-            Of<T>::get(take(slot(s, r, 2, v)), rf);
+            get2<T>(take(slot(s, r, 2, v)), gf);
 #pragma unroll
-            for (int j = 0; j < N; ++j) o[j] += rf[j];
+            for (int j = 0; j < M; ++j) xf[j] = f2_add(xf[j], gf[j]);
           }
-          reinterpret_cast<uint4*>(dx + (size_t)(u * R + r) * D)[i] = Of<T>::put(o);
+          reinterpret_cast<uint4*>(dx + (size_t)(u * R + r) * D)[i] = put2<T>(xf);
         }
       }
     }
@@ -317,29 +345,23 @@ bwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict
   // the groups of a block in their order, through the ring, which nothing is copied into any more
   asm volatile("cp.async.wait_all;" ::: "memory");
   float* out = partial + (size_t)blockIdx.x * 2 * D;
-  if (G == 1) {
+  auto put_sums = [&](float* dst) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int i = gl + 32 * W * v;
       if (i < nv) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) { out[i * N + j] = dwa[v][j]; out[D + i * N + j] = dba[v][j]; }
+        for (int j = 0; j < M; ++j) {
+          reinterpret_cast<float2*>(dst + i * N)[j] = f2_unpack(dwa[v][j]);
+          reinterpret_cast<float2*>(dst + D + i * N)[j] = f2_unpack(dba[v][j]);
+        }
       }
     }
-    return;
-  }
+  };
+  if (G == 1) { put_sums(out); return; }
   __syncthreads();
   float* sh = reinterpret_cast<float*>(smem);
-  if (grp < G) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int i = gl + 32 * W * v;
-      if (i < nv) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) { sh[(size_t)grp * 2 * D + i * N + j] = dwa[v][j]; sh[(size_t)grp * 2 * D + D + i * N + j] = dba[v][j]; }
-      }
-    }
-  }
+  put_sums(sh + (size_t)grp * 2 * D);
   __syncthreads();
   for (int c = threadIdx.x; c < 2 * D; c += blockDim.x) {
     float t = 0.f;
@@ -444,22 +466,34 @@ static int launch_fwd(const void* x, const void* w, const void* b, void* y, floa
 
 template <class T, int VEC>
 static int forward(const void* x, const void* w, const void* b, void* y, float* stats, int rows, int D, float eps, cudaStream_t st) {
-  const int nv = D / VEC, lanes = (nv + 31) / 32;        // warps that hold a row with one vector a lane
+  // A warp alone on a row has no barrier and the fewest sums to join, and with many rows that is what counts; with few rows on an SM a row is
+  // spread so that its loads and its sums are short.  us, more vectors a lane / fewer (bf16): D = 1024 200 rows 2.97 / 2.37, 8192 rows 8.6 / 12.4;
+  // D = 2048 1000 rows 3.8 / 3.2, 4000 rows 8.8 / 10.8; D = 4096 200 rows 3.3 / 3.0, 1000 rows 5.4 / 7.8; D = 8192 8 rows 3.3 / 3.0, 200 rows
+  // 3.7 / 4.5; D = 16384 1000 rows 17.9 / 17.3, 4000 rows 51.2 / 52.1.  Single values: D = 1027, 8192 rows 24.3 with 8 x 8, 26.9 with 16 x 4,
+  // 34.9 with 4 x 16.
+  const int lanes = (D / VEC + 31) / 32;                 // warps that hold a row with one vector a lane
+  const int per_sm = (rows + num_sms() - 1) / num_sms();
 #define LN_FWD(V, W) return launch_fwd<T, VEC, V, W>(x, w, b, y, stats, rows, D, eps, st)
-  if (lanes <= 1) LN_FWD(1, 1);
-  if (lanes <= 2) LN_FWD(2, 1);
-  if (lanes <= 4) LN_FWD(4, 1);
-  if (lanes <= 8) LN_FWD(2, 4);
-  if (lanes <= 16) LN_FWD(4, 4);
-  if (lanes <= 32) LN_FWD(4, 8);
-  if (lanes <= 64) LN_FWD(4, 16);
-  if (lanes <= 128) LN_FWD(8, 16);
   if constexpr (VEC == 1) {
+    if (lanes <= 4) LN_FWD(4, 1);
+    if (lanes <= 8) LN_FWD(8, 1);
+    if (lanes <= 16) LN_FWD(8, 2);
+    if (lanes <= 32) LN_FWD(8, 4);
+    if (lanes <= 64) LN_FWD(8, 8);
+    if (lanes <= 128) LN_FWD(16, 8);
     if (lanes <= 256) LN_FWD(8, 32);
     LN_FWD(16, 32);
+  } else {
+    if (lanes <= 1) LN_FWD(1, 1);
+    if (lanes <= 2) { if (per_sm <= 4) LN_FWD(1, 2); LN_FWD(2, 1); }
+    if (lanes <= 4) { if (per_sm <= 7) LN_FWD(1, 4); LN_FWD(4, 1); }
+    if (lanes <= 8) { if (per_sm <= 7) LN_FWD(2, 4); LN_FWD(4, 2); }
+    if (lanes <= 16) { if (per_sm <= 2) LN_FWD(2, 8); LN_FWD(4, 4); }
+    if (lanes <= 32) { if (per_sm <= 1) LN_FWD(2, 16); LN_FWD(4, 8); }
+    if (lanes <= 64) { if (per_sm <= 7) LN_FWD(4, 16); LN_FWD(8, 8); }
+    LN_FWD(8, 16);
   }
 #undef LN_FWD
-  return -3;
 }
 
 struct Plan { int W, V, threads, grid; };
@@ -486,12 +520,12 @@ static Plan plan_any(int rows, int D) {
   return p;
 }
 
-template <class T, int V, int R, int S, bool RES>
+template <class T, int V, int R, int S, bool RES, bool W16>
 static int launch_bwd(const Plan& p, const void* x, const void* w, const void* dy, const float* stats, const void* gres, void* dx, float* partial,
                       int rows, int D, cudaStream_t st) {
   const int ring = S * R * (RES ? 3 : 2) * V * p.threads * 16;
-  if (ring > 40 * 1024 && cudaFuncSetAttribute(bwd_kernel<T, V, R, S, RES>, cudaFuncAttributeMaxDynamicSharedMemorySize, ring) != cudaSuccess) return -2;
-  bwd_kernel<T, V, R, S, RES><<<p.grid, p.threads, ring, st>>>((const T*)x, (const T*)w, (const T*)dy, (const float2*)stats, (const T*)gres, (T*)dx,
+  if (ring > 40 * 1024 && cudaFuncSetAttribute(bwd_kernel<T, V, R, S, RES, W16>, cudaFuncAttributeMaxDynamicSharedMemorySize, ring) != cudaSuccess) return -2;
+  bwd_kernel<T, V, R, S, RES, W16><<<p.grid, p.threads, ring, st>>>((const T*)x, (const T*)w, (const T*)dy, (const float2*)stats, (const T*)gres, (T*)dx,
                                                                partial, rows, D, p.W);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
@@ -501,16 +535,17 @@ static int backward(const void* x, const void* w, const void* dy, const float* s
                     int rows, int D, bool vec, cudaStream_t st) {
   const Plan p = vec ? plan_vec(rows, D, Of<T>::N) : plan_any(rows, D);
   int rc = 0;
-#define LN_BWD(V, R, S) rc = gres ? launch_bwd<T, V, R, S, true>(p, x, w, dy, stats, gres, dx, partial, rows, D, st) \
-                                  : launch_bwd<T, V, R, S, false>(p, x, w, dy, stats, gres, dx, partial, rows, D, st)
+#define LN_BWD(V, R, S, W16) rc = gres ? launch_bwd<T, V, R, S, true, W16>(p, x, w, dy, stats, gres, dx, partial, rows, D, st) \
+                                       : launch_bwd<T, V, R, S, false, W16>(p, x, w, dy, stats, gres, dx, partial, rows, D, st)
 #define LN_ANY(V) bwd_any_kernel<T, V><<<p.grid, p.threads, 0, st>>>((const T*)x, (const T*)w, (const T*)dy, (const float2*)stats, (const T*)gres, \
                                                                      (T*)dx, partial, rows, D)
   if (rows > 0) {
     if (vec) {
-      if (p.V == 1) LN_BWD(1, 2, 2);
-      else if (p.V == 2) LN_BWD(2, 2, 2);
-      else if (p.V == 4) LN_BWD(4, 1, 2);
-      else if constexpr (Of<T>::N == 4) LN_BWD(8, 1, 1);
+      if (p.V == 1 && p.W == 16) LN_BWD(1, 2, 2, true);
+      else if (p.V == 1) LN_BWD(1, 2, 2, false);
+      else if (p.V == 2) LN_BWD(2, 2, 2, true);
+      else if (p.V == 4) LN_BWD(4, 1, 2, true);
+      else if constexpr (Of<T>::N == 4) LN_BWD(8, 1, 1, true);
       else rc = -3;
       if (rc) return rc;
     } else {

@@ -50,7 +50,7 @@ def act_quantize(x):
     xf = F.pad(x.detach().float(), (0, n * ACT_BLOCK - D)).view(*x.shape[:-1], n, ACT_BLOCK)
     amax = xf.abs().amax(-1, keepdim=True)
     q = torch.round(xf * (127.0 / amax.clamp(min=1e-30))).nan_to_num(0.0, 127.0, -127.0).clamp(-127, 127).to(torch.int8)
-    return q.view(*x.shape[:-1], n * ACT_BLOCK)[..., :D].contiguous(), (amax / 127.0).squeeze(-1)
+    return q.view(*x.shape[:-1], n * ACT_BLOCK)[..., :D].contiguous(), torch.where(amax.isfinite(), amax / 127.0, torch.nan).squeeze(-1)
 
 
 def act_dequantize(q, scale, dtype):
