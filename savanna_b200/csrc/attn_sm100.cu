@@ -21,7 +21,12 @@
 // the attention start earlier still, as soon as the last rotary blocks run, gains nothing more (38.1).
 //
 // Every wait is bounded (sm100.cuh); on a timeout the CTA records a status code, frees TMEM and returns.
+#include <cooperative_groups.h>
+
+#include <atomic>
+
 #include "entries.h"
+#include "f32x2.cuh"
 #include "pdl.cuh"
 #include "sm100.cuh"
 
@@ -48,6 +53,45 @@ struct FwdParams {
   int heads_fast;            // grid order (H, B, query blocks) instead of (query blocks, H, B)
   int pingpong;              // 1: the two softmax warpgroups take turns on the exponentials (see the kernel)
 };
+
+// ------------------------------------------------------------------------------------ bias by relative position
+// s = q k^T scale + bias_scale table[bucket(q - k), h], the bucket of a distance from a map: 0 .. far (causal), or -far .. far; beyond it the
+// last entry counts.  Variants of both kernels (template parameter RPE) add it to the scores in registers, so that no [L, L] bias exists:
+//   - A tile all of whose pairs are at least `far` apart has one bias, which is folded into the constant of the exponent: nothing per pair.
+//     With far = 128 those are all but two or three tiles of a row.
+//   - In the others ("near") a pair's bias is read from the head's values by distance; consecutive lanes have consecutive distances.
+//   - The table's gradient needs the sums of dS along the diagonals of the near tiles: 32 x 32 pairs a warp, by accumulators that travel along
+//     the diagonals from lane to lane.  Each warp writes its 64 sums to a place of its own, and rpe_table_kernel adds them up in a fixed
+//     order, with one sum per warp of the far tiles.
+//   - delta = sum(dO O) must be good to the rounding of dS itself: the forward divides O by the sum of the ROUNDED probabilities, so that it is
+//     an exact average under slightly other weights, and hands on what O lost in rounding (out_lo); lse has the sum of the unrounded ones.  What error e is left in a row's delta adds
+//     P e to each dS.  In a causal row the far keys' true sum is as small as that of the near ones (both add up to zero), so their error,
+//     e times nearly all of P, would be a percent of it at 8192 keys.  Minus the sum of all other distances is off by e times the near
+//     keys' P instead.  The gradient of the last distance is an average of the two, weighted by what of P lies near and far.
+constexpr int RPE_MAX_FAR = 2048;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+enum { RPE_NONE = 0, RPE_CAUSAL = 1, RPE_BOTH = 2 };
+struct RpeParams {
+  const void* table;         // [nb, H], fp32 or bf16
+  const int* buckets;        // [far + 1] (causal) or [2 far + 1]
+  int table_f32, nb, far;
+  float scale_log2;          // bias_scale * log2(e)
+  __nv_bfloat16* out_lo;     // like out, or null: what the output lost in rounding
+  // backward
+  const float* values;       // [H, width] log2(e) * bias by distance, entry `origin` at distance 0
+  int width, origin;
+  float* diag;               // [B * H * key blocks, 8 warps, near tiles, 64]: sums along the diagonals of the near tiles
+  float* outer;              // [B * H * key blocks, 8 warps, 2]: sums of dS of the tiles beyond +far, and beyond -far or (causal) of P of the near ones
+  int x_lo, x_hi;            // near tiles: query tile start - key block start, in units of 64
+};
+// log2(e) * bias at distance d of head h; a bucket that does not exist has none
+__device__ __forceinline__ float rpe_value(const RpeParams& r, int mode, int H, int h, int d) {
+  const int i = mode == RPE_CAUSAL ? min(max(d, 0), r.far) : min(max(d, -r.far), r.far) + r.far;
+  const int b = r.buckets[i];
+  if (b < 0 || b >= r.nb) return 0.f;
+  const size_t at = (size_t)b * H + h;
+  return r.scale_log2 * (r.table_f32 ? reinterpret_cast<const float*>(r.table)[at] : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(r.table)[at]));
+}
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int c0, int c1, int c2, int c3, uint32_t bar) {
   asm volatile(
@@ -91,10 +135,11 @@ __device__ __forceinline__ uint64_t desc_mnmajor(uint32_t tile, int kk) {
 // (a single-CTA M = 128 product with both operands in shared memory uses the whole shared-memory bandwidth of the SM).
 // The price is an ordering constraint: the scores of block j+1 overwrite P(j), so S_t(j+1) is issued behind P_t(j) V(j)
 // on the (in-order) tensor pipe instead of during softmax j; the other query tile fills the gap.
-template <bool P_TMEM>
+template <bool P_TMEM, int RPE>
 __global__ void __launch_bounds__(FWD_THREADS, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                const __grid_constant__ CUtensorMap tmV, FwdParams p) {
+                const __grid_constant__ CUtensorMap tmV, FwdParams p, const __grid_constant__ RpeParams rp) {
+  static_assert(!RPE || P_TMEM, "the bias by distance takes the shared memory of P");
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -254,8 +299,19 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     const uint32_t t_o = tmem_base + (uint32_t(quarter * 32) << 16) + 256 + t * 128;
     const uint32_t p_tile = sP + t * TILE_BYTES;
     const float sl2 = p.scale_log2;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f;                    // RPE: m in units of log2, bias included
+    float lr = 0.f;                                  // RPE: sum of the rounded probabilities, where l is that of the unrounded ones
     bool ok = true;
+    // near tiles reach distances of far + 253: 127 beyond their first column's
+    float* bias_s = reinterpret_cast<float*>(smem_gen + 5 * TILE_BYTES);
+    const int origin = RPE == RPE_BOTH ? rp.far + 256 : 128;
+    float beyond[2] = {0.f, 0.f};                    // of the tiles beyond +far, -far
+    if (RPE) {
+      for (int i = (int)threadIdx.x - 64; i < origin + rp.far + 256; i += 256) bias_s[i] = rpe_value(rp, RPE, p.H, h, i - origin);
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      beyond[0] = bias_s[origin + rp.far];
+      beyond[1] = bias_s[RPE == RPE_BOTH ? origin - rp.far : origin];
+    }
     for (int j = 0; j < nb[t] && ok; ++j) {
       const uint32_t par = uint32_t(j) & 1u;
       if (!mbar_wait(s_full(t), par, abort_flag, p.status, ST_ATTN + 7)) { ok = false; break; }
@@ -270,6 +326,20 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       tmem_wait_ld();
       tc_fence_before();
       mbar_arrive(s_free(t));
+      float mul = sl2, add = 0.f;                    // RPE: x = v * mul + add in units of log2
+      if (RPE) {
+        const int base = q0 + t * BQ - k0;           // distance of the tile's first row and column
+        if (base - 127 < rp.far && (RPE == RPE_CAUSAL || base + 127 > -rp.far)) {
+          const float* bt = bias_s + origin + base + r;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[c][i] = __float_as_uint(fmaf(__uint_as_float(v[c][i]), sl2, bt[-(c * 32 + i)]));
+          mul = 1.f;
+        } else {
+          add = base > 0 ? beyond[0] : beyond[1];
+        }
+      }
       if (edge) {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
@@ -285,12 +355,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 #pragma unroll
         for (int i = 1; i < 32; ++i) bm4[c] = fmaxf(bm4[c], __uint_as_float(v[c][i]));
       }
-      const float bm = fmaxf(fmaxf(bm4[0], bm4[1]), fmaxf(bm4[2], bm4[3]));
+      float bm = fmaxf(fmaxf(bm4[0], bm4[1]), fmaxf(bm4[2], bm4[3]));
+      if (RPE) bm = fmaf(bm, mul, add);              // of the row, in the units of m
+      const float unit = RPE ? 1.f : sl2;
       // keep the old reference maximum unless the new one exceeds it by more than 2^8 (P stays below 256)
       float m_new = m;
-      if (bm > m && (m == -INFINITY || (bm - m) * sl2 > 8.f)) m_new = bm;
+      if (bm > m && (m == -INFINITY || (bm - m) * unit > 8.f)) m_new = bm;
       const float m_ref = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = (m == -INFINITY) ? 0.f : ex2((m - m_ref) * sl2);
+      const float alpha = (m == -INFINITY) ? 0.f : ex2((m - m_ref) * unit);
       const bool rescale = (j > 0) && (m_new != m);
       m = m_new;
       if (j > 0) {
@@ -309,8 +381,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         }
       }
       // P = exp2((S - m) * scale) as bf16 into the swizzled P tile; row sum in fp32
-      const float moff = -m_ref * sl2;
+      const float moff = RPE ? add - m_ref : -m_ref * sl2;
       float rs4[4] = {0.f, 0.f, 0.f, 0.f};
+      f2 rs2[2] = {0, 0}, rounded[2] = {0, 0};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
 #pragma unroll
@@ -318,11 +391,16 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           uint32_t w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float xa = fmaf(__uint_as_float(v[c][g * 8 + 2 * i]), sl2, moff);
-            const float xb = fmaf(__uint_as_float(v[c][g * 8 + 2 * i + 1]), sl2, moff);
+            const float xa = fmaf(__uint_as_float(v[c][g * 8 + 2 * i]), RPE ? mul : sl2, moff);
+            const float xb = fmaf(__uint_as_float(v[c][g * 8 + 2 * i + 1]), RPE ? mul : sl2, moff);
             const float ea = ex2(xa), eb = ex2(xb);        // exp2(-inf) = 0 for masked keys
-            rs4[i] += ea + eb;
             w[i] = pack_bf16(ea, eb);
+            if (RPE) {
+              rs2[i & 1] = f2_add(rs2[i & 1], f2_pack(ea, eb));
+              rounded[i & 1] = f2_add(rounded[i & 1], f2_bf(w[i]));      // what enters the product
+            } else {
+              rs4[i] += ea + eb;
+            }
           }
           if (P_TMEM) {
             // the score registers of these 8 keys are dead: keep the packed probabilities in their place
@@ -341,7 +419,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       }
       if (P_TMEM) tmem_wait_st();
       if (p.pingpong) mbar_arrive(turn(t ^ 1));               // hand the unit to the other warpgroup
-      const float rs = (rs4[0] + rs4[1]) + (rs4[2] + rs4[3]);
+      float rs = (rs4[0] + rs4[1]) + (rs4[2] + rs4[3]);
+      if (RPE) {
+        const float2 e = f2_unpack(f2_add(rs2[0], rs2[1])), d = f2_unpack(f2_add(rounded[0], rounded[1]));
+        rs = e.x + e.y;
+        lr = lr * alpha + (d.x + d.y);
+      }
       l = l * alpha + rs;
       if (__any_sync(0xffffffffu, rescale)) {
 #pragma unroll 1
@@ -363,7 +446,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       const uint32_t par = uint32_t(nb[t] - 1) & 1u;
       if (mbar_wait(pv_done(t), par, abort_flag, p.status, ST_ATTN + 9)) {
         tc_fence_after();
-        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const float div = RPE ? lr : l, inv = div > 0.f ? 1.f / div : 0.f;
         __nv_bfloat16* orow = p.out + (long long)b * p.o_sb + (long long)row * p.o_sl + (long long)h * p.o_sh;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
@@ -379,11 +462,20 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
               o.z = pack_bf16(__uint_as_float(v[g * 8 + 4]) * inv, __uint_as_float(v[g * 8 + 5]) * inv);
               o.w = pack_bf16(__uint_as_float(v[g * 8 + 6]) * inv, __uint_as_float(v[g * 8 + 7]) * inv);
               *reinterpret_cast<uint4*>(orow + c * 32 + g * 8) = o;
+              if (RPE && rp.out_lo) {
+                const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
+                uint32_t lw[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  lw[i] = pack_bf16(fmaf(__uint_as_float(v[g * 8 + 2 * i]), inv, -__uint_as_float(ow[i] << 16)),
+                                    fmaf(__uint_as_float(v[g * 8 + 2 * i + 1]), inv, -__uint_as_float(ow[i] & 0xffff0000u)));
+                *reinterpret_cast<uint4*>(rp.out_lo + (orow - p.out) + c * 32 + g * 8) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+              }
             }
           }
         }
         if (row < p.Lq)
-          p.lse[((long long)b * p.H + h) * p.Lq + row] = (m == -INFINITY ? 0.f : m) * p.scale + __logf(fmaxf(l, 1e-37f));
+          p.lse[((long long)b * p.H + h) * p.Lq + row] = (m == -INFINITY ? 0.f : m) * (RPE ? LN2 : p.scale) + __logf(fmaxf(l, 1e-37f));
       }
     }
   }
@@ -457,11 +549,11 @@ __device__ __forceinline__ uint64_t pdesc_mnmajor(uint32_t tile, int kk) { retur
 // P_TMEM: P^T stays in tensor memory (written over the consumed S^T columns, two bf16 per 32-bit cell) and feeds the dV
 // product as the A operand from TMEM; the shared memory this frees holds a third Q/dO stage, which takes the tile loads
 // off the critical path.  Otherwise P^T goes through shared memory like dS^T and there are two Q/dO stages.
-template <bool P_TMEM>
+template <bool P_TMEM, int RPE>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
-                const __grid_constant__ CUtensorMap tmDQ, BwdParams p) {
+                const __grid_constant__ CUtensorMap tmDQ, BwdParams p, const __grid_constant__ RpeParams rp) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -647,6 +739,14 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     const uint32_t lane_off = uint32_t(quarter * 32) << 16;
     const float sl2 = p.scale_log2;
     bool ok = n > 0;
+    const float* values = nullptr;                   // of this key: entry d at distance d
+    float beyond[2] = {0.f, 0.f}, outer[2] = {0.f, 0.f};
+    const long long place = (((long long)b * p.H + h) * gridDim.x + blockIdx.x) * 8 + wg * 4 + quarter;
+    if (RPE) {
+      values = rp.values + (size_t)h * rp.width + rp.origin;
+      beyond[0] = values[rp.far];
+      if (RPE == RPE_BOTH) beyond[1] = values[-rp.far];
+    }
     for (int it = 0; it < n && ok; ++it) {
       const int s = it & 1;
       const int qi = (i_start + it) * BQ2 + wg * 32;   // first query of this thread's 32 columns
@@ -663,15 +763,44 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       tc_fence_before();
       mbar_arrive(dp_free);
       uint32_t pw[16], dw[16];
+      const int x = RPE ? (i_start + it) - k0 / BQ2 : 0;
+      const bool near = RPE && x >= rp.x_lo && x <= rp.x_hi;
+      if (near) {
+        // column i is at distance qi + i - key; `up` gathers the diagonals i - lane = 31 - lane >= 0, `down` -1 - lane, while they travel
+        const float* bv = values + (qi - key);
+        const int vis = key >= p.Lk ? 32 : RPE == RPE_CAUSAL ? key - qi : 0;      // columns 0 .. vis - 1 are masked
+        const float* sf = reinterpret_cast<const float*>(st);
+        float up = 0.f, down = 0.f, pl = 0.f, dl = 0.f, mass = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float4 sd = st[i];
-        const float pa = ex2(fmaf(__uint_as_float(sv[2 * i]), sl2, sd.x));
-        const float pb = ex2(fmaf(__uint_as_float(sv[2 * i + 1]), sl2, sd.z));
-        const float da = pa * fmaf(__uint_as_float(dp[2 * i]), p.scale, -sd.y);
-        const float db = pb * fmaf(__uint_as_float(dp[2 * i + 1]), p.scale, -sd.w);
-        pw[i] = pack_bf16(pa, pb);
-        dw[i] = pack_bf16(da, db);
+        for (int i = 0; i < 32; ++i) {
+          float pp = ex2(fmaf(__uint_as_float(sv[i]), sl2, sf[2 * i]) + bv[i]);
+          float ds = pp * fmaf(__uint_as_float(dp[i]), p.scale, -sf[2 * i + 1]);
+          if (i < vis) { pp = 0.f; ds = 0.f; }
+          if (i) { up = __shfl_sync(0xffffffffu, up, (lane + 31) & 31); down = __shfl_sync(0xffffffffu, down, (lane + 31) & 31); }
+          if (lane <= i) up += ds; else down += ds;
+          if (RPE == RPE_CAUSAL) mass += pp;
+          if (i & 1) { pw[i >> 1] = pack_bf16(pl, pp); dw[i >> 1] = pack_bf16(dl, ds); }
+          else { pl = pp; dl = ds; }
+        }
+        float* to = rp.diag + (place * (rp.x_hi - rp.x_lo + 1) + (x - rp.x_lo)) * 64;
+        to[63 - lane] = up;                          // sum of diagonal e at 32 + e
+        to[31 - lane] = down;
+        outer[1] += mass;                            // zero unless causal
+      } else {
+        const float far = x > 0 ? beyond[0] : beyond[1];
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float4 sd = st[i];
+          const float pa = ex2(fmaf(__uint_as_float(sv[2 * i]), sl2, RPE ? sd.x + far : sd.x));
+          const float pb = ex2(fmaf(__uint_as_float(sv[2 * i + 1]), sl2, RPE ? sd.z + far : sd.z));
+          const float da = pa * fmaf(__uint_as_float(dp[2 * i]), p.scale, -sd.y);
+          const float db = pb * fmaf(__uint_as_float(dp[2 * i + 1]), p.scale, -sd.w);
+          if (RPE) sum += da + db;
+          pw[i] = pack_bf16(pa, pb);
+          dw[i] = pack_bf16(da, db);
+        }
+        if (RPE && key < p.Lk) { if (RPE == RPE_CAUSAL || x > 0) outer[0] += sum; else outer[1] += sum; }
       }
       if ((p.causal && key > qi) || key >= p.Lk) {
         // some of this row's 32 columns are masked (only the tiles on the diagonal, and the key rows beyond Lk)
@@ -700,6 +829,14 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       fence_proxy_async();
       tc_fence_before();
       mbar_arrive(pds_ready(s));
+    }
+    if (RPE) {
+#pragma unroll
+      for (int o = 16; o; o >>= 1) {
+        outer[0] += __shfl_xor_sync(0xffffffffu, outer[0], o);
+        outer[1] += __shfl_xor_sync(0xffffffffu, outer[1], o);
+      }
+      if (lane < 2) rp.outer[place * 2 + lane] = outer[lane & 1];
     }
     if (ok && mbar_wait(dkv_done, 0u, abort_flag, p.status, ST_ATTN + 29)) {
       tc_fence_after();
@@ -735,14 +872,22 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 }
 
 // stats[b, h, i] = (-lse * log2(e), scale * (sum_d dO[b, i, h, d] * O[b, i, h, d] - dlse[b, h, i])) for i < L and (0, 0)
-// for the padding rows L <= i < Lpad.  A block takes one row i of one batch entry, sixteen lanes with 16-byte loads a head
+// for the padding rows L <= i < Lpad; with a bias (-inf, 0) there, whose exponential is 0 whatever the bias.  A block takes one row i of one batch entry, sixteen lanes with 16-byte loads a head
 // (one warp per head with 8-byte loads and 64-bit index divisions per row ran at a third of the copy bandwidth).
+// RPE: O + out_lo stands for O, and the last row of blocks writes the heads' values by distance.
 constexpr int STATS_THREADS = 256;
+template <int RPE>
 __global__ void __launch_bounds__(STATS_THREADS)
 attn_stats_kernel(const __nv_bfloat16* __restrict__ go, const __nv_bfloat16* __restrict__ o, const float* __restrict__ lse,
                   const float* __restrict__ glse, float* __restrict__ stats, int H, int L, int Lpad, float scale, long long g_sb,
-                  long long g_sl, long long g_sh, long long o_sb, long long o_sl, long long o_sh) {
+                  long long g_sl, long long g_sh, long long o_sb, long long o_sl, long long o_sh, const __grid_constant__ RpeParams rp) {
   const int i = blockIdx.x, bb = blockIdx.y, lane = threadIdx.x & 15;
+  if (RPE && bb == gridDim.y - 1) {
+    for (int hh = blockIdx.x; hh < H; hh += gridDim.x)
+      for (int e = threadIdx.x; e < rp.width; e += STATS_THREADS)
+        const_cast<float*>(rp.values)[(size_t)hh * rp.width + e] = rpe_value(rp, RPE, H, hh, e - rp.origin);
+    return;
+  }
   for (int hh = threadIdx.x >> 4; hh < (H + 1) / 2 * 2; hh += STATS_THREADS / 16) {      // whole warps stay in the shuffles
     float sum = 0.f;
     if (i < L && hh < H) {
@@ -752,7 +897,11 @@ attn_stats_kernel(const __nv_bfloat16* __restrict__ go, const __nv_bfloat16* __r
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&aw[j]));
-        const float2 g = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&cw[j]));
+        float2 g = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&cw[j]));
+        if (RPE) {
+          const __nv_bfloat162 lo = *reinterpret_cast<const __nv_bfloat162*>(rp.out_lo + bb * o_sb + i * o_sl + hh * o_sh + lane * 8 + 2 * j);
+          g.x += __low2float(lo); g.y += __high2float(lo);
+        }
         sum += f.x * g.x + f.y * g.y;
       }
     }
@@ -760,7 +909,7 @@ attn_stats_kernel(const __nv_bfloat16* __restrict__ go, const __nv_bfloat16* __r
     for (int off = 8; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
     if (lane == 0 && hh < H) {
       const long long row = (long long)bb * H + hh;
-      float2 v = make_float2(0.f, 0.f);
+      float2 v = make_float2(RPE ? -INFINITY : 0.f, 0.f);
       if (i < L) v = make_float2(-lse[row * L + i] * 1.4426950408889634f, scale * (sum - (glse ? glse[row * L + i] : 0.f)));
       reinterpret_cast<float2*>(stats)[row * Lpad + i] = v;
     }
@@ -887,6 +1036,100 @@ __global__ void attn_dq_cast_kernel(const float* __restrict__ acc, __nv_bfloat16
   *reinterpret_cast<uint4*>(dq + bb * sb_ + i * sl_ + hh * sh_ + c) = o;
 }
 
+// dtable[b, h] = factor * sum over the distances d of bucket b of (the sums of dS at distance d).  Eight blocks (a cluster) a head: each takes
+// every eighth key block's sums, the first adds the eight up in order.  Distances of near tiles: 0 (or -far - 191) .. far + 191, the outermost
+// of which count as far.
+constexpr int TABLE_THREADS = 512, TABLE_SPLIT = 8;
+template <int RPE>
+__global__ void __cluster_dims__(TABLE_SPLIT, 1, 1) __launch_bounds__(TABLE_THREADS)
+rpe_table_kernel(const __grid_constant__ RpeParams rp, void* dtable, float factor, int B, int H, int L, int kblocks) {
+  extern __shared__ float sums[];                  // [count] by distance, then [4][128] while they are formed
+  __shared__ float total, ends[2];
+  const int rank = blockIdx.x % TABLE_SPLIT, h = blockIdx.x / TABLE_SPLIT, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int low = RPE == RPE_BOTH ? -(rp.far + 191) : 0, count = rp.far + 192 - low;
+  const int nq = (L + BQ2 - 1) / BQ2, tiles = rp.x_hi - rp.x_lo + 1, rows = B * kblocks;
+  float* part = sums + count;
+  wait_for_previous();
+  for (int c0 = 0; c0 < count; c0 += 128) {
+    const int c = c0 + (tid & 127);
+    float s = 0.f;
+    if (c < count) {
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {                // the warps of a block: queries 32 (w / 4), keys 32 (w % 4) into the tile
+        const int y = low + c - 32 * (w >> 2) + 32 * (w & 3) + 32, x = y >> 6, e = y & 63;      // floor: y may be negative
+        if (x < rp.x_lo || x > rp.x_hi) continue;
+        for (int row = rank + TABLE_SPLIT * (tid >> 7); row < rows; row += TABLE_SPLIT * 4) {
+          const int bb = row / kblocks, kb = row - bb * kblocks, q = kb * (BK / BQ2) + x;
+          if (q >= 0 && q < nq) s += rp.diag[((((long long)bb * H + h) * kblocks + kb) * 8 + w) * tiles * 64 + (x - rp.x_lo) * 64 + e];
+        }
+      }
+    }
+    part[tid] = s;
+    __syncthreads();
+    if (tid < 128 && c < count) sums[c] = (part[tid] + part[tid + 128]) + (part[tid + 256] + part[tid + 384]);
+    __syncthreads();
+  }
+  if (warp < 2) {
+    float s = 0.f;
+    for (int k = lane; k < rows * 8; k += 32) {
+      const int row = k >> 3, bb = row / kblocks, kb = row - bb * kblocks;
+      if (row % TABLE_SPLIT == rank) s += rp.outer[((((long long)bb * H + h) * kblocks + kb) * 8 + (k & 7)) * 2 + warp];
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) ends[warp] = s;
+  }
+  auto cluster = cooperative_groups::this_cluster();
+  cluster.sync();
+  if (rank == 0) {
+    for (int c = tid; c < count; c += TABLE_THREADS) {
+      float s = 0.f;
+#pragma unroll
+      for (int k = 0; k < TABLE_SPLIT; ++k) s += *cluster.map_shared_rank(&sums[c], k);
+      sums[c] = s;                                 // read by this thread alone before
+    }
+    if (tid < 2) {
+      float s = 0.f;
+      for (int k = 0; k < TABLE_SPLIT; ++k) s += *cluster.map_shared_rank(&ends[tid], k);
+      part[tid] = s;
+    }
+    __syncthreads();
+    if (RPE == RPE_CAUSAL && warp == 0) {            // the last distance: its own sum, or minus that of all others
+      float near = 0.f, own = 0.f;
+      for (int c = lane; c < count; c += 32) { if (c < rp.far) near += sums[c]; else own += sums[c]; }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) {
+        near += __shfl_xor_sync(0xffffffffu, near, o);
+        own += __shfl_xor_sync(0xffffffffu, own, o);
+      }
+      if (lane == 0) {
+        const float rows_p = (float)B * L, mn = part[1] / rows_p, mf = fmaxf(0.f, 1.f - mn), w = mn * mn / (mn * mn + mf * mf);
+        total = w * (own + part[0]) - (1.f - w) * near;
+      }
+    }
+    __syncthreads();
+    for (int bk = warp; bk < rp.nb; bk += TABLE_THREADS / 32) {
+      float s = 0.f;
+      for (int c = lane; c < count; c += 32) {
+        const int d = low + c, i = RPE == RPE_BOTH ? min(max(d, -rp.far), rp.far) + rp.far : d;
+        if ((RPE == RPE_BOTH || d < rp.far) && rp.buckets[i] == bk) s += sums[c];
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if (lane == 0) {
+        if (RPE == RPE_CAUSAL) { if (rp.buckets[rp.far] == bk) s += total; }
+        else {
+          if (rp.buckets[2 * rp.far] == bk) s += part[0];
+          if (rp.buckets[0] == bk) s += part[1];
+        }
+        if (rp.table_f32) reinterpret_cast<float*>(dtable)[(size_t)bk * H + h] = s * factor;
+        else reinterpret_cast<__nv_bfloat16*>(dtable)[(size_t)bk * H + h] = __float2bfloat16_rn(s * factor);
+      }
+    }
+  }
+  cluster.sync();                                  // the others' shared memory stays until it has been read
+}
+
 // ------------------------------------------------------------------------------------ host side
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -933,13 +1176,12 @@ extern "C" int sb_attn_set_bwd_variant(int p_in_tmem) { sb::attn::g_p_tmem = p_i
 extern "C" int sb_attn_set_fwd_variant(int pingpong) { sb::attn::g_pingpong = pingpong ? 1 : 0; return 0; }
 extern "C" int sb_attn_set_fwd_p_tmem(int on) { sb::attn::g_fwd_p_tmem = on ? 1 : 0; return 0; }
 
-// Attention forward.  q [B, Lq, H, 128], k and v [B, Lk, H, 128], out like q: bf16, last dimension contiguous, the
-// other strides (in elements) multiples of 8.  lse [B, H, Lq] fp32.  causal needs Lq == Lk (row i sees keys 0..i).
-extern "C" int sb_attn_fwd(const void* q, const void* k, const void* v, void* out, float* lse, int B, int H, int Lq, int Lk,
-                           const long long* q_str, const long long* k_str, const long long* v_str, const long long* o_str,
-                           int causal, float scale, unsigned int* status, cudaStream_t stream) {
-  using namespace sb;
-  using namespace sb::attn;
+namespace sb {
+namespace attn {
+template <int RPE>
+static int attn_forward(const void* q, const void* k, const void* v, void* out, float* lse, int B, int H, int Lq, int Lk, const long long* q_str,
+                        const long long* k_str, const long long* v_str, const long long* o_str, int causal, float scale, const RpeParams& rp,
+                        unsigned int* status, cudaStream_t stream) {
   if (B <= 0 || H <= 0 || Lq <= 0 || Lk <= 0) return 0;
   if (causal && Lq != Lk) return -3;
   static thread_local bool ctx_bound = false;
@@ -950,11 +1192,13 @@ extern "C" int sb_attn_fwd(const void* q, const void* k, const void* v, void* ou
   if ((rc = make_tmap(&tq, q, B, Lq, H, q_str[0], q_str[1], q_str[2]))) return rc;
   if ((rc = make_tmap(&tk, k, B, Lk, H, k_str[0], k_str[1], k_str[2]))) return rc;
   if ((rc = make_tmap(&tv, v, B, Lk, H, v_str[0], v_str[1], v_str[2]))) return rc;
-  static bool attr_set = false;
-  if (!attr_set) {
-    if (cudaFuncSetAttribute(attn_fwd_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, FWD_SMEM) != cudaSuccess) return -5;
-    if (cudaFuncSetAttribute(attn_fwd_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, FWD_SMEM) != cudaSuccess) return -5;
-    attr_set = true;
+  static std::atomic<unsigned long long> attr_set{0};          // by device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -5;
+  if (!(attr_set.load() >> dev & 1)) {
+    if (!RPE && cudaFuncSetAttribute(attn_fwd_kernel<false, RPE_NONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, FWD_SMEM) != cudaSuccess) return -5;
+    if (cudaFuncSetAttribute(attn_fwd_kernel<true, RPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, FWD_SMEM) != cudaSuccess) return -5;
+    attr_set.fetch_or(1ull << dev);
   }
   FwdParams p{reinterpret_cast<__nv_bfloat16*>(out), lse, o_str[0], o_str[1], o_str[2], B, H, Lq, Lk, causal,
               scale * 1.4426950408889634f, scale, status, 0, g_pingpong};
@@ -967,20 +1211,17 @@ extern "C" int sb_attn_fwd(const void* q, const void* k, const void* v, void* ou
   // measured gain at 128 MB, and nothing to gain at 256 MB.
   p.heads_fast = causal && (long long)B * H * Lk * HD * 4 <= (128LL << 20) && qblocks <= 65535 && B <= 65535;
   const dim3 grid = p.heads_fast ? dim3(H, B, qblocks) : dim3(qblocks, H, B);
-  return launch_chained(false, g_fwd_p_tmem ? attn_fwd_kernel<true> : attn_fwd_kernel<false>, grid, FWD_THREADS, FWD_SMEM, stream, tq, tk, tv, p) ? -6 : 0;
+  auto* kernel = RPE || g_fwd_p_tmem ? attn_fwd_kernel<true, RPE> : attn_fwd_kernel<false, RPE_NONE>;
+  return launch_chained(false, kernel, grid, FWD_THREADS, FWD_SMEM, stream, tq, tk, tv, p, rp) ? -6 : 0;
 }
 
-// Attention backward.  go/q/out [B, Lq, H, 128], k/v [B, Lk, H, 128] (bf16, strided as in the forward); lse and the
-// optional dlse [B, H, Lq] fp32; scratch: stats (2 * B * H * 64 * ceil(Lq / 64) floats) and dq_acc [B, Lq, H, 128] fp32
-// (the kernel adds into it: zero it before the first of the calls that share it).  Results: dq (strided, bf16; null =
-// leave the sum in dq_acc), dk and dv (contiguous [B, Lk, H, 128], bf16).  Three launches (two without dq).
-extern "C" int sb_attn_bwd(const void* go, const void* q, const void* k, const void* v, const void* out, const float* lse,
-                           const float* glse, float* stats, float* dq_acc, void* dq, void* dk, int B, int H, int Lq, int Lk,
-                           void* dv, const long long* g_str, const long long* q_str, const long long* k_str,
-                           const long long* v_str, const long long* o_str, const long long* dq_str, const long long* dk_str,
-                           const long long* dv_str, int causal, float scale, unsigned int* status, cudaStream_t stream) {
-  using namespace sb;
-  using namespace sb::attn;
+
+template <int RPE>
+static int attn_backward(const void* go, const void* q, const void* k, const void* v, const void* out, const float* lse, const float* glse,
+                         float* stats, float* dq_acc, void* dq, void* dk, int B, int H, int Lq, int Lk, void* dv, const long long* g_str,
+                         const long long* q_str, const long long* k_str, const long long* v_str, const long long* o_str, const long long* dq_str,
+                         const long long* dk_str, const long long* dv_str, int causal, float scale, const RpeParams& rp, unsigned int* status,
+                         cudaStream_t stream) {
   if (B <= 0 || H <= 0 || Lq <= 0 || Lk <= 0) return 0;
   if (causal && Lq != Lk) return -3;
   static thread_local bool ctx_bound = false;
@@ -1008,27 +1249,123 @@ extern "C" int sb_attn_bwd(const void* go, const void* q, const void* k, const v
                      CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) { g_last_encode = (int)r; return -2; }
   }
-  static bool attr_set = false;
-  if (!attr_set) {
-    if (cudaFuncSetAttribute(attn_bwd_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, BWD_SMEM) != cudaSuccess) return -5;
-    if (cudaFuncSetAttribute(attn_bwd_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, BWD_SMEM) != cudaSuccess) return -5;
-    attr_set = true;
+  static std::atomic<unsigned long long> attr_set{0};          // by device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -5;
+  if (!(attr_set.load() >> dev & 1)) {
+    if (cudaFuncSetAttribute(attn_bwd_kernel<true, RPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, BWD_SMEM) != cudaSuccess) return -5;
+    if (!RPE && cudaFuncSetAttribute(attn_bwd_kernel<false, RPE_NONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, BWD_SMEM) != cudaSuccess) return -5;
+    attr_set.fetch_or(1ull << dev);
   }
   const int lpad = (Lq + BQ2 - 1) / BQ2 * BQ2;
-  attn_stats_kernel<<<dim3(lpad, B), STATS_THREADS, 0, stream>>>(
+  attn_stats_kernel<RPE><<<dim3(lpad, B + (RPE ? 1 : 0)), STATS_THREADS, 0, stream>>>(
       (const __nv_bfloat16*)go, (const __nv_bfloat16*)out, lse, glse, stats, H, Lq, lpad, scale, g_str[0], g_str[1], g_str[2],
-      o_str[0], o_str[1], o_str[2]);
+      o_str[0], o_str[1], o_str[2], rp);
   BwdParams p{stats, reinterpret_cast<__nv_bfloat16*>(dk), reinterpret_cast<__nv_bfloat16*>(dv),
               {dk_str[0], dk_str[1], dk_str[2]}, {dv_str[0], dv_str[1], dv_str[2]}, B, H, Lq, Lk,
               causal, scale * 1.4426950408889634f, scale, status};
   dim3 grid((Lk + BK - 1) / BK, H, B);
-  if (launch_chained(false, g_p_tmem ? attn_bwd_kernel<true> : attn_bwd_kernel<false>, grid, BWD_THREADS, BWD_SMEM, stream, tq, tk, tv, tg, tdq, p)) return -6;
+  auto* kernel = RPE || g_p_tmem ? attn_bwd_kernel<true, RPE> : attn_bwd_kernel<false, RPE_NONE>;
+  if (launch_chained(false, kernel, grid, BWD_THREADS, BWD_SMEM, stream, tq, tk, tv, tg, tdq, p, rp)) return -6;
   const long long orows = (long long)B * Lq * H;
   // dq == null: the caller keeps accumulating into dq_acc over several calls (ring attention) and casts at the end
   if (dq)
     attn_dq_cast_kernel<<<(unsigned)((orows * 16 + 255) / 256), 256, 0, stream>>>(dq_acc, (__nv_bfloat16*)dq, orows, H, Lq,
                                                                                  dq_str[0], dq_str[1], dq_str[2]);
   return cudaGetLastError() == cudaSuccess ? 0 : -6;
+}
+
+}  // namespace attn
+}  // namespace sb
+
+// Attention forward.  q [B, Lq, H, 128], k and v [B, Lk, H, 128], out like q: bf16, last dimension contiguous, the
+// other strides (in elements) multiples of 8.  lse [B, H, Lq] fp32.  causal needs Lq == Lk (row i sees keys 0..i).
+extern "C" int sb_attn_fwd(const void* q, const void* k, const void* v, void* out, float* lse, int B, int H, int Lq, int Lk,
+                           const long long* q_str, const long long* k_str, const long long* v_str, const long long* o_str,
+                           int causal, float scale, unsigned int* status, cudaStream_t stream) {
+  return sb::attn::attn_forward<sb::attn::RPE_NONE>(q, k, v, out, lse, B, H, Lq, Lk, q_str, k_str, v_str, o_str, causal, scale, {}, status, stream);
+}
+
+// Attention backward.  go/q/out [B, Lq, H, 128], k/v [B, Lk, H, 128] (bf16, strided as in the forward); lse and the
+// optional dlse [B, H, Lq] fp32; scratch: stats (2 * B * H * 64 * ceil(Lq / 64) floats) and dq_acc [B, Lq, H, 128] fp32
+// (the kernel adds into it: zero it before the first of the calls that share it).  Results: dq (strided, bf16; null =
+// leave the sum in dq_acc), dk and dv (contiguous [B, Lk, H, 128], bf16).  Three launches (two without dq).
+extern "C" int sb_attn_bwd(const void* go, const void* q, const void* k, const void* v, const void* out, const float* lse,
+                           const float* glse, float* stats, float* dq_acc, void* dq, void* dk, int B, int H, int Lq, int Lk,
+                           void* dv, const long long* g_str, const long long* q_str, const long long* k_str,
+                           const long long* v_str, const long long* o_str, const long long* dq_str, const long long* dk_str,
+                           const long long* dv_str, int causal, float scale, unsigned int* status, cudaStream_t stream) {
+  return sb::attn::attn_backward<sb::attn::RPE_NONE>(go, q, k, v, out, lse, glse, stats, dq_acc, dq, dk, B, H, Lq, Lk, dv, g_str, q_str, k_str,
+                                                     v_str, o_str, dq_str, dk_str, dv_str, causal, scale, {}, status, stream);
+}
+
+namespace sb {
+namespace attn {
+static int rpe_params(RpeParams& r, const void* table, int table_f32, const int* buckets, int nb, int far, float bias_scale) {
+  if (far < 0 || far > RPE_MAX_FAR || nb < 1) return -3;
+  r.table = table; r.buckets = buckets; r.table_f32 = table_f32; r.nb = nb; r.far = far;
+  r.scale_log2 = bias_scale * LOG2E;
+  return 0;
+}
+// Where the backward's scratch lies; its size in floats.
+static long long rpe_scratch(RpeParams& r, float* work, int B, int H, int L, int far, int causal) {
+  const long long blocks = (long long)B * H * ((L + BK - 1) / BK) * 8;
+  r.x_lo = causal ? 0 : -((far + 62) / 64);
+  r.x_hi = (far + 126) / 64;
+  r.origin = causal ? 128 : far + 192;
+  r.width = r.origin + far + 192;
+  const long long values = ((long long)H * r.width + 3) / 4 * 4, diag = blocks * (r.x_hi - r.x_lo + 1) * 64;
+  r.values = work;
+  r.diag = work + values;
+  r.outer = r.diag + diag;
+  return values + diag + blocks * 2;
+}
+}  // namespace attn
+}  // namespace sb
+
+// Attention forward with a bias by relative position: as sb_attn_fwd with Lq == Lk == L, plus bias_scale * table[bucket(q - k), h] on the scaled
+// scores.  table [nb, H] (fp32 or bf16), buckets [far + 1] (causal: of the distances 0 .. far) or [2 far + 1] (-far .. far), int32.  out_lo
+// (like out, or null): what the output lost in rounding, for the backward.
+extern "C" int sb_attn_rpe_fwd(const void* q, const void* k, const void* v, void* out, void* out_lo, float* lse, int B, int H, int L,
+                               const long long* q_str, const long long* k_str, const long long* v_str, const long long* o_str, int causal,
+                               float scale, const void* table, int table_f32, const int* buckets, int nb, int far, float bias_scale,
+                               unsigned int* status, cudaStream_t stream) {
+  using namespace sb::attn;
+  RpeParams r{};
+  if (int rc = rpe_params(r, table, table_f32, buckets, nb, far, bias_scale)) return rc;
+  if (reinterpret_cast<uintptr_t>(out_lo) & 15) return -4;
+  r.out_lo = (__nv_bfloat16*)out_lo;
+  return causal ? attn_forward<RPE_CAUSAL>(q, k, v, out, lse, B, H, L, L, q_str, k_str, v_str, o_str, 1, scale, r, status, stream)
+                : attn_forward<RPE_BOTH>(q, k, v, out, lse, B, H, L, L, q_str, k_str, v_str, o_str, 0, scale, r, status, stream);
+}
+
+// Floats of scratch that sb_attn_rpe_bwd needs.
+extern "C" long long sb_attn_rpe_bwd_work(int B, int H, int L, int far, int causal) {
+  sb::attn::RpeParams r{};
+  return sb::attn::rpe_scratch(r, nullptr, B, H, L, far, causal);
+}
+
+// Its backward: as sb_attn_bwd (dq_acc zeroed by the caller), plus dtable [nb, H] of table's type, written.  Four launches.
+extern "C" int sb_attn_rpe_bwd(const void* go, const void* q, const void* k, const void* v, const void* out, const void* out_lo, const float* lse,
+                               float* stats, float* dq_acc, void* dq, void* dk, void* dv, int B, int H, int L, const long long* g_str,
+                               const long long* q_str, const long long* k_str, const long long* v_str, const long long* o_str,
+                               const long long* dq_str, const long long* dk_str, const long long* dv_str, int causal, float scale,
+                               const void* table, int table_f32, const int* buckets, int nb, int far, float bias_scale, float* work,
+                               void* dtable, unsigned int* status, cudaStream_t stream) {
+  using namespace sb::attn;
+  if (B <= 0 || H <= 0 || L <= 0 || B >= 65535) return -3;
+  RpeParams r{};
+  if (int rc = rpe_params(r, table, table_f32, buckets, nb, far, bias_scale)) return rc;
+  rpe_scratch(r, work, B, H, L, far, causal);
+  r.out_lo = const_cast<__nv_bfloat16*>((const __nv_bfloat16*)out_lo);
+  const int rc = causal ? attn_backward<RPE_CAUSAL>(go, q, k, v, out, lse, nullptr, stats, dq_acc, dq, dk, B, H, L, L, dv, g_str, q_str, k_str, v_str,
+                                                    o_str, dq_str, dk_str, dv_str, 1, scale, r, status, stream)
+                        : attn_backward<RPE_BOTH>(go, q, k, v, out, lse, nullptr, stats, dq_acc, dq, dk, B, H, L, L, dv, g_str, q_str, k_str, v_str,
+                                                  o_str, dq_str, dk_str, dv_str, 0, scale, r, status, stream);
+  if (rc) return rc;
+  const int smem = 4 * ((causal ? far + 192 : 2 * (far + 191) + 1) + TABLE_THREADS);
+  return sb::launch_chained(false, causal ? rpe_table_kernel<RPE_CAUSAL> : rpe_table_kernel<RPE_BOTH>, dim3(H * TABLE_SPLIT), TABLE_THREADS, smem, stream,
+                            r, dtable, bias_scale / scale, B, H, L, (L + BK - 1) / BK) ? -6 : 0;
 }
 
 // Rotary embedding of `n` (1 or 2) tensors [B, L, H, 128] with tables cs / sn [L, rd] fp32 (rd a multiple of 16, at most

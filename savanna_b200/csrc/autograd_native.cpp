@@ -45,7 +45,7 @@ constexpr auto F32 = at::kFloat;
   X(sb_se_fwd) X(sb_se_fwd_taps) X(sb_se_bwd) X(sb_mr_fwd) X(sb_mr_bwd) X(sb_mr_tc_fwd) X(sb_mr_tc_bwd) X(sb_mr_umma_fwd) X(sb_mr_umma_bwd) \
   X(sb_li_fwd_tiled) \
   X(sb_li_bwd_tiled_chunk) X(sb_li_bwd_tiled) X(sb_attn_fwd) X(sb_attn_bwd) X(sb_attn_rope) \
-  X(sb_layernorm_fwd) X(sb_layernorm_bwd_blocks) X(sb_layernorm_bwd) X(sb_act8_quantize) X(sb_act8_dequantize)
+  X(sb_attn_rpe_fwd) X(sb_attn_rpe_bwd_work) X(sb_attn_rpe_bwd) X(sb_layernorm_fwd) X(sb_layernorm_bwd_blocks) X(sb_layernorm_bwd) X(sb_act8_quantize) X(sb_act8_dequantize)
 
 struct {
 #define SB_DECLARE(name) decltype(&::name) name = nullptr;
@@ -717,6 +717,53 @@ struct FlashPacked : Function<FlashPacked> {
   }
 };
 
+// The same without rotary embedding and with a learned bias by relative position: bias_scale * table[buckets[q - k], head] on the scores.
+// A row of one key has a softmax that is constant: only v has a gradient then, and it is exact.
+struct FlashRpe : Function<FlashRpe> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& qkv, const Tensor& table, const Tensor& buckets, double bias_scale, bool causal, bool train) {
+    const int64_t B = qkv.size(0), Ln = qkv.size(1), H = qkv.size(2), far = causal ? buckets.size(0) - 1 : buckets.size(0) / 2;
+    const at::Device dev = qkv.device();
+    Tensor q = qkv.slice(3, 0, 128), k = qkv.slice(3, 128, 256), v = qkv.slice(3, 256, 384), tc = contiguous(table), bc = contiguous(buckets);
+    Tensor o = alloc({B, Ln, H, 128}, BF16, dev), lo = train ? alloc_like(o) : Tensor(), lse = alloc({B, H, Ln}, F32, dev);
+    const Strides qs(q), ks(k), vs(v), os(o);
+    const int rc = SB_RUN(sb_attn_rpe_fwd, B * Ln * H > 0, ptr(q), ptr(k), ptr(v), out(o), out(lo), f32o(lse), (int)B, (int)H, (int)Ln, qs.s, ks.s, vs.s,
+                          os.s, (int)causal, 0.08838834764831845f, ptr(tc), (int)(tc.scalar_type() == F32), static_cast<const int*>(ptr(bc)),
+                          (int)tc.size(0), (int)far, (float)bias_scale, status_word(dev), stream());
+    TORCH_CHECK(rc == 0, "attention with relative position bias failed (code ", rc, ", encode ", L.sb_attn_last_encode_result(), "): ",
+                layouts({{"q", &q}, {"k", &k}, {"v", &v}, {"table", &tc}, {"buckets", &bc}}));
+    ctx->save_for_backward({qkv, tc, bc, o, lo, lse});
+    ctx->saved_data["bias_scale"] = bias_scale;
+    ctx->saved_data["causal"] = causal;
+    return o;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &qkv = s[0], &table = s[1], &buckets = s[2], &o = s[3], &lo = s[4], &lse = s[5];
+    const bool causal = ctx->saved_data["causal"].toBool();
+    const int64_t B = qkv.size(0), Ln = qkv.size(1), H = qkv.size(2), far = causal ? buckets.size(0) - 1 : buckets.size(0) / 2;
+    const at::Device dev = qkv.device();
+    Tensor dqkv = alloc(qkv.sizes(), BF16, dev), dtable = alloc_like(table);
+    if (Ln <= 1 || B * H == 0) {
+      cleared(dqkv);
+      if (dqkv.numel() > 0) dqkv.slice(3, 256, 384).copy_(g[0]);
+      return {dqkv, cleared(dtable), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+    Tensor q = qkv.slice(3, 0, 128), k = qkv.slice(3, 128, 256), v = qkv.slice(3, 256, 384);
+    Tensor dq = dqkv.slice(3, 0, 128), dk = dqkv.slice(3, 128, 256), dv = dqkv.slice(3, 256, 384);
+    Tensor go = packed_rows(g[0]) ? g[0] : g[0].contiguous();
+    Tensor acc = zeros({B, Ln, H, 128}, F32, dev), stats = alloc({2 * B * H * ((Ln + 63) / 64 * 64)}, F32, dev),
+           work = alloc({(int64_t)L.sb_attn_rpe_bwd_work(B, H, Ln, far, causal)}, F32, dev);
+    const Strides gs(go), qs(q), ks(k), vs(v), os(o), dqs(dq), dks(dk), dvs(dv);
+    const int rc = SB_RUN(sb_attn_rpe_bwd, 4, ptr(go), ptr(q), ptr(k), ptr(v), ptr(o), ptr(lo), f32(lse), f32o(stats), f32o(acc), out(dq), out(dk), out(dv),
+                          (int)B, (int)H, (int)Ln, gs.s, qs.s, ks.s, vs.s, os.s, dqs.s, dks.s, dvs.s, (int)causal, 0.08838834764831845f, ptr(table),
+                          (int)(table.scalar_type() == F32), static_cast<const int*>(ptr(buckets)), (int)table.size(0), (int)far,
+                          (float)ctx->saved_data["bias_scale"].toDouble(), f32o(work), out(dtable), status_word(dev), stream());
+    TORCH_CHECK(rc == 0, "backward of attention with relative position bias failed (code ", rc, ", encode ", L.sb_attn_last_encode_result(), "): ",
+                layouts({{"dout", &go}, {"q", &q}, {"k", &k}, {"v", &v}}));
+    return {dqkv, dtable, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
 // ------------------------------------------------------------------------------------ what Python calls
 bool fused(const py::handle& w) {          // the parameter's gradient lives in a persistent flat buffer (set by the ZeRO optimizers)
   PyObject* v = PyObject_GetAttrString(w.ptr(), "_fuse_grad_accum");
@@ -802,6 +849,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     no_transforms();
     variable_list r = HyenaLI::apply(feat, gamma, R, p, bias, state_in, want_state, tc);
     return std::make_tuple(r[0], want_state ? OptTensor(r[1]) : OptTensor());
+  });
+  m.def("attention_rpe", [](const Tensor& qkv, const Tensor& table, const Tensor& buckets, double bias_scale, bool causal) {
+    no_transforms();
+    const c10::cuda::CUDAGuard device(qkv.device());
+    return FlashRpe::apply(qkv, table, buckets, bias_scale, causal, wants_grad({&qkv, &table}));
   });
   m.def("attention_packed", [](const Tensor& qkv, const OptTensor& cos, const OptTensor& sin, bool causal) {
     no_transforms();

@@ -226,6 +226,45 @@ def attention_packed(qkv, cos, sin, causal=True):
     return flash_sm100.attention_packed(qkv, cos, sin, causal)
 
 
+RPE_MAX_FAR = 2048       # distances of their own that the kernels' bias by relative position has on a side
+
+
+def _check_rpe(table, buckets, heads, device, causal):
+    n = buckets.shape[0] if buckets.dim() == 1 else 0
+    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] != heads or not table.is_floating_point():
+        raise ValueError(f"relative position table {table.dtype} {tuple(table.shape)} for {heads} heads: [buckets, heads] expected")
+    if buckets.dtype != torch.int32 or n < 1 or (not causal and n % 2 == 0):
+        raise ValueError(f"bucket map {buckets.dtype} {tuple(buckets.shape)}: int32 [far + 1] (causal) or [2 far + 1] expected")
+    if table.device != device or buckets.device != device:
+        raise ValueError("relative position table and bucket map belong on the device of the attention's inputs")
+
+
+def attention_rpe_covers(qkv, far: int) -> bool:
+    """Whether `attention_rpe` runs the flash kernels: CUDA, contiguous bf16, heads of 128, `far` at most 2048.  It materialises the scores
+    otherwise."""
+    if not _k(qkv):
+        return False
+    from . import flash_sm100
+    return flash_sm100.packed_supported(qkv) and 0 <= far <= RPE_MAX_FAR
+
+
+def attention_rpe(qkv, table, buckets, scale: float = 1.0, causal: bool = True):
+    """Self-attention on the packed projection qkv [B, L, H, 3 * hd] with a learned bias by relative position on the scores:
+    softmax(q k^T / sqrt(hd) + scale * table[bucket, h]) v -> [B, L, H, hd], differentiated for qkv and the table.
+
+    table [nb, H]; buckets int32, the bucket of each distance query - key: [far + 1] for 0 .. far (causal) or [2 far + 1] for -far .. far,
+    where what lies further away has the outermost entry's (`RelativePositionBias.bucket_map`).  An entry outside 0 .. nb - 1 has no bias on the
+    kernel path.  The kernels form no [L, L] bias or scores; their query gradient is added up in an order that varies, as that of
+    `attention_packed` does, the table's in a fixed one."""
+    if qkv.dim() != 4 or qkv.shape[3] % 3 or qkv.shape[3] == 0:
+        raise ValueError(f"attention_rpe takes qkv [B, L, H, 3 * hd], got {tuple(qkv.shape)}")
+    _check_rpe(table, buckets, qkv.shape[2], qkv.device, causal)
+    far = buckets.shape[0] - 1 if causal else buckets.shape[0] // 2
+    if attention_rpe_covers(qkv, far):
+        return _co().attention_rpe(qkv, table, buckets, scale, causal)
+    return ref.attention_rpe(qkv, table, buckets, scale, causal)
+
+
 # ----------------------------------------------------------------------------- activation checkpoints
 
 

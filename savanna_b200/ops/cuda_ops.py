@@ -1076,6 +1076,12 @@ def layernorm_residual(x, weight, bias, eps):
     return _native("layernorm_residual", x, weight, bias, float(eps))
 
 
+def attention_rpe(qkv, table, buckets, scale, causal):
+    if table.dtype not in (torch.bfloat16, torch.float32):
+        table = table.float()
+    return _native("attention_rpe", qkv, table, buckets, float(scale), bool(causal))
+
+
 def act_quantize(x):
     return _N.act_quantize(x)
 

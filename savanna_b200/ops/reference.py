@@ -292,6 +292,22 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     return o
 
 
+def relative_bias(table, buckets, scale, Lq: int, Lk: int, causal: bool = True):
+    """[H, Lq, Lk]: scale * table[bucket of the distance query - key, h].  The last query stands at the last key.  `buckets` maps the distances
+    0 .. far (causal; what lies ahead counts as 0) or -far .. far; beyond them the outermost entry counts."""
+    far = buckets.shape[0] - 1 if causal else buckets.shape[0] // 2
+    d = torch.arange(Lk - Lq, Lk, device=table.device)[:, None] - torch.arange(Lk, device=table.device)[None, :]
+    at = d.clamp(0, far) if causal else d.clamp(-far, far) + far
+    return table[buckets.long()[at]].permute(2, 0, 1) * scale
+
+
+def attention_rpe(qkv, table, buckets, scale, causal: bool = True):
+    """Self-attention on qkv [B, L, H, 3 * hd] with a learned bias by relative position -> [B, L, H, hd]."""
+    L, hd = qkv.shape[1], qkv.shape[3] // 3
+    q, k, v = qkv[..., :hd], qkv[..., hd: 2 * hd], qkv[..., 2 * hd:]
+    return attention(q, k, v, causal, bias=relative_bias(table.float(), buckets, scale, L, L, causal))
+
+
 # ----------------------------------------------------------------------------- mlp / loss
 
 

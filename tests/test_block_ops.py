@@ -52,3 +52,49 @@ def test_activation_refusals():
     for bad in ((q.float(), scale, torch.bfloat16), (q, scale[:, :1], torch.bfloat16), (q, scale.double(), torch.bfloat16), (q, scale, torch.float64)):
         with pytest.raises(ValueError):
             ops.act_dequantize(*bad)
+
+
+def _rpe_inputs(B=1, L=6, H=2, nb=8, far=4, causal=True):
+    g = torch.Generator().manual_seed(2)
+    n = far + 1 if causal else 2 * far + 1
+    return torch.randn(B, L, H, 12, generator=g), torch.randn(nb, H, generator=g), torch.randint(0, nb, (n,), generator=g, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_rpe_statement(causal):
+    """Against the formula pair by pair, its gradient for the table against differences."""
+    qkv, table, buckets = _rpe_inputs(causal=causal)
+    qkv, table = qkv.double(), table.double().requires_grad_(True)
+    far = 4
+    q, k, v = qkv.split(4, dim=-1)
+    want = torch.zeros(1, 6, 2, 4, dtype=torch.float64)
+    for h in range(2):
+        for i in range(6):
+            js = range(i + 1) if causal else range(6)
+            at = [min(i - j, far) if causal else max(-far, min(far, i - j)) + far for j in js]
+            s = torch.stack([q[0, i, h] @ k[0, j, h] / 2 + 1.5 * table[int(buckets[a]), h] for j, a in zip(js, at)])
+            want[0, i, h] = (torch.softmax(s, 0)[:, None] * torch.stack([v[0, j, h] for j in js])).sum(0).detach()
+    got = ops.attention_rpe(qkv, table, buckets, 1.5, causal)
+    # the statement computes in fp32: scores of a few units, six keys
+    assert float((got - want).abs().max()) <= 64 * 2.0 ** -24 * 16
+    w = torch.randn(got.shape, generator=torch.Generator().manual_seed(3)).double()
+    (grad,) = torch.autograd.grad((got * w).sum(), table)
+    with torch.no_grad():
+        for b, h in ((0, 0), (int(buckets[0]), 1), (int(buckets[-1]), 0)):
+            step = torch.zeros_like(table)
+            step[b, h] = 0.05
+            diff = ((ops.attention_rpe(qkv, table + step, buckets, 1.5, causal) - ops.attention_rpe(qkv, table - step, buckets, 1.5, causal)) * w).sum() / 0.1
+            # third derivative times step^2 / 6 of sums of about 50 values, and fp32 differences divided by the step
+            assert abs(float(diff - grad[b, h])) <= 0.05 ** 2 * 1.5 ** 3 * 50 + 64 * 2.0 ** -24 * 50 / 0.1
+
+
+def test_attention_rpe_refusals():
+    qkv, table, buckets = _rpe_inputs()
+    both = torch.zeros(9, dtype=torch.int32)
+    for bad in ((qkv[..., :11], table, buckets, 1.0, True), (qkv[0], table, buckets, 1.0, True), (qkv, table[:, :1], buckets, 1.0, True),
+                (qkv, table, buckets.long(), 1.0, True), (qkv, table, buckets[:0], 1.0, True), (qkv, table, both[:8], 1.0, False),
+                (qkv, table.to(torch.int32), buckets, 1.0, True), (qkv, table[0], buckets, 1.0, True)):
+        with pytest.raises(ValueError):
+            ops.attention_rpe(*bad)
+    assert ops.attention_rpe(qkv, table, both, 1.0, False).shape == (1, 6, 2, 4)
+    assert not ops.attention_rpe_covers(qkv, 4)
