@@ -1,0 +1,289 @@
+// Attention of one new token of every sequence over its cached keys and values, with a bias by relative position:
+//
+//   s_j = q k_j / sqrt(hd) + scale table[bucket(len - 1 - j), h],  o = sum_j softmax(s)_j v_j  over the sequence's len keys (0 of them: o = 0)
+//
+// Every key and value is read once, so memory bounds it, and with few heads or short caches the latency of one block's chain.  A key's hd values
+// lie over hd / 8 lanes with a 16-byte load each; such a group takes four keys at a time, all of whose loads are under way together, keeps its own
+// running maximum and sum, and the groups are joined at the end.  A row (sequence and head) is split over so many blocks that all SMs read: up
+// to eight in a cluster, joined through distributed shared memory; more than that leave their results in scratch and a second kernel joins them.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "device_info.h"
+#include "entries.h"
+#include "pdl.cuh"
+
+namespace sb {
+namespace step {
+namespace cg = cooperative_groups;
+typedef __nv_bfloat16 bf16;
+
+constexpr int WARPS = 4, THREADS = 32 * WARPS;
+constexpr int U = 4;                     // keys of a group under way
+constexpr int MAX_HD = 256;
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Args {
+  const void *q, *k, *v;
+  void* out;                             // [B, H, hd]
+  long long q_sb, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;      // element strides
+  const int* lengths;                    // [B], or null: T everywhere
+  const void* table;                     // [nb, H] of type table_type (0 bf16, 1 fp16, 2 fp32)
+  const int* buckets;                    // [far + 1]
+  float* part;                           // [B, H, splits, hd + 2] of the form with a second kernel
+  int T, H, hd, nb, far, table_type, splits;
+  float scale_log2, bias_log2;           // 1 / sqrt(hd) and the bias' scale, times log2(e)
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint4 stream16(const void* p) {             // read once by this block: not into L1
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+template <class T> __device__ __forceinline__ void eight(const uint4& v, float (&f)[8]);
+template <> __device__ __forceinline__ void eight<bf16>(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+template <> __device__ __forceinline__ void eight<__half>(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    f[2 * i] = t.x; f[2 * i + 1] = t.y;
+  }
+}
+__device__ __forceinline__ bf16 to(float v, bf16) { return __float2bfloat16_rn(v); }
+__device__ __forceinline__ __half to(float v, __half) { return __float2half_rn(v); }
+
+// log2(e) * bias at distance d >= 0; a bucket that does not exist has none
+__device__ __forceinline__ float bias(const Args& a, int h, int d) {
+  const int b = a.buckets[min(d, a.far)];
+  if (b < 0 || b >= a.nb) return 0.f;
+  const size_t i = (size_t)b * a.H + h;
+  const float t = a.table_type == 2 ? static_cast<const float*>(a.table)[i]
+                  : a.table_type == 1 ? __half2float(static_cast<const __half*>(a.table)[i]) : __bfloat162float(static_cast<const bf16*>(a.table)[i]);
+  return t * a.bias_log2;
+}
+
+// A weighted sum under a maximum: what joins two of them.
+__device__ __forceinline__ void weights(float m1, float m2, float& m, float& w1, float& w2) {
+  m = fmaxf(m1, m2);
+  const float r = m == -INFINITY ? 0.f : m;
+  w1 = ex2(m1 - r);
+  w2 = ex2(m2 - r);
+}
+
+template <class T, int LPK>                // LPK lanes a key: hd <= 8 LPK
+__global__ void __launch_bounds__(THREADS)
+step_kernel(const Args a) {
+  constexpr int G = 32 / LPK;              // groups of a warp
+  __shared__ float wm[WARPS], wl[WARPS], wo[WARPS][8 * LPK];
+  __shared__ float cm, cl, co[8 * LPK];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, grp = lane / LPK, c0 = (lane % LPK) * 8;
+  const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+  const int chunk = ((len + a.splits - 1) / a.splits + U - 1) / U * U, j0 = min(len, split * chunk), j1 = min(len, j0 + chunk);
+  const bool have = c0 < a.hd;
+  const T* kp = static_cast<const T*>(a.k) + b * a.k_sb + h * a.k_sh + (have ? c0 : 0);
+  const T* vp = static_cast<const T*>(a.v) + b * a.v_sb + h * a.v_sh + (have ? c0 : 0);
+  float q[8], o[8], m = -INFINITY, l = 0.f;
+  eight<T>(have ? *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.q_sb + h * a.q_sh + c0) : make_uint4(0, 0, 0, 0), q);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) { q[i] *= a.scale_log2; o[i] = 0.f; }
+  const float far_bias = bias(a, h, a.far);
+  for (int j = j0 + (warp * G + grp) * U; __any_sync(0xffffffffu, j < j1); j += WARPS * G * U) {
+    uint4 kr[U], vr[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {          // a key beyond the last reads the last one again
+      const long long at = max(min(j + u, j1 - 1), j0);
+      kr[u] = stream16(kp + at * a.k_st);
+      vr[u] = stream16(vp + at * a.v_st);
+    }
+    float s[U], mx = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float f[8];
+      eight<T>(kr[u], f);
+      s[u] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[u] = fmaf(q[i], f[i], s[u]);
+    }
+#pragma unroll
+    for (int d = LPK / 2; d; d >>= 1)
+#pragma unroll
+      for (int u = 0; u < U; ++u) s[u] += __shfl_xor_sync(0xffffffffu, s[u], d);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int d = len - 1 - (j + u);
+      s[u] = j + u < j1 ? s[u] + (d >= a.far ? far_bias : bias(a, h, d)) : -INFINITY;
+      mx = fmaxf(mx, s[u]);
+    }
+    const float ref = mx == -INFINITY ? 0.f : mx, al = ex2(m - ref);
+    m = mx;
+    l *= al;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] *= al;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float p = ex2(s[u] - ref);
+      float f[8];
+      eight<T>(vr[u], f);
+      l += p;
+      if (j + u < j1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = fmaf(p, f[i], o[i]);
+      }
+    }
+  }
+  // the groups of a warp, the warps of a block, the blocks of a cluster
+#pragma unroll
+  for (int d = LPK; d < 32; d <<= 1) {
+    float mm, w1, w2;
+    weights(m, __shfl_xor_sync(0xffffffffu, m, d), mm, w1, w2);
+    m = mm;
+    l = l * w1 + __shfl_xor_sync(0xffffffffu, l, d) * w2;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = o[i] * w1 + __shfl_xor_sync(0xffffffffu, o[i], d) * w2;
+  }
+  if (grp == 0) {
+    if (lane == 0) { wm[warp] = m; wl[warp] = l; }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) wo[warp][c0 + i] = o[i];
+  }
+  __syncthreads();
+  float bm = wm[0];
+#pragma unroll
+  for (int w = 1; w < WARPS; ++w) bm = fmaxf(bm, wm[w]);
+  float e[WARPS], bl = 0.f;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) { e[w] = ex2(wm[w] - (bm == -INFINITY ? 0.f : bm)); bl += e[w] * wl[w]; }
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = cluster.num_blocks();
+  const long long row = (long long)b * a.H + h;
+  T* out = static_cast<T*>(a.out) + row * a.hd;
+  for (int c = threadIdx.x; c < a.hd; c += THREADS) {
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) t += e[w] * wo[w][c];
+    if (a.splits == 1) out[c] = to(bl > 0.f ? t / bl : 0.f, T());
+    else if (blocks > 1) co[c] = t;
+    else a.part[(row * a.splits + split) * (a.hd + 2) + 2 + c] = t;
+  }
+  if (a.splits == 1) return;
+  if (threadIdx.x == 0) {
+    if (blocks > 1) { cm = bm; cl = bl; }
+    else { a.part[(row * a.splits + split) * (a.hd + 2)] = bm; a.part[(row * a.splits + split) * (a.hd + 2) + 1] = bl; }
+  }
+  if (blocks == 1) return;
+  cluster.sync();
+  if (cluster.block_rank() == 0) {
+    float pm[8], tm = -INFINITY, tl = 0.f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) { pm[r] = r < blocks ? *cluster.map_shared_rank(&cm, r) : -INFINITY; tm = fmaxf(tm, pm[r]); }
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      pm[r] = ex2(pm[r] - (tm == -INFINITY ? 0.f : tm));
+      if (r < blocks) tl += pm[r] * *cluster.map_shared_rank(&cl, r);
+    }
+    for (int c = threadIdx.x; c < a.hd; c += THREADS) {
+      float t = 0.f;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) if (r < blocks) t += pm[r] * *cluster.map_shared_rank(&co[c], r);
+      out[c] = to(tl > 0.f ? t / tl : 0.f, T());
+    }
+  }
+  cluster.sync();                          // the others' shared memory stays until it has been read
+}
+
+// Joins the splits of a row: a block a row, a thread a column, the weights by one warp.
+template <class T>
+__global__ void __launch_bounds__(MAX_HD)
+join_kernel(const float* part, T* out, int splits, int hd) {
+  extern __shared__ float e[];             // [splits]
+  __shared__ float sum;
+  const float* p = part + (long long)blockIdx.x * splits * (hd + 2);
+  wait_for_previous();
+  if (threadIdx.x < 32) {
+    float m = -INFINITY, l = 0.f;
+    for (int s = threadIdx.x; s < splits; s += 32) m = fmaxf(m, p[(long long)s * (hd + 2)]);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    for (int s = threadIdx.x; s < splits; s += 32) {
+      const float w = ex2(p[(long long)s * (hd + 2)] - (m == -INFINITY ? 0.f : m));
+      e[s] = w;
+      l += w * p[(long long)s * (hd + 2) + 1];
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+    if (threadIdx.x == 0) sum = l;
+  }
+  __syncthreads();
+  if ((int)threadIdx.x >= hd) return;
+  float t = 0.f;
+#pragma unroll 8
+  for (int s = 0; s < splits; ++s) t += e[s] * p[(long long)s * (hd + 2) + 2 + threadIdx.x];
+  out[(long long)blockIdx.x * hd + threadIdx.x] = to(sum > 0.f ? t / sum : 0.f, T());
+}
+
+// Blocks a row: four a SM where the cache is long enough for 64 keys a block.
+static int choose_splits(long long rows, int T) {
+  const long long want = (4LL * num_sms() + rows - 1) / rows, most = (T + 63) / 64;
+  long long s = want < most ? want : most;
+  if (s <= 1) return 1;
+  if (s <= 8) return s <= 2 ? 2 : s <= 4 ? 4 : 8;
+  return rows * 8 >= 2LL * num_sms() ? 8 : (int)s;
+}
+
+template <class T>
+static int launch(const Args& a, int B, cudaStream_t st) {
+  const dim3 grid(a.splits, a.H, B);
+  auto* kernel = a.hd <= 64 ? step_kernel<T, 8> : a.hd <= 128 ? step_kernel<T, 16> : step_kernel<T, 32>;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = a.splits;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = a.splits > 1 && a.splits <= 8 ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) { (void)cudaGetLastError(); return -2; }
+  if (a.splits <= 8) return 0;
+  return launch_chained(false, join_kernel<T>, dim3((unsigned)(B * a.H)), MAX_HD, a.splits * 4, st, (const float*)a.part, (T*)a.out, a.splits, a.hd);
+}
+
+}  // namespace step
+}  // namespace sb
+
+using namespace sb::step;
+
+// Blocks a row of sb_attn_step; above eight it needs scratch of B * H * splits * (hd + 2) floats.
+extern "C" int sb_attn_step_splits(int B, int H, int T) { return B < 1 || H < 1 || T < 1 ? 1 : choose_splits((long long)B * H, T); }
+
+// q [B, H, hd], k and v [B, T, H, hd] (type 0 bf16, 1 fp16; 16-byte boundaries, strides in elements multiples of 8, unit inner stride), out
+// [B, H, hd] contiguous.  lengths [B] int32 (clamped to 0 .. T) or null; table [nb, H] of table_type (0, 1 or 2: fp32), buckets [far + 1] int32
+// of the distances 0 .. far.
+extern "C" int sb_attn_step(const void* q, const void* k, const void* v, void* out, const int* lengths, int B, int T, int H, int hd,
+                            const long long* q_str, const long long* k_str, const long long* v_str, int type, const void* table, int table_type,
+                            const int* buckets, int nb, int far, float scale, float bias_scale, float* part, int splits, cudaStream_t st) {
+  if (hd < 8 || hd > MAX_HD || hd % 8 || nb < 1 || far < 0 || type < 0 || type > 1 || splits < 1 || splits > 8192 || (splits > 8 && !part)) return -1;
+  if (splits != 1 && splits != 2 && splits != 4 && splits < 8) return -1;
+  if (B < 0 || H < 0 || T < 0 || B > 65535 || H > 65535) return -1;
+  if (B == 0 || H == 0) return 0;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) return -4;
+  if ((q_str[0] | q_str[1] | k_str[0] | k_str[1] | k_str[2] | v_str[0] | v_str[1] | v_str[2]) & 7) return -4;
+  const Args a{q, k, v, out, q_str[0], q_str[1], k_str[0], k_str[1], k_str[2], v_str[0], v_str[1], v_str[2], lengths, table, buckets, part, T, H, hd, nb,
+               far, table_type, splits, scale * LOG2E, bias_scale * LOG2E};
+  return type == 0 ? launch<bf16>(a, B, st) : launch<__half>(a, B, st);
+}

@@ -12,6 +12,7 @@
 #include <dlfcn.h>
 
 #include <atomic>
+#include <cmath>
 #include <mutex>
 #include <sstream>
 
@@ -45,7 +46,7 @@ constexpr auto F32 = at::kFloat;
   X(sb_se_fwd) X(sb_se_fwd_taps) X(sb_se_bwd) X(sb_mr_fwd) X(sb_mr_bwd) X(sb_mr_tc_fwd) X(sb_mr_tc_bwd) X(sb_mr_umma_fwd) X(sb_mr_umma_bwd) \
   X(sb_li_fwd_tiled) \
   X(sb_li_bwd_tiled_chunk) X(sb_li_bwd_tiled) X(sb_attn_fwd) X(sb_attn_bwd) X(sb_attn_rope) \
-  X(sb_attn_rpe_fwd) X(sb_attn_rpe_bwd_work) X(sb_attn_rpe_bwd) X(sb_layernorm_fwd) X(sb_layernorm_bwd_blocks) X(sb_layernorm_bwd) X(sb_act8_quantize) X(sb_act8_dequantize)
+  X(sb_attn_step_splits) X(sb_attn_step) X(sb_attn_rpe_fwd) X(sb_attn_rpe_bwd_work) X(sb_attn_rpe_bwd) X(sb_layernorm_fwd) X(sb_layernorm_bwd_blocks) X(sb_layernorm_bwd) X(sb_act8_quantize) X(sb_act8_dequantize)
 
 struct {
 #define SB_DECLARE(name) decltype(&::name) name = nullptr;
@@ -854,6 +855,24 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     no_transforms();
     const c10::cuda::CUDAGuard device(qkv.device());
     return FlashRpe::apply(qkv, table, buckets, bias_scale, causal, wants_grad({&qkv, &table}));
+  });
+  m.def("attention_rpe_step", [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& buckets, double bias_scale,
+                                 const OptTensor& lengths) {
+    no_transforms();
+    const c10::cuda::CUDAGuard device(q.device());
+    const int64_t B = q.size(0), H = q.size(1), hd = q.size(2), T = k.size(1);
+    const Tensor tc = contiguous(table), bc = contiguous(buckets), lc = lengths.has_value() ? contiguous(*lengths) : Tensor();
+    Tensor o = alloc({B, H, hd}, q.scalar_type(), q.device());
+    const int splits = L.sb_attn_step_splits(B, H, T);
+    Tensor part = splits > 8 ? alloc({B * H * splits * (hd + 2)}, F32, q.device()) : Tensor();
+    const long long qs[2] = {q.stride(0), q.stride(1)};
+    const Strides ks(k), vs(v);
+    const int rc = SB_RUN(sb_attn_step, B * H == 0 ? 0 : splits > 8 ? 2 : 1, ptr(q), ptr(k), ptr(v), out(o), static_cast<const int*>(ptr(lc)), (int)B, (int)T,
+                          (int)H, (int)hd, qs, ks.s, vs.s, type_code(q.scalar_type()), ptr(tc), type_code(tc.scalar_type()),
+                          static_cast<const int*>(ptr(bc)), (int)tc.size(0), (int)bc.size(0) - 1, (float)(1.0 / std::sqrt((double)hd)), (float)bias_scale,
+                          f32o(part), splits, stream());
+    TORCH_CHECK(rc == 0, "attention step failed (code ", rc, "): ", layouts({{"q", &q}, {"k", &k}, {"v", &v}, {"table", &tc}, {"buckets", &bc}}));
+    return o;
   });
   m.def("attention_packed", [](const Tensor& qkv, const OptTensor& cos, const OptTensor& sin, bool causal) {
     no_transforms();

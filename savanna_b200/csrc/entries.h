@@ -55,6 +55,11 @@ int sb_li_bwd_tiled_chunk();
 int sb_li_bwd_tiled(const void* feat, const void* dz, const float* modal, const float* bias, const float* state_in, const float* dstate_out,
                     float* S, float* A, float* dRp, float* dBp, void* dfeat, float* dR, float* dll, float* db, float* dstate_in, int B,
                     int L, int D, int O, cudaStream_t st);
+// attn_step.cu
+int sb_attn_step_splits(int B, int H, int T);
+int sb_attn_step(const void* q, const void* k, const void* v, void* out, const int* lengths, int B, int T, int H, int hd,
+                 const long long* q_str, const long long* k_str, const long long* v_str, int type, const void* table, int table_type,
+                 const int* buckets, int nb, int far, float scale, float bias_scale, float* part, int splits, cudaStream_t st);
 // layernorm.cu
 int sb_layernorm_fwd(const void* x, const void* w, const void* b, void* y, float* stats, int rows, int D, float eps, int type, cudaStream_t st);
 int sb_layernorm_bwd_blocks(int rows, int D, int type);

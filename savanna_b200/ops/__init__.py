@@ -265,6 +265,24 @@ def attention_rpe(qkv, table, buckets, scale: float = 1.0, causal: bool = True):
     return ref.attention_rpe(qkv, table, buckets, scale, causal)
 
 
+def attention_rpe_step(q, k, v, table, buckets, scale: float = 1.0, lengths=None):
+    """Attention of one new token of every sequence over its cache, the decoding form of causal `attention_rpe`: q [B, H, hd], k and v
+    [B, T, H, hd] (any strides with 16-byte rows are read in place), the new token's own key and value the last of the sequence's.  `lengths`
+    [B] int32 on the device: keys of each sequence, 0 .. T (values outside are clamped; rows of length 0 give zeros; what lies behind a
+    sequence's last key is not looked at); None: T.  CUDA: bf16 or fp16, heads of up to 256; no gradients (with them the statement runs)."""
+    if q.dim() != 3 or k.dim() != 4 or k.shape != v.shape or (k.shape[0], k.shape[2], k.shape[3]) != tuple(q.shape) or q.shape[2] == 0:
+        raise ValueError(f"attention_rpe_step takes q [B, H, hd], k and v [B, T, H, hd], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if k.dtype != q.dtype or v.dtype != q.dtype or k.device != q.device or v.device != q.device:
+        raise ValueError("attention_rpe_step: q, k and v are of one type on one device")
+    _check_rpe(table, buckets, q.shape[1], q.device, True)
+    if lengths is not None and (lengths.dtype != torch.int32 or tuple(lengths.shape) != (q.shape[0],) or lengths.device != q.device):
+        raise ValueError(f"attention_rpe_step: lengths int32 [{q.shape[0]}] on the inputs' device, got {lengths.dtype} {tuple(lengths.shape)}")
+    grad = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, table))
+    if _k(q) and not grad and _co().attention_rpe_step_covers(q, k, v):
+        return _co().attention_rpe_step(q, k, v, table, buckets, scale, lengths)
+    return ref.attention_rpe_step(q, k, v, table, buckets, scale, lengths)
+
+
 # ----------------------------------------------------------------------------- activation checkpoints
 
 

@@ -1082,6 +1082,19 @@ def attention_rpe(qkv, table, buckets, scale, causal):
     return _native("attention_rpe", qkv, table, buckets, float(scale), bool(causal))
 
 
+def attention_rpe_step_covers(q, k, v) -> bool:
+    """What the kernels read in place: bf16 or fp16 heads of up to 256 in steps of 8, 16-byte rows."""
+    return (q.dtype in (torch.bfloat16, torch.float16) and q.shape[2] % 8 == 0 and 8 <= q.shape[2] <= 256 and q.shape[0] <= 65535
+            and q.shape[1] <= 65535 and k.shape[1] < 2 ** 31
+            and all(t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1]) for t in (q, k, v)))
+
+
+def attention_rpe_step(q, k, v, table, buckets, scale, lengths):
+    if table.dtype not in _TYPES:
+        table = table.float()
+    return _N.attention_rpe_step(q, k, v, table, buckets, float(scale), lengths)
+
+
 def act_quantize(x):
     return _N.act_quantize(x)
 

@@ -308,6 +308,19 @@ def attention_rpe(qkv, table, buckets, scale, causal: bool = True):
     return attention(q, k, v, causal, bias=relative_bias(table.float(), buckets, scale, L, L, causal))
 
 
+def attention_rpe_step(q, k, v, table, buckets, scale, lengths=None):
+    """One new token a sequence, at the last of its `lengths` keys: q [B, H, hd], k / v [B, T, H, hd] -> [B, H, hd]; zero without keys."""
+    B, T, H, hd = k.shape
+    n = torch.full((B,), T, device=k.device) if lengths is None else lengths.long().clamp(0, T)
+    j = torch.arange(T, device=k.device)
+    d = (n[:, None] - 1 - j[None, :]).clamp(0, buckets.shape[0] - 1)
+    s = torch.einsum("bhd,bthd->bht", q.float(), k.float()) / math.sqrt(hd) + (table.float()[buckets.long()[d]] * scale).permute(0, 2, 1)
+    s = s.masked_fill((j[None, :] >= n[:, None])[:, None], float("-inf"))
+    p = torch.nan_to_num(torch.exp(s - torch.logsumexp(s, dim=-1, keepdim=True)), nan=0.0)
+    v = v.float().masked_fill((j[None, :] >= n[:, None])[..., None, None], 0.0)          # what lies behind the last key may be anything
+    return torch.einsum("bht,bthd->bhd", p, v).to(q.dtype)
+
+
 # ----------------------------------------------------------------------------- mlp / loss
 
 

@@ -98,3 +98,27 @@ def test_attention_rpe_refusals():
             ops.attention_rpe(*bad)
     assert ops.attention_rpe(qkv, table, both, 1.0, False).shape == (1, 6, 2, 4)
     assert not ops.attention_rpe_covers(qkv, 4)
+
+
+def test_attention_rpe_step_statement_is_the_last_row():
+    qkv, table, buckets = _rpe_inputs(B=2)
+    q, k, v = qkv.split(4, dim=-1)
+    full = ops.attention_rpe(qkv, table, buckets, 1.5, True)
+    for n in range(1, 7):
+        lengths = torch.tensor([n, 0], dtype=torch.int32)
+        got = ops.attention_rpe_step(q[:, n - 1], k, v, table, buckets, 1.5, lengths)
+        assert float((got[0] - full[0, n - 1]).abs().max()) <= 64 * 2.0 ** -24 * 16 and float(got[1].abs().max()) == 0
+
+
+def test_attention_rpe_step_refusals():
+    qkv, table, buckets = _rpe_inputs(B=2)
+    q, k, v = qkv.split(4, dim=-1)
+    q = q[:, 0]
+    n = torch.tensor([1, 2], dtype=torch.int32)
+    for bad in ((q[0], k, v, table, buckets), (q, k, v[:, :3], table, buckets), (q, k, v.double(), table, buckets), (q[..., :3], k, v, table, buckets),
+                (q, k, v, table[:, :1], buckets), (q, k, v, table, buckets.long())):
+        with pytest.raises(ValueError):
+            ops.attention_rpe_step(*bad, 1.0, n)
+    for bad in (n.long(), n[:1], torch.tensor([[1, 2]], dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            ops.attention_rpe_step(q, k, v, table, buckets, 1.0, bad)
