@@ -64,10 +64,10 @@ struct FwdParams {
 //     the diagonals from lane to lane.  Each warp writes its 64 sums to a place of its own, and rpe_table_kernel adds them up in a fixed
 //     order, with one sum per warp of the far tiles.
 //   - delta = sum(dO O) must be good to the rounding of dS itself: the forward divides O by the sum of the ROUNDED probabilities, so that it is
-//     an exact average under slightly other weights, and hands on what O lost in rounding (out_lo); lse has the sum of the unrounded ones.  What error e is left in a row's delta adds
-//     P e to each dS.  In a causal row the far keys' true sum is as small as that of the near ones (both add up to zero), so their error,
-//     e times nearly all of P, would be a percent of it at 8192 keys.  Minus the sum of all other distances is off by e times the near
-//     keys' P instead.  The gradient of the last distance is an average of the two, weighted by what of P lies near and far.
+//     an exact average under slightly other weights, and hands on what O lost in rounding (out_lo); lse has the sum of the unrounded ones.
+//     What error e is left in a row's delta adds P e to each dS, and the sum of e over the rows is that of all dS, which should be zero: it is
+//     taken off the distances in proportion to their share of P, whose diagonals are summed up the same way.  (In a long causal row the far
+//     keys hold nearly all of P while their true sum is as small as that of the near ones: their error without this is a percent at 8192 keys.)
 constexpr int RPE_MAX_FAR = 2048;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 enum { RPE_NONE = 0, RPE_CAUSAL = 1, RPE_BOTH = 2 };
@@ -80,8 +80,8 @@ struct RpeParams {
   // backward
   const float* values;       // [H, width] log2(e) * bias by distance, entry `origin` at distance 0
   int width, origin;
-  float* diag;               // [B * H * key blocks, 8 warps, near tiles, 64]: sums along the diagonals of the near tiles
-  float* outer;              // [B * H * key blocks, 8 warps, 2]: sums of dS of the tiles beyond +far, and beyond -far or (causal) of P of the near ones
+  float* diag;               // [B * H * key blocks, dS | P, 8 warps, near tiles, 64]: sums along the diagonals of the near tiles
+  float* outer;              // [B * H * key blocks, 8 warps, 4]: sums of dS of the tiles beyond +far and beyond -far, of P beyond +far
   int x_lo, x_hi;            // near tiles: query tile start - key block start, in units of 64
 };
 // log2(e) * bias at distance d of head h; a bucket that does not exist has none
@@ -740,8 +740,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     const float sl2 = p.scale_log2;
     bool ok = n > 0;
     const float* values = nullptr;                   // of this key: entry d at distance d
-    float beyond[2] = {0.f, 0.f}, outer[2] = {0.f, 0.f};
-    const long long place = (((long long)b * p.H + h) * gridDim.x + blockIdx.x) * 8 + wg * 4 + quarter;
+    float beyond[2] = {0.f, 0.f}, outer[3] = {0.f, 0.f, 0.f};
+    const long long place = ((long long)b * p.H + h) * gridDim.x + blockIdx.x;
     if (RPE) {
       values = rp.values + (size_t)h * rp.width + rp.origin;
       beyond[0] = values[rp.far];
@@ -770,25 +770,31 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         const float* bv = values + (qi - key);
         const int vis = key >= p.Lk ? 32 : RPE == RPE_CAUSAL ? key - qi : 0;      // columns 0 .. vis - 1 are masked
         const float* sf = reinterpret_cast<const float*>(st);
-        float up = 0.f, down = 0.f, pl = 0.f, dl = 0.f, mass = 0.f;
+        float up = 0.f, down = 0.f, up_p = 0.f, down_p = 0.f, pl = 0.f, dl = 0.f;
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
           float pp = ex2(fmaf(__uint_as_float(sv[i]), sl2, sf[2 * i]) + bv[i]);
           float ds = pp * fmaf(__uint_as_float(dp[i]), p.scale, -sf[2 * i + 1]);
           if (i < vis) { pp = 0.f; ds = 0.f; }
-          if (i) { up = __shfl_sync(0xffffffffu, up, (lane + 31) & 31); down = __shfl_sync(0xffffffffu, down, (lane + 31) & 31); }
-          if (lane <= i) up += ds; else down += ds;
-          if (RPE == RPE_CAUSAL) mass += pp;
+          if (i) {
+            const int from = (lane + 31) & 31;
+            up = __shfl_sync(0xffffffffu, up, from); down = __shfl_sync(0xffffffffu, down, from);
+            up_p = __shfl_sync(0xffffffffu, up_p, from); down_p = __shfl_sync(0xffffffffu, down_p, from);
+          }
+          if (lane <= i) { up += ds; up_p += pp; } else { down += ds; down_p += pp; }
           if (i & 1) { pw[i >> 1] = pack_bf16(pl, pp); dw[i >> 1] = pack_bf16(dl, ds); }
           else { pl = pp; dl = ds; }
         }
-        float* to = rp.diag + (place * (rp.x_hi - rp.x_lo + 1) + (x - rp.x_lo)) * 64;
+        const int tiles = rp.x_hi - rp.x_lo + 1;
+        float* to = rp.diag + ((place * 16 + wg * 4 + quarter) * tiles + (x - rp.x_lo)) * 64;
         to[63 - lane] = up;                          // sum of diagonal e at 32 + e
         to[31 - lane] = down;
-        outer[1] += mass;                            // zero unless causal
+        to += 8 * 64 * tiles;
+        to[63 - lane] = up_p;
+        to[31 - lane] = down_p;
       } else {
         const float far = x > 0 ? beyond[0] : beyond[1];
-        float sum = 0.f;
+        float sum = 0.f, sum_p = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const float4 sd = st[i];
@@ -797,10 +803,13 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           const float da = pa * fmaf(__uint_as_float(dp[2 * i]), p.scale, -sd.y);
           const float db = pb * fmaf(__uint_as_float(dp[2 * i + 1]), p.scale, -sd.w);
           if (RPE) sum += da + db;
+          if (RPE == RPE_BOTH) sum_p += pa + pb;
           pw[i] = pack_bf16(pa, pb);
           dw[i] = pack_bf16(da, db);
         }
-        if (RPE && key < p.Lk) { if (RPE == RPE_CAUSAL || x > 0) outer[0] += sum; else outer[1] += sum; }
+        if (RPE && key < p.Lk) {
+          if (RPE == RPE_CAUSAL || x > 0) { outer[0] += sum; outer[2] += sum_p; } else { outer[1] += sum; }
+        }
       }
       if ((p.causal && key > qi) || key >= p.Lk) {
         // some of this row's 32 columns are masked (only the tiles on the diagonal, and the key rows beyond Lk)
@@ -832,11 +841,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     }
     if (RPE) {
 #pragma unroll
-      for (int o = 16; o; o >>= 1) {
-        outer[0] += __shfl_xor_sync(0xffffffffu, outer[0], o);
-        outer[1] += __shfl_xor_sync(0xffffffffu, outer[1], o);
-      }
-      if (lane < 2) rp.outer[place * 2 + lane] = outer[lane & 1];
+      for (int o = 16; o; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < 3; ++k) outer[k] += __shfl_xor_sync(0xffffffffu, outer[k], o);
+      if (lane == 0) reinterpret_cast<float4*>(rp.outer)[place * 8 + wg * 4 + quarter] = make_float4(outer[0], outer[1], outer[2], 0.f);
     }
     if (ok && mbar_wait(dkv_done, 0u, abort_flag, p.status, ST_ATTN + 29)) {
       tc_fence_after();
@@ -1036,92 +1044,106 @@ __global__ void attn_dq_cast_kernel(const float* __restrict__ acc, __nv_bfloat16
   *reinterpret_cast<uint4*>(dq + bb * sb_ + i * sl_ + hh * sh_ + c) = o;
 }
 
-// dtable[b, h] = factor * sum over the distances d of bucket b of (the sums of dS at distance d).  Eight blocks (a cluster) a head: each takes
-// every eighth key block's sums, the first adds the eight up in order.  Distances of near tiles: 0 (or -far - 191) .. far + 191, the outermost
-// of which count as far.
+// dtable[b, h] = factor * sum over the distances d of bucket b of (the sums of dS at distance d, less their share of what all dS add up to).
+// Eight blocks (a cluster) a head: each adds up the columns of every eighth key block's sums, four columns a thread, gathers them by distance
+// (eight warps have sums of each), and the first adds the eight blocks' up in order.  Distances of near tiles: 0 (or -far - 191) .. far + 191,
+// the outermost of which count as far.  8192 tokens, 32 heads, far = 128: 33 MB.
 constexpr int TABLE_THREADS = 512, TABLE_SPLIT = 8;
+__host__ __device__ constexpr int table_low(int rpe, int far) { return rpe == RPE_BOTH ? -(far + 191) : 0; }
+__host__ __device__ constexpr int table_count(int rpe, int far) { return far + 192 - table_low(rpe, far); }
 template <int RPE>
 __global__ void __cluster_dims__(TABLE_SPLIT, 1, 1) __launch_bounds__(TABLE_THREADS)
 rpe_table_kernel(const __grid_constant__ RpeParams rp, void* dtable, float factor, int B, int H, int L, int kblocks) {
-  extern __shared__ float sums[];                  // [count] by distance, then [4][128] while they are formed
-  __shared__ float total, ends[2];
+  extern __shared__ float4 table_smem[];
+  __shared__ float ends[3], total[4];
   const int rank = blockIdx.x % TABLE_SPLIT, h = blockIdx.x / TABLE_SPLIT, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int low = RPE == RPE_BOTH ? -(rp.far + 191) : 0, count = rp.far + 192 - low;
-  const int nq = (L + BQ2 - 1) / BQ2, tiles = rp.x_hi - rp.x_lo + 1, rows = B * kblocks;
-  float* part = sums + count;
+  const int low = table_low(RPE, rp.far), count = table_count(RPE, rp.far), tiles = rp.x_hi - rp.x_lo + 1;
+  const int nq = (L + BQ2 - 1) / BQ2, rows = B * kblocks, cols = 8 * tiles * 16;      // columns in fours
+  float4* col = table_smem;                        // [cols]
+  float* sums = reinterpret_cast<float*>(table_smem + cols);      // [dS | P][count] by distance
   wait_for_previous();
-  for (int c0 = 0; c0 < count; c0 += 128) {
-    const int c = c0 + (tid & 127);
-    float s = 0.f;
-    if (c < count) {
+  for (int what = 0; what < 2; ++what) {
+    for (int c = tid; c < cols; c += TABLE_THREADS) {
+      const int x = rp.x_lo + (c >> 4) % tiles;
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+      for (int row = rank; row < rows; row += TABLE_SPLIT) {
+        const int bb = row / kblocks, kb = row - bb * kblocks, q = kb * (BK / BQ2) + x;
+        if (q >= 0 && q < nq) {
+          const float4 v = reinterpret_cast<const float4*>(rp.diag)[((((long long)bb * H + h) * kblocks + kb) * 2 + what) * cols + c];
+          s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        }
+      }
+      col[c] = s;
+    }
+    __syncthreads();
+    for (int c = tid; c < count; c += TABLE_THREADS) {
+      float s = 0.f;
 #pragma unroll
       for (int w = 0; w < 8; ++w) {                // the warps of a block: queries 32 (w / 4), keys 32 (w % 4) into the tile
         const int y = low + c - 32 * (w >> 2) + 32 * (w & 3) + 32, x = y >> 6, e = y & 63;      // floor: y may be negative
-        if (x < rp.x_lo || x > rp.x_hi) continue;
-        for (int row = rank + TABLE_SPLIT * (tid >> 7); row < rows; row += TABLE_SPLIT * 4) {
-          const int bb = row / kblocks, kb = row - bb * kblocks, q = kb * (BK / BQ2) + x;
-          if (q >= 0 && q < nq) s += rp.diag[((((long long)bb * H + h) * kblocks + kb) * 8 + w) * tiles * 64 + (x - rp.x_lo) * 64 + e];
-        }
+        if (x >= rp.x_lo && x <= rp.x_hi) s += reinterpret_cast<const float*>(col)[(w * tiles + x - rp.x_lo) * 64 + e];
       }
+      sums[what * count + c] = s;
     }
-    part[tid] = s;
-    __syncthreads();
-    if (tid < 128 && c < count) sums[c] = (part[tid] + part[tid + 128]) + (part[tid + 256] + part[tid + 384]);
     __syncthreads();
   }
-  if (warp < 2) {
-    float s = 0.f;
+  if (warp == 0) {
+    float s[3] = {0.f, 0.f, 0.f};
     for (int k = lane; k < rows * 8; k += 32) {
       const int row = k >> 3, bb = row / kblocks, kb = row - bb * kblocks;
-      if (row % TABLE_SPLIT == rank) s += rp.outer[((((long long)bb * H + h) * kblocks + kb) * 8 + (k & 7)) * 2 + warp];
+      if (row % TABLE_SPLIT == rank) {
+        const float4 v = reinterpret_cast<const float4*>(rp.outer)[(((long long)bb * H + h) * kblocks + kb) * 8 + (k & 7)];
+        s[0] += v.x; s[1] += v.y; s[2] += v.z;
+      }
     }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) ends[warp] = s;
+    for (int o = 16; o; o >>= 1)
+#pragma unroll
+      for (int k = 0; k < 3; ++k) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
+    if (lane == 0) { ends[0] = s[0]; ends[1] = s[1]; ends[2] = s[2]; }
   }
   auto cluster = cooperative_groups::this_cluster();
   cluster.sync();
   if (rank == 0) {
-    for (int c = tid; c < count; c += TABLE_THREADS) {
+    for (int c = tid; c < 2 * count; c += TABLE_THREADS) {
       float s = 0.f;
 #pragma unroll
       for (int k = 0; k < TABLE_SPLIT; ++k) s += *cluster.map_shared_rank(&sums[c], k);
       sums[c] = s;                                 // read by this thread alone before
     }
-    if (tid < 2) {
-      float s = 0.f;
-      for (int k = 0; k < TABLE_SPLIT; ++k) s += *cluster.map_shared_rank(&ends[tid], k);
-      part[tid] = s;
-    }
+    float end = 0.f;
+    if (tid < 3)
+      for (int k = 0; k < TABLE_SPLIT; ++k) end += *cluster.map_shared_rank(&ends[tid], k);
     __syncthreads();
-    if (RPE == RPE_CAUSAL && warp == 0) {            // the last distance: its own sum, or minus that of all others
-      float near = 0.f, own = 0.f;
-      for (int c = lane; c < count; c += 32) { if (c < rp.far) near += sums[c]; else own += sums[c]; }
+    if (tid < 3) ends[tid] = end;                  // after the reads above, which other blocks do not make
+    __syncthreads();
+    if (warp == 0) {                               // what all dS add up to, as a multiple of P; then the far distances of either side
+      float ds = 0.f, pr = 0.f;
+      for (int c = lane; c < count; c += 32) { ds += sums[c]; pr += sums[count + c]; }
 #pragma unroll
-      for (int o = 16; o; o >>= 1) {
-        near += __shfl_xor_sync(0xffffffffu, near, o);
-        own += __shfl_xor_sync(0xffffffffu, own, o);
-      }
+      for (int o = 16; o; o >>= 1) { ds += __shfl_xor_sync(0xffffffffu, ds, o); pr += __shfl_xor_sync(0xffffffffu, pr, o); }
       if (lane == 0) {
-        const float rows_p = (float)B * L, mn = part[1] / rows_p, mf = fmaxf(0.f, 1.f - mn), w = mn * mn / (mn * mn + mf * mf);
-        total = w * (own + part[0]) - (1.f - w) * near;
+        const float all = (float)B * L, rest = fmaxf(0.f, all - pr), ahead = RPE == RPE_BOTH ? fminf(ends[2], rest) : rest;
+        const float e = (ds + ends[0] + ends[1]) / all;
+        total[0] = e;
+        total[1] = ends[0] - e * ahead;
+        total[2] = RPE == RPE_BOTH ? ends[1] - e * (rest - ahead) : 0.f;
       }
     }
     __syncthreads();
+    const float e = total[0];
     for (int bk = warp; bk < rp.nb; bk += TABLE_THREADS / 32) {
       float s = 0.f;
       for (int c = lane; c < count; c += 32) {
-        const int d = low + c, i = RPE == RPE_BOTH ? min(max(d, -rp.far), rp.far) + rp.far : d;
-        if ((RPE == RPE_BOTH || d < rp.far) && rp.buckets[i] == bk) s += sums[c];
+        const int d = low + c, i = RPE == RPE_BOTH ? min(max(d, -rp.far), rp.far) + rp.far : min(d, rp.far);
+        if (rp.buckets[i] == bk) s += sums[c] - e * sums[count + c];
       }
 #pragma unroll
       for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
       if (lane == 0) {
-        if (RPE == RPE_CAUSAL) { if (rp.buckets[rp.far] == bk) s += total; }
-        else {
-          if (rp.buckets[2 * rp.far] == bk) s += part[0];
-          if (rp.buckets[0] == bk) s += part[1];
-        }
+        if (rp.buckets[RPE == RPE_BOTH ? 2 * rp.far : rp.far] == bk) s += total[1];
+        if (RPE == RPE_BOTH && rp.buckets[0] == bk) s += total[2];
         if (rp.table_f32) reinterpret_cast<float*>(dtable)[(size_t)bk * H + h] = s * factor;
         else reinterpret_cast<__nv_bfloat16*>(dtable)[(size_t)bk * H + h] = __float2bfloat16_rn(s * factor);
       }
@@ -1309,16 +1331,16 @@ static int rpe_params(RpeParams& r, const void* table, int table_f32, const int*
 }
 // Where the backward's scratch lies; its size in floats.
 static long long rpe_scratch(RpeParams& r, float* work, int B, int H, int L, int far, int causal) {
-  const long long blocks = (long long)B * H * ((L + BK - 1) / BK) * 8;
+  const long long blocks = (long long)B * H * ((L + BK - 1) / BK);
   r.x_lo = causal ? 0 : -((far + 62) / 64);
   r.x_hi = (far + 126) / 64;
   r.origin = causal ? 128 : far + 192;
   r.width = r.origin + far + 192;
-  const long long values = ((long long)H * r.width + 3) / 4 * 4, diag = blocks * (r.x_hi - r.x_lo + 1) * 64;
+  const long long values = ((long long)H * r.width + 3) / 4 * 4, diag = blocks * 16 * (r.x_hi - r.x_lo + 1) * 64;
   r.values = work;
   r.diag = work + values;
   r.outer = r.diag + diag;
-  return values + diag + blocks * 2;
+  return values + diag + blocks * 32;
 }
 }  // namespace attn
 }  // namespace sb
@@ -1340,9 +1362,11 @@ extern "C" int sb_attn_rpe_fwd(const void* q, const void* k, const void* v, void
 }
 
 // Floats of scratch that sb_attn_rpe_bwd needs.
-extern "C" long long sb_attn_rpe_bwd_work(int B, int H, int L, int far, int causal) {
+extern "C" int sb_attn_rpe_bwd_work(int B, int H, int L, int far, int causal, long long* floats) {
+  if (B < 0 || H < 0 || L < 0 || far < 0 || far > sb::attn::RPE_MAX_FAR) return -3;
   sb::attn::RpeParams r{};
-  return sb::attn::rpe_scratch(r, nullptr, B, H, L, far, causal);
+  *floats = sb::attn::rpe_scratch(r, nullptr, B, H, L, far, causal);
+  return 0;
 }
 
 // Its backward: as sb_attn_bwd (dq_acc zeroed by the caller), plus dtable [nb, H] of table's type, written.  Four launches.
@@ -1363,9 +1387,11 @@ extern "C" int sb_attn_rpe_bwd(const void* go, const void* q, const void* k, con
                         : attn_backward<RPE_BOTH>(go, q, k, v, out, lse, nullptr, stats, dq_acc, dq, dk, B, H, L, L, dv, g_str, q_str, k_str, v_str,
                                                   o_str, dq_str, dk_str, dv_str, 0, scale, r, status, stream);
   if (rc) return rc;
-  const int smem = 4 * ((causal ? far + 192 : 2 * (far + 191) + 1) + TABLE_THREADS);
-  return sb::launch_chained(false, causal ? rpe_table_kernel<RPE_CAUSAL> : rpe_table_kernel<RPE_BOTH>, dim3(H * TABLE_SPLIT), TABLE_THREADS, smem, stream,
-                            r, dtable, bias_scale / scale, B, H, L, (L + BK - 1) / BK) ? -6 : 0;
+  const int mode = causal ? RPE_CAUSAL : RPE_BOTH, smem = 8 * (r.x_hi - r.x_lo + 1) * 256 + 8 * table_count(mode, far);
+  auto* kernel = causal ? rpe_table_kernel<RPE_CAUSAL> : rpe_table_kernel<RPE_BOTH>;
+  if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -5;
+  return sb::launch_chained(false, kernel, dim3(H * TABLE_SPLIT), TABLE_THREADS, smem, stream, r, dtable, bias_scale / scale, B, H, L,
+                            (L + BK - 1) / BK) ? -6 : 0;
 }
 
 // Rotary embedding of `n` (1 or 2) tensors [B, L, H, 128] with tables cs / sn [L, rd] fp32 (rd a multiple of 16, at most

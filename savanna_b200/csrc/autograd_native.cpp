@@ -752,8 +752,9 @@ struct FlashRpe : Function<FlashRpe> {
     Tensor q = qkv.slice(3, 0, 128), k = qkv.slice(3, 128, 256), v = qkv.slice(3, 256, 384);
     Tensor dq = dqkv.slice(3, 0, 128), dk = dqkv.slice(3, 128, 256), dv = dqkv.slice(3, 256, 384);
     Tensor go = packed_rows(g[0]) ? g[0] : g[0].contiguous();
-    Tensor acc = zeros({B, Ln, H, 128}, F32, dev), stats = alloc({2 * B * H * ((Ln + 63) / 64 * 64)}, F32, dev),
-           work = alloc({(int64_t)L.sb_attn_rpe_bwd_work(B, H, Ln, far, causal)}, F32, dev);
+    long long floats = 0;
+    SB_CALL(sb_attn_rpe_bwd_work, 0, (int)B, (int)H, (int)Ln, (int)far, (int)causal, &floats);
+    Tensor acc = zeros({B, Ln, H, 128}, F32, dev), stats = alloc({2 * B * H * ((Ln + 63) / 64 * 64)}, F32, dev), work = alloc({floats}, F32, dev);
     const Strides gs(go), qs(q), ks(k), vs(v), os(o), dqs(dq), dks(dk), dvs(dv);
     const int rc = SB_RUN(sb_attn_rpe_bwd, 4, ptr(go), ptr(q), ptr(k), ptr(v), ptr(o), ptr(lo), f32(lse), f32o(stats), f32o(acc), out(dq), out(dk), out(dv),
                           (int)B, (int)H, (int)Ln, gs.s, qs.s, ks.s, vs.s, os.s, dqs.s, dks.s, dvs.s, (int)causal, 0.08838834764831845f, ptr(table),

@@ -79,7 +79,7 @@ int sb_attn_bwd(const void* go, const void* q, const void* k, const void* v, con
 int sb_attn_rpe_fwd(const void* q, const void* k, const void* v, void* out, void* out_lo, float* lse, int B, int H, int L, const long long* q_str,
                     const long long* k_str, const long long* v_str, const long long* o_str, int causal, float scale, const void* table,
                     int table_f32, const int* buckets, int nb, int far, float bias_scale, unsigned int* status, cudaStream_t stream);
-long long sb_attn_rpe_bwd_work(int B, int H, int L, int far, int causal);
+int sb_attn_rpe_bwd_work(int B, int H, int L, int far, int causal, long long* floats);
 int sb_attn_rpe_bwd(const void* go, const void* q, const void* k, const void* v, const void* out, const void* out_lo, const float* lse,
                     float* stats, float* dq_acc, void* dq, void* dk, void* dv, int B, int H, int L, const long long* g_str,
                     const long long* q_str, const long long* k_str, const long long* v_str, const long long* o_str, const long long* dq_str,

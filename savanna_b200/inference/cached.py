@@ -14,8 +14,8 @@ from the layers' inputs (forward pre-hooks; the Hyena-LI state comes from the sc
 recurrent Hyena inference lives in the separate vortex project).  Decode steps are matrix-vector work on one token: on CUDA
 one native call per step runs five kernels per layer (csrc/decode.cu, see `_FusedStep` for what it covers); everything else
 uses plain PyTorch operations on the model's own parameters.  Supported: one device (no tensor / context / pipeline
-parallelism), pre-norm blocks with the gated MLP, rotary or no position embedding, implicit-modal Hyena-LI filters; any
-other configuration raises NotImplementedError and the caller falls back to `stream_tokens` (recompute).  So does a sequence
+parallelism), pre-norm blocks with the gated MLP, rotary embedding, causal bias by relative position or neither, implicit-modal
+Hyena-LI filters; any other configuration raises NotImplementedError and the caller falls back to `stream_tokens` (recompute).  So does a sequence
 longer than `rotary_emb_max_unscaled_seq_len` under `rotary_ntk_scaled`: from there on the rotary base of all positions changes
 with every token, and with it every key and everything computed from them.
 """
@@ -33,7 +33,8 @@ from ..models.filters import ExplicitSingleDecayFilter, ImplicitModalFilter
 from ..models.hyena import HyenaOperator, ShortHyenaOperator
 from ..models.mixer import SelfAttention
 from ..models.mlp import ParallelGLU
-from ..models.norms import RMSNorm
+from ..models.norms import LayerNorm, RMSNorm
+from ..models.rope import RelativePositionBias
 from .. import ops
 from ..ops import cuda_ops
 from ..ops import reference as ref
@@ -41,6 +42,8 @@ from ..parallel import state
 
 
 def _rms(x, norm):
+    if isinstance(norm, LayerNorm):                  # x comes from the parameters' type: nothing is lost
+        return norm(x.to(norm.weight.dtype))
     return ref.rmsnorm(x, norm.gain, norm.eps, norm.form) if hasattr(norm, "gain") else norm(x)
 
 
@@ -123,6 +126,8 @@ def _layer_form(blk, D, at):
             form["eps" + i], form["form" + i] = at(n, "eps"), int(not te)
             ws.append((f"norm{i}_w", at(n, "weight" if te else "scale"), (D,), False))
     if isinstance(op, SelfAttention):
+        if at(op, "score_bias") is not None:
+            return None
         if at(op, "hd") != 128 or at(op, "heads") * 128 != H:
             return None
         form.update(kind=3, heads=op.heads, rd=0, pos_scale=1.0, base=0.0)
@@ -397,7 +402,7 @@ class CachedDecoder:
             raise NotImplementedError("cached generation runs on one device")
         if not cfg.prenorm or cfg.postnorm or cfg.outer_mlp_norm or cfg.gpt_j_residual:
             raise NotImplementedError("cached generation supports pre-norm blocks")
-        if cfg.pos_emb not in ("rotary", "rotary_linear_scaled", "rotary_ntk_scaled", "rotary2", "none", None):
+        if cfg.pos_emb not in ("rotary", "rotary_linear_scaled", "rotary_ntk_scaled", "rotary2", "none", "rpe", None):
             raise NotImplementedError(f"cached generation does not support pos_emb={cfg.pos_emb!r}")
         self.model, self.cfg = model, cfg
         self.blocks = model.blocks()
@@ -409,6 +414,8 @@ class CachedDecoder:
             m = b.mixer.mixer
             if isinstance(m, HyenaOperator) and not m.is_mr and not isinstance(m.filter, ImplicitModalFilter):
                 raise NotImplementedError("cached generation needs the implicit modal filter for Hyena-LI")
+            if getattr(m, "score_bias", None) is not None and not (isinstance(m.score_bias, RelativePositionBias) and m.causal and m.score_bias.far >= 0):
+                raise NotImplementedError("cached generation covers the causal bias by relative position only")
             if getattr(m, "sparse", False):
                 raise NotImplementedError("cached generation does not cover the block-sparse attention operators")
             if isinstance(m, HyenaOperator) and (m.bidirectional or m.slow_heads):
@@ -569,6 +576,10 @@ class CachedDecoder:
             k = ref.apply_rope(k.float(), cos, sin).to(proj.dtype)
         st["k"] = torch.cat([st["k"], k], dim=1)
         st["v"] = torch.cat([st["v"], v], dim=1)
+        rpe = inner.score_bias
+        if rpe is not None:
+            o = ops.attention_rpe_step(q[:, 0], st["k"], st["v"], rpe.weight, rpe.bucket_map(), rpe.scale)
+            return o.reshape(B, inner.heads * inner.hd)
         scores = torch.einsum("bqhd,bkhd->bhqk", q.float(), st["k"].float()) / math.sqrt(inner.hd)
         o = torch.einsum("bhqk,bkhd->bqhd", scores.softmax(-1), st["v"].float())
         return o.reshape(B, inner.heads * inner.hd)

@@ -20,6 +20,7 @@ from .embedding import Embedding
 from .init_functions import get_init_methods
 from .mlp import ParallelLinear
 from .norms import get_norm
+from .rope import are_consecutive, consecutive_positions, mark_consecutive
 
 
 class _Placeholder(nn.Module):
@@ -114,9 +115,12 @@ class Backbone(nn.Module):
                 x = b(self._watch(x, i + 1), positions)
             return x
         n = self.checkpoint_num_layers
+        consecutive = are_consecutive(positions)
 
         def chunk_fn(start, end):
             def fn(h, pos):
+                if consecutive:                  # the re-entrant checkpoint hands over detached copies, without the mark
+                    mark_consecutive(pos)
                 for b in blocks[start:end]:
                     h = b(h, pos)
                 return h
@@ -137,8 +141,14 @@ class Backbone(nn.Module):
         back for the recomputation; `partition_activations` keeps 1 / tp of a tensor that is replicated over the
         tensor-parallel group (no sequence parallelism) and all-gathers it for the recomputation.  Both are saved-tensor
         hooks, so the chunk then runs through the re-entrant checkpoint, which hands its inputs to `save_for_backward`
-        (the non-re-entrant one keeps them in a closure that no hook sees).  None when neither option is on."""
+        (the non-re-entrant one keeps them in a closure that no hook sees).  `checkpoint_in_8bit` keeps them as int8 with a
+        scale for 128 values (ops.act_quantize), with `checkpoint_in_cpu` those on the host: half of the memory or transfer of
+        bf16, and a recomputation, with its gradients, at inputs that are off by up to half a step.  None when no option is on."""
         cfg = self.cfg
+        if cfg.checkpoint_in_8bit:
+            if cfg.partition_activations and state.get_model_parallel_world_size() > 1:
+                raise NotImplementedError("checkpoint_in_8bit does not combine with partition_activations")
+            return _saved_tensors_in_8bit(cfg.checkpoint_in_cpu)
         if cfg.checkpoint_in_cpu:
             return torch.autograd.graph.save_on_cpu(pin_memory=torch.cuda.is_available())
         tp = state.get_model_parallel_world_size()
@@ -167,7 +177,7 @@ class Backbone(nn.Module):
         Pipeline stages pass `hidden_in` instead of tokens and set `return_hidden`."""
         if positions is None:
             ref_t = tokens if tokens is not None else hidden_in
-            positions = torch.arange(ref_t.shape[1], device=ref_t.device)
+            positions = consecutive_positions(ref_t.shape[1], ref_t.device)
         x = self.embedding(tokens, positions) if hidden_in is None else hidden_in
         x = self._run_blocks(x, positions)
         if return_hidden or not self.has_head:
@@ -189,6 +199,29 @@ def build_model(cfg, device=None) -> Backbone:
                     if id(p) in ids:
                         p.mul_(mult ** -0.5)
     return model
+
+
+def _saved_tensors_in_8bit(on_host: bool):
+    """Saved-tensor hooks that keep floating-point activations [B, L, D] as int8 with scales, on the device or in pinned host memory."""
+    def put(t):
+        if not (on_host and t.is_cuda):
+            return t
+        host = torch.empty(t.shape, dtype=t.dtype, pin_memory=True)
+        host.copy_(t, non_blocking=False)
+        return host
+
+    def pack(t):
+        if t.dim() == 3 and t.dtype in (torch.bfloat16, torch.float16, torch.float32) and t.numel() > 0 and not isinstance(t, nn.Parameter):
+            q, scale = ops.act_quantize(t)
+            return ("8bit", put(q), put(scale), t.dtype, t.device)
+        return ("whole", t, None, None, None)
+
+    def unpack(packed):
+        kind, q, scale, dtype, device = packed
+        if kind == "whole":
+            return q
+        return ops.act_dequantize(q.to(device, non_blocking=True), scale.to(device, non_blocking=True), dtype)
+    return torch.autograd.graph.saved_tensors_hooks(pack, unpack)
 
 
 def _partitioned_saved_tensors(tp: int, rank: int, group):

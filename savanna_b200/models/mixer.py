@@ -56,8 +56,9 @@ class SelfAttention(nn.Module):
             self._rotary.append(RotaryEmbedding(rd, cfg.rotary_emb_base, cfg.rotary_emb_scaling_factor,
                                                 "rotary" if cfg.pos_emb == "rotary2" else cfg.pos_emb,
                                                 cfg.rotary_emb_max_unscaled_seq_len, device=device))
-        # score biases (ALiBi slopes, bucketed relative positions): only the legacy `global` operator takes them; its
-        # scores are materialised (the flash kernels have no bias input), as in the reference's non-flash attention
+        # score biases (ALiBi slopes, bucketed relative positions): only the legacy `global` operator takes them.  The bucketed one runs
+        # the flash kernels where they cover the shape and the positions are consecutive (ops.attention_rpe); otherwise, and with ALiBi,
+        # the scores are materialised, as in the reference's non-flash attention
         self.score_bias = None
         if cfg.pos_emb in ("alibi", "rpe"):
             if operator_type != "global":
@@ -99,6 +100,10 @@ class SelfAttention(nn.Module):
         if self.score_bias is not None:
             if cp > 1:
                 raise NotImplementedError("score-bias attention (alibi / rpe) does not run under context parallelism")
+            from .rope import RelativePositionBias, are_consecutive
+            rpe = self.score_bias
+            if isinstance(rpe, RelativePositionBias) and are_consecutive(positions) and ops.attention_rpe_covers(qkv, rpe.far):
+                return ops.attention_rpe(qkv, rpe.weight, rpe.bucket_map(), rpe.scale, self.causal).reshape(B, L, self.heads * self.hd)
             from ..ops import reference as ref
             q, k, v = qkv[..., : self.hd], qkv[..., self.hd: 2 * self.hd], qkv[..., 2 * self.hd:]
             o = ref.attention(q, k, v, self.causal, positions, positions, bias=self.score_bias.bias(positions, positions))

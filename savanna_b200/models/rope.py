@@ -15,6 +15,22 @@ from ..ops import reference as ref
 from ..parallel import state
 
 
+def consecutive_positions(n: int, device=None) -> torch.Tensor:
+    """0 .. n - 1, marked as such: operators that work by distance need not look at the values then."""
+    return mark_consecutive(torch.arange(n, device=device))
+
+
+def mark_consecutive(positions: torch.Tensor) -> torch.Tensor:
+    positions._consecutive = 0 if positions.is_inference() else positions._version
+    return positions
+
+
+def are_consecutive(positions: torch.Tensor) -> bool:
+    """Whether `positions` were made by `consecutive_positions` and not written to since; False says nothing about the values."""
+    mark = getattr(positions, "_consecutive", None)
+    return mark is not None and mark == (0 if positions.is_inference() else positions._version)
+
+
 class RotaryEmbedding(nn.Module):
     def __init__(self, dim: int, base: float = 10000.0, scaling_factor: float = 1.0, kind: str = "rotary",
                  max_unscaled_len: int = 8192, device=None):
@@ -70,7 +86,7 @@ class AliBi(nn.Module):
 
 
 class RelativePositionBias(nn.Module):
-    """T5-style bucketed relative-position bias: a table [num_buckets, heads / tp] indexed by the bucket of
+    """Bucketed relative-position bias: a table [num_buckets, heads / tp] indexed by the bucket of
     (key position - query position); half of the buckets are exact small distances, the rest grow logarithmically up
     to `max_distance`.  `bias(q_pos, k_pos)` -> [heads / tp, Lq, Lk] * scale, added to the attention scores
     (reference: savanna/mpu/layers.py:194-349 `ParallelRelativePositionBias`, heads split over tensor-parallel ranks)."""
@@ -85,6 +101,29 @@ class RelativePositionBias(nn.Module):
         (init_method or nn.init.xavier_normal_)(full)              # the whole table, then this rank's head columns
         self.weight = nn.Parameter(full[:, mp_rank * per:(mp_rank + 1) * per].to(dtype=dtype, device=device).contiguous())
         self._log_ratio = math.log
+        self._map = None                # (what it depends on, bucket map)
+
+    @property
+    def far(self) -> int:
+        """The distance from which on all share the last bucket of their side (`max_distance`, where buckets grow up to it at all), or -1."""
+        side = self.num_buckets if self.causal else self.num_buckets // 2
+        return self.max_distance if self.max_distance > side // 2 >= 1 else -1
+
+    def bucket_map(self) -> torch.Tensor:
+        """Buckets by distance query - key, int32 on the table's device: of 0 .. far (causal) or -far .. far, as ops.attention_rpe takes them."""
+        far = self.far
+        if far < 0:
+            raise ValueError(f"no bucket map: max_distance {self.max_distance} does not exceed the {self.num_buckets} buckets' single distances")
+        key = (self.num_buckets, self.max_distance, self.causal, self.weight.device)
+        if self._map is not None and self._map[0] == key:
+            return self._map[1]
+        with torch.inference_mode(False), torch.no_grad():
+            d = torch.arange(0 if self.causal else -far, far + 1, device=self.weight.device)
+            made = self.bucket(-d).to(torch.int32)
+        # one made while a graph is captured has no values before the graph runs: it stays that graph's own
+        if not (made.is_cuda and torch.cuda.is_current_stream_capturing()):
+            self._map = key, made
+        return made
 
     def bucket(self, relative_position: torch.Tensor) -> torch.Tensor:
         import math

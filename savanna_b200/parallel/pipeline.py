@@ -15,6 +15,7 @@ from typing import List, Optional, Tuple
 import torch
 import torch.distributed as dist
 
+from ..models.rope import consecutive_positions
 from ..train import batch as batch_mod
 from . import state
 
@@ -163,7 +164,7 @@ def pipeline_train_step(trainer, data_iterator) -> torch.Tensor:
             out = model(tokens, b["positions"], return_hidden=not last)
         else:
             x_in.requires_grad_()
-            positions = b["positions"] if b is not None else torch.arange(L, device=dev)
+            positions = b["positions"] if b is not None else consecutive_positions(L, dev)
             out = model(None, positions, hidden_in=x_in, return_hidden=not last)
         if last:
             loss = trainer.compute_loss(out, b)

@@ -15,6 +15,7 @@ from typing import Dict, Optional
 
 import torch
 
+from ..models.rope import consecutive_positions
 from ..parallel import broadcast_data, state, zigzag_indices
 
 
@@ -70,8 +71,7 @@ def ltor_masks_and_position_ids(tokens: torch.Tensor, eod: int, eod_mask_loss: b
         loss_mask[tokens == eod] = 0.0
     if pad_mask_loss and pad is not None:
         loss_mask[tokens == pad] = 0.0
-    positions = torch.arange(L, device=tokens.device)
-    return loss_mask, positions
+    return loss_mask, consecutive_positions(L, tokens.device)
 
 
 def _dna_only(tokens: torch.Tensor) -> torch.Tensor:
@@ -189,7 +189,7 @@ def build_batch(cfg, text: torch.Tensor, generator=None) -> Dict[str, torch.Tens
             tokens, loss_mask, _ = _oadm_corrupt(clean, **kw)
         else:
             raise ValueError(f"pretraining strategy {strategy!r} unknown")
-        positions = torch.arange(clean.shape[1], device=clean.device)
+        positions = consecutive_positions(clean.shape[1], clean.device)
     if cfg.mask_loss_control_tags:
         loss_mask = mask_control_tags(labels, loss_mask, eod)
     batch = {"tokens": tokens, "labels": labels, "loss_mask": loss_mask, "positions": positions}

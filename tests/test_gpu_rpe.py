@@ -81,13 +81,9 @@ def _exact(qkv, table, buckets, scale, causal, go):
     one = (p * e + SMALL * (p * (dp.abs() + delta.abs())) + 2.0 ** -16 * p * mag + SMALL * ds.abs()).sum(0).reshape(H, -1)
     gd = torch.zeros(n, H, dtype=torch.float64, device=DEV).index_add_(0, at, ds.sum(0).reshape(H, -1).t())
     bd = torch.zeros(n, H, dtype=torch.float64, device=DEV).index_add_(0, at, one.t())
-    if causal:
-        # the last distance is w times its own sum and 1 - w times minus the sum of the others (whose exact values agree), by the shares of P
-        # in the tiles of 64 queries and 128 keys that reach nearer than it
-        near = (i[:, None] // 64 - 2 * (i[None, :] // 128)) <= (far + 126) // 64
-        mn = (p * near).sum((0, 2, 3)) / (B * L)
-        w = mn ** 2 / (mn ** 2 + (1 - mn) ** 2)
-        bd[far] = (w + 1e-4) * bd[far] + (1 - w + 1e-4) * bd[:far].sum(0)
+    # what all distances add up to (their errors: exactly, they add up to 0) is taken off each in proportion to its share of P
+    mass = torch.zeros(n, H, dtype=torch.float64, device=DEV).index_add_(0, at, p.sum(0).reshape(H, -1).t()) / (B * L)
+    bd = bd + (mass + 1e-4) * bd.sum(0)
     gt = torch.zeros(nb, H, dtype=torch.float64, device=DEV).index_add_(0, buckets.long(), gd) * scale
     bt = torch.zeros(nb, H, dtype=torch.float64, device=DEV).index_add_(0, buckets.long(), bd) * abs(scale)
     return (o.transpose(1, 2), bo.transpose(1, 2)), (torch.cat([dq, dk, dv], -1).transpose(1, 2), torch.cat([bq, bk, bv], -1).transpose(1, 2)), \
