@@ -61,14 +61,14 @@ struct FwdParams {
 //     With far = 128 those are all but two or three tiles of a row.
 //   - In the others ("near") a pair's bias is read from the head's values by distance; consecutive lanes have consecutive distances.
 //   - The table's gradient needs the sums of dS along the diagonals of the near tiles: 32 x 32 pairs a warp, by accumulators that travel along
-//     the diagonals from lane to lane.  Each warp writes its 64 sums to a place of its own, and rpe_table_kernel adds them up in a fixed
+//     the diagonals from lane to lane.  Each warp writes its 64 sums to a place of its own, and rpe_finish_kernel adds them up in a fixed
 //     order, with one sum per warp of the far tiles.
-//   - delta = sum(dO O) must be good to the rounding of dS itself: the forward divides O by the sum of the ROUNDED probabilities, so that it is
-//     an exact average under slightly other weights, and hands on what O lost in rounding (out_lo); lse has the sum of the unrounded ones.
-//     What error e is left in a row's delta adds P e to each dS, and the sum of e over the rows is that of all dS, which should be zero: it is
+//   - delta = sum(dO O) must be good to the rounding of dS itself: the forward divides by the sum of the ROUNDED probabilities, so that O is an
+//     exact average under slightly other weights, and hands on what O lost in rounding (out_lo).  (The unrounded sum beside it, for lse, took
+//     the forward from 555 to 640 us at 8192 tokens; without it the backward's P is off by up to 2^-8, as much as its roundings.)  What error e is left in a row's delta adds P e to each dS, and the sum of e over the rows is that of all dS, which should be zero: it is
 //     taken off the distances in proportion to their share of P, whose diagonals are summed up the same way.  (In a long causal row the far
 //     keys hold nearly all of P while their true sum is as small as that of the near ones: their error without this is a percent at 8192 keys.)
-constexpr int RPE_MAX_FAR = 2048;
+constexpr int RPE_MAX_FAR = 1024;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 enum { RPE_NONE = 0, RPE_CAUSAL = 1, RPE_BOTH = 2 };
 struct RpeParams {
@@ -76,14 +76,19 @@ struct RpeParams {
   const int* buckets;        // [far + 1] (causal) or [2 far + 1]
   int table_f32, nb, far;
   float scale_log2;          // bias_scale * log2(e)
-  __nv_bfloat16* out_lo;     // like out, or null: what the output lost in rounding
+  int8_t* out_lo;            // like out, or null: what the output lost in rounding, in 256ths of a step
   // backward
   const float* values;       // [H, width] log2(e) * bias by distance, entry `origin` at distance 0
   int width, origin;
   float* diag;               // [B * H * key blocks, dS | P, 8 warps, near tiles, 64]: sums along the diagonals of the near tiles
   float* outer;              // [B * H * key blocks, 8 warps, 4]: sums of dS of the tiles beyond +far and beyond -far, of P beyond +far
   int x_lo, x_hi;            // near tiles: query tile start - key block start, in units of 64
+  float* acc;                // dq_acc, which the statistics kernel clears
 };
+// What fp32 bits x lost in being rounded to the bf16 bits hi (shifted up): their difference, of which the second byte is kept.  The integer
+// difference holds across an exponent's border too; 0x8000 (a tie that was rounded down) would come back as its negative.
+__device__ __forceinline__ uint32_t lost(float x, uint32_t hi) { return (uint32_t)min(int(__float_as_uint(x) - hi), 0x7fff); }
+__device__ __forceinline__ float regained(uint32_t hi, int8_t lo) { return __uint_as_float(hi + (uint32_t)((int)lo * 256)); }
 // log2(e) * bias at distance d of head h; a bucket that does not exist has none
 __device__ __forceinline__ float rpe_value(const RpeParams& r, int mode, int H, int h, int d) {
   const int i = mode == RPE_CAUSAL ? min(max(d, 0), r.far) : min(max(d, -r.far), r.far) + r.far;
@@ -103,6 +108,11 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int 
 __device__ __forceinline__ void load_tile(uint32_t dst, const void* tmap, int l0, int h, int b, uint32_t bar) {
   tma_load_4d(dst, tmap, 0, h, l0, b, bar);
   tma_load_4d(dst + BOX_BYTES, tmap, 64, h, l0, b, bar);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -300,7 +310,6 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     const uint32_t p_tile = sP + t * TILE_BYTES;
     const float sl2 = p.scale_log2;
     float m = -INFINITY, l = 0.f;                    // RPE: m in units of log2, bias included
-    float lr = 0.f;                                  // RPE: sum of the rounded probabilities, where l is that of the unrounded ones
     bool ok = true;
     // near tiles reach distances of far + 253: 127 beyond their first column's
     float* bias_s = reinterpret_cast<float*>(smem_gen + 5 * TILE_BYTES);
@@ -352,8 +361,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         bm4[c] = __uint_as_float(v[c][0]);
+        if (RPE) {
 #pragma unroll
-        for (int i = 1; i < 32; ++i) bm4[c] = fmaxf(bm4[c], __uint_as_float(v[c][i]));
+          for (int i = 1; i < 31; i += 2) bm4[c] = max3(bm4[c], __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
+          bm4[c] = fmaxf(bm4[c], __uint_as_float(v[c][31]));
+        } else {
+#pragma unroll
+          for (int i = 1; i < 32; ++i) bm4[c] = fmaxf(bm4[c], __uint_as_float(v[c][i]));
+        }
       }
       float bm = fmaxf(fmaxf(bm4[0], bm4[1]), fmaxf(bm4[2], bm4[3]));
       if (RPE) bm = fmaf(bm, mul, add);              // of the row, in the units of m
@@ -383,7 +398,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       // P = exp2((S - m) * scale) as bf16 into the swizzled P tile; row sum in fp32
       const float moff = RPE ? add - m_ref : -m_ref * sl2;
       float rs4[4] = {0.f, 0.f, 0.f, 0.f};
-      f2 rs2[2] = {0, 0}, rounded[2] = {0, 0};
+      f2 rounded[2] = {0, 0};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
 #pragma unroll
@@ -396,7 +411,6 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             const float ea = ex2(xa), eb = ex2(xb);        // exp2(-inf) = 0 for masked keys
             w[i] = pack_bf16(ea, eb);
             if (RPE) {
-              rs2[i & 1] = f2_add(rs2[i & 1], f2_pack(ea, eb));
               rounded[i & 1] = f2_add(rounded[i & 1], f2_bf(w[i]));      // what enters the product
             } else {
               rs4[i] += ea + eb;
@@ -421,9 +435,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       if (p.pingpong) mbar_arrive(turn(t ^ 1));               // hand the unit to the other warpgroup
       float rs = (rs4[0] + rs4[1]) + (rs4[2] + rs4[3]);
       if (RPE) {
-        const float2 e = f2_unpack(f2_add(rs2[0], rs2[1])), d = f2_unpack(f2_add(rounded[0], rounded[1]));
-        rs = e.x + e.y;
-        lr = lr * alpha + (d.x + d.y);
+        const float2 d = f2_unpack(f2_add(rounded[0], rounded[1]));
+        rs = d.x + d.y;
       }
       l = l * alpha + rs;
       if (__any_sync(0xffffffffu, rescale)) {
@@ -446,7 +459,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       const uint32_t par = uint32_t(nb[t] - 1) & 1u;
       if (mbar_wait(pv_done(t), par, abort_flag, p.status, ST_ATTN + 9)) {
         tc_fence_after();
-        const float div = RPE ? lr : l, inv = div > 0.f ? 1.f / div : 0.f;
+        const float inv = l > 0.f ? 1.f / l : 0.f;
         __nv_bfloat16* orow = p.out + (long long)b * p.o_sb + (long long)row * p.o_sl + (long long)h * p.o_sh;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
@@ -462,14 +475,25 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
               o.z = pack_bf16(__uint_as_float(v[g * 8 + 4]) * inv, __uint_as_float(v[g * 8 + 5]) * inv);
               o.w = pack_bf16(__uint_as_float(v[g * 8 + 6]) * inv, __uint_as_float(v[g * 8 + 7]) * inv);
               *reinterpret_cast<uint4*>(orow + c * 32 + g * 8) = o;
-              if (RPE && rp.out_lo) {
+              if (RPE && rp.out_lo) {              // in place of these eight values
                 const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
-                uint32_t lw[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  lw[i] = pack_bf16(fmaf(__uint_as_float(v[g * 8 + 2 * i]), inv, -__uint_as_float(ow[i] << 16)),
-                                    fmaf(__uint_as_float(v[g * 8 + 2 * i + 1]), inv, -__uint_as_float(ow[i] & 0xffff0000u)));
-                *reinterpret_cast<uint4*>(rp.out_lo + (orow - p.out) + c * 32 + g * 8) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+                for (int i = 0; i < 4; ++i) {
+                  v[g * 8 + 2 * i] = lost(__uint_as_float(v[g * 8 + 2 * i]) * inv, ow[i] << 16);
+                  v[g * 8 + 2 * i + 1] = lost(__uint_as_float(v[g * 8 + 2 * i + 1]) * inv, ow[i] & 0xffff0000u);
+                }
+              }
+            }
+            if (RPE && rp.out_lo) {
+#pragma unroll
+              for (int g = 0; g < 2; ++g) {
+                uint32_t b[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const uint32_t* w = v + g * 16 + i * 4;
+                  b[i] = __byte_perm(__byte_perm(w[0], w[1], 0x0051), __byte_perm(w[2], w[3], 0x0051), 0x5410);
+                }
+                *reinterpret_cast<uint4*>(rp.out_lo + (orow - p.out) + c * 32 + g * 16) = make_uint4(b[0], b[1], b[2], b[3]);
               }
             }
           }
@@ -882,14 +906,20 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 // stats[b, h, i] = (-lse * log2(e), scale * (sum_d dO[b, i, h, d] * O[b, i, h, d] - dlse[b, h, i])) for i < L and (0, 0)
 // for the padding rows L <= i < Lpad; with a bias (-inf, 0) there, whose exponential is 0 whatever the bias.  A block takes one row i of one batch entry, sixteen lanes with 16-byte loads a head
 // (one warp per head with 8-byte loads and 64-bit index divisions per row ran at a third of the copy bandwidth).
-// RPE: O + out_lo stands for O, and the last row of blocks writes the heads' values by distance.
+// RPE: O and out_lo together stand for O, a block clears its row of the query gradient's accumulator, and the last row of blocks writes the heads' values
+// by distance.
 constexpr int STATS_THREADS = 256;
 template <int RPE>
 __global__ void __launch_bounds__(STATS_THREADS)
-attn_stats_kernel(const __nv_bfloat16* __restrict__ go, const __nv_bfloat16* __restrict__ o, const float* __restrict__ lse,
-                  const float* __restrict__ glse, float* __restrict__ stats, int H, int L, int Lpad, float scale, long long g_sb,
-                  long long g_sl, long long g_sh, long long o_sb, long long o_sl, long long o_sh, const __grid_constant__ RpeParams rp) {
+attn_stats_kernel(const __nv_bfloat16* go, const __nv_bfloat16* o, const float* lse, const float* glse, float* stats, int H, int L, int Lpad, float scale,
+                  long long g_sb, long long g_sl, long long g_sh, long long o_sb, long long o_sl, long long o_sh,
+                  const __grid_constant__ RpeParams rp) {
   const int i = blockIdx.x, bb = blockIdx.y, lane = threadIdx.x & 15;
+  if (RPE) wait_for_previous();
+  if (RPE && bb < gridDim.y - 1 && i < L) {
+    float4* row = reinterpret_cast<float4*>(rp.acc) + ((long long)bb * L + i) * H * (HD / 4);
+    for (int c = threadIdx.x; c < H * (HD / 4); c += STATS_THREADS) row[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
   if (RPE && bb == gridDim.y - 1) {
     for (int hh = blockIdx.x; hh < H; hh += gridDim.x)
       for (int e = threadIdx.x; e < rp.width; e += STATS_THREADS)
@@ -902,14 +932,13 @@ attn_stats_kernel(const __nv_bfloat16* __restrict__ go, const __nv_bfloat16* __r
       const uint4 a = *reinterpret_cast<const uint4*>(go + bb * g_sb + i * g_sl + hh * g_sh + lane * 8);
       const uint4 c = *reinterpret_cast<const uint4*>(o + bb * o_sb + i * o_sl + hh * o_sh + lane * 8);
       const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, cw[4] = {c.x, c.y, c.z, c.w};
+      alignas(8) int8_t lo[8];
+      if (RPE) *reinterpret_cast<uint2*>(lo) = *reinterpret_cast<const uint2*>(rp.out_lo + bb * o_sb + i * o_sl + hh * o_sh + lane * 8);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&aw[j]));
         float2 g = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&cw[j]));
-        if (RPE) {
-          const __nv_bfloat162 lo = *reinterpret_cast<const __nv_bfloat162*>(rp.out_lo + bb * o_sb + i * o_sl + hh * o_sh + lane * 8 + 2 * j);
-          g.x += __low2float(lo); g.y += __high2float(lo);
-        }
+        if (RPE) g = make_float2(regained(cw[j] << 16, lo[2 * j]), regained(cw[j] & 0xffff0000u, lo[2 * j + 1]));
         sum += f.x * g.x + f.y * g.y;
       }
     }
@@ -1026,73 +1055,86 @@ attn_rope_kernel(const RopeArgs a) {
   else rope_row<false>(a, d, blockIdx.x, blockIdx.y);
 }
 
-// dq[b, i, h, :] (bf16, strided) = dq_acc (fp32, contiguous [B, L, H, 128])
-__global__ void attn_dq_cast_kernel(const float* __restrict__ acc, __nv_bfloat16* __restrict__ dq, long long rows, int H, int L,
-                                    long long sb_, long long sl_, long long sh_) {
-  const long long idx = blockIdx.x * (long long)blockDim.x + threadIdx.x;     // one thread per 8 values
+// dq[b, i, h, :] (bf16, strided) = dq_acc (fp32, contiguous [B, L, H, 128]): eight values
+__device__ __forceinline__ void dq_cast(const float* acc, __nv_bfloat16* dq, long long idx, long long rows, int H, int L, long long sb_, long long sl_,
+                                        long long sh_) {
   if (idx >= rows * 16) return;
   const long long row = idx >> 4;
   const int c = int(idx & 15) * 8;
-  const int hh = int(row % H);
-  const long long bl = row / H;
-  const int i = int(bl % L);
-  const long long bb = bl / L;
+  int hh, i;
+  long long bb;
+  if (rows < 0x80000000LL) {                       // 64-bit divisions would take longer than the copy
+    const uint32_t r = (uint32_t)row, bl = r / (uint32_t)H;
+    hh = int(r - bl * H); bb = bl / (uint32_t)L; i = int(bl - (uint32_t)bb * L);
+  } else {
+    const long long bl = row / H;
+    hh = int(row - bl * H); bb = bl / L; i = int(bl - bb * L);
+  }
   const float4 x = *reinterpret_cast<const float4*>(acc + row * HD + c);
   const float4 y = *reinterpret_cast<const float4*>(acc + row * HD + c + 4);
   uint4 o;
   o.x = pack_bf16(x.x, x.y); o.y = pack_bf16(x.z, x.w); o.z = pack_bf16(y.x, y.y); o.w = pack_bf16(y.z, y.w);
   *reinterpret_cast<uint4*>(dq + bb * sb_ + i * sl_ + hh * sh_ + c) = o;
 }
+__global__ void attn_dq_cast_kernel(const float* __restrict__ acc, __nv_bfloat16* __restrict__ dq, long long rows, int H, int L,
+                                    long long sb_, long long sl_, long long sh_) {
+  dq_cast(acc, dq, blockIdx.x * (long long)blockDim.x + threadIdx.x, rows, H, L, sb_, sl_, sh_);      // one thread per 8 values
+}
 
 // dtable[b, h] = factor * sum over the distances d of bucket b of (the sums of dS at distance d, less their share of what all dS add up to).
 // Eight blocks (a cluster) a head: each adds up the columns of every eighth key block's sums, four columns a thread, gathers them by distance
 // (eight warps have sums of each), and the first adds the eight blocks' up in order.  Distances of near tiles: 0 (or -far - 191) .. far + 191,
 // the outermost of which count as far.  8192 tokens, 32 heads, far = 128: 33 MB.
-constexpr int TABLE_THREADS = 512, TABLE_SPLIT = 8;
+// The chain of one such cluster is long and its work small, so the other blocks of the launch turn the query gradient into bf16 meanwhile.
+constexpr int TABLE_THREADS = 512, TABLE_SPLIT = 8, TABLE_CAST = 4;      // TABLE_CAST: eights of the query gradient a thread casts
 __host__ __device__ constexpr int table_low(int rpe, int far) { return rpe == RPE_BOTH ? -(far + 191) : 0; }
 __host__ __device__ constexpr int table_count(int rpe, int far) { return far + 192 - table_low(rpe, far); }
 template <int RPE>
 __global__ void __cluster_dims__(TABLE_SPLIT, 1, 1) __launch_bounds__(TABLE_THREADS)
-rpe_table_kernel(const __grid_constant__ RpeParams rp, void* dtable, float factor, int B, int H, int L, int kblocks) {
+rpe_finish_kernel(const __grid_constant__ RpeParams rp, void* dtable, float factor, int B, int H, int L, int kblocks, __nv_bfloat16* dq,
+                  long long q_sb, long long q_sl, long long q_sh) {
   extern __shared__ float4 table_smem[];
-  __shared__ float ends[3], total[4];
+  __shared__ float total[3];
   const int rank = blockIdx.x % TABLE_SPLIT, h = blockIdx.x / TABLE_SPLIT, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int low = table_low(RPE, rp.far), count = table_count(RPE, rp.far), tiles = rp.x_hi - rp.x_lo + 1;
-  const int nq = (L + BQ2 - 1) / BQ2, rows = B * kblocks, cols = 8 * tiles * 16;      // columns in fours
+  const int nq = (L + BQ2 - 1) / BQ2, rows = B * kblocks, cols = 2 * 8 * tiles * 16;      // columns in fours: dS, then P
   float4* col = table_smem;                        // [cols]
-  float* sums = reinterpret_cast<float*>(table_smem + cols);      // [dS | P][count] by distance
+  float* sums = reinterpret_cast<float*>(table_smem + cols);      // [dS | P][count] by distance, then the three sums of the far tiles
+  int* bucket = reinterpret_cast<int*>(sums + 2 * count + 3);     // [count] of each distance
   wait_for_previous();
-  for (int what = 0; what < 2; ++what) {
-    for (int c = tid; c < cols; c += TABLE_THREADS) {
-      const int x = rp.x_lo + (c >> 4) % tiles;
-      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-      for (int row = rank; row < rows; row += TABLE_SPLIT) {
-        const int bb = row / kblocks, kb = row - bb * kblocks, q = kb * (BK / BQ2) + x;
-        if (q >= 0 && q < nq) {
-          const float4 v = reinterpret_cast<const float4*>(rp.diag)[((((long long)bb * H + h) * kblocks + kb) * 2 + what) * cols + c];
-          s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
-        }
-      }
-      col[c] = s;
-    }
-    __syncthreads();
-    for (int c = tid; c < count; c += TABLE_THREADS) {
-      float s = 0.f;
+  if (h >= H) {
 #pragma unroll
-      for (int w = 0; w < 8; ++w) {                // the warps of a block: queries 32 (w / 4), keys 32 (w % 4) into the tile
-        const int y = low + c - 32 * (w >> 2) + 32 * (w & 3) + 32, x = y >> 6, e = y & 63;      // floor: y may be negative
-        if (x >= rp.x_lo && x <= rp.x_hi) s += reinterpret_cast<const float*>(col)[(w * tiles + x - rp.x_lo) * 64 + e];
-      }
-      sums[what * count + c] = s;
+    for (int k = 0; k < TABLE_CAST; ++k)
+      dq_cast(rp.acc, dq, ((long long)(blockIdx.x - H * TABLE_SPLIT) * TABLE_CAST + k) * TABLE_THREADS + tid, (long long)B * L * H, H, L, q_sb, q_sl, q_sh);
+    return;
+  }
+  if (rank == 0)
+    for (int c = tid; c < count; c += TABLE_THREADS) {
+      const int d = low + c;
+      bucket[c] = rp.buckets[RPE == RPE_BOTH ? min(max(d, -rp.far), rp.far) + rp.far : min(d, rp.far)];
     }
-    __syncthreads();
+  for (int c = tid; c < cols; c += TABLE_THREADS) {
+    const int x = rp.x_lo + (c >> 4) % tiles;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int r0 = rank; r0 < rows; r0 += TABLE_SPLIT * 4) {       // tiles that no query reaches were not written
+      float4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int row = r0 + TABLE_SPLIT * k, bb = row / kblocks, kb = row - bb * kblocks, q = kb * (BK / BQ2) + x;
+        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (row < rows && q >= 0 && q < nq) v[k] = reinterpret_cast<const float4*>(rp.diag)[(((long long)bb * H + h) * kblocks + kb) * cols + c];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) { s.x += v[k].x; s.y += v[k].y; s.z += v[k].z; s.w += v[k].w; }
+    }
+    col[c] = s;
   }
   if (warp == 0) {
     float s[3] = {0.f, 0.f, 0.f};
-    for (int k = lane; k < rows * 8; k += 32) {
-      const int row = k >> 3, bb = row / kblocks, kb = row - bb * kblocks;
-      if (row % TABLE_SPLIT == rank) {
+    for (int k = lane; k < (rows + TABLE_SPLIT - 1) / TABLE_SPLIT * 8; k += 32) {
+      const int row = rank + TABLE_SPLIT * (k >> 3);
+      if (row < rows) {
+        const int bb = row / kblocks, kb = row - bb * kblocks;
         const float4 v = reinterpret_cast<const float4*>(rp.outer)[(((long long)bb * H + h) * kblocks + kb) * 8 + (k & 7)];
         s[0] += v.x; s[1] += v.y; s[2] += v.z;
       }
@@ -1101,22 +1143,30 @@ rpe_table_kernel(const __grid_constant__ RpeParams rp, void* dtable, float facto
     for (int o = 16; o; o >>= 1)
 #pragma unroll
       for (int k = 0; k < 3; ++k) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
-    if (lane == 0) { ends[0] = s[0]; ends[1] = s[1]; ends[2] = s[2]; }
+    if (lane < 3) sums[2 * count + lane] = lane == 0 ? s[0] : lane == 1 ? s[1] : s[2];
+  }
+  __syncthreads();
+  for (int c = tid; c < 2 * count; c += TABLE_THREADS) {
+    const int what = c >= count;
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {                  // the warps of a block: queries 32 (w / 4), keys 32 (w % 4) into the tile
+      const int y = low + c - what * count - 32 * (w >> 2) + 32 * (w & 3) + 32, x = y >> 6, e = y & 63;      // floor: y may be negative
+      if (x >= rp.x_lo && x <= rp.x_hi) s += reinterpret_cast<const float*>(col)[((what * 8 + w) * tiles + x - rp.x_lo) * 64 + e];
+    }
+    sums[c] = s;
   }
   auto cluster = cooperative_groups::this_cluster();
   cluster.sync();
   if (rank == 0) {
-    for (int c = tid; c < 2 * count; c += TABLE_THREADS) {
-      float s = 0.f;
+    for (int c = tid; c < 2 * count + 3; c += TABLE_THREADS) {
+      float v[TABLE_SPLIT], s = 0.f;
 #pragma unroll
-      for (int k = 0; k < TABLE_SPLIT; ++k) s += *cluster.map_shared_rank(&sums[c], k);
+      for (int k = 0; k < TABLE_SPLIT; ++k) v[k] = *cluster.map_shared_rank(&sums[c], k);
+#pragma unroll
+      for (int k = 0; k < TABLE_SPLIT; ++k) s += v[k];
       sums[c] = s;                                 // read by this thread alone before
     }
-    float end = 0.f;
-    if (tid < 3)
-      for (int k = 0; k < TABLE_SPLIT; ++k) end += *cluster.map_shared_rank(&ends[tid], k);
-    __syncthreads();
-    if (tid < 3) ends[tid] = end;                  // after the reads above, which other blocks do not make
     __syncthreads();
     if (warp == 0) {                               // what all dS add up to, as a multiple of P; then the far distances of either side
       float ds = 0.f, pr = 0.f;
@@ -1124,6 +1174,7 @@ rpe_table_kernel(const __grid_constant__ RpeParams rp, void* dtable, float facto
 #pragma unroll
       for (int o = 16; o; o >>= 1) { ds += __shfl_xor_sync(0xffffffffu, ds, o); pr += __shfl_xor_sync(0xffffffffu, pr, o); }
       if (lane == 0) {
+        const float* ends = sums + 2 * count;
         const float all = (float)B * L, rest = fmaxf(0.f, all - pr), ahead = RPE == RPE_BOTH ? fminf(ends[2], rest) : rest;
         const float e = (ds + ends[0] + ends[1]) / all;
         total[0] = e;
@@ -1135,15 +1186,14 @@ rpe_table_kernel(const __grid_constant__ RpeParams rp, void* dtable, float facto
     const float e = total[0];
     for (int bk = warp; bk < rp.nb; bk += TABLE_THREADS / 32) {
       float s = 0.f;
-      for (int c = lane; c < count; c += 32) {
-        const int d = low + c, i = RPE == RPE_BOTH ? min(max(d, -rp.far), rp.far) + rp.far : min(d, rp.far);
-        if (rp.buckets[i] == bk) s += sums[c] - e * sums[count + c];
-      }
+#pragma unroll 4
+      for (int c = lane; c < count; c += 32)
+        if (bucket[c] == bk) s += sums[c] - e * sums[count + c];
 #pragma unroll
       for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
       if (lane == 0) {
-        if (rp.buckets[RPE == RPE_BOTH ? 2 * rp.far : rp.far] == bk) s += total[1];
-        if (RPE == RPE_BOTH && rp.buckets[0] == bk) s += total[2];
+        if (bucket[count - 1] == bk) s += total[1];
+        if (RPE == RPE_BOTH && bucket[0] == bk) s += total[2];
         if (rp.table_f32) reinterpret_cast<float*>(dtable)[(size_t)bk * H + h] = s * factor;
         else reinterpret_cast<__nv_bfloat16*>(dtable)[(size_t)bk * H + h] = __float2bfloat16_rn(s * factor);
       }
@@ -1280,9 +1330,9 @@ static int attn_backward(const void* go, const void* q, const void* k, const voi
     attr_set.fetch_or(1ull << dev);
   }
   const int lpad = (Lq + BQ2 - 1) / BQ2 * BQ2;
-  attn_stats_kernel<RPE><<<dim3(lpad, B + (RPE ? 1 : 0)), STATS_THREADS, 0, stream>>>(
-      (const __nv_bfloat16*)go, (const __nv_bfloat16*)out, lse, glse, stats, H, Lq, lpad, scale, g_str[0], g_str[1], g_str[2],
-      o_str[0], o_str[1], o_str[2], rp);
+  if (launch_chained(!RPE, attn_stats_kernel<RPE>, dim3(lpad, B + (RPE ? 1 : 0)), STATS_THREADS, 0, stream, (const __nv_bfloat16*)go,
+                     (const __nv_bfloat16*)out, lse, glse, stats, H, Lq, lpad, scale, g_str[0], g_str[1], g_str[2], o_str[0], o_str[1], o_str[2], rp))
+    return -6;
   BwdParams p{stats, reinterpret_cast<__nv_bfloat16*>(dk), reinterpret_cast<__nv_bfloat16*>(dv),
               {dk_str[0], dk_str[1], dk_str[2]}, {dv_str[0], dv_str[1], dv_str[2]}, B, H, Lq, Lk,
               causal, scale * 1.4426950408889634f, scale, status};
@@ -1347,7 +1397,7 @@ static long long rpe_scratch(RpeParams& r, float* work, int B, int H, int L, int
 
 // Attention forward with a bias by relative position: as sb_attn_fwd with Lq == Lk == L, plus bias_scale * table[bucket(q - k), h] on the scaled
 // scores.  table [nb, H] (fp32 or bf16), buckets [far + 1] (causal: of the distances 0 .. far) or [2 far + 1] (-far .. far), int32.  out_lo
-// (like out, or null): what the output lost in rounding, for the backward.
+// (int8, laid out like out, or null): what the output lost in rounding, for the backward.
 extern "C" int sb_attn_rpe_fwd(const void* q, const void* k, const void* v, void* out, void* out_lo, float* lse, int B, int H, int L,
                                const long long* q_str, const long long* k_str, const long long* v_str, const long long* o_str, int causal,
                                float scale, const void* table, int table_f32, const int* buckets, int nb, int far, float bias_scale,
@@ -1356,7 +1406,7 @@ extern "C" int sb_attn_rpe_fwd(const void* q, const void* k, const void* v, void
   RpeParams r{};
   if (int rc = rpe_params(r, table, table_f32, buckets, nb, far, bias_scale)) return rc;
   if (reinterpret_cast<uintptr_t>(out_lo) & 15) return -4;
-  r.out_lo = (__nv_bfloat16*)out_lo;
+  r.out_lo = (int8_t*)out_lo;
   return causal ? attn_forward<RPE_CAUSAL>(q, k, v, out, lse, B, H, L, L, q_str, k_str, v_str, o_str, 1, scale, r, status, stream)
                 : attn_forward<RPE_BOTH>(q, k, v, out, lse, B, H, L, L, q_str, k_str, v_str, o_str, 0, scale, r, status, stream);
 }
@@ -1369,7 +1419,7 @@ extern "C" int sb_attn_rpe_bwd_work(int B, int H, int L, int far, int causal, lo
   return 0;
 }
 
-// Its backward: as sb_attn_bwd (dq_acc zeroed by the caller), plus dtable [nb, H] of table's type, written.  Four launches.
+// Its backward: as sb_attn_bwd, but dq_acc is scratch that need not be zero, plus dtable [nb, H] of table's type, written.  Three launches.
 extern "C" int sb_attn_rpe_bwd(const void* go, const void* q, const void* k, const void* v, const void* out, const void* out_lo, const float* lse,
                                float* stats, float* dq_acc, void* dq, void* dk, void* dv, int B, int H, int L, const long long* g_str,
                                const long long* q_str, const long long* k_str, const long long* v_str, const long long* o_str,
@@ -1381,17 +1431,20 @@ extern "C" int sb_attn_rpe_bwd(const void* go, const void* q, const void* k, con
   RpeParams r{};
   if (int rc = rpe_params(r, table, table_f32, buckets, nb, far, bias_scale)) return rc;
   rpe_scratch(r, work, B, H, L, far, causal);
-  r.out_lo = const_cast<__nv_bfloat16*>((const __nv_bfloat16*)out_lo);
-  const int rc = causal ? attn_backward<RPE_CAUSAL>(go, q, k, v, out, lse, nullptr, stats, dq_acc, dq, dk, B, H, L, L, dv, g_str, q_str, k_str, v_str,
+  r.out_lo = const_cast<int8_t*>((const int8_t*)out_lo);
+  r.acc = dq_acc;
+  if (reinterpret_cast<uintptr_t>(dq) & 15) return -4;
+  const int rc = causal ? attn_backward<RPE_CAUSAL>(go, q, k, v, out, lse, nullptr, stats, dq_acc, nullptr, dk, B, H, L, L, dv, g_str, q_str, k_str, v_str,
                                                     o_str, dq_str, dk_str, dv_str, 1, scale, r, status, stream)
-                        : attn_backward<RPE_BOTH>(go, q, k, v, out, lse, nullptr, stats, dq_acc, dq, dk, B, H, L, L, dv, g_str, q_str, k_str, v_str,
+                        : attn_backward<RPE_BOTH>(go, q, k, v, out, lse, nullptr, stats, dq_acc, nullptr, dk, B, H, L, L, dv, g_str, q_str, k_str, v_str,
                                                   o_str, dq_str, dk_str, dv_str, 0, scale, r, status, stream);
   if (rc) return rc;
-  const int mode = causal ? RPE_CAUSAL : RPE_BOTH, smem = 8 * (r.x_hi - r.x_lo + 1) * 256 + 8 * table_count(mode, far);
-  auto* kernel = causal ? rpe_table_kernel<RPE_CAUSAL> : rpe_table_kernel<RPE_BOTH>;
+  const int mode = causal ? RPE_CAUSAL : RPE_BOTH, smem = 16 * (r.x_hi - r.x_lo + 1) * 256 + 12 * table_count(mode, far) + 12;
+  auto* kernel = causal ? rpe_finish_kernel<RPE_CAUSAL> : rpe_finish_kernel<RPE_BOTH>;
   if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -5;
-  return sb::launch_chained(false, kernel, dim3(H * TABLE_SPLIT), TABLE_THREADS, smem, stream, r, dtable, bias_scale / scale, B, H, L,
-                            (L + BK - 1) / BK) ? -6 : 0;
+  const long long per = TABLE_THREADS * TABLE_SPLIT * TABLE_CAST, cast = ((long long)B * L * H * 16 + per - 1) / per;
+  return sb::launch_chained(false, kernel, dim3((unsigned)((H + cast) * TABLE_SPLIT)), TABLE_THREADS, smem, stream, r, dtable, bias_scale / scale, B, H, L,
+                            (L + BK - 1) / BK, (__nv_bfloat16*)dq, dq_str[0], dq_str[1], dq_str[2]) ? -6 : 0;
 }
 
 // Rotary embedding of `n` (1 or 2) tensors [B, L, H, 128] with tables cs / sn [L, rd] fp32 (rd a multiple of 16, at most

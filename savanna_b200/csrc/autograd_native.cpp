@@ -725,7 +725,7 @@ struct FlashRpe : Function<FlashRpe> {
     const int64_t B = qkv.size(0), Ln = qkv.size(1), H = qkv.size(2), far = causal ? buckets.size(0) - 1 : buckets.size(0) / 2;
     const at::Device dev = qkv.device();
     Tensor q = qkv.slice(3, 0, 128), k = qkv.slice(3, 128, 256), v = qkv.slice(3, 256, 384), tc = contiguous(table), bc = contiguous(buckets);
-    Tensor o = alloc({B, Ln, H, 128}, BF16, dev), lo = train ? alloc_like(o) : Tensor(), lse = alloc({B, H, Ln}, F32, dev);
+    Tensor o = alloc({B, Ln, H, 128}, BF16, dev), lo = train ? alloc({B, Ln, H, 128}, at::kChar, dev) : Tensor(), lse = alloc({B, H, Ln}, F32, dev);
     const Strides qs(q), ks(k), vs(v), os(o);
     const int rc = SB_RUN(sb_attn_rpe_fwd, B * Ln * H > 0, ptr(q), ptr(k), ptr(v), out(o), out(lo), f32o(lse), (int)B, (int)H, (int)Ln, qs.s, ks.s, vs.s,
                           os.s, (int)causal, 0.08838834764831845f, ptr(tc), (int)(tc.scalar_type() == F32), static_cast<const int*>(ptr(bc)),
@@ -754,9 +754,9 @@ struct FlashRpe : Function<FlashRpe> {
     Tensor go = packed_rows(g[0]) ? g[0] : g[0].contiguous();
     long long floats = 0;
     SB_CALL(sb_attn_rpe_bwd_work, 0, (int)B, (int)H, (int)Ln, (int)far, (int)causal, &floats);
-    Tensor acc = zeros({B, Ln, H, 128}, F32, dev), stats = alloc({2 * B * H * ((Ln + 63) / 64 * 64)}, F32, dev), work = alloc({floats}, F32, dev);
+    Tensor acc = alloc({B, Ln, H, 128}, F32, dev), stats = alloc({2 * B * H * ((Ln + 63) / 64 * 64)}, F32, dev), work = alloc({floats}, F32, dev);
     const Strides gs(go), qs(q), ks(k), vs(v), os(o), dqs(dq), dks(dk), dvs(dv);
-    const int rc = SB_RUN(sb_attn_rpe_bwd, 4, ptr(go), ptr(q), ptr(k), ptr(v), ptr(o), ptr(lo), f32(lse), f32o(stats), f32o(acc), out(dq), out(dk), out(dv),
+    const int rc = SB_RUN(sb_attn_rpe_bwd, 3, ptr(go), ptr(q), ptr(k), ptr(v), ptr(o), ptr(lo), f32(lse), f32o(stats), f32o(acc), out(dq), out(dk), out(dv),
                           (int)B, (int)H, (int)Ln, gs.s, qs.s, ks.s, vs.s, os.s, dqs.s, dks.s, dvs.s, (int)causal, 0.08838834764831845f, ptr(table),
                           (int)(table.scalar_type() == F32), static_cast<const int*>(ptr(buckets)), (int)table.size(0), (int)far,
                           (float)ctx->saved_data["bias_scale"].toDouble(), f32o(work), out(dtable), status_word(dev), stream());

@@ -226,7 +226,7 @@ def attention_packed(qkv, cos, sin, causal=True):
     return flash_sm100.attention_packed(qkv, cos, sin, causal)
 
 
-RPE_MAX_FAR = 2048       # distances of their own that the kernels' bias by relative position has on a side
+RPE_MAX_FAR = 1024       # distances of their own that the kernels' bias by relative position has on a side
 
 
 def _check_rpe(table, buckets, heads, device, causal):
@@ -240,7 +240,7 @@ def _check_rpe(table, buckets, heads, device, causal):
 
 
 def attention_rpe_covers(qkv, far: int) -> bool:
-    """Whether `attention_rpe` runs the flash kernels: CUDA, contiguous bf16, heads of 128, `far` at most 2048.  It materialises the scores
+    """Whether `attention_rpe` runs the flash kernels: CUDA, contiguous bf16, heads of 128, `far` at most 1024.  It materialises the scores
     otherwise."""
     if not _k(qkv):
         return False
