@@ -64,10 +64,17 @@ struct FwdParams {
 //     the diagonals from lane to lane.  Each warp writes its 64 sums to a place of its own, and rpe_finish_kernel adds them up in a fixed
 //     order, with one sum per warp of the far tiles.
 //   - delta = sum(dO O) must be good to the rounding of dS itself: the forward divides by the sum of the ROUNDED probabilities, so that O is an
-//     exact average under slightly other weights, and hands on what O lost in rounding (out_lo).  (The unrounded sum beside it, for lse, took
-//     the forward from 555 to 640 us at 8192 tokens; without it the backward's P is off by up to 2^-8, as much as its roundings.)  What error e is left in a row's delta adds P e to each dS, and the sum of e over the rows is that of all dS, which should be zero: it is
+//     exact average under slightly other weights, and hands on what O lost in rounding (out_lo).  The divisor in lse, which the backward's P
+//     has, gets back what the largest probability of each tile lost, which is most of it where a few keys have all the weight.  (A sum of
+//     the unrounded probabilities took the forward from 555 to 640 us at 8192 tokens, 32 heads.)
+//     What error e is left in a row's delta adds P e to each dS, and the sum of e over the rows is that of all dS, which should be zero: it is
 //     taken off the distances in proportion to their share of P, whose diagonals are summed up the same way.  (In a long causal row the far
 //     keys hold nearly all of P while their true sum is as small as that of the near ones: their error without this is a percent at 8192 keys.)
+//
+// Measured beside the same kernels without bias, us, causal with far = 128 / both sides with far = 256: forward 8192 x 32 heads 565 / -
+// (542), 2 x 2048 x 16 heads - / 95 (82); with the backward pass 2137 / - (2058), - / 381 (316), 3 x 777 x 4 heads 66 / - (53).  A tile that
+// is not near costs what it costs without bias (8192 x 16 heads, far = 1: 822 us in the backward kernel, 823 without bias); a near one a third more
+// there, for the read of the values and the travelling sums.
 constexpr int RPE_MAX_FAR = 1024;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 enum { RPE_NONE = 0, RPE_CAUSAL = 1, RPE_BOTH = 2 };
@@ -310,6 +317,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     const uint32_t p_tile = sP + t * TILE_BYTES;
     const float sl2 = p.scale_log2;
     float m = -INFINITY, l = 0.f;                    // RPE: m in units of log2, bias included
+    float lost_top = 0.f;                            // RPE: what the largest probability of each tile lost in rounding
     bool ok = true;
     // near tiles reach distances of far + 253: 127 beyond their first column's
     float* bias_s = reinterpret_cast<float*>(smem_gen + 5 * TILE_BYTES);
@@ -371,6 +379,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         }
       }
       float bm = fmaxf(fmaxf(bm4[0], bm4[1]), fmaxf(bm4[2], bm4[3]));
+      const float top = bm;
       if (RPE) bm = fmaf(bm, mul, add);              // of the row, in the units of m
       const float unit = RPE ? 1.f : sl2;
       // keep the old reference maximum unless the new one exceeds it by more than 2^8 (P stays below 256)
@@ -439,6 +448,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         rs = d.x + d.y;
       }
       l = l * alpha + rs;
+      if (RPE) {
+        const float e = ex2(fmaf(top, mul, moff));
+        lost_top = lost_top * alpha + (e - __uint_as_float(pack_bf16(0.f, e) & 0xffff0000u));
+      }
       if (__any_sync(0xffffffffu, rescale)) {
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
@@ -499,7 +512,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           }
         }
         if (row < p.Lq)
-          p.lse[((long long)b * p.H + h) * p.Lq + row] = (m == -INFINITY ? 0.f : m) * (RPE ? LN2 : p.scale) + __logf(fmaxf(l, 1e-37f));
+          p.lse[((long long)b * p.H + h) * p.Lq + row] = (m == -INFINITY ? 0.f : m) * (RPE ? LN2 : p.scale) + __logf(fmaxf(RPE ? l + lost_top : l, 1e-37f));
       }
     }
   }
@@ -790,7 +803,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       const int x = RPE ? (i_start + it) - k0 / BQ2 : 0;
       const bool near = RPE && x >= rp.x_lo && x <= rp.x_hi;
       if (near) {
-        // column i is at distance qi + i - key; `up` gathers the diagonals i - lane = 31 - lane >= 0, `down` -1 - lane, while they travel
+        // Column i is at distance qi + i - key.  The sum of diagonal e = i - lane travels with it: a column later it is one lane further.  `up`
+        // has those with e >= 0, `down` those with e < 0, which are complete once they are past lane 31 and are carried on from lane 0; the
+        // last column finds e = 31 - lane and -1 - lane.  (One sum for both whose lane 0 writes down what is complete, with half of the
+        // shuffles: 277 us instead of 265 for two of 2048, 16 heads, far = 256; four shorter chains side by side, joined at the end: 264.)
         const float* bv = values + (qi - key);
         const int vis = key >= p.Lk ? 32 : RPE == RPE_CAUSAL ? key - qi : 0;      // columns 0 .. vis - 1 are masked
         const float* sf = reinterpret_cast<const float*>(st);
