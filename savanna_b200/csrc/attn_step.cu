@@ -6,6 +6,9 @@
 // lie over hd / 8 lanes with a 16-byte load each; such a group takes four keys at a time, all of whose loads are under way together, keeps its own
 // running maximum and sum, and the groups are joined at the end.  A row (sequence and head) is split over so many blocks that all SMs read: up
 // to eight in a cluster, joined through distributed shared memory; more than that leave their results in scratch and a second kernel joins them.
+//
+// One sequence of 32768 keys, 32 heads of 128, bf16: 82.8 us for 537 MB, the rate of a copy.  Eight warps a block instead of four: 101 -> 82 us there;
+// reading the first keys before the query and the bias, two or eight keys a group, or a limit on registers for more blocks gained nothing.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -21,7 +24,7 @@ namespace step {
 namespace cg = cooperative_groups;
 typedef __nv_bfloat16 bf16;
 
-constexpr int WARPS = 4, THREADS = 32 * WARPS;
+constexpr int WARPS = 8, THREADS = 32 * WARPS;
 constexpr int U = 4;                     // keys of a group under way
 constexpr int MAX_HD = 256;
 constexpr float LOG2E = 1.4426950408889634f;
@@ -33,7 +36,7 @@ struct Args {
   const int* lengths;                    // [B], or null: T everywhere
   const void* table;                     // [nb, H] of type table_type (0 bf16, 1 fp16, 2 fp32)
   const int* buckets;                    // [far + 1]
-  float* part;                           // [B, H, splits, hd + 2] of the form with a second kernel
+  float* part;                           // of the form with a second kernel: (maximum, sum) [B, H, splits], then [B, H, splits, hd]
   int T, H, hd, nb, far, table_type, splits;
   float scale_log2, bias_log2;           // 1 / sqrt(hd) and the bias' scale, times log2(e)
 };
@@ -177,12 +180,12 @@ step_kernel(const Args a) {
     for (int w = 0; w < WARPS; ++w) t += e[w] * wo[w][c];
     if (a.splits == 1) out[c] = to(bl > 0.f ? t / bl : 0.f, T());
     else if (blocks > 1) co[c] = t;
-    else a.part[(row * a.splits + split) * (a.hd + 2) + 2 + c] = t;
+    else a.part[(long long)gridDim.z * a.H * a.splits * 2 + (row * a.splits + split) * a.hd + c] = t;
   }
   if (a.splits == 1) return;
   if (threadIdx.x == 0) {
     if (blocks > 1) { cm = bm; cl = bl; }
-    else { a.part[(row * a.splits + split) * (a.hd + 2)] = bm; a.part[(row * a.splits + split) * (a.hd + 2) + 1] = bl; }
+    else reinterpret_cast<float2*>(a.part)[row * a.splits + split] = make_float2(bm, bl);
   }
   if (blocks == 1) return;
   cluster.sync();
@@ -205,43 +208,67 @@ step_kernel(const Args a) {
   cluster.sync();                          // the others' shared memory stays until it has been read
 }
 
-// Joins the splits of a row: a block a row, a thread a column, the weights by one warp.
+// Joins the splits of a row: a block a row, two columns a thread, the splits in as many groups as there are threads for.
+constexpr int JOIN_THREADS = 512;
 template <class T>
-__global__ void __launch_bounds__(MAX_HD)
-join_kernel(const float* part, T* out, int splits, int hd) {
-  extern __shared__ float e[];             // [splits]
-  __shared__ float sum;
-  const float* p = part + (long long)blockIdx.x * splits * (hd + 2);
+__global__ void __launch_bounds__(JOIN_THREADS)
+join_kernel(const float* part, T* out, long long rows, int splits, int hd) {
+  extern __shared__ float e[];             // [splits], then [JOIN_THREADS][2]
+  __shared__ float red[JOIN_THREADS / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cols = hd / 2, groups = JOIN_THREADS / cols, g = tid / cols;
+  const float2* ml = reinterpret_cast<const float2*>(part) + (long long)blockIdx.x * splits;
+  const float2* o = reinterpret_cast<const float2*>(part) + rows * splits + (long long)blockIdx.x * splits * cols + tid - g * cols;
+  auto block = [&](float v, bool sum) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) { const float w = __shfl_xor_sync(0xffffffffu, v, d); v = sum ? v + w : fmaxf(v, w); }
+    __syncthreads();
+    if (lane == 0) red[warp] = v;
+    __syncthreads();
+    v = red[0];
+#pragma unroll
+    for (int k = 1; k < JOIN_THREADS / 32; ++k) v = sum ? v + red[k] : fmaxf(v, red[k]);
+    return v;
+  };
   wait_for_previous();
-  if (threadIdx.x < 32) {
-    float m = -INFINITY, l = 0.f;
-    for (int s = threadIdx.x; s < splits; s += 32) m = fmaxf(m, p[(long long)s * (hd + 2)]);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    for (int s = threadIdx.x; s < splits; s += 32) {
-      const float w = ex2(p[(long long)s * (hd + 2)] - (m == -INFINITY ? 0.f : m));
-      e[s] = w;
-      l += w * p[(long long)s * (hd + 2) + 1];
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-    if (threadIdx.x == 0) sum = l;
+  float m = -INFINITY, l = 0.f;
+  for (int s = tid; s < splits; s += JOIN_THREADS) m = fmaxf(m, ml[s].x);
+  m = block(m, false);
+  const float ref = m == -INFINITY ? 0.f : m;
+  for (int s = tid; s < splits; s += JOIN_THREADS) {
+    const float2 v = ml[s];
+    const float w = ex2(v.x - ref);
+    e[s] = w;
+    l += w * v.y;
   }
-  __syncthreads();
-  if ((int)threadIdx.x >= hd) return;
-  float t = 0.f;
+  l = block(l, true);                      // and e is there
+  float2 t = make_float2(0.f, 0.f);
+  if (g < groups) {
 #pragma unroll 8
-  for (int s = 0; s < splits; ++s) t += e[s] * p[(long long)s * (hd + 2) + 2 + threadIdx.x];
-  out[(long long)blockIdx.x * hd + threadIdx.x] = to(sum > 0.f ? t / sum : 0.f, T());
+    for (int s = g; s < splits; s += groups) { const float2 v = o[(long long)s * cols]; t.x += e[s] * v.x; t.y += e[s] * v.y; }
+  }
+  float2* sh = reinterpret_cast<float2*>(e + (splits + 1) / 2 * 2);
+  sh[tid] = t;
+  __syncthreads();
+  if (tid < cols) {
+    for (int k = 1; k < groups; ++k) { t.x += sh[tid + k * cols].x; t.y += sh[tid + k * cols].y; }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    T* dst = out + (long long)blockIdx.x * hd + 2 * tid;
+    dst[0] = to(t.x * inv, T());
+    dst[1] = to(t.y * inv, T());
+  }
 }
 
-// Blocks a row: four a SM where the cache is long enough for 64 keys a block.
+// Blocks a row: so many that there are four on a SM (no more: they would run one after the other), each with 64 keys or more.  Up to eight are a
+// cluster; more, with a second kernel, where a row is so long that eight blocks would leave SMs idle for longer than that kernel takes.  us, by
+// blocks a row: one sequence of 32768, 32 heads of 128 8: 93, 16: 82.4, 18: 81.7, 24: 87.5; twelve of up to 1500, 16 heads of 64 1: 19, 2: 15.9,
+// 4: 19.9; one of 1000, 32 heads 4: 10, 8: 8, 16: 11; 64 of 512, 16 heads 1: 36, 2: 47; one of 65536, 2 heads 8: 280, 64: 28, 128: 20, 256: 21.5.
 static int choose_splits(long long rows, int T) {
-  const long long want = (4LL * num_sms() + rows - 1) / rows, most = (T + 63) / 64;
-  long long s = want < most ? want : most;
-  if (s <= 1) return 1;
-  if (s <= 8) return s <= 2 ? 2 : s <= 4 ? 4 : 8;
-  return rows * 8 >= 2LL * num_sms() ? 8 : (int)s;
+  const long long want = 4LL * num_sms() / rows, keys = (T + 63) / 64;
+  int s = 1;
+  while (s < 8 && 2 * s <= want && s < keys) s *= 2;
+  if (s < 8 || want <= 8 || T < 8192) return s;
+  const long long longest = T / 256;
+  return (int)(want < longest ? want : longest);
 }
 
 template <class T>
@@ -260,7 +287,8 @@ static int launch(const Args& a, int B, cudaStream_t st) {
   cfg.numAttrs = a.splits > 1 && a.splits <= 8 ? 1 : 0;
   if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) { (void)cudaGetLastError(); return -2; }
   if (a.splits <= 8) return 0;
-  return launch_chained(false, join_kernel<T>, dim3((unsigned)(B * a.H)), MAX_HD, a.splits * 4, st, (const float*)a.part, (T*)a.out, a.splits, a.hd);
+  return launch_chained(false, join_kernel<T>, dim3((unsigned)(B * a.H)), JOIN_THREADS, (a.splits + 1) / 2 * 8 + JOIN_THREADS * 8, st,
+                        (const float*)a.part, (T*)a.out, (long long)B * a.H, a.splits, a.hd);
 }
 
 }  // namespace step
