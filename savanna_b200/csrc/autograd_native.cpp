@@ -346,23 +346,31 @@ struct RmsNormResidual : Function<RmsNormResidual> {
 // ------------------------------------------------------------------------------------ layer norm
 int type_code(at::ScalarType t) { return t == BF16 ? 0 : t == at::kHalf ? 1 : 2; }
 
+struct LnForward { Tensor x2, w, stats, y; };
+LnForward layernorm_fwd(const Tensor& x, const Tensor& w, const Tensor& b, double eps, bool train) {
+  LnForward n{rows_contiguous(x), contiguous(w), Tensor(), Tensor()};
+  const Tensor bc = contiguous(b);
+  const int64_t T = n.x2.size(0), D = n.x2.size(1);
+  n.y = alloc_like(n.x2);
+  if (train) n.stats = alloc({T, 2}, F32, x.device());
+  SB_CALL(sb_layernorm_fwd, T > 0, ptr(n.x2), ptr(n.w), ptr(bc), out(n.y), f32o(n.stats), (int)T, (int)D, (float)eps, type_code(x.scalar_type()), stream());
+  if (x.dim() != 2) n.y = n.y.view(x.sizes());
+  return n;
+}
 // Layer norm; with `residual` the second output carries x down the residual branch and the gradient arriving there is added inside the
 // backward kernel.
 struct LayerNorm : Function<LayerNorm> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& b, double eps, bool residual, bool train) {
-    Tensor x2 = rows_contiguous(x), wc = contiguous(w), bc = contiguous(b), y = alloc_like(x2), st;
-    const int64_t T = x2.size(0), D = x2.size(1);
-    if (train) st = alloc({T, 2}, F32, x.device());
-    SB_CALL(sb_layernorm_fwd, 1, ptr(x2), ptr(wc), ptr(bc), out(y), f32o(st), (int)T, (int)D, (float)eps, type_code(x.scalar_type()), stream());
-    ctx->save_for_backward({x2, wc, st});
-    ctx->saved_data["shape"] = x.sizes().vec();
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& b, double eps, bool residual) {
+    LnForward n = layernorm_fwd(x, w, b, eps, true);
+    ctx->save_for_backward({n.x2, n.w, n.stats});
+    if (x.dim() != 2) ctx->saved_data["shape"] = x.sizes().vec();
     ctx->set_materialize_grads(false);
-    if (residual) return {y.view(x.sizes()), x.view_as(x)};
-    return {y.view(x.sizes())};
+    if (residual) return {n.y, x.view_as(x)};
+    return {n.y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const Tensor gres = g.size() > 1 ? g[1] : Tensor();
-    if (!g[0].defined()) return {gres, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    if (!g[0].defined()) return {gres, Tensor(), Tensor(), Tensor(), Tensor()};
     const variable_list s = ctx->get_saved_variables();
     const Tensor &x2 = s[0], &w = s[1], &st = s[2];
     const int64_t T = x2.size(0), D = x2.size(1);
@@ -372,9 +380,21 @@ struct LayerNorm : Function<LayerNorm> {
            partial = alloc({(int64_t)L.sb_layernorm_bwd_blocks(T, D, type) * 2 * D}, F32, x2.device());
     SB_CALL(sb_layernorm_bwd, T > 0 ? 2 : 1, ptr(x2), ptr(w), ptr(g2), f32(st), ptr(r2), out(dx), out(dw), out(db), f32o(partial), (int)T, (int)D,
             type, stream());
-    return {dx.view(ctx->saved_data["shape"].toIntVector()), dw, db, Tensor(), Tensor(), Tensor()};
+    const auto shape = ctx->saved_data.find("shape");
+    if (shape != ctx->saved_data.end()) dx = dx.view(shape->second.toIntVector());
+    return {dx, dw, db, Tensor(), Tensor()};
   }
 };
+// The kernels' part of layer norms: one type, rows of up to 16384 values that 32 bits count.  Shapes that make no sense are refused.
+bool layernorm_covers(const Tensor& x, const Tensor& w, const Tensor& b) {
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "layernorm takes [..., D] with D >= 1, got ", x.sizes());
+  const int64_t D = x.size(-1);
+  TORCH_CHECK_VALUE(w.dim() == 1 && w.size(0) == D && b.dim() == 1 && b.size(0) == D, "layernorm weight ", w.sizes(), " and bias ", b.sizes(),
+                    " for rows of ", D, " values");
+  const at::ScalarType t = x.scalar_type();
+  return (t == BF16 || t == at::kHalf || t == F32) && w.scalar_type() == t && b.scalar_type() == t && D <= 16384 && x.numel() / D < (1LL << 31) &&
+         w.device() == x.device() && b.device() == x.device();
+}
 
 // (linear(norm(x)), x) as one node
 struct NormLinear : Function<NormLinear> {
@@ -720,22 +740,28 @@ struct FlashPacked : Function<FlashPacked> {
 
 // The same without rotary embedding and with a learned bias by relative position: bias_scale * table[buckets[q - k], head] on the scores.
 // A row of one key has a softmax that is constant: only v has a gradient then, and it is exact.
+struct RpeForward { Tensor table, buckets, o, lo, lse; };
+RpeForward rpe_fwd(const Tensor& qkv, const Tensor& table, const Tensor& buckets, double bias_scale, bool causal, bool train) {
+  const int64_t B = qkv.size(0), Ln = qkv.size(1), H = qkv.size(2), far = causal ? buckets.size(0) - 1 : buckets.size(0) / 2;
+  const at::Device dev = qkv.device();
+  const Tensor q = qkv.slice(3, 0, 128), k = qkv.slice(3, 128, 256), v = qkv.slice(3, 256, 384);
+  RpeForward f{contiguous(table), contiguous(buckets), alloc({B, Ln, H, 128}, BF16, dev), train ? alloc({B, Ln, H, 128}, at::kChar, dev) : Tensor(),
+               alloc({B, H, Ln}, F32, dev)};
+  const Strides qs(q), ks(k), vs(v), os(f.o);
+  const int rc = SB_RUN(sb_attn_rpe_fwd, B * Ln * H > 0, ptr(q), ptr(k), ptr(v), out(f.o), out(f.lo), f32o(f.lse), (int)B, (int)H, (int)Ln, qs.s, ks.s, vs.s,
+                        os.s, (int)causal, 0.08838834764831845f, ptr(f.table), (int)(f.table.scalar_type() == F32), static_cast<const int*>(ptr(f.buckets)),
+                        (int)f.table.size(0), (int)far, (float)bias_scale, status_word(dev), stream());
+  TORCH_CHECK(rc == 0, "attention with relative position bias failed (code ", rc, ", encode ", L.sb_attn_last_encode_result(), "): ",
+              layouts({{"q", &q}, {"k", &k}, {"v", &v}, {"table", &f.table}, {"buckets", &f.buckets}}));
+  return f;
+}
 struct FlashRpe : Function<FlashRpe> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& qkv, const Tensor& table, const Tensor& buckets, double bias_scale, bool causal, bool train) {
-    const int64_t B = qkv.size(0), Ln = qkv.size(1), H = qkv.size(2), far = causal ? buckets.size(0) - 1 : buckets.size(0) / 2;
-    const at::Device dev = qkv.device();
-    Tensor q = qkv.slice(3, 0, 128), k = qkv.slice(3, 128, 256), v = qkv.slice(3, 256, 384), tc = contiguous(table), bc = contiguous(buckets);
-    Tensor o = alloc({B, Ln, H, 128}, BF16, dev), lo = train ? alloc({B, Ln, H, 128}, at::kChar, dev) : Tensor(), lse = alloc({B, H, Ln}, F32, dev);
-    const Strides qs(q), ks(k), vs(v), os(o);
-    const int rc = SB_RUN(sb_attn_rpe_fwd, B * Ln * H > 0, ptr(q), ptr(k), ptr(v), out(o), out(lo), f32o(lse), (int)B, (int)H, (int)Ln, qs.s, ks.s, vs.s,
-                          os.s, (int)causal, 0.08838834764831845f, ptr(tc), (int)(tc.scalar_type() == F32), static_cast<const int*>(ptr(bc)),
-                          (int)tc.size(0), (int)far, (float)bias_scale, status_word(dev), stream());
-    TORCH_CHECK(rc == 0, "attention with relative position bias failed (code ", rc, ", encode ", L.sb_attn_last_encode_result(), "): ",
-                layouts({{"q", &q}, {"k", &k}, {"v", &v}, {"table", &tc}, {"buckets", &bc}}));
-    ctx->save_for_backward({qkv, tc, bc, o, lo, lse});
+  static Tensor forward(AutogradContext* ctx, const Tensor& qkv, const Tensor& table, const Tensor& buckets, double bias_scale, bool causal) {
+    RpeForward f = rpe_fwd(qkv, table, buckets, bias_scale, causal, true);
+    ctx->save_for_backward({qkv, f.table, f.buckets, f.o, f.lo, f.lse});
     ctx->saved_data["bias_scale"] = bias_scale;
     ctx->saved_data["causal"] = causal;
-    return o;
+    return f.o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const variable_list s = ctx->get_saved_variables();
@@ -747,7 +773,7 @@ struct FlashRpe : Function<FlashRpe> {
     if (Ln <= 1 || B * H == 0) {
       cleared(dqkv);
       if (dqkv.numel() > 0) dqkv.slice(3, 256, 384).copy_(g[0]);
-      return {dqkv, cleared(dtable), Tensor(), Tensor(), Tensor(), Tensor()};
+      return {dqkv, cleared(dtable), Tensor(), Tensor(), Tensor()};
     }
     Tensor q = qkv.slice(3, 0, 128), k = qkv.slice(3, 128, 256), v = qkv.slice(3, 256, 384);
     Tensor dq = dqkv.slice(3, 0, 128), dk = dqkv.slice(3, 128, 256), dv = dqkv.slice(3, 256, 384);
@@ -762,9 +788,17 @@ struct FlashRpe : Function<FlashRpe> {
                           (float)ctx->saved_data["bias_scale"].toDouble(), f32o(work), out(dtable), status_word(dev), stream());
     TORCH_CHECK(rc == 0, "backward of attention with relative position bias failed (code ", rc, ", encode ", L.sb_attn_last_encode_result(), "): ",
                 layouts({{"dout", &go}, {"q", &q}, {"k", &k}, {"v", &v}}));
-    return {dqkv, dtable, Tensor(), Tensor(), Tensor(), Tensor()};
+    return {dqkv, dtable, Tensor(), Tensor(), Tensor()};
   }
 };
+void check_rpe(const Tensor& table, const Tensor& buckets, int64_t heads, at::Device device, bool causal) {
+  TORCH_CHECK_VALUE(table.dim() == 2 && table.size(0) >= 1 && table.size(1) == heads && table.is_floating_point(), "relative position table ",
+                    table.scalar_type(), " ", table.sizes(), " for ", heads, " heads: [buckets, heads] expected");
+  TORCH_CHECK_VALUE(buckets.dim() == 1 && buckets.scalar_type() == at::kInt && buckets.size(0) >= 1 && (causal || buckets.size(0) % 2 == 1), "bucket map ",
+                    buckets.scalar_type(), " ", buckets.sizes(), ": int32 [far + 1] (causal) or [2 far + 1] expected");
+  TORCH_CHECK_VALUE(table.device() == device && buckets.device() == device,
+                    "relative position table and bucket map belong on the device of the attention's inputs");
+}
 
 // ------------------------------------------------------------------------------------ what Python calls
 bool fused(const py::handle& w) {          // the parameter's gradient lives in a persistent flat buffer (set by the ZeRO optimizers)
@@ -795,30 +829,43 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   });
   m.def("layernorm", [](const Tensor& x, const Tensor& w, const Tensor& b, double eps) {
     no_transforms();
+    if (!layernorm_covers(x, w, b)) return at::layer_norm(x, {x.size(-1)}, w, b, eps);
     const c10::cuda::CUDAGuard device(x.device());
-    return LayerNorm::apply(x, w, b, eps, false, wants_grad({&x, &w, &b}))[0];
+    if (!wants_grad({&x, &w, &b})) return layernorm_fwd(x, w, b, eps, false).y;
+    return LayerNorm::apply(x, w, b, eps, false)[0];
   });
   m.def("layernorm_residual", [](const Tensor& x, const Tensor& w, const Tensor& b, double eps) {
     no_transforms();
+    if (!layernorm_covers(x, w, b)) return std::make_tuple(at::layer_norm(x, {x.size(-1)}, w, b, eps), x);
     const c10::cuda::CUDAGuard device(x.device());
-    variable_list r = LayerNorm::apply(x, w, b, eps, true, wants_grad({&x, &w, &b}));
+    if (!wants_grad({&x, &w, &b})) return std::make_tuple(layernorm_fwd(x, w, b, eps, false).y, x);
+    variable_list r = LayerNorm::apply(x, w, b, eps, true);
     return std::make_tuple(r[0], r[1]);
   });
   m.def("act_quantize", [](const Tensor& x) {
     no_transforms();
+    const at::ScalarType type = x.scalar_type();
+    TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && (type == BF16 || type == at::kHalf || type == F32),
+                      "act_quantize takes bf16, fp16 or fp32 [..., D] with D >= 1, got ", type, " ", x.sizes());
     const c10::cuda::CUDAGuard device(x.device());
-    const Tensor xc = contiguous(x.detach());
-    const int64_t D = xc.size(-1), T = D ? xc.numel() / D : 0;
+    const at::AutoDispatchBelowADInplaceOrView no_graph;
+    const Tensor xc = contiguous(x);
+    const int64_t D = xc.size(-1), T = xc.numel() / D;
     Tensor q = alloc(xc.sizes(), at::kChar, xc.device()), s = alloc(with_last(xc.sizes(), (D + 127) / 128), F32, xc.device());
     SB_CALL(sb_act8_quantize, T > 0, ptr(xc), out(q), f32o(s), (long long)T, (int)D, type_code(xc.scalar_type()), stream());
     return std::make_tuple(q, s);
   });
   m.def("act_dequantize", [](const Tensor& q, const Tensor& scale, int64_t type) {
     no_transforms();
+    TORCH_CHECK_VALUE(q.scalar_type() == at::kChar && q.dim() >= 1 && q.size(-1) >= 1 && scale.scalar_type() == F32 && scale.device() == q.device() &&
+                      scale.sizes().vec() == with_last(q.sizes(), (q.size(-1) + 127) / 128),
+                      "act_dequantize takes what act_quantize returned, got q ", q.scalar_type(), " ", q.sizes(), ", scale ", scale.scalar_type(), " ",
+                      scale.sizes());
     const c10::cuda::CUDAGuard device(q.device());
+    const at::AutoDispatchBelowADInplaceOrView no_graph;
     const Tensor qc = contiguous(q), sc = contiguous(scale);
     const at::ScalarType t = type == 0 ? BF16 : type == 1 ? at::kHalf : F32;
-    const int64_t D = qc.size(-1), T = D ? qc.numel() / D : 0;
+    const int64_t D = qc.size(-1), T = qc.numel() / D;
     Tensor x = alloc(qc.sizes(), t, qc.device());
     SB_CALL(sb_act8_dequantize, T > 0, ptr(qc), f32(sc), out(x), (long long)T, (int)D, (int)type, stream());
     return x;
@@ -852,17 +899,43 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     variable_list r = HyenaLI::apply(feat, gamma, R, p, bias, state_in, want_state, tc);
     return std::make_tuple(r[0], want_state ? OptTensor(r[1]) : OptTensor());
   });
-  m.def("attention_rpe", [](const Tensor& qkv, const Tensor& table, const Tensor& buckets, double bias_scale, bool causal) {
+  // nothing where the kernels do not cover the shape
+  m.def("attention_rpe", [](const Tensor& qkv, const Tensor& table, const Tensor& buckets, double bias_scale, bool causal, int64_t max_far) -> OptTensor {
     no_transforms();
+    TORCH_CHECK_VALUE(qkv.dim() == 4 && qkv.size(3) % 3 == 0 && qkv.size(3) > 0, "attention_rpe takes qkv [B, L, H, 3 * hd], got ", qkv.sizes());
+    check_rpe(table, buckets, qkv.size(2), qkv.device(), causal);
+    if (qkv.scalar_type() != BF16 || qkv.size(3) != 384 || !qkv.is_contiguous() || !on16(qkv) || qkv.size(0) >= 65535 || qkv.size(1) >= (1LL << 30) ||
+        (causal ? buckets.size(0) - 1 : buckets.size(0) / 2) > max_far)
+      return std::nullopt;
     const c10::cuda::CUDAGuard device(qkv.device());
-    return FlashRpe::apply(qkv, table, buckets, bias_scale, causal, wants_grad({&qkv, &table}));
+    const Tensor t = table.scalar_type() == BF16 || table.scalar_type() == F32 ? table : table.to(F32);
+    if (!wants_grad({&qkv, &table})) return rpe_fwd(qkv, t, buckets, bias_scale, causal, false).o;
+    return FlashRpe::apply(qkv, t, buckets, bias_scale, causal);
   });
   m.def("attention_rpe_step", [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& buckets, double bias_scale,
-                                 const OptTensor& lengths) {
+                                 const OptTensor& lengths) -> OptTensor {
     no_transforms();
-    const c10::cuda::CUDAGuard device(q.device());
+    TORCH_CHECK_VALUE(q.dim() == 3 && k.dim() == 4 && k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(2) == q.size(1) && k.size(3) == q.size(2) &&
+                      q.size(2) > 0, "attention_rpe_step takes q [B, H, hd], k and v [B, T, H, hd], got ", q.sizes(), ", ", k.sizes(), ", ", v.sizes());
+    TORCH_CHECK_VALUE(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type() && k.device() == q.device() && v.device() == q.device(),
+                      "attention_rpe_step: q, k and v are of one type on one device");
     const int64_t B = q.size(0), H = q.size(1), hd = q.size(2), T = k.size(1);
-    const Tensor tc = contiguous(table), bc = contiguous(buckets), lc = lengths.has_value() ? contiguous(*lengths) : Tensor();
+    check_rpe(table, buckets, H, q.device(), true);
+    TORCH_CHECK_VALUE(!lengths.has_value() || (lengths->scalar_type() == at::kInt && lengths->dim() == 1 && lengths->size(0) == B &&
+                                               lengths->device() == q.device()), "attention_rpe_step: lengths int32 [", B, "] on the inputs' device");
+    const auto readable = [](const Tensor& t) {
+      for (int64_t i = 0; i + 1 < t.dim(); ++i)
+        if (t.stride(i) % 8) return false;
+      return t.stride(t.dim() - 1) == 1 && on16(t);
+    };
+    const bool half = q.scalar_type() == BF16 || q.scalar_type() == at::kHalf;
+    if (!half || hd % 8 || hd > 256 || B > 65535 || H > 65535 || T >= (1LL << 31) || wants_grad({&q, &k, &v, &table}) || !readable(q) || !readable(k) ||
+        !readable(v))
+      return std::nullopt;
+    const c10::cuda::CUDAGuard device(q.device());
+    const at::ScalarType tt = table.scalar_type();
+    const Tensor tc = contiguous(tt == BF16 || tt == at::kHalf || tt == F32 ? table : table.to(F32)), bc = contiguous(buckets),
+                 lc = lengths.has_value() ? contiguous(*lengths) : Tensor();
     Tensor o = alloc({B, H, hd}, q.scalar_type(), q.device());
     const int splits = L.sb_attn_step_splits(B, H, T);
     Tensor part = splits > 8 ? alloc({B * H * splits * (hd + 2)}, F32, q.device()) : Tensor();

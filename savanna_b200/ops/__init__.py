@@ -107,15 +107,17 @@ def _check_layernorm(x, weight, bias):
 def layernorm(x, weight, bias, eps: float):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension.  CUDA: bf16, fp16 or fp32 (x, weight and bias alike), rows of
     up to 16384 values of any width, statistics and the gradients' sums over the rows in fp32."""
+    if _k(x):
+        return _CO.layernorm(x, weight, bias, eps)
     _check_layernorm(x, weight, bias)
-    return _co().layernorm(x, weight, bias, eps) if _k(x) else ref.layernorm(x, weight, bias, eps)
+    return ref.layernorm(x, weight, bias, eps)
 
 
 def layernorm_residual(x, weight, bias, eps: float):
     """(layernorm(x), x): as `rmsnorm_residual`."""
-    _check_layernorm(x, weight, bias)
     if _k(x):
-        return _co().layernorm_residual(x, weight, bias, eps)
+        return _CO.layernorm_residual(x, weight, bias, eps)
+    _check_layernorm(x, weight, bias)
     return ref.layernorm(x, weight, bias, eps), x
 
 
@@ -256,12 +258,13 @@ def attention_rpe(qkv, table, buckets, scale: float = 1.0, causal: bool = True):
     where what lies further away has the outermost entry's (`RelativePositionBias.bucket_map`).  An entry outside 0 .. nb - 1 has no bias on the
     kernel path.  The kernels form no [L, L] bias or scores; their query gradient is added up in an order that varies, as that of
     `attention_packed` does, the table's in a fixed one."""
+    if _k(qkv):
+        o = _CO.attention_rpe(qkv, table, buckets, scale, causal, RPE_MAX_FAR)
+        if o is not None:
+            return o
     if qkv.dim() != 4 or qkv.shape[3] % 3 or qkv.shape[3] == 0:
         raise ValueError(f"attention_rpe takes qkv [B, L, H, 3 * hd], got {tuple(qkv.shape)}")
     _check_rpe(table, buckets, qkv.shape[2], qkv.device, causal)
-    far = buckets.shape[0] - 1 if causal else buckets.shape[0] // 2
-    if attention_rpe_covers(qkv, far):
-        return _co().attention_rpe(qkv, table, buckets, scale, causal)
     return ref.attention_rpe(qkv, table, buckets, scale, causal)
 
 
@@ -270,6 +273,10 @@ def attention_rpe_step(q, k, v, table, buckets, scale: float = 1.0, lengths=None
     [B, T, H, hd] (any strides with 16-byte rows are read in place), the new token's own key and value the last of the sequence's.  `lengths`
     [B] int32 on the device: keys of each sequence, 0 .. T (values outside are clamped; rows of length 0 give zeros; what lies behind a
     sequence's last key is not looked at); None: T.  CUDA: bf16 or fp16, heads of up to 256; no gradients (with them the statement runs)."""
+    if _k(q):
+        o = _CO.attention_rpe_step(q, k, v, table, buckets, scale, lengths)
+        if o is not None:
+            return o
     if q.dim() != 3 or k.dim() != 4 or k.shape != v.shape or (k.shape[0], k.shape[2], k.shape[3]) != tuple(q.shape) or q.shape[2] == 0:
         raise ValueError(f"attention_rpe_step takes q [B, H, hd], k and v [B, T, H, hd], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     if k.dtype != q.dtype or v.dtype != q.dtype or k.device != q.device or v.device != q.device:
@@ -277,9 +284,6 @@ def attention_rpe_step(q, k, v, table, buckets, scale: float = 1.0, lengths=None
     _check_rpe(table, buckets, q.shape[1], q.device, True)
     if lengths is not None and (lengths.dtype != torch.int32 or tuple(lengths.shape) != (q.shape[0],) or lengths.device != q.device):
         raise ValueError(f"attention_rpe_step: lengths int32 [{q.shape[0]}] on the inputs' device, got {lengths.dtype} {tuple(lengths.shape)}")
-    grad = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, table))
-    if _k(q) and not grad and _co().attention_rpe_step_covers(q, k, v):
-        return _co().attention_rpe_step(q, k, v, table, buckets, scale, lengths)
     return ref.attention_rpe_step(q, k, v, table, buckets, scale, lengths)
 
 
@@ -290,19 +294,23 @@ def act_quantize(x):
     """x [..., D] (bf16, fp16 or fp32) -> (q int8 of x's shape, scale fp32 [..., ceil(D / 128)]): 128 consecutive values of a row share
     a scale of amax / 127, so that a value comes back within amax / 254 of itself and a rounding to its type.  A block that holds an infinity
     or NaN comes back as NaN.  Not differentiated: the form in which a checkpointed activation waits for its recomputation."""
+    if _k(x):
+        return _CO.act_quantize(x)
     if x.dim() < 1 or x.shape[-1] < 1 or x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise ValueError(f"act_quantize takes bf16, fp16 or fp32 [..., D] with D >= 1, got {x.dtype} {tuple(x.shape)}")
-    return _co().act_quantize(x) if _k(x) else ref.act_quantize(x)
+    return ref.act_quantize(x)
 
 
 def act_dequantize(q, scale, dtype=torch.bfloat16):
     """q * scale as `dtype`: what `act_quantize` kept."""
     if dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise ValueError(f"act_dequantize gives bf16, fp16 or fp32, not {dtype}")
+    if _k(q):
+        return _CO.act_dequantize(q, scale, dtype)
     if q.dtype != torch.int8 or q.dim() < 1 or q.shape[-1] < 1 or scale.dtype != torch.float32 or scale.device != q.device \
             or tuple(scale.shape) != tuple(q.shape[:-1]) + (-(-q.shape[-1] // ref.ACT_BLOCK),):
         raise ValueError(f"act_dequantize takes what act_quantize returned, got q {q.dtype} {tuple(q.shape)}, scale {scale.dtype} {tuple(scale.shape)}")
-    return _co().act_dequantize(q, scale, dtype) if _k(q) else ref.act_dequantize(q, scale, dtype)
+    return ref.act_dequantize(q, scale, dtype)
 
 
 # ----------------------------------------------------------------------------- loss / optimizer

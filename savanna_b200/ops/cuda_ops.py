@@ -1057,50 +1057,35 @@ def rmsnorm(x, weight, eps, form="te"):
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}       # type codes of csrc/layernorm.cu and csrc/act8.cu
 
 
-def _layernorm_covers(x, weight, bias) -> bool:
-    """One type, rows of up to 16384 values that 32 bits count; anything else runs PyTorch's layer norm."""
-    return (x.dtype in _TYPES and weight.dtype == x.dtype and bias is not None and bias.dtype == x.dtype and 1 <= x.shape[-1] <= 16384
-            and x.numel() // max(1, x.shape[-1]) < 2 ** 31 and weight.device == x.device and bias.device == x.device)
+# These check their arguments in C++ (a few microseconds less than here: what a small call takes is the host's time).
 
 
 def layernorm(x, weight, bias, eps):
-    if not _layernorm_covers(x, weight, bias):
-        return torch.nn.functional.layer_norm(x, (x.shape[-1],), weight, bias, eps)
-    return _native("layernorm", x, weight, bias, float(eps))
+    """PyTorch's layer norm runs where the kernels do not cover types or sizes."""
+    return _native("layernorm", x, weight, bias, eps)
 
 
 def layernorm_residual(x, weight, bias, eps):
     """(layernorm(x), x) with the two gradients combined in one backward kernel."""
-    if not _layernorm_covers(x, weight, bias):
-        return torch.nn.functional.layer_norm(x, (x.shape[-1],), weight, bias, eps), x
-    return _native("layernorm_residual", x, weight, bias, float(eps))
+    return _native("layernorm_residual", x, weight, bias, eps)
 
 
-def attention_rpe(qkv, table, buckets, scale, causal):
-    if table.dtype not in (torch.bfloat16, torch.float32):
-        table = table.float()
-    return _native("attention_rpe", qkv, table, buckets, float(scale), bool(causal))
-
-
-def attention_rpe_step_covers(q, k, v) -> bool:
-    """What the kernels read in place: bf16 or fp16 heads of up to 256 in steps of 8, 16-byte rows."""
-    return (q.dtype in (torch.bfloat16, torch.float16) and q.shape[2] % 8 == 0 and 8 <= q.shape[2] <= 256 and q.shape[0] <= 65535
-            and q.shape[1] <= 65535 and k.shape[1] < 2 ** 31
-            and all(t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1]) for t in (q, k, v)))
+def attention_rpe(qkv, table, buckets, scale, causal, max_far):
+    """None where the kernels do not cover the shape."""
+    return _native("attention_rpe", qkv, table, buckets, scale, causal, max_far)
 
 
 def attention_rpe_step(q, k, v, table, buckets, scale, lengths):
-    if table.dtype not in _TYPES:
-        table = table.float()
-    return _N.attention_rpe_step(q, k, v, table, buckets, float(scale), lengths)
+    """None where the kernels do not cover types, sizes or strides, or a gradient is wanted."""
+    return _native("attention_rpe_step", q, k, v, table, buckets, scale, lengths)
 
 
 def act_quantize(x):
-    return _N.act_quantize(x)
+    return _native("act_quantize", x)
 
 
 def act_dequantize(q, scale, dtype):
-    return _N.act_dequantize(q, scale, _TYPES[dtype])
+    return _native("act_dequantize", q, scale, _TYPES[dtype])
 
 
 # ----------------------------------------------------------------------------- gated activation

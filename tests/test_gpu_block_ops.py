@@ -242,3 +242,44 @@ def test_activations_guarded_and_empty():
             q, scale = ops.act_quantize(x)
             assert ops.act_dequantize(q, scale).shape == shape
         assert cuda_ops.check_guards() > 0
+
+
+def test_refusals():
+    x, w = torch.randn(2, 8, device=DEV), torch.ones(8, device=DEV)
+    for bad in ((x, w[:7], w), (x, w, torch.ones(8, 1, device=DEV)), (torch.randn(3, 0, device=DEV), w, w), (torch.tensor(1.0, device=DEV), w, w)):
+        with pytest.raises(ValueError):
+            ops.layernorm(*bad, 1e-5)
+        with pytest.raises(ValueError):
+            ops.layernorm_residual(*bad, 1e-5)
+    for bad in (torch.zeros(3, 4, dtype=torch.int32, device=DEV), torch.zeros(3, 0, device=DEV), torch.tensor(1.0, device=DEV)):
+        with pytest.raises(ValueError):
+            ops.act_quantize(bad)
+    q, scale = ops.act_quantize(torch.randn(3, 200, device=DEV))
+    for bad in ((q.float(), scale, torch.bfloat16), (q, scale[:, :1], torch.bfloat16), (q, scale.double(), torch.bfloat16), (q, scale, torch.float64),
+                (q, scale.cpu(), torch.bfloat16)):
+        with pytest.raises(ValueError):
+            ops.act_dequantize(*bad)
+
+
+def test_types_and_sizes_that_the_kernels_do_not_cover_run_pytorchs():
+    g = _gen(8)
+    with pytest.raises(RuntimeError):                # as there
+        ops.layernorm(torch.randn(3, 64, device=DEV).to(torch.bfloat16), torch.randn(64, device=DEV), torch.randn(64, device=DEV), 1e-5)
+    for x, w in ((torch.randn(2, 20000, generator=g, device=DEV), torch.randn(20000, generator=g, device=DEV)),
+                 (torch.randn(2, 10, generator=g, device=DEV).double(), torch.randn(10, generator=g, device=DEV).double())):
+        want = torch.nn.functional.layer_norm(x, (x.shape[-1],), w, w, 1e-5)
+        assert torch.equal(ops.layernorm(x, w, w, 1e-5), want)
+        y, xr = ops.layernorm_residual(x, w, w, 1e-5)
+        assert torch.equal(y, want) and xr is x
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_traced_operators_run_on_new_inputs():
+    w, b = torch.randn(64, device=DEV), torch.randn(64, device=DEV)
+
+    def f(x):
+        return ops.act_dequantize(*ops.act_quantize(ops.layernorm(x, w, b, 1e-5)), torch.float32)
+    g = _gen(2)
+    x, z = torch.randn(5, 64, generator=g, device=DEV), torch.randn(5, 64, generator=g, device=DEV)
+    traced = torch.jit.trace(f, x, check_trace=False)
+    assert torch.equal(traced(z), f(z)) and not torch.equal(traced(z), f(x))

@@ -241,3 +241,38 @@ def test_empty_batch():
     o = ops.attention_rpe(qkv, table, _map(32, 128, True), 1.0, True)
     gq, gt = torch.autograd.grad(o, (qkv, table), torch.empty_like(o))
     assert o.shape == (0, 5, 2, 128) and gq.shape == qkv.shape and float(gt.abs().sum()) == 0
+
+
+def test_refusals():
+    qkv, table, buckets, _ = _case(1, 6, 2, 8, 4, True)
+    both = torch.zeros(9, dtype=torch.int32, device=DEV)
+    for bad in ((qkv[..., :383], table, buckets, 1.0, True), (qkv[0], table, buckets, 1.0, True), (qkv, table[:, :1], buckets, 1.0, True),
+                (qkv, table, buckets.long(), 1.0, True), (qkv, table, buckets[:0], 1.0, True), (qkv, table, both[:8], 1.0, False),
+                (qkv, table.to(torch.int32), buckets, 1.0, True), (qkv, table[0], buckets, 1.0, True), (qkv, table.cpu(), buckets, 1.0, True),
+                (qkv, table, buckets.cpu(), 1.0, True)):
+        with pytest.raises(ValueError):
+            ops.attention_rpe(*bad)
+
+
+def test_buckets_that_do_not_exist_have_no_bias_and_no_gradient():
+    qkv, table, buckets, go = _case(1, 150, 2, 32, 128, True)
+    odd = buckets.clone()
+    odd[buckets == 3], odd[buckets == 9] = -1, 40
+    zero = table.clone()
+    zero[3], zero[9] = 0, 0
+    a, b = _run(qkv, table, odd, 2.0, True, go), _run(qkv, zero, buckets, 2.0, True, go)
+    assert torch.equal(a[0], b[0])
+    keep = torch.ones(32, dtype=torch.bool, device=DEV)
+    keep[3] = keep[9] = False
+    assert torch.equal(a[2][keep], b[2][keep]) and float(a[2][~keep].abs().max()) == 0
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_traced_on_new_inputs():
+    qkv, table, buckets, _ = _case(1, 70, 2, 32, 64, True)
+    other = _case(1, 70, 2, 32, 64, True, seed=9)[0]
+
+    def f(x):
+        return ops.attention_rpe(x, table, buckets, 2.0, True)
+    traced = torch.jit.trace(f, qkv, check_trace=False)
+    assert torch.equal(traced(other), f(other))

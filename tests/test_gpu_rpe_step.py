@@ -155,3 +155,24 @@ def test_empty_batch_and_cache():
     q, k, v, table, buckets, _ = _case(2, 0, 2, 64, torch.bfloat16)
     assert float(ops.attention_rpe_step(q, k, v, table, buckets).abs().max()) == 0
     assert ops.attention_rpe_step(q[:0], k[:0], v[:0], table, buckets).shape == (0, 2, 64)
+
+
+def test_refusals():
+    q, k, v, table, buckets, n = _case(2, 6, 2, 64, torch.bfloat16)
+    for bad in ((q[0], k, v, table, buckets), (q, k, v[:, :3], table, buckets), (q, k, v.half(), table, buckets), (q[..., :8], k, v, table, buckets),
+                (q, k, v, table[:, :1], buckets), (q, k, v, table, buckets.long()), (q, k.cpu(), v, table, buckets)):
+        with pytest.raises(ValueError):
+            ops.attention_rpe_step(*bad, 1.0, n)
+    for bad in (n.long(), n[:1], n.cpu()):
+        with pytest.raises(ValueError):
+            ops.attention_rpe_step(q, k, v, table, buckets, 1.0, bad)
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_traced_on_new_inputs():
+    q, k, v, table, buckets, n = _case(2, 40, 2, 64, torch.bfloat16)
+
+    def f(x):
+        return ops.attention_rpe_step(x, k, v, table, buckets, 1.0, n)
+    traced = torch.jit.trace(f, q, check_trace=False)
+    assert torch.equal(traced(-q), f(-q))
