@@ -6,7 +6,8 @@
 // infinity: a block that holds one of them has a scale of NaN and comes back as NaN, so that an overflow stays visible.  A block below 1e-30
 // comes back as nearly zero.
 //
-// Bound by memory: 2 + 1 bytes a value for 16-bit types, one pass; a lane has four 16-byte loads on their way.
+// Bound by memory: 2 + 1 bytes a value for 16-bit types, one pass; a lane has four 16-byte loads on their way.  8192 x 4096 bf16: 20.5 us there and
+// 19.7 back (a copy of as many bytes takes 15.5).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -33,8 +34,9 @@ template <class T, int N> struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16
 __device__ __forceinline__ uint32_t magnitude(float f) { return __float_as_uint(f) & 0x7fffffffu; }
 __device__ __forceinline__ float inverse(float amax) { return 127.f / (amax < TINY ? TINY : amax); }     // NaN stays NaN
 // rint(x * inv), whose magnitude is at most 127, in the low byte: a product of up to 2^22 added to 1.5 * 2^23 is rounded to an integer, half
-// to even.  (A conversion instruction for each value ran at a quarter of the rate.)
-__device__ __forceinline__ uint32_t code(float x, float inv) { return __float_as_uint(fmaf(x, inv, 12582912.f)); }
+// to even.  (A conversion instruction for each value ran at a quarter of the rate.)  The product is rounded by itself: 16-bit values often lie
+// halfway between two codes, and there its rounding makes good that of inv, where a fused one would fall to a side by chance.
+__device__ __forceinline__ uint32_t code(float x, float inv) { return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.f)); }
 __device__ __forceinline__ uint32_t four(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }

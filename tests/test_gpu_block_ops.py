@@ -283,3 +283,12 @@ def test_traced_operators_run_on_new_inputs():
     x, z = torch.randn(5, 64, generator=g, device=DEV), torch.randn(5, 64, generator=g, device=DEV)
     traced = torch.jit.trace(f, x, check_trace=False)
     assert torch.equal(traced(z), f(z)) and not torch.equal(traced(z), f(x))
+
+
+def test_values_halfway_between_two_codes_go_to_the_even_one():
+    """With amax = 127 a code is the value itself: halves are ties."""
+    x = torch.arange(-127, 128, device=DEV).float().div(2).repeat(2)[:384].clone()
+    x[::128] = 127.0
+    for dtype in (torch.float16, torch.float32):
+        q, scale = ops.act_quantize(x.to(dtype).view(1, 384))
+        assert torch.equal(scale, torch.ones_like(scale)) and torch.equal(q[0].float(), torch.round(x))
