@@ -385,14 +385,14 @@ struct LayerNorm : Function<LayerNorm> {
     return {dx, dw, db, Tensor(), Tensor()};
   }
 };
-// The kernels' part of layer norms: one type, rows of up to 16384 values that 32 bits count.  Shapes that make no sense are refused.
+// The kernels' part of layer norms: one type, up to 2^30 rows of up to 16384 values.  Shapes that make no sense are refused.
 bool layernorm_covers(const Tensor& x, const Tensor& w, const Tensor& b) {
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "layernorm takes [..., D] with D >= 1, got ", x.sizes());
   const int64_t D = x.size(-1);
   TORCH_CHECK_VALUE(w.dim() == 1 && w.size(0) == D && b.dim() == 1 && b.size(0) == D, "layernorm weight ", w.sizes(), " and bias ", b.sizes(),
                     " for rows of ", D, " values");
   const at::ScalarType t = x.scalar_type();
-  return (t == BF16 || t == at::kHalf || t == F32) && w.scalar_type() == t && b.scalar_type() == t && D <= 16384 && x.numel() / D < (1LL << 31) &&
+  return (t == BF16 || t == at::kHalf || t == F32) && w.scalar_type() == t && b.scalar_type() == t && D <= 16384 && x.numel() / D <= (1LL << 30) &&
          w.device() == x.device() && b.device() == x.device();
 }
 

@@ -101,22 +101,75 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// Widths that N = 16 / sizeof(T) does not divide (SHIFT): a row is `head` values up to the next 16-byte boundary, nv vectors, and `tail` values.  The
+// single ones, 14 at most, are spread over the lanes of the row's first warp.  Rows that are N (or N / 2, ..: `classes`) apart are cut alike.
+// bf16, us, single values throughout -> here: forward 8192 x 1027 22.6 -> 12.3, 8192 x 4095 95 -> 37; backward 45 -> 27, 1045 -> 62.  (Whole vectors
+// with the neighbours' values masked: 69 and 88 at 8192 x 4095, most of it spent on the two ends.)
+template <class T> struct Cut {
+  int head, nv, tail;
+  __device__ __forceinline__ Cut(int row, int D) {
+    constexpr int N = Of<T>::N;
+    const int a = row % N * (D % N) % N;
+    head = min((N - a) % N, D);
+    nv = (D - head) / N;
+    tail = D - head - nv * N;
+  }
+  __device__ __forceinline__ int single(int lane) const {        // the column of a lane's single value, or -1
+    constexpr int N = Of<T>::N;
+    return lane < head ? lane : lane >= 16 && lane - 16 < tail ? head + nv * N + lane - 16 : -1;
+  }
+};
+
+__device__ __forceinline__ uint4 halves(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e) {
+  return make_uint4(__funnelshift_r(a, b, 16), __funnelshift_r(b, c, 16), __funnelshift_r(c, d, 16), __funnelshift_r(d, e, 16));
+}
+// The N weights from column c on (c + N <= D) out of two vectors of w, which lies on a 16-byte boundary.  `c` is the same modulo N in all lanes.
+template <class T> __device__ __forceinline__ uint4 weights_at(const T* w, int c, int D) {
+  constexpr int N = Of<T>::N;
+  const int k = c / N, e = c - k * N;                    // first vector, values into it
+  const uint4 lo = __ldg(reinterpret_cast<const uint4*>(w) + k);
+  if (e == 0) return lo;
+  uint4 hi;
+  if ((k + 2) * N <= D) {
+    hi = __ldg(reinterpret_cast<const uint4*>(w) + k + 1);
+  } else {                                               // the last vector ends beyond the row
+    float t[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) t[j] = j < e ? Of<T>::one(w[(k + 1) * N + j]) : 0.f;
+    hi = Of<T>::put(t);
+  }
+  const bool half = sizeof(T) == 2 && (e & 1);           // whole words, then half a one
+  switch (e * (int)sizeof(T) / 4) {
+    case 0: return halves(lo.x, lo.y, lo.z, lo.w, hi.x);
+    case 1: return half ? halves(lo.y, lo.z, lo.w, hi.x, hi.y) : make_uint4(lo.y, lo.z, lo.w, hi.x);
+    case 2: return half ? halves(lo.z, lo.w, hi.x, hi.y, hi.z) : make_uint4(lo.z, lo.w, hi.x, hi.y);
+    default: return half ? halves(lo.w, hi.x, hi.y, hi.z, hi.w) : make_uint4(lo.w, hi.x, hi.y, hi.z);
+  }
+}
+
 // ------------------------------------------------------------------------------------ forward
 // W warps take a row, V vectors a lane, all loaded before the first sum.  Bound by memory with many rows: 8192 x 4096 bf16 25.1 us (a copy
 // takes 22.2); a few rows take the chain load, two sums, barrier, store.
 __host__ __device__ constexpr int fwd_rows(int W) { return W == 1 ? 4 : 1; }
 
-template <class T, int VEC, int V, int W>
+template <class T, int VEC, int V, int W, bool SHIFT>
 __global__ void __launch_bounds__(32 * W * fwd_rows(W))
 fwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict__ b, T* __restrict__ y, float2* __restrict__ stats, int rows,
            int D, float eps) {
   __shared__ float4 red[W];
-  const int lane = threadIdx.x & 31, warp = W > 1 ? threadIdx.x >> 5 : 0, i0 = warp * 32 + lane, nv = D / VEC;
+  const int lane = threadIdx.x & 31, warp = W > 1 ? threadIdx.x >> 5 : 0, i0 = warp * 32 + lane;
   const size_t row = (size_t)blockIdx.x * fwd_rows(W) + threadIdx.x / (32 * W);
   if (row >= (size_t)rows) return;                       // a whole warp of W == 1, never part of a row
-  const T* src = x + row * D;
+  const Cut<T> cut((int)(row % Of<T>::N), D);            // SHIFT
+  const int nv = SHIFT ? cut.nv : D / VEC, head = SHIFT ? cut.head : 0;
+  const T* src = x + row * D + head;
+  const int sc = SHIFT && warp == 0 ? cut.single(lane) : -1;
+  float fs = 0.f, gs = 0.f, cs = 0.f;                    // a lane's single value, its weight and bias
+  if constexpr (SHIFT) {
+    if (sc >= 0) { fs = Of<T>::one(x[row * D + sc]); gs = Of<T>::one(w[sc]); cs = Of<T>::one(b[sc]); }
+  }
   // the weights as well where a lane has few of them: a row alone on its SM then waits once
-  constexpr bool AHEAD = V * VEC <= 16;
+  constexpr bool AHEAD = V * VEC <= 16 && !SHIFT;
   float f[V][VEC], g[AHEAD ? V : 1][VEC], c[AHEAD ? V : 1][VEC];
   int n = 0;                                             // values of this warp
   float s = 0.f;
@@ -124,8 +177,9 @@ fwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict
   for (int v = 0; v < V; ++v) {
     const int i = i0 + 32 * W * v;
     n += min(max(nv - (warp * 32 + 32 * W * v), 0), 32) * VEC;
-    if (i < nv) load<T, VEC>(src, i, f[v]);
-    else {
+    if (i < nv) {
+      load<T, VEC>(src, i, f[v]);
+    } else {
 #pragma unroll
       for (int j = 0; j < VEC; ++j) f[v][j] = 0.f;
     }
@@ -139,6 +193,7 @@ fwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict
   for (int v = 0; v < V; ++v)
 #pragma unroll
     for (int j = 0; j < VEC; ++j) s += f[v][j];
+  if (SHIFT && warp == 0) { n += cut.head + cut.tail; s += fs; }
   s = warp_sum(s);
   float mean = n ? __fdividef(s, (float)n) : 0.f, m2 = 0.f;
 #pragma unroll
@@ -147,6 +202,7 @@ fwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict
 #pragma unroll
       for (int j = 0; j < VEC; ++j) { const float d = f[v][j] - mean; m2 = fmaf(d, d, m2); }
     }
+  if (SHIFT && sc >= 0) m2 = fmaf(fs - mean, fs - mean, m2);
   m2 = warp_sum(m2);
   if (W > 1) {                                           // the warps' results, one a lane: the same sums in every warp
     if (lane == 0) red[warp] = make_float4(s, m2, mean, (float)n);
@@ -168,17 +224,56 @@ fwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict
     const int i = i0 + 32 * W * v;
     if (i < nv) {
       const int k = AHEAD ? v : 0;
-      if (!AHEAD) { load<T, VEC>(w, i, g[k]); load<T, VEC>(b, i, c[k]); }
+      if constexpr (SHIFT) { Of<T>::get(weights_at<T>(w, head + i * VEC, D), g[k]); Of<T>::get(weights_at<T>(b, head + i * VEC, D), c[k]); }
+      else if (!AHEAD) { load<T, VEC>(w, i, g[k]); load<T, VEC>(b, i, c[k]); }
 #pragma unroll
       for (int j = 0; j < VEC; ++j) f[v][j] = fmaf((f[v][j] - mean) * rstd, g[k][j], c[k][j]);
-      store<T, VEC>(y + row * D, i, f[v]);
+      store<T, VEC>(y + row * D + head, i, f[v]);
     }
   }
+  if constexpr (SHIFT) {
+    if (sc >= 0) y[row * D + sc] = Of<T>::from(fmaf((fs - mean) * rstd, gs, cs));
+  }
+}
+
+// Rows of up to LPR = 8 or 16 vectors: as many lanes a row.  262144 x 64 bf16: 17 us, 58 with a warp a row.
+template <class T, int LPR>
+__global__ void __launch_bounds__(256)
+fwd_narrow_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict__ b, T* __restrict__ y, float2* __restrict__ stats, int rows,
+                  int D, float eps) {
+  constexpr int N = Of<T>::N;
+  const int i = threadIdx.x % LPR, row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const bool have = row < rows && i < D / N;
+  float f[N], g[N], c[N], s = 0.f, m2 = 0.f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) f[j] = g[j] = c[j] = 0.f;
+  if (have) {
+    load<T, N>(x + (size_t)row * D, i, f);
+    load<T, N>(w, i, g);
+    load<T, N>(b, i, c);
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) s += f[j];
+#pragma unroll
+  for (int o = LPR / 2; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const float mean = __fdividef(s, (float)D);
+#pragma unroll
+  for (int j = 0; j < N; ++j) { const float d = have ? f[j] - mean : 0.f; m2 = fmaf(d, d, m2); }
+#pragma unroll
+  for (int o = LPR / 2; o; o >>= 1) m2 += __shfl_xor_sync(0xffffffffu, m2, o);
+  const float rstd = rsqrtf(__fdividef(m2, (float)D) + eps);
+  if (!have) return;
+  if (stats && i == 0) stats[row] = make_float2(mean, rstd);
+#pragma unroll
+  for (int j = 0; j < N; ++j) f[j] = fmaf((f[j] - mean) * rstd, g[j], c[j]);
+  store<T, N>(y + (size_t)row * D, i, f);
 }
 
 // ------------------------------------------------------------------------------------ backward
 // A thread owns V vectors of columns and keeps their dw and db sums in registers; W warps share a row, a block holds several such groups
 // and walks over the rows.  partial[block] = [dw | db] of the block's rows, added up by reduce_kernel in a fixed order.
+//
+// SHIFT: a group takes rows of one class, which are cut alike, so that it owns fixed columns all the same, single ones among them.
 //
 // The rows come through a ring in shared memory, R rows at a time and S of those ahead: a thread copies the 16 bytes of each row and
 // tensor that it owns, nobody else reads them, so there is no barrier for them, only the thread's own wait.  8192 x 4096 bf16 with residual:
@@ -230,27 +325,33 @@ __device__ __forceinline__ void group_sums(float (&s)[2 * R], float* red, int wa
   for (int k = 0; k < P; ++k) s[k] = __shfl_sync(0xffffffffu, t, k * (32 / P));
 }
 
-template <class T, int V, int R, int S, bool RES, bool W16>
+template <class T, int V, int R, int S, bool RES, bool W16, bool SHIFT>
 __global__ void __launch_bounds__(BWD_THREADS, V == 1 ? 2 : 1)
 bwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict__ dy, const float2* __restrict__ stats,
-           const T* __restrict__ gres, T* __restrict__ dx, float* __restrict__ partial, int rows, int D, int warps) {
+           const T* __restrict__ gres, T* __restrict__ dx, float* __restrict__ partial, int rows, int D, int warps, int classes) {
   const int W = W16 ? 16 : warps;
   constexpr int N = Of<T>::N, NT = RES ? 3 : 2;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float red_all[2][16][2 * R];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, grp = warp / W, wid = warp - grp * W, gl = wid * 32 + lane;
-  const int nv = D / N, G = (blockDim.x >> 5) / W, units = (rows + R - 1) / R;
+  const int G = (blockDim.x >> 5) / W, group = blockIdx.x * G + grp, groups = gridDim.x * G;
+  const int cls = SHIFT ? group % classes : 0;
+  const Cut<T> cut(cls, D);
+  const int nv = SHIFT ? cut.nv : D / N, head = SHIFT ? cut.head : 0;
+  const int live_rows = SHIFT ? (rows - cls + classes - 1) / classes : rows, units = (live_rows + R - 1) / R;
+  auto row_of = [&](int i) { return SHIFT ? cls + i * classes : i; };
+  const int sc = SHIFT && wid == 0 ? cut.single(lane) : -1;
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + threadIdx.x * 16, part = blockDim.x * 16;
   auto slot = [&](int s, int r, int t, int v) { return ring + (((s * R + r) * NT + t) * V + v) * part; };
   auto fetch = [&](int u, int s) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int row = u * R + r;
-      if (u < units && row < rows) {
+      const int i = u * R + r;
+      if (u < units && i < live_rows) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           if (gl + 32 * W * v < nv) {
-            const size_t o = (size_t)row * D + (gl + 32 * W * v) * N;
+            const size_t o = (size_t)row_of(i) * D + head + (gl + 32 * W * v) * N;
             copy16(slot(s, r, 0, v), x + o);
             copy16(slot(s, r, 1, v), dy + o);
             if (RES) copy16(slot(s, r, 2, v), gres + o);
@@ -262,23 +363,46 @@ bwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict
   };
   constexpr int M = N / 2;
   f2 wf[V][M], dwa[V][M], dba[V][M];
-  const int step = gridDim.x * G;
-  int u = blockIdx.x * G + grp;
+  const int step = SHIFT ? (groups - cls + classes - 1) / classes : groups;
+  int u = SHIFT ? group / classes : group;
 #pragma unroll
   for (int s = 0; s < S; ++s) fetch(u + s * step, s);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int i = gl + 32 * W * v;
-    get2<T>(i < nv ? reinterpret_cast<const uint4*>(w)[i] : make_uint4(0, 0, 0, 0), wf[v]);
+    if (SHIFT) {
+#pragma unroll
+      for (int j = 0; j < M; ++j) {
+        const int c = head + i * N + 2 * j;
+        wf[v][j] = i < nv ? f2_pack(Of<T>::one(w[c]), Of<T>::one(w[c + 1])) : f2(0);
+      }
+    } else {
+      get2<T>(i < nv ? reinterpret_cast<const uint4*>(w)[i] : make_uint4(0, 0, 0, 0), wf[v]);
+    }
 #pragma unroll
     for (int j = 0; j < M; ++j) dwa[v][j] = dba[v][j] = 0;
   }
   auto row_stats = [&](int un, float2 (&st)[R]) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) st[r] = un < units && un * R + r < rows ? stats[un * R + r] : make_float2(0.f, 0.f);
+    for (int r = 0; r < R; ++r) st[r] = un < units && un * R + r < live_rows ? stats[row_of(un * R + r)] : make_float2(0.f, 0.f);
   };
   float2 next[R];                                        // of the next rows: as far away as they are
   row_stats(u, next);
+  const float ws = SHIFT && sc >= 0 ? Of<T>::one(w[sc]) : 0.f;
+  float dws = 0.f, dbs = 0.f;                            // a lane's single column
+  T sx[R], sg[R], sr[R];
+  auto singles = [&](int un) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      sx[r] = sg[r] = sr[r] = Of<T>::from(0.f);
+      if (SHIFT && sc >= 0 && un < units && un * R + r < live_rows) {
+        const size_t o = (size_t)row_of(un * R + r) * D + sc;
+        sx[r] = x[o]; sg[r] = dy[o];
+        if (RES) sr[r] = gres[o];
+      }
+    }
+  };
+  if (SHIFT) singles(u);
   const float inv = 1.f / D;
   int s = 0;
   for (int it = 0; u < units; u += step, ++it) {
@@ -295,7 +419,7 @@ bwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict
     float sums[2 * R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const bool live = u * R + r < rows;
+      const bool live = u * R + r < live_rows;
       f2 a = 0, c = 0;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
@@ -314,11 +438,18 @@ bwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict
       }
       const float2 ta = f2_unpack(a), tc = f2_unpack(c);
       sums[2 * r] = ta.x + ta.y; sums[2 * r + 1] = tc.x + tc.y;
+      if (SHIFT && sc >= 0 && live) {
+        const float xh = fmaf(Of<T>::one(sx[r]), rstd[r], f2_unpack(off[r]).x), gf = Of<T>::one(sg[r]);
+        dws = fmaf(gf, xh, dws);
+        dbs += gf;
+        sums[2 * r] = fmaf(gf, ws, sums[2 * r]);
+        sums[2 * r + 1] = fmaf(gf * ws, xh, sums[2 * r + 1]);
+      }
     }
     group_sums<R, W16>(sums, &red_all[it & 1][grp * W][0], W, 1 + grp, wid, lane);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (u * R + r >= rows) break;
+      if (u * R + r >= live_rows) break;
       const float k1 = -rstd[r] * (sums[2 * r] * inv), k2 = -rstd[r] * (sums[2 * r + 1] * inv);
       const f2 c1 = f2_pack(k1, k1), c2 = f2_pack(k2, k2);
 #pragma unroll
@@ -335,10 +466,15 @@ bwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict
 #pragma unroll
             for (int j = 0; j < M; ++j) xf[j] = f2_add(xf[j], gf[j]);
           }
-          reinterpret_cast<uint4*>(dx + (size_t)(u * R + r) * D)[i] = put2<T>(xf);
+          reinterpret_cast<uint4*>(dx + (size_t)row_of(u * R + r) * D + head)[i] = put2<T>(xf);
         }
       }
+      if (SHIFT && sc >= 0) {
+        const float xh = fmaf(Of<T>::one(sx[r]), rstd[r], f2_unpack(off[r]).x);
+        dx[(size_t)row_of(u * R + r) * D + sc] = Of<T>::from(fmaf(xh, k2, fmaf(Of<T>::one(sg[r]) * ws, rstd[r], k1)) + Of<T>::one(sr[r]));
+      }
     }
+    if (SHIFT) singles(u + step);
     fetch(u + S * step, s);                              // this thread has read the slot that it fills again
     if (++s == S) s = 0;
   }
@@ -352,11 +488,14 @@ bwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict
       if (i < nv) {
 #pragma unroll
         for (int j = 0; j < M; ++j) {
-          reinterpret_cast<float2*>(dst + i * N)[j] = f2_unpack(dwa[v][j]);
-          reinterpret_cast<float2*>(dst + D + i * N)[j] = f2_unpack(dba[v][j]);
+          const float2 pw = f2_unpack(dwa[v][j]), pb = f2_unpack(dba[v][j]);
+          const int c = head + i * N + 2 * j;
+          if (SHIFT) { dst[c] = pw.x; dst[c + 1] = pw.y; dst[D + c] = pb.x; dst[D + c + 1] = pb.y; }
+          else { *reinterpret_cast<float2*>(dst + c) = pw; *reinterpret_cast<float2*>(dst + D + c) = pb; }
         }
       }
     }
+    if (SHIFT && sc >= 0) { dst[sc] = dws; dst[D + sc] = dbs; }
   };
   if (G == 1) { put_sums(out); return; }
   __syncthreads();
@@ -370,8 +509,7 @@ bwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict
   }
 }
 
-// Widths that 16-byte vectors do not divide, and rows off a 16-byte boundary: a block per row, V single values a thread, the next row's on
-// their way while this one is summed.
+// Tensors off a 16-byte boundary: a block per row, V single values a thread, the next row's on their way while this one is summed.
 template <class T, int V>
 __global__ void __launch_bounds__(V > 8 ? 1024 : 256)
 bwd_any_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict__ dy, const float2* __restrict__ stats,
@@ -455,12 +593,12 @@ reduce_kernel(const float* partial, T* dw, T* db, int nblk, int D) {
 }
 
 // ------------------------------------------------------------------------------------ launchers
-constexpr int MAX_D = 16384;
+constexpr int MAX_D = 16384, MAX_ROWS = 1 << 30;
 
-template <class T, int VEC, int V, int W>
+template <class T, int VEC, int V, int W, bool SHIFT = false>
 static int launch_fwd(const void* x, const void* w, const void* b, void* y, float* stats, int rows, int D, float eps, cudaStream_t st) {
   const int per = fwd_rows(W);
-  fwd_kernel<T, VEC, V, W><<<(rows + per - 1) / per, 32 * W * per, 0, st>>>((const T*)x, (const T*)w, (const T*)b, (T*)y, (float2*)stats, rows, D, eps);
+  fwd_kernel<T, VEC, V, W, SHIFT><<<(rows + per - 1) / per, 32 * W * per, 0, st>>>((const T*)x, (const T*)w, (const T*)b, (T*)y, (float2*)stats, rows, D, eps);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
@@ -484,6 +622,12 @@ static int forward(const void* x, const void* w, const void* b, void* y, float* 
     if (lanes <= 256) LN_FWD(8, 32);
     LN_FWD(16, 32);
   } else {
+    if (D / VEC <= 16) {
+      auto* kernel = D / VEC <= 8 ? fwd_narrow_kernel<T, 8> : fwd_narrow_kernel<T, 16>;
+      const int per = D / VEC <= 8 ? 32 : 16;
+      kernel<<<(rows + per - 1) / per, 256, 0, st>>>((const T*)x, (const T*)w, (const T*)b, (T*)y, (float2*)stats, rows, D, eps);
+      return cudaGetLastError() == cudaSuccess ? 0 : -2;
+    }
     if (lanes <= 1) LN_FWD(1, 1);
     if (lanes <= 2) { if (per_sm <= 4) LN_FWD(1, 2); LN_FWD(2, 1); }
     if (lanes <= 4) { if (per_sm <= 7) LN_FWD(1, 4); LN_FWD(4, 1); }
@@ -496,17 +640,19 @@ static int forward(const void* x, const void* w, const void* b, void* y, float* 
 #undef LN_FWD
 }
 
-struct Plan { int W, V, threads, grid; };
-// Backward by vectors: `n` values a vector
+struct Plan { int W, V, threads, grid, classes; };
+// Groups of warps a row by vectors of n values.
 static Plan plan_vec(int rows, int D, int n) {
-  const int lanes = (D / n + 31) / 32;                   // 1 .. 128
   Plan p;
+  p.classes = D % n == 0 ? 1 : D % 2 ? n : D % 4 ? n / 2 : 2;
+  const int lanes = D < n ? 1 : (D / n + 31) / 32;       // 1 .. 128
   p.V = lanes <= 16 ? 1 : lanes <= 32 ? 2 : lanes <= 64 ? 4 : 8;
   p.W = p.V == 1 ? lanes : 16;
   const int G = p.V == 1 ? 16 / p.W : 1, R = p.V <= 2 ? 2 : 1;
   p.threads = 32 * p.W * G;
-  const int units = (rows + R - 1) / R, blocks = (units + G - 1) / G, most = (p.V == 1 ? 2 : 1) * num_sms();
+  const int units = (rows + R - 1) / R, blocks = (units + G - 1) / G, most = (p.V == 1 ? 2 : 1) * num_sms(), least = (p.classes + G - 1) / G;
   p.grid = blocks < most ? blocks : most;
+  if (p.grid < least) p.grid = least;                    // a group for every class
   return p;
 }
 static Plan plan_any(int rows, int D) {
@@ -520,13 +666,28 @@ static Plan plan_any(int rows, int D) {
   return p;
 }
 
-template <class T, int V, int R, int S, bool RES, bool W16>
+template <class T>
+static int forward_shift(const void* x, const void* w, const void* b, void* y, float* stats, int rows, int D, float eps, cudaStream_t st) {
+  constexpr int N = Of<T>::N;
+  const int lanes = (D / N + 31) / 32;
+#define LN_FWD(V, W) if (lanes <= V * W) return launch_fwd<T, N, V, W, true>(x, w, b, y, stats, rows, D, eps, st)
+  LN_FWD(1, 1); LN_FWD(2, 1); LN_FWD(3, 1); LN_FWD(4, 1);
+  LN_FWD(3, 2); LN_FWD(4, 2);
+  LN_FWD(3, 4); LN_FWD(4, 4);
+  LN_FWD(3, 8); LN_FWD(4, 8);
+  LN_FWD(3, 16); LN_FWD(4, 16);
+  if constexpr (N == 4) LN_FWD(8, 16);
+#undef LN_FWD
+  return -3;
+}
+
+template <class T, int V, int R, int S, bool RES, bool W16, bool SHIFT>
 static int launch_bwd(const Plan& p, const void* x, const void* w, const void* dy, const float* stats, const void* gres, void* dx, float* partial,
                       int rows, int D, cudaStream_t st) {
   const int ring = S * R * (RES ? 3 : 2) * V * p.threads * 16;
-  if (ring > 40 * 1024 && cudaFuncSetAttribute(bwd_kernel<T, V, R, S, RES, W16>, cudaFuncAttributeMaxDynamicSharedMemorySize, ring) != cudaSuccess) return -2;
-  bwd_kernel<T, V, R, S, RES, W16><<<p.grid, p.threads, ring, st>>>((const T*)x, (const T*)w, (const T*)dy, (const float2*)stats, (const T*)gres, (T*)dx,
-                                                               partial, rows, D, p.W);
+  if (ring > 40 * 1024 && cudaFuncSetAttribute(bwd_kernel<T, V, R, S, RES, W16, SHIFT>, cudaFuncAttributeMaxDynamicSharedMemorySize, ring) != cudaSuccess) return -2;
+  bwd_kernel<T, V, R, S, RES, W16, SHIFT><<<p.grid, p.threads, ring, st>>>((const T*)x, (const T*)w, (const T*)dy, (const float2*)stats, (const T*)gres, (T*)dx,
+                                                               partial, rows, D, p.W, p.classes);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
@@ -535,8 +696,10 @@ static int backward(const void* x, const void* w, const void* dy, const float* s
                     int rows, int D, bool vec, cudaStream_t st) {
   const Plan p = vec ? plan_vec(rows, D, Of<T>::N) : plan_any(rows, D);
   int rc = 0;
-#define LN_BWD(V, R, S, W16) rc = gres ? launch_bwd<T, V, R, S, true, W16>(p, x, w, dy, stats, gres, dx, partial, rows, D, st) \
-                                       : launch_bwd<T, V, R, S, false, W16>(p, x, w, dy, stats, gres, dx, partial, rows, D, st)
+#define LN_ARGS p, x, w, dy, stats, gres, dx, partial, rows, D, st
+#define LN_BWD(V, R, S, W16)                                                                                                              \
+  rc = p.classes == 1 ? (gres ? launch_bwd<T, V, R, S, true, W16, false>(LN_ARGS) : launch_bwd<T, V, R, S, false, W16, false>(LN_ARGS)) \
+                      : (gres ? launch_bwd<T, V, R, S, true, W16, true>(LN_ARGS) : launch_bwd<T, V, R, S, false, W16, true>(LN_ARGS))
 #define LN_ANY(V) bwd_any_kernel<T, V><<<p.grid, p.threads, 0, st>>>((const T*)x, (const T*)w, (const T*)dy, (const float2*)stats, (const T*)gres, \
                                                                      (T*)dx, partial, rows, D)
   if (rows > 0) {
@@ -546,7 +709,7 @@ static int backward(const void* x, const void* w, const void* dy, const float* s
       else if (p.V == 2) LN_BWD(2, 2, 2, true);
       else if (p.V == 4) LN_BWD(4, 1, 2, true);
       else if constexpr (Of<T>::N == 4) LN_BWD(8, 1, 1, true);
-      else rc = -3;
+      else return -3;
       if (rc) return rc;
     } else {
       if (p.V == 2) LN_ANY(2);
@@ -556,6 +719,7 @@ static int backward(const void* x, const void* w, const void* dy, const float* s
       if (cudaGetLastError() != cudaSuccess) return -2;
     }
   }
+#undef LN_ARGS
 #undef LN_BWD
 #undef LN_ANY
   return launch_chained(false, reduce_kernel<T>, dim3((2 * D + 31) / 32), 1024, 0, st, (const float*)partial, (T*)dw, (T*)db, rows > 0 ? p.grid : 0, D);
@@ -575,9 +739,13 @@ using namespace sb::ln;
 // x, y [rows, D], w and b [D] of one type (0: bf16, 1: fp16, 2: fp32); stats [rows, 2] fp32 (mean, rstd) for the backward, or null.
 extern "C" int sb_layernorm_fwd(const void* x, const void* w, const void* b, void* y, float* stats, int rows, int D, float eps, int type,
                                 cudaStream_t st) {
-  if (D < 1 || D > MAX_D || rows < 0 || type < 0 || type > 2) return -1;
+  if (D < 1 || D > MAX_D || rows < 0 || rows > MAX_ROWS || type < 0 || type > 2) return -1;
   if (rows == 0) return 0;
-  const bool vec = D % (type == 2 ? 4 : 8) == 0 && on16({x, w, b, y});
+  const int n = type == 2 ? 4 : 8;
+  const bool vec = D % n == 0 && on16({x, w, b, y}), shift = D % n != 0 && on16({x, w, b, y});
+  if (shift) return type == 0   ? forward_shift<bf16>(x, w, b, y, stats, rows, D, eps, st)
+                    : type == 1 ? forward_shift<__half>(x, w, b, y, stats, rows, D, eps, st)
+                                : forward_shift<float>(x, w, b, y, stats, rows, D, eps, st);
   if (type == 0) return vec ? forward<bf16, 8>(x, w, b, y, stats, rows, D, eps, st) : forward<bf16, 1>(x, w, b, y, stats, rows, D, eps, st);
   if (type == 1) return vec ? forward<__half, 8>(x, w, b, y, stats, rows, D, eps, st) : forward<__half, 1>(x, w, b, y, stats, rows, D, eps, st);
   return vec ? forward<float, 4>(x, w, b, y, stats, rows, D, eps, st) : forward<float, 1>(x, w, b, y, stats, rows, D, eps, st);
@@ -586,16 +754,16 @@ extern "C" int sb_layernorm_fwd(const void* x, const void* w, const void* b, voi
 // Rows of 2 D floats that sb_layernorm_bwd needs as scratch.
 extern "C" int sb_layernorm_bwd_blocks(int rows, int D, int type) {
   if (rows <= 0 || D < 1) return 1;
-  const int n = type == 2 ? 4 : 8, any = plan_any(rows, D).grid;
-  const int vec = D % n == 0 ? plan_vec(rows, D, n).grid : 0;
+  const int n = type == 2 ? 4 : 8, any = plan_any(rows, D).grid, vec = plan_vec(rows, D, n).grid;
   return vec > any ? vec : any;
 }
 
 // dx [rows, D] (gres, the gradient that came along the residual branch, added; may be null), dw and db [D], written.  Two launches.
 extern "C" int sb_layernorm_bwd(const void* x, const void* w, const void* dy, const float* stats, const void* gres, void* dx, void* dw, void* db,
                                 float* partial, int rows, int D, int type, cudaStream_t st) {
-  if (D < 1 || D > MAX_D || rows < 0 || type < 0 || type > 2) return -1;
-  const bool vec = D % (type == 2 ? 4 : 8) == 0 && on16({x, w, dy, gres, dx});
+  if (D < 1 || D > MAX_D || rows < 0 || rows > MAX_ROWS || type < 0 || type > 2) return -1;
+  const int n = type == 2 ? 4 : 8;
+  const bool vec = on16({x, dy, gres, dx}) && (D % n || on16({w}));
   if (type == 0) return backward<bf16>(x, w, dy, stats, gres, dx, dw, db, partial, rows, D, vec, st);
   if (type == 1) return backward<__half>(x, w, dy, stats, gres, dx, dw, db, partial, rows, D, vec, st);
   return backward<float>(x, w, dy, stats, gres, dx, dw, db, partial, rows, D, vec, st);

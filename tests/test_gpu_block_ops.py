@@ -74,7 +74,7 @@ def _norm_exact(x, w, b, gy, gr, eps, dtype):
     return out
 
 
-WIDTHS = [1, 3, 8, 33, 64, 100, 136, 256, 257, 1000, 1024, 1027, 2048, 2056, 4096, 4104, 5001, 8192, 12000, 16383, 16384]
+WIDTHS = [1, 2, 3, 4, 6, 8, 12, 33, 64, 100, 136, 256, 257, 1000, 1024, 1027, 2048, 2056, 4096, 4104, 5001, 8191, 8192, 8196, 12000, 12001, 16370, 16372, 16383, 16384]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=["bf16", "fp16", "fp32"])
@@ -292,3 +292,24 @@ def test_values_halfway_between_two_codes_go_to_the_even_one():
     for dtype in (torch.float16, torch.float32):
         q, scale = ops.act_quantize(x.to(dtype).view(1, 384))
         assert torch.equal(scale, torch.ones_like(scale)) and torch.equal(q[0].float(), torch.round(x))
+
+
+@pytest.mark.parametrize("D", [33, 100, 1027, 4095])
+def test_layernorm_of_odd_widths_leaves_neighbours_alone(D):
+    """A row of NaN between others, and nothing written outside: vectors reach into the rows before and behind."""
+    from savanna_b200.ops import cuda_ops
+    for rows in (1, 3, 40):
+        x, w, b, gy, gr = _norm_case(rows, D, torch.bfloat16, seed=rows)
+        want = _norm_exact(x, w, b, gy, gr, 1e-5, torch.bfloat16)
+        bad = rows // 2
+        x[bad], gy[bad], gr[bad] = float("nan"), float("inf"), float("nan")
+        leaves = [t.requires_grad_(True) for t in (x, w, b)]
+        with cuda_ops.guarded_allocations():
+            y, xr = ops.layernorm_residual(*leaves, 1e-5)
+            dx, dw, db = torch.autograd.grad((y, xr), leaves, (gy, gr))
+            assert cuda_ops.check_guards() >= 5
+        keep = torch.arange(rows, device=DEV) != bad
+        for name, v in (("y", y.detach()), ("dx", dx)):
+            assert bool(v[bad].isnan().all())
+            _inside(v[keep], want[name][0][keep], want[name][1][keep], name)
+        assert bool(dw.isnan().all())
