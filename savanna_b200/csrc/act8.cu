@@ -6,8 +6,8 @@
 // infinity: a block that holds one of them has a scale of NaN and comes back as NaN, so that an overflow stays visible.  A block below 1e-30
 // comes back as nearly zero.
 //
-// Bound by memory: 2 + 1 bytes a value for 16-bit types, one pass; a lane has four 16-byte loads on their way.  8192 x 4096 bf16: 20.5 us there and
-// 19.7 back (a copy of as many bytes takes 15.5).
+// Bound by memory: 2 + 1 bytes a value for 16-bit types, one pass; a lane has two 16-byte loads on their way.  8192 x 4096 bf16: 18.6 us there and
+// 20.2 back (a copy of as many bytes takes 15.5); four loads a lane 19.0 and 24.2, eight 20.4 and 24.1.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -200,7 +200,7 @@ dequantize_any_kernel(const int8_t* __restrict__ q, const float* __restrict__ sc
 
 template <class T>
 static int quantize(const void* x, void* q, float* scale, long long rows, int D, bool vec, cudaStream_t st) {
-  constexpr int U = sizeof(T) == 4 ? 2 : 4;
+  constexpr int U = 2;
   const Rows r{(uint32_t)((D + BLOCK - 1) / BLOCK), (uint32_t)D};
   const long long blocks = rows * r.per_row, per = vec ? 16 * U : 8, grid = (blocks + per - 1) / per;
   if (grid > 0x7fffffffLL) return -1;
@@ -211,7 +211,7 @@ static int quantize(const void* x, void* q, float* scale, long long rows, int D,
 }
 template <class T>
 static int dequantize(const void* q, const float* scale, void* x, long long rows, int D, bool vec, cudaStream_t st) {
-  constexpr int U = 4;
+  constexpr int U = 2;
   const Rows r{(uint32_t)((D + BLOCK - 1) / BLOCK), (uint32_t)D};
   const bool wide = vec && D % BLOCK == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
   const long long blocks = rows * r.per_row, per = wide ? 32 * U : vec ? 16 * U : 8, grid = (blocks + per - 1) / per;

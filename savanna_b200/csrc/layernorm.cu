@@ -396,7 +396,7 @@ bwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict
     for (int r = 0; r < R; ++r) {
       sx[r] = sg[r] = sr[r] = Of<T>::from(0.f);
       if (SHIFT && sc >= 0 && un < units && un * R + r < live_rows) {
-        const size_t o = (size_t)row_of(un * R + r) * D + sc;
+        const size_t o = (size_t)row_of(un * R + r) * D + (unsigned)sc;
         sx[r] = x[o]; sg[r] = dy[o];
         if (RES) sr[r] = gres[o];
       }
@@ -471,7 +471,7 @@ bwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict
       }
       if (SHIFT && sc >= 0) {
         const float xh = fmaf(Of<T>::one(sx[r]), rstd[r], f2_unpack(off[r]).x);
-        dx[(size_t)row_of(u * R + r) * D + sc] = Of<T>::from(fmaf(xh, k2, fmaf(Of<T>::one(sg[r]) * ws, rstd[r], k1)) + Of<T>::one(sr[r]));
+        dx[(size_t)row_of(u * R + r) * D + (unsigned)sc] = Of<T>::from(fmaf(xh, k2, fmaf(Of<T>::one(sg[r]) * ws, rstd[r], k1)) + Of<T>::one(sr[r]));
       }
     }
     if (SHIFT) singles(u + step);
