@@ -13,14 +13,17 @@
 
 #include <atomic>
 #include <cmath>
+#include <limits>
 #include <mutex>
 #include <sstream>
 
+#include <ATen/autocast_mode.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime_api.h>
 #include <nvtx3/nvToolsExt.h>
+#include <torch/csrc/autograd/autograd.h>
 #include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
@@ -170,9 +173,18 @@ unsigned int* status_word(at::Device device) {
 }
 
 // The functions of this file know nothing of functorch's wrappers (forward-mode tangents are refused by Function::apply itself).
+bool in_transform() { return c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode); }
 void no_transforms() {
-  TORCH_CHECK(!c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode),
+  TORCH_CHECK(!in_transform(),
               "the CUDA operators of savanna_b200 do not support functorch transforms (vmap, grad, jvp)");
+}
+
+// functorch's transforms or forward-mode tangents: operators that have a form in PyTorch's own operations beside them leave it to that
+bool differs_forward(std::initializer_list<const Tensor*> ts) {
+  if (in_transform()) return true;
+  for (const Tensor* t : ts)
+    if (t->_fw_grad(0).defined()) return true;
+  return false;
 }
 
 // ------------------------------------------------------------------------------------ GEMM
@@ -362,8 +374,7 @@ LnForward layernorm_fwd(const Tensor& x, const Tensor& w, const Tensor& b, doubl
 struct LayerNorm : Function<LayerNorm> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& b, double eps, bool residual) {
     LnForward n = layernorm_fwd(x, w, b, eps, true);
-    ctx->save_for_backward({n.x2, n.w, n.stats});
-    if (x.dim() != 2) ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->save_for_backward({x, w, b, n.stats});          // as they came: a second derivative goes on from them
     ctx->set_materialize_grads(false);
     if (residual) return {n.y, x.view_as(x)};
     return {n.y};
@@ -372,20 +383,29 @@ struct LayerNorm : Function<LayerNorm> {
     const Tensor gres = g.size() > 1 ? g[1] : Tensor();
     if (!g[0].defined()) return {gres, Tensor(), Tensor(), Tensor(), Tensor()};
     const variable_list s = ctx->get_saved_variables();
-    const Tensor &x2 = s[0], &w = s[1], &st = s[2];
-    const int64_t T = x2.size(0), D = x2.size(1);
+    const Tensor &x = s[0], &st = s[3];
+    const int64_t D = x.size(-1);
+    if (at::GradMode::is_enabled()) {                    // create_graph: PyTorch's backward, which has a derivative of its own
+      std::vector<int64_t> per_row = x.sizes().vec();
+      per_row.back() = 1;
+      const Tensor mean = st.select(1, 0).contiguous().view(per_row), rstd = st.select(1, 1).contiguous().view(per_row);
+      auto d = at::native_layer_norm_backward(g[0], x, {D}, mean, rstd, s[1], s[2], {true, true, true});
+      const Tensor dx = std::get<0>(d);
+      return {gres.defined() ? dx + gres : dx, std::get<1>(d), std::get<2>(d), Tensor(), Tensor()};
+    }
+    const Tensor x2 = rows_contiguous(x), w = contiguous(s[1]);
+    const int64_t T = x2.size(0);
     const int type = type_code(x2.scalar_type());
     Tensor g2 = contiguous(g[0].reshape({T, D})), r2 = gres.defined() ? contiguous(gres.reshape({T, D})) : Tensor();
     Tensor dx = alloc_like(x2), dw = alloc({D}, x2.scalar_type(), x2.device()), db = alloc_like(dw),
            partial = alloc({(int64_t)L.sb_layernorm_bwd_blocks(T, D, type) * 2 * D}, F32, x2.device());
     SB_CALL(sb_layernorm_bwd, T > 0 ? 2 : 1, ptr(x2), ptr(w), ptr(g2), f32(st), ptr(r2), out(dx), out(dw), out(db), f32o(partial), (int)T, (int)D,
             type, stream());
-    const auto shape = ctx->saved_data.find("shape");
-    if (shape != ctx->saved_data.end()) dx = dx.view(shape->second.toIntVector());
-    return {dx, dw, db, Tensor(), Tensor()};
+    return {x.dim() == 2 ? dx : dx.view(x.sizes()), dw, db, Tensor(), Tensor()};
   }
 };
-// The kernels' part of layer norms: one type, up to 2^30 rows of up to 16384 values.  Shapes that make no sense are refused.
+// The kernels' part of layer norms: one type, up to 2^30 rows of up to 16384 values, outside of autocast (which wants fp32), functorch's transforms and
+// forward-mode differentiation.  Shapes that make no sense are refused.
 bool layernorm_covers(const Tensor& x, const Tensor& w, const Tensor& b) {
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "layernorm takes [..., D] with D >= 1, got ", x.sizes());
   const int64_t D = x.size(-1);
@@ -393,7 +413,7 @@ bool layernorm_covers(const Tensor& x, const Tensor& w, const Tensor& b) {
                     " for rows of ", D, " values");
   const at::ScalarType t = x.scalar_type();
   return (t == BF16 || t == at::kHalf || t == F32) && w.scalar_type() == t && b.scalar_type() == t && D <= 16384 && x.numel() / D <= (1LL << 30) &&
-         w.device() == x.device() && b.device() == x.device();
+         w.device() == x.device() && b.device() == x.device() && !at::autocast::is_autocast_enabled(at::kCUDA) && !differs_forward({&x, &w, &b});
 }
 
 // (linear(norm(x)), x) as one node
@@ -755,18 +775,40 @@ RpeForward rpe_fwd(const Tensor& qkv, const Tensor& table, const Tensor& buckets
               layouts({{"q", &q}, {"k", &k}, {"v", &v}, {"table", &f.table}, {"buckets", &f.buckets}}));
   return f;
 }
+// The same by elementary operations, scores materialised: what a second derivative goes through.
+Tensor rpe_statement(const Tensor& qkv, const Tensor& table, const Tensor& buckets, double bias_scale, bool causal) {
+  const int64_t Ln = qkv.size(1), far = causal ? buckets.size(0) - 1 : buckets.size(0) / 2;
+  const Tensor f = qkv.to(F32).transpose(1, 2), i = at::arange(Ln, buckets.options().dtype(at::kLong)), d = i.unsqueeze(1) - i.unsqueeze(0);
+  const Tensor at_ = causal ? d.clamp(0, far) : d.clamp(-far, far) + far, b = buckets.to(at::kLong).index({at_});
+  const Tensor valid = (b >= 0).logical_and(b < table.size(0));
+  Tensor bias = table.to(F32).index({b.clamp(0, table.size(0) - 1)}) * bias_scale;
+  bias = at::where(valid.unsqueeze(-1), bias, at::zeros({}, bias.options())).permute({2, 0, 1});
+  Tensor s = at::matmul(f.slice(3, 0, 128), f.slice(3, 128, 256).transpose(2, 3)) * 0.08838834764831845 + bias;
+  if (causal) s = s.masked_fill(d < 0, -std::numeric_limits<double>::infinity());
+  return at::matmul(at::softmax(s, -1), f.slice(3, 256, 384)).transpose(1, 2).to(BF16);
+}
 struct FlashRpe : Function<FlashRpe> {
   static Tensor forward(AutogradContext* ctx, const Tensor& qkv, const Tensor& table, const Tensor& buckets, double bias_scale, bool causal) {
     RpeForward f = rpe_fwd(qkv, table, buckets, bias_scale, causal, true);
-    ctx->save_for_backward({qkv, f.table, f.buckets, f.o, f.lo, f.lse});
+    ctx->save_for_backward({qkv, table, f.buckets, f.o, f.lo, f.lse});
     ctx->saved_data["bias_scale"] = bias_scale;
     ctx->saved_data["causal"] = causal;
     return f.o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const variable_list s = ctx->get_saved_variables();
-    const Tensor &qkv = s[0], &table = s[1], &buckets = s[2], &o = s[3], &lo = s[4], &lse = s[5];
+    const Tensor &qkv = s[0], &buckets = s[2], &o = s[3], &lo = s[4], &lse = s[5];
     const bool causal = ctx->saved_data["causal"].toBool();
+    if (at::GradMode::is_enabled()) {                    // create_graph
+      const Tensor again = rpe_statement(qkv, s[1], buckets, ctx->saved_data["bias_scale"].toDouble(), causal);
+      variable_list wanted;
+      for (const Tensor* t : {&s[0], &s[1]})
+        if (t->requires_grad()) wanted.push_back(*t);
+      variable_list d = torch::autograd::grad({again}, wanted, {g[0]}, true, true);
+      Tensor none;
+      return {s[0].requires_grad() ? d.front() : none, s[1].requires_grad() ? d.back() : none, none, none, none};
+    }
+    const Tensor table = contiguous(s[1]);
     const int64_t B = qkv.size(0), Ln = qkv.size(1), H = qkv.size(2), far = causal ? buckets.size(0) - 1 : buckets.size(0) / 2;
     const at::Device dev = qkv.device();
     Tensor dqkv = alloc(qkv.sizes(), BF16, dev), dtable = alloc_like(table);
@@ -828,14 +870,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return std::make_tuple(r[0], r[1]);
   });
   m.def("layernorm", [](const Tensor& x, const Tensor& w, const Tensor& b, double eps) {
-    no_transforms();
     if (!layernorm_covers(x, w, b)) return at::layer_norm(x, {x.size(-1)}, w, b, eps);
     const c10::cuda::CUDAGuard device(x.device());
     if (!wants_grad({&x, &w, &b})) return layernorm_fwd(x, w, b, eps, false).y;
     return LayerNorm::apply(x, w, b, eps, false)[0];
   });
   m.def("layernorm_residual", [](const Tensor& x, const Tensor& w, const Tensor& b, double eps) {
-    no_transforms();
     if (!layernorm_covers(x, w, b)) return std::make_tuple(at::layer_norm(x, {x.size(-1)}, w, b, eps), x);
     const c10::cuda::CUDAGuard device(x.device());
     if (!wants_grad({&x, &w, &b})) return std::make_tuple(layernorm_fwd(x, w, b, eps, false).y, x);
@@ -901,7 +941,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   });
   // nothing where the kernels do not cover the shape
   m.def("attention_rpe", [](const Tensor& qkv, const Tensor& table, const Tensor& buckets, double bias_scale, bool causal, int64_t max_far) -> OptTensor {
-    no_transforms();
+    if (differs_forward({&qkv, &table})) return std::nullopt;
     TORCH_CHECK_VALUE(qkv.dim() == 4 && qkv.size(3) % 3 == 0 && qkv.size(3) > 0, "attention_rpe takes qkv [B, L, H, 3 * hd], got ", qkv.sizes());
     check_rpe(table, buckets, qkv.size(2), qkv.device(), causal);
     if (qkv.scalar_type() != BF16 || qkv.size(3) != 384 || !qkv.is_contiguous() || !on16(qkv) || qkv.size(0) >= 65535 || qkv.size(1) >= (1LL << 30) ||
@@ -914,7 +954,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   });
   m.def("attention_rpe_step", [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& buckets, double bias_scale,
                                  const OptTensor& lengths) -> OptTensor {
-    no_transforms();
+    if (differs_forward({&q, &k, &v, &table})) return std::nullopt;
     TORCH_CHECK_VALUE(q.dim() == 3 && k.dim() == 4 && k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(2) == q.size(1) && k.size(3) == q.size(2) &&
                       q.size(2) > 0, "attention_rpe_step takes q [B, H, hd], k and v [B, T, H, hd], got ", q.sizes(), ", ", k.sizes(), ", ", v.sizes());
     TORCH_CHECK_VALUE(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type() && k.device() == q.device() && v.device() == q.device(),

@@ -313,3 +313,38 @@ def test_layernorm_of_odd_widths_leaves_neighbours_alone(D):
             assert bool(v[bad].isnan().all())
             _inside(v[keep], want[name][0][keep], want[name][1][keep], name)
         assert bool(dw.isnan().all())
+
+
+@pytest.mark.parametrize("residual", [False, True])
+def test_layernorm_second_derivatives(residual):
+    g = _gen(4)
+    x, w, b = (torch.randn(*s, generator=g, device=DEV) for s in ((6, 40), (40,), (40,)))
+    r, q = torch.randn(6, 40, generator=g, device=DEV), torch.randn(6, 40, generator=g, device=DEV)
+
+    def second(f, t):
+        leaves = [v.clone().to(t).requires_grad_(True) for v in (x, w, b)]
+        y, xr = f(*leaves)
+        dx, dw, db = torch.autograd.grad((y * r.to(t)).sum() + (xr * xr).sum(), leaves, create_graph=True)
+        return torch.autograd.grad((dx * q.to(t)).sum() + (dw * dw).sum(), leaves, allow_unused=True)
+    plain = lambda x, w, b: (torch.nn.functional.layer_norm(x, (40,), w, b, 1e-5), x)  # noqa: E731
+    own = (lambda x, w, b: ops.layernorm_residual(x, w, b, 1e-5)) if residual else (lambda x, w, b: (ops.layernorm(x, w, b, 1e-5), x))
+    for a, c in zip(second(own, torch.float32), second(plain, torch.float64)):
+        if c is None or float(c.abs().max()) == 0:
+            assert a is None or float(a.abs().max()) <= 1e-3
+        else:                                        # 40-term sums of products of up to five factors in fp32: a few hundred roundings
+            assert float((a.double() - c).abs().max()) <= 1024 * U * float(c.abs().max()) * 8
+
+
+def test_layernorm_leaves_transforms_and_autocast_to_pytorch():
+    g = _gen(6)
+    x, w, b = torch.randn(4, 32, generator=g, device=DEV), torch.randn(32, generator=g, device=DEV), torch.randn(32, generator=g, device=DEV)
+    t = torch.randn(4, 32, generator=g, device=DEV)
+    f = lambda v: ops.layernorm(v, w, b, 1e-5)  # noqa: E731
+    p = lambda v: torch.nn.functional.layer_norm(v, (32,), w, b, 1e-5)  # noqa: E731
+    assert torch.allclose(torch.func.jvp(f, (x,), (t,))[1], torch.func.jvp(p, (x,), (t,))[1])
+    assert torch.allclose(torch.vmap(f)(x), p(x), atol=1e-5)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        assert f(x.to(torch.bfloat16).float()).dtype == p(x).dtype == torch.float32
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        h = [v.to(torch.bfloat16) for v in (x, w, b)]
+        assert ops.layernorm(*h, 1e-5).dtype == torch.nn.functional.layer_norm(h[0], (32,), h[1], h[2], 1e-5).dtype

@@ -276,3 +276,26 @@ def test_traced_on_new_inputs():
         return ops.attention_rpe(x, table, buckets, 2.0, True)
     traced = torch.jit.trace(f, qkv, check_trace=False)
     assert torch.equal(traced(other), f(other))
+
+
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "both"])
+def test_second_derivatives(causal):
+    """create_graph goes through elementary operations, whose gradients are those of the statement."""
+    qkv, table, buckets, go = _case(1, 20, 2, 32, 16, causal, table_dtype=torch.float32)
+
+    def second(f):
+        a, t = qkv.clone().requires_grad_(True), table.clone().requires_grad_(True)
+        ga, gt = torch.autograd.grad(f(a, t), (a, t), go, create_graph=True)
+        return torch.autograd.grad(ga.float().square().sum() + gt.square().sum(), (a, t))
+    got = second(lambda a, t: ops.attention_rpe(a, t, buckets, 2.0, causal))
+    want = second(lambda a, t: ref.attention_rpe(a, t, buckets, 2.0, causal))
+    for x, y in zip(got, want):                      # the same sums in another order, then bf16
+        assert (x.float() - y.float()).norm() <= 2 * H1 * y.float().norm()
+
+
+def test_forward_mode_runs_the_statement():
+    qkv, table, buckets, _ = _case(1, 12, 2, 32, 16, True, table_dtype=torch.float32)
+    t = torch.randn_like(table)
+    f = lambda v: ops.attention_rpe(qkv, v, buckets, 2.0, True)  # noqa: E731
+    p = lambda v: ref.attention_rpe(qkv, v, buckets, 2.0, True)  # noqa: E731
+    assert torch.equal(torch.func.jvp(f, (table,), (t,))[1], torch.func.jvp(p, (table,), (t,))[1])
