@@ -325,8 +325,8 @@ __device__ __forceinline__ void group_sums(float (&s)[2 * R], float* red, int wa
   for (int k = 0; k < P; ++k) s[k] = __shfl_sync(0xffffffffu, t, k * (32 / P));
 }
 
-template <class T, int V, int R, int S, bool RES, bool W16, bool SHIFT>
-__global__ void __launch_bounds__(BWD_THREADS, V == 1 ? 2 : 1)
+template <class T, int V, int R, int S, bool RES, bool W16, bool SHIFT, int THREADS>
+__global__ void __launch_bounds__(THREADS, V == 1 ? 2 : 1)
 bwd_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict__ dy, const float2* __restrict__ stats,
            const T* __restrict__ gres, T* __restrict__ dx, float* __restrict__ partial, int rows, int D, int warps, int classes) {
   const int W = W16 ? 16 : warps;
@@ -648,7 +648,7 @@ static Plan plan_vec(int rows, int D, int n) {
   const int lanes = D < n ? 1 : (D / n + 31) / 32;       // 1 .. 128
   p.V = lanes <= 16 ? 1 : lanes <= 32 ? 2 : lanes <= 64 ? 4 : 8;
   p.W = p.V == 1 ? lanes : 16;
-  const int G = p.V == 1 ? 16 / p.W : 1, R = p.V <= 2 ? 2 : 1;
+  const int G = p.V > 1 ? 1 : p.classes > 1 && p.W <= 12 ? 12 / p.W : 16 / p.W, R = p.V <= 2 ? 2 : 1;      // 384 threads have registers for the single values
   p.threads = 32 * p.W * G;
   const int units = (rows + R - 1) / R, blocks = (units + G - 1) / G, most = (p.V == 1 ? 2 : 1) * num_sms(), least = (p.classes + G - 1) / G;
   p.grid = blocks < most ? blocks : most;
@@ -681,12 +681,12 @@ static int forward_shift(const void* x, const void* w, const void* b, void* y, f
   return -3;
 }
 
-template <class T, int V, int R, int S, bool RES, bool W16, bool SHIFT>
+template <class T, int V, int R, int S, bool RES, bool W16, bool SHIFT, int THREADS = BWD_THREADS>
 static int launch_bwd(const Plan& p, const void* x, const void* w, const void* dy, const float* stats, const void* gres, void* dx, float* partial,
                       int rows, int D, cudaStream_t st) {
   const int ring = S * R * (RES ? 3 : 2) * V * p.threads * 16;
-  if (ring > 40 * 1024 && cudaFuncSetAttribute(bwd_kernel<T, V, R, S, RES, W16, SHIFT>, cudaFuncAttributeMaxDynamicSharedMemorySize, ring) != cudaSuccess) return -2;
-  bwd_kernel<T, V, R, S, RES, W16, SHIFT><<<p.grid, p.threads, ring, st>>>((const T*)x, (const T*)w, (const T*)dy, (const float2*)stats, (const T*)gres, (T*)dx,
+  if (ring > 40 * 1024 && cudaFuncSetAttribute(bwd_kernel<T, V, R, S, RES, W16, SHIFT, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, ring) != cudaSuccess) return -2;
+  bwd_kernel<T, V, R, S, RES, W16, SHIFT, THREADS><<<p.grid, p.threads, ring, st>>>((const T*)x, (const T*)w, (const T*)dy, (const float2*)stats, (const T*)gres, (T*)dx,
                                                                partial, rows, D, p.W, p.classes);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
@@ -705,6 +705,8 @@ static int backward(const void* x, const void* w, const void* dy, const float* s
   if (rows > 0) {
     if (vec) {
       if (p.V == 1 && p.W == 16) LN_BWD(1, 2, 2, true);
+      else if (p.V == 1 && p.threads <= 384 && p.classes > 1)
+        rc = gres ? launch_bwd<T, 1, 2, 2, true, false, true, 384>(LN_ARGS) : launch_bwd<T, 1, 2, 2, false, false, true, 384>(LN_ARGS);
       else if (p.V == 1) LN_BWD(1, 2, 2, false);
       else if (p.V == 2) LN_BWD(2, 2, 2, true);
       else if (p.V == 4) LN_BWD(4, 1, 2, true);
