@@ -178,7 +178,7 @@ step_kernel(const Args a) {
     float t = 0.f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) t += e[w] * wo[w][c];
-    if (a.splits == 1) out[c] = to(bl > 0.f ? t / bl : 0.f, T());
+    if (a.splits == 1) out[c] = to(bl == 0.f ? 0.f : t / bl, T());     // 0: no keys; NaN stays
     else if (blocks > 1) co[c] = t;
     else a.part[(long long)gridDim.z * a.H * a.splits * 2 + (row * a.splits + split) * a.hd + c] = t;
   }
@@ -202,7 +202,7 @@ step_kernel(const Args a) {
       float t = 0.f;
 #pragma unroll
       for (int r = 0; r < 8; ++r) if (r < blocks) t += pm[r] * *cluster.map_shared_rank(&co[c], r);
-      out[c] = to(tl > 0.f ? t / tl : 0.f, T());
+      out[c] = to(tl == 0.f ? 0.f : t / tl, T());
     }
   }
   cluster.sync();                          // the others' shared memory stays until it has been read
@@ -251,7 +251,7 @@ join_kernel(const float* part, T* out, long long rows, int splits, int hd) {
   __syncthreads();
   if (tid < cols) {
     for (int k = 1; k < groups; ++k) { t.x += sh[tid + k * cols].x; t.y += sh[tid + k * cols].y; }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
     T* dst = out + (long long)blockIdx.x * hd + 2 * tid;
     dst[0] = to(t.x * inv, T());
     dst[1] = to(t.y * inv, T());

@@ -316,7 +316,8 @@ def attention_rpe_step(q, k, v, table, buckets, scale, lengths=None):
     d = (n[:, None] - 1 - j[None, :]).clamp(0, buckets.shape[0] - 1)
     s = torch.einsum("bhd,bthd->bht", q.float(), k.float()) / math.sqrt(hd) + (table.float()[buckets.long()[d]] * scale).permute(0, 2, 1)
     s = s.masked_fill((j[None, :] >= n[:, None])[:, None], float("-inf"))
-    p = torch.nan_to_num(torch.exp(s - torch.logsumexp(s, dim=-1, keepdim=True)), nan=0.0)
+    total = torch.logsumexp(s, dim=-1, keepdim=True)
+    p = torch.exp(s - total).masked_fill(total == float("-inf"), 0.0)
     v = v.float().masked_fill((j[None, :] >= n[:, None])[..., None, None], 0.0)          # what lies behind the last key may be anything
     return torch.einsum("bht,bthd->bhd", p, v).to(q.dtype)
 

@@ -110,6 +110,14 @@ def test_attention_rpe_step_statement_is_the_last_row():
         assert float((got[0] - full[0, n - 1]).abs().max()) <= 64 * 2.0 ** -24 * 16 and float(got[1].abs().max()) == 0
 
 
+def test_attention_rpe_step_statement_keeps_nan_and_empties_rows_without_keys():
+    q, k, v = torch.randn(3, 2, 8), torch.randn(3, 5, 2, 8), torch.randn(3, 5, 2, 8)
+    q[1, 0, 0] = float("nan")
+    n = torch.tensor([0, 4, 5], dtype=torch.int32)
+    out = ops.attention_rpe_step(q, k, v, torch.randn(4, 2), torch.arange(4, dtype=torch.int32), 1.0, n)
+    assert float(out[0].abs().max()) == 0 and bool(out[1, 0].isnan().all()) and bool(out[1, 1].isfinite().all()) and bool(out[2].isfinite().all())
+
+
 def test_attention_rpe_step_refusals():
     qkv, table, buckets = _rpe_inputs(B=2)
     q, k, v = qkv.split(4, dim=-1)

@@ -81,6 +81,28 @@ def test_buckets_of_minus_infinity_may_empty_a_row():
     assert torch.equal(got, v[:, -1])
 
 
+@pytest.mark.parametrize("B,T,H", [(300, 40, 4), (2, 900, 2), (1, 9000, 2)], ids=["one block", "cluster", "two kernels"])
+@pytest.mark.parametrize("where", ["q", "k", "v", "overflow", "table"])
+def test_nan_stays_visible_in_its_row(B, T, H, where):
+    q, k, v, table, buckets, _ = _case(B, T, H, 64, torch.bfloat16, seed=7)
+    want = ops.attention_rpe_step(q, k, v, table, buckets, 1.0)
+    hit = torch.zeros(B, H, dtype=torch.bool, device=DEV)
+    if where == "table":
+        table[int(buckets[0]), 1] = float("nan")     # of the newest key
+        hit[:, 1] = True
+    else:
+        hit[-1, 1] = True
+        if where == "q":
+            q[-1, 1, 3] = float("nan")
+        elif where == "overflow":                    # a score of +inf: inf - inf in the softmax
+            q[-1, 1, 3], k[-1, T // 2, 1, 3] = 3e38, 3e38
+        else:
+            (k if where == "k" else v)[-1, T // 2, 1] = float("nan")
+    got = ops.attention_rpe_step(q, k, v, table, buckets, 1.0)
+    assert bool(got[hit].isnan().all())
+    assert torch.equal(got[~hit], want[~hit])
+
+
 def test_strided_caches_and_queries():
     g = torch.Generator(device=DEV).manual_seed(4)
     qkv = torch.randn(3, 2, 3 * 128, generator=g, device=DEV).to(torch.bfloat16)
