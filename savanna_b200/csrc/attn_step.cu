@@ -26,7 +26,7 @@ typedef __nv_bfloat16 bf16;
 
 constexpr int WARPS = 8, THREADS = 32 * WARPS;
 constexpr int U = 4;                     // keys of a group under way
-constexpr int MAX_HD = 256;
+constexpr int MAX_HD = 256, MAX_T = 1 << 30;             // indexes of keys run a little past T in 32 bits
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Args {
@@ -301,13 +301,13 @@ extern "C" int sb_attn_step_splits(int B, int H, int T) { return B < 1 || H < 1 
 
 // q [B, H, hd], k and v [B, T, H, hd] (type 0 bf16, 1 fp16; 16-byte boundaries, strides in elements multiples of 8, unit inner stride), out
 // [B, H, hd] contiguous.  lengths [B] int32 (clamped to 0 .. T) or null; table [nb, H] of table_type (0, 1 or 2: fp32), buckets [far + 1] int32
-// of the distances 0 .. far.
+// of the distances 0 .. far.  T <= 2^30.
 extern "C" int sb_attn_step(const void* q, const void* k, const void* v, void* out, const int* lengths, int B, int T, int H, int hd,
                             const long long* q_str, const long long* k_str, const long long* v_str, int type, const void* table, int table_type,
                             const int* buckets, int nb, int far, float scale, float bias_scale, float* part, int splits, cudaStream_t st) {
   if (hd < 8 || hd > MAX_HD || hd % 8 || nb < 1 || far < 0 || type < 0 || type > 1 || splits < 1 || splits > 8192 || (splits > 8 && !part)) return -1;
   if (splits != 1 && splits != 2 && splits != 4 && splits < 8) return -1;
-  if (B < 0 || H < 0 || T < 0 || B > 65535 || H > 65535) return -1;
+  if (B < 0 || H < 0 || T < 0 || T > MAX_T || B > 65535 || H > 65535) return -1;
   if (B == 0 || H == 0) return 0;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) return -4;
   if ((q_str[0] | q_str[1] | k_str[0] | k_str[1] | k_str[2] | v_str[0] | v_str[1] | v_str[2]) & 7) return -4;

@@ -969,7 +969,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       return t.stride(t.dim() - 1) == 1 && on16(t);
     };
     const bool half = q.scalar_type() == BF16 || q.scalar_type() == at::kHalf;
-    if (!half || hd % 8 || hd > 256 || B > 65535 || H > 65535 || T >= (1LL << 31) || wants_grad({&q, &k, &v, &table}) || !readable(q) || !readable(k) ||
+    if (!half || hd % 8 || hd > 256 || B > 65535 || H > 65535 || T > (1LL << 30) || wants_grad({&q, &k, &v, &table}) || !readable(q) || !readable(k) ||
         !readable(v))
       return std::nullopt;
     const c10::cuda::CUDAGuard device(q.device());

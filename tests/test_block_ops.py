@@ -1,4 +1,6 @@
 """Layer norm and 8-bit activations on CPU: the statements against 64 bits, and what the entry points refuse."""
+import os
+
 import pytest
 import torch
 
@@ -130,3 +132,17 @@ def test_attention_rpe_step_refusals():
     for bad in (n.long(), n[:1], torch.tensor([[1, 2]], dtype=torch.int32)):
         with pytest.raises(ValueError):
             ops.attention_rpe_step(q, k, v, table, buckets, 1.0, bad)
+
+
+def test_attention_step_entry_refuses_caches_beyond_its_indexes():
+    import ctypes
+
+    from savanna_b200.ops import cuda_ops
+    if not os.path.exists(cuda_ops._LIB_PATH):
+        pytest.skip("library not built")
+    entry, strides = ctypes.CDLL(cuda_ops._LIB_PATH).sb_attn_step, (ctypes.c_longlong * 3)(8, 8, 8)
+
+    def call(T):                                     # no heads: nothing is launched
+        return entry(None, None, None, None, None, 1, T, 0, 64, strides, strides, strides, 0, None, 2, None, 1, 0, ctypes.c_float(1), ctypes.c_float(1),
+                     None, 1, None)
+    assert call(2 ** 30) == 0 and call(2 ** 30 + 1) != 0 and call(-1) != 0
