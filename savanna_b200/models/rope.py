@@ -122,6 +122,8 @@ class RelativePositionBias(nn.Module):
             made = self.bucket(-d).to(torch.int32)
         # one made while a graph is captured has no values before the graph runs: it stays that graph's own
         if not (made.is_cuda and torch.cuda.is_current_stream_capturing()):
+            if made.is_cuda:                # once: other streams read it without a wait
+                torch.cuda.current_stream(made.device).synchronize()
             self._map = key, made
         return made
 

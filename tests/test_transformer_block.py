@@ -217,6 +217,21 @@ def test_cached_generation_on_the_kernels_follows_the_model():
 
 
 @pytest.mark.gpu
+def test_bucket_map_is_there_for_other_streams():
+    rpe = RelativePositionBias(1.0, heads=2, device="cuda")
+    want = rpe.bucket_map().cpu()
+    rpe._map = None
+    first, second = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(first):
+        torch.cuda._sleep(200_000_000)               # a tenth of a second before the map's values
+        rpe.bucket_map()
+    with torch.cuda.stream(second):
+        got = rpe.bucket_map().clone()
+    torch.cuda.synchronize()
+    assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("host", [False, True])
 def test_checkpoints_in_8_bits_on_the_kernels(host):
     # the query gradient is added up in an order that varies: a few units of its 32-bit sums, then one rounding to bf16 that may fall on
