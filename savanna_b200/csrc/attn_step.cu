@@ -70,12 +70,12 @@ __device__ __forceinline__ __half to(float v, __half) { return __float2half_rn(v
 
 // log2(e) * bias at distance d >= 0; a bucket that does not exist has none
 __device__ __forceinline__ float bias(const Args& a, int h, int d) {
-  const int b = a.buckets[min(d, a.far)];
-  if (b < 0 || b >= a.nb) return 0.f;
-  const size_t i = (size_t)b * a.H + h;
+  const int b = __ldg(a.buckets + min(d, a.far));
+  const bool ok = b >= 0 && b < a.nb;
+  const size_t i = ok ? (size_t)b * a.H + h : h;
   const float t = a.table_type == 2 ? static_cast<const float*>(a.table)[i]
                   : a.table_type == 1 ? __half2float(static_cast<const __half*>(a.table)[i]) : __bfloat162float(static_cast<const bf16*>(a.table)[i]);
-  return t * a.bias_log2;
+  return ok ? t * a.bias_log2 : 0.f;
 }
 
 // A weighted sum under a maximum: what joins two of them.
@@ -86,8 +86,9 @@ __device__ __forceinline__ void weights(float m1, float m2, float& m, float& w1,
   w2 = ex2(m2 - r);
 }
 
-template <class T, int LPK>                // LPK lanes a key: hd <= 8 LPK
-__global__ void __launch_bounds__(THREADS)
+// LPK lanes a key: hd <= 8 LPK.  EARLY: the biases of a group's keys are read beside the keys themselves.
+template <class T, int LPK, bool EARLY>
+__global__ void __launch_bounds__(THREADS, 4)
 step_kernel(const Args a) {
   constexpr int G = 32 / LPK;              // groups of a warp
   __shared__ float wm[WARPS], wl[WARPS], wo[WARPS][8 * LPK];
@@ -103,7 +104,7 @@ step_kernel(const Args a) {
   eight<T>(have ? *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.q_sb + h * a.q_sh + c0) : make_uint4(0, 0, 0, 0), q);
 #pragma unroll
   for (int i = 0; i < 8; ++i) { q[i] *= a.scale_log2; o[i] = 0.f; }
-  const float far_bias = bias(a, h, a.far);
+  const float far_bias = EARLY ? 0.f : bias(a, h, a.far);
   for (int j = j0 + (warp * G + grp) * U; __any_sync(0xffffffffu, j < j1); j += WARPS * G * U) {
     uint4 kr[U], vr[U];
 #pragma unroll
@@ -111,6 +112,17 @@ step_kernel(const Args a) {
       const long long at = max(min(j + u, j1 - 1), j0);
       kr[u] = stream16(kp + at * a.k_st);
       vr[u] = stream16(vp + at * a.v_st);
+    }
+    float bs[U];
+    if (EARLY) {
+      if (j + U > len - a.far) {           // some of them nearer than far
+#pragma unroll
+        for (int u = 0; u < U; ++u) bs[u] = bias(a, h, max(len - 1 - (j + u), 0));
+      } else {
+        const float t = bias(a, h, a.far);
+#pragma unroll
+        for (int u = 0; u < U; ++u) bs[u] = t;
+      }
     }
     float s[U], mx = m;
 #pragma unroll
@@ -128,7 +140,7 @@ step_kernel(const Args a) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int d = len - 1 - (j + u);
-      s[u] = j + u < j1 ? s[u] + (d >= a.far ? far_bias : bias(a, h, d)) : -INFINITY;
+      s[u] = j + u < j1 ? s[u] + (EARLY ? bs[u] : d >= a.far ? far_bias : bias(a, h, d)) : -INFINITY;
       mx = fmaxf(mx, s[u]);
     }
     const float ref = mx == -INFINITY ? 0.f : mx, al = ex2(m - ref);
@@ -274,7 +286,13 @@ static int choose_splits(long long rows, int T) {
 template <class T>
 static int launch(const Args& a, int B, cudaStream_t st) {
   const dim3 grid(a.splits, a.H, B);
-  auto* kernel = a.hd <= 64 ? step_kernel<T, 8> : a.hd <= 128 ? step_kernel<T, 16> : step_kernel<T, 32>;
+  // A block's chain counts where it is short, or where lengths differ and the longest sequences' blocks end last: the biases are read early then.
+  // With long blocks on all SMs alike the reads of the far bias in every step cost more.  us, late / early: 8 sequences of 300, 32 heads of 128
+  // 13.4 / 12.4; of up to 2000 28.9 / 25.4, of 2000 each 43.3 / 43.8; 12 of up to 1500, 16 heads of 64 15.7 / 14.1; one of 7000 28.4 / 25.2, of
+  // 16000 44.1 / 44.9, of 32768 82.9 / 87.5; 8 of 16384, 16 heads of 64 82.8 / 93, of up to 16384 50.5 / 45.4.
+  const bool early = (a.lengths && B > 1) || a.T <= 1024 * a.splits;
+  auto* kernel = early ? a.hd <= 64 ? step_kernel<T, 8, true> : a.hd <= 128 ? step_kernel<T, 16, true> : step_kernel<T, 32, true>
+                       : a.hd <= 64 ? step_kernel<T, 8, false> : a.hd <= 128 ? step_kernel<T, 16, false> : step_kernel<T, 32, false>;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = a.splits;
