@@ -32,10 +32,12 @@ __device__ __forceinline__ void down(float f, float& v) { v = f; }
 template <class T, int N> struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack { T v[N]; };
 
 __device__ __forceinline__ uint32_t magnitude(float f) { return __float_as_uint(f) & 0x7fffffffu; }
-__device__ __forceinline__ float inverse(float amax) { return 127.f / (amax < TINY ? TINY : amax); }     // NaN stays NaN
+// 127 / amax as the statement in PyTorch's operations rounds it, so that both give the same codes: a value at the border between two codes goes
+// to the same side.  NaN stays NaN.
+__device__ __forceinline__ float inverse(float amax) { return __fmul_rn(__frcp_rn(amax < TINY ? TINY : amax), 127.f); }
 // rint(x * inv), whose magnitude is at most 127, in the low byte: a product of up to 2^22 added to 1.5 * 2^23 is rounded to an integer, half
-// to even.  (A conversion instruction for each value ran at a quarter of the rate.)  The product is rounded by itself: 16-bit values often lie
-// halfway between two codes, and there its rounding makes good that of inv, where a fused one would fall to a side by chance.
+// to even.  (A conversion instruction for each value ran at a quarter of the rate.)  The product is rounded by itself, as the statement's is: 16-bit values
+// often lie halfway between two codes, and there its rounding mostly makes good that of inv, where a fused one would fall to a side by chance.
 __device__ __forceinline__ uint32_t code(float x, float inv) { return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.f)); }
 __device__ __forceinline__ uint32_t four(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);

@@ -348,3 +348,17 @@ def test_layernorm_leaves_transforms_and_autocast_to_pytorch():
     with torch.autocast("cuda", dtype=torch.bfloat16):
         h = [v.to(torch.bfloat16) for v in (x, w, b)]
         assert ops.layernorm(*h, 1e-5).dtype == torch.nn.functional.layer_norm(h[0], (32,), h[1], h[2], 1e-5).dtype
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("T,D", [(743, 7091), (1000, 1024), (3000, 200)])
+def test_codes_are_those_of_the_statement(T, D, dtype):
+    from savanna_b200.ops import reference as ref
+    g = torch.Generator(device=DEV).manual_seed(T)
+    x = (torch.randn(T, D, generator=g, device=DEV) * torch.exp2(torch.randint(-60, 60, (T, 1), generator=g, device=DEV))).to(dtype)
+    x = x.nan_to_num(0.0, 1000.0, -1000.0)           # what fp16 does not hold
+    q, scale = ops.act_quantize(x)
+    for want, s in (ref.act_quantize(x), [t.to(DEV) for t in ref.act_quantize(x.cpu())]):
+        assert torch.equal(q, want)
+        # amax / 127 by a division or by a product with 1 / 127
+        assert float(((scale - s).abs() / s.clamp(min=1e-30)).max()) <= 2 * 2.0 ** -23
