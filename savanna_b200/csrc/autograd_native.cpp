@@ -358,15 +358,14 @@ struct RmsNormResidual : Function<RmsNormResidual> {
 // ------------------------------------------------------------------------------------ layer norm
 int type_code(at::ScalarType t) { return t == BF16 ? 0 : t == at::kHalf ? 1 : 2; }
 
-struct LnForward { Tensor x2, w, stats, y; };
+struct LnForward { Tensor x, w, stats, y; };
 LnForward layernorm_fwd(const Tensor& x, const Tensor& w, const Tensor& b, double eps, bool train) {
-  LnForward n{rows_contiguous(x), contiguous(w), Tensor(), Tensor()};
+  LnForward n{contiguous(x), contiguous(w), Tensor(), Tensor()};
   const Tensor bc = contiguous(b);
-  const int64_t T = n.x2.size(0), D = n.x2.size(1);
-  n.y = alloc_like(n.x2);
+  const int64_t D = x.size(-1), T = x.numel() / D;
+  n.y = alloc_like(x);
   if (train) n.stats = alloc({T, 2}, F32, x.device());
-  SB_CALL(sb_layernorm_fwd, T > 0, ptr(n.x2), ptr(n.w), ptr(bc), out(n.y), f32o(n.stats), (int)T, (int)D, (float)eps, type_code(x.scalar_type()), stream());
-  if (x.dim() != 2) n.y = n.y.view(x.sizes());
+  SB_CALL(sb_layernorm_fwd, T > 0, ptr(n.x), ptr(n.w), ptr(bc), out(n.y), f32o(n.stats), (int)T, (int)D, (float)eps, type_code(x.scalar_type()), stream());
   return n;
 }
 // Layer norm; with `residual` the second output carries x down the residual branch and the gradient arriving there is added inside the
@@ -393,15 +392,14 @@ struct LayerNorm : Function<LayerNorm> {
       const Tensor dx = std::get<0>(d);
       return {gres.defined() ? dx + gres : dx, std::get<1>(d), std::get<2>(d), Tensor(), Tensor()};
     }
-    const Tensor x2 = rows_contiguous(x), w = contiguous(s[1]);
-    const int64_t T = x2.size(0);
-    const int type = type_code(x2.scalar_type());
-    Tensor g2 = contiguous(g[0].reshape({T, D})), r2 = gres.defined() ? contiguous(gres.reshape({T, D})) : Tensor();
-    Tensor dx = alloc_like(x2), dw = alloc({D}, x2.scalar_type(), x2.device()), db = alloc_like(dw),
-           partial = alloc({(int64_t)L.sb_layernorm_bwd_blocks(T, D, type) * 2 * D}, F32, x2.device());
-    SB_CALL(sb_layernorm_bwd, T > 0 ? 2 : 1, ptr(x2), ptr(w), ptr(g2), f32(st), ptr(r2), out(dx), out(dw), out(db), f32o(partial), (int)T, (int)D,
+    const Tensor xc = contiguous(x), w = contiguous(s[1]), gy = contiguous(g[0]), gr = gres.defined() ? contiguous(gres) : Tensor();
+    const int64_t T = x.numel() / D;
+    const int type = type_code(x.scalar_type());
+    Tensor dx = alloc_like(x), dw = alloc({D}, x.scalar_type(), x.device()), db = alloc_like(dw),
+           partial = alloc({(int64_t)L.sb_layernorm_bwd_blocks(T, D, type) * 2 * D}, F32, x.device());
+    SB_CALL(sb_layernorm_bwd, T > 0 ? 2 : 1, ptr(xc), ptr(w), ptr(gy), f32(st), ptr(gr), out(dx), out(dw), out(db), f32o(partial), (int)T, (int)D,
             type, stream());
-    return {x.dim() == 2 ? dx : dx.view(x.sizes()), dw, db, Tensor(), Tensor()};
+    return {dx, dw, db, Tensor(), Tensor()};
   }
 };
 // The kernels' part of layer norms: one type, up to 2^30 rows of up to 16384 values, outside of autocast (which wants fp32), functorch's transforms and
@@ -761,18 +759,28 @@ struct FlashPacked : Function<FlashPacked> {
 // The same without rotary embedding and with a learned bias by relative position: bias_scale * table[buckets[q - k], head] on the scores.
 // A row of one key has a softmax that is constant: only v has a gradient then, and it is exact.
 struct RpeForward { Tensor table, buckets, o, lo, lse; };
+// A contiguous [B, L, H, N] with strides that follow from its sizes (those of a dimension of size one may be anything), and the address of 128
+// columns of it: q, k and v of a packed projection without views, nine of which would take a small forward and backward longer on the host than
+// its launches.
+struct Dense {
+  char* p;
+  long long s[3];
+  explicit Dense(const Tensor& t)
+      : p(static_cast<char*>(const_cast<void*>(t.const_data_ptr()))), s{t.size(1) * t.size(2) * t.size(3), t.size(2) * t.size(3), t.size(3)} {}
+  void* part(int i) const { return p + i * 256; }
+};
 RpeForward rpe_fwd(const Tensor& qkv, const Tensor& table, const Tensor& buckets, double bias_scale, bool causal, bool train) {
   const int64_t B = qkv.size(0), Ln = qkv.size(1), H = qkv.size(2), far = causal ? buckets.size(0) - 1 : buckets.size(0) / 2;
   const at::Device dev = qkv.device();
-  const Tensor q = qkv.slice(3, 0, 128), k = qkv.slice(3, 128, 256), v = qkv.slice(3, 256, 384);
+  const Dense in(qkv);
   RpeForward f{contiguous(table), contiguous(buckets), alloc({B, Ln, H, 128}, BF16, dev), train ? alloc({B, Ln, H, 128}, at::kChar, dev) : Tensor(),
                alloc({B, H, Ln}, F32, dev)};
-  const Strides qs(q), ks(k), vs(v), os(f.o);
-  const int rc = SB_RUN(sb_attn_rpe_fwd, B * Ln * H > 0, ptr(q), ptr(k), ptr(v), out(f.o), out(f.lo), f32o(f.lse), (int)B, (int)H, (int)Ln, qs.s, ks.s, vs.s,
-                        os.s, (int)causal, 0.08838834764831845f, ptr(f.table), (int)(f.table.scalar_type() == F32), static_cast<const int*>(ptr(f.buckets)),
+  const Dense os(f.o);
+  const int rc = SB_RUN(sb_attn_rpe_fwd, B * Ln * H > 0, in.part(0), in.part(1), in.part(2), out(f.o), out(f.lo), f32o(f.lse), (int)B, (int)H, (int)Ln, in.s,
+                        in.s, in.s, os.s, (int)causal, 0.08838834764831845f, ptr(f.table), (int)(f.table.scalar_type() == F32), static_cast<const int*>(ptr(f.buckets)),
                         (int)f.table.size(0), (int)far, (float)bias_scale, status_word(dev), stream());
   TORCH_CHECK(rc == 0, "attention with relative position bias failed (code ", rc, ", encode ", L.sb_attn_last_encode_result(), "): ",
-              layouts({{"q", &q}, {"k", &k}, {"v", &v}, {"table", &f.table}, {"buckets", &f.buckets}}));
+              layouts({{"qkv", &qkv}, {"table", &f.table}, {"buckets", &f.buckets}}));
   return f;
 }
 // The same by elementary operations, scores materialised: what a second derivative goes through.
@@ -817,19 +825,21 @@ struct FlashRpe : Function<FlashRpe> {
       if (dqkv.numel() > 0) dqkv.slice(3, 256, 384).copy_(g[0]);
       return {dqkv, cleared(dtable), Tensor(), Tensor(), Tensor()};
     }
-    Tensor q = qkv.slice(3, 0, 128), k = qkv.slice(3, 128, 256), v = qkv.slice(3, 256, 384);
-    Tensor dq = dqkv.slice(3, 0, 128), dk = dqkv.slice(3, 128, 256), dv = dqkv.slice(3, 256, 384);
-    Tensor go = packed_rows(g[0]) ? g[0] : g[0].contiguous();
+    const Dense in(qkv), d(dqkv), os(o);
+    const Tensor go = packed_rows(g[0]) ? g[0] : aligned(g[0]);
+    const Strides as_is(go);
+    const long long* gs = go.is_contiguous() ? os.s : as_is.s;
     long long floats = 0;
     SB_CALL(sb_attn_rpe_bwd_work, 0, (int)B, (int)H, (int)Ln, (int)far, (int)causal, &floats);
-    Tensor acc = alloc({B, Ln, H, 128}, F32, dev), stats = alloc({2 * B * H * ((Ln + 63) / 64 * 64)}, F32, dev), work = alloc({floats}, F32, dev);
-    const Strides gs(go), qs(q), ks(k), vs(v), os(o), dqs(dq), dks(dk), dvs(dv);
-    const int rc = SB_RUN(sb_attn_rpe_bwd, 3, ptr(go), ptr(q), ptr(k), ptr(v), ptr(o), ptr(lo), f32(lse), f32o(stats), f32o(acc), out(dq), out(dk), out(dv),
-                          (int)B, (int)H, (int)Ln, gs.s, qs.s, ks.s, vs.s, os.s, dqs.s, dks.s, dvs.s, (int)causal, 0.08838834764831845f, ptr(table),
+    const int64_t accs = B * Ln * H * 128, stats = 2 * B * H * ((Ln + 63) / 64 * 64);          // multiples of 128 floats
+    Tensor scratch = alloc({accs + stats + floats}, F32, dev);
+    float* acc = f32o(scratch);
+    const int rc = SB_RUN(sb_attn_rpe_bwd, 3, ptr(go), in.part(0), in.part(1), in.part(2), ptr(o), ptr(lo), f32(lse), acc + accs, acc, d.part(0), d.part(1),
+                          d.part(2), (int)B, (int)H, (int)Ln, gs, in.s, in.s, in.s, os.s, d.s, d.s, d.s, (int)causal, 0.08838834764831845f, ptr(table),
                           (int)(table.scalar_type() == F32), static_cast<const int*>(ptr(buckets)), (int)table.size(0), (int)far,
-                          (float)ctx->saved_data["bias_scale"].toDouble(), f32o(work), out(dtable), status_word(dev), stream());
+                          (float)ctx->saved_data["bias_scale"].toDouble(), acc + accs + stats, out(dtable), status_word(dev), stream());
     TORCH_CHECK(rc == 0, "backward of attention with relative position bias failed (code ", rc, ", encode ", L.sb_attn_last_encode_result(), "): ",
-                layouts({{"dout", &go}, {"q", &q}, {"k", &k}, {"v", &v}}));
+                layouts({{"dout", &go}, {"qkv", &qkv}}));
     return {dqkv, dtable, Tensor(), Tensor(), Tensor()};
   }
 };

@@ -103,8 +103,9 @@ __device__ __forceinline__ float warp_sum(float v) {
 
 // Widths that N = 16 / sizeof(T) does not divide (SHIFT): a row is `head` values up to the next 16-byte boundary, nv vectors, and `tail` values.  The
 // single ones, 14 at most, are spread over the lanes of the row's first warp.  Rows that are N (or N / 2, ..: `classes`) apart are cut alike.
-// bf16, us, single values throughout -> here: forward 8192 x 1027 22.6 -> 12.3, 8192 x 4095 95 -> 37; backward 45 -> 27, 1045 -> 62.  (Whole vectors
-// with the neighbours' values masked: 69 and 88 at 8192 x 4095, most of it spent on the two ends.)
+// bf16, us, single values throughout -> here: forward 8192 x 1027 22.6 -> 12.3, 8192 x 4095 95 -> 37; backward 45 -> 22.5, 1045 -> 62.  (Whole vectors
+// with the neighbours' values masked: 69 and 88 at 8192 x 4095, most of it spent on the two ends.)  In the backward the single values' registers fit
+// blocks of 384 threads where a row has no more than 12 warps: 8192 x 3001 63 -> 48, 40000 x 203 with residual 35 -> 25 against 512.
 template <class T> struct Cut {
   int head, nv, tail;
   __device__ __forceinline__ Cut(int row, int D) {

@@ -209,6 +209,29 @@ def test_strided_output_gradient_and_other_stream():
     assert torch.equal(expanded[2], same[2])
 
 
+def test_odd_strides_of_dimensions_of_size_one_and_gradients_off_16_bytes():
+    qkv, table, buckets, go = _case(1, 150, 2, 32, 64, True)
+
+    def run(x, g):
+        x, t = x.detach().requires_grad_(True), table.clone().requires_grad_(True)
+        o = ops.attention_rpe(x, t, buckets, 2.0, True)
+        return (o.detach(), *torch.autograd.grad(o, (x, t), g))
+
+    def after(t, start, end):                        # the same values in the middle of a longer row
+        row = torch.zeros(1, start + t.numel() + end, device=DEV, dtype=BF)[:, start: start + t.numel()]
+        row.copy_(t.view(1, -1))
+        return row.view(t.shape)
+    want = run(qkv, go)
+    for x, g in ((after(qkv, 0, 3), go), (qkv, after(go, 0, 5)), (qkv, after(go, 1, 0)), (after(qkv, 8, 1), after(go, 3, 2))):
+        assert x.is_contiguous() and g.is_contiguous()
+        got = run(x, g)
+        _status_ok()
+        assert torch.equal(want[0], got[0]) and torch.equal(want[2], got[2])
+        # dq is added up in an order that varies: a step of bf16 between two sums; dk and dv are not
+        assert torch.equal(want[1][..., 128:], got[1][..., 128:])
+        assert bool(((want[1].double() - got[1].double()).abs() <= 2.0 ** -7 * want[1].double().abs() + 2.0 ** -20 * want[1].abs().max()).all())
+
+
 def test_captured_forward_and_backward():
     qkv, table, buckets, go = _case(1, 400, 2, 32, 128, True)
     want = _run(qkv, table, buckets, 2.0, True, go)
