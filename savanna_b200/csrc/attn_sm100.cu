@@ -56,7 +56,8 @@ struct FwdParams {
 
 // ------------------------------------------------------------------------------------ bias by relative position
 // s = q k^T scale + bias_scale table[bucket(q - k), h], the bucket of a distance from a map: 0 .. far (causal), or -far .. far; beyond it the
-// last entry counts.  Variants of both kernels (template parameter RPE) add it to the scores in registers, so that no [L, L] bias exists:
+// last entry counts.  A forward kernel of its own and variants of the backward's (template parameter RPE) add it to the scores in registers, so that
+// no [L, L] bias exists:
 //   - A tile all of whose pairs are at least `far` apart has one bias, which is folded into the constant of the exponent: nothing per pair.
 //     With far = 128 those are all but two or three tiles of a row.
 //   - In the others ("near") a pair's bias is read from the head's values by distance; consecutive lanes have consecutive distances.
@@ -66,15 +67,15 @@ struct FwdParams {
 //   - delta = sum(dO O) must be good to the rounding of dS itself: the forward divides by the sum of the ROUNDED probabilities, so that O is an
 //     exact average under slightly other weights, and hands on what O lost in rounding (out_lo).  The divisor in lse, which the backward's P
 //     has, gets back what the largest probability of each tile lost, which is most of it where a few keys have all the weight.  (A sum of
-//     the unrounded probabilities took the forward from 555 to 640 us at 8192 tokens, 32 heads.)
+//     the unrounded probabilities too cost the forward an eighth.)
 //     What error e is left in a row's delta adds P e to each dS, and the sum of e over the rows is that of all dS, which should be zero: it is
 //     taken off the distances in proportion to their share of P, whose diagonals are summed up the same way.  (In a long causal row the far
 //     keys hold nearly all of P while their true sum is as small as that of the near ones: their error without this is a percent at 8192 keys.)
 //
-// Measured beside the same kernels without bias, us, causal with far = 128 / both sides with far = 256: forward 8192 x 32 heads 565 / -
-// (542), 2 x 2048 x 16 heads - / 95 (82); with the backward pass 2137 / - (2058), - / 381 (316), 3 x 777 x 4 heads 66 / - (53).  A tile that
-// is not near costs what it costs without bias (8192 x 16 heads, far = 1: 822 us in the backward kernel, 823 without bias); a near one a third more
-// there, for the read of the values and the travelling sums.
+// Measured beside the kernels without bias, us, causal with far = 128 / both sides with far = 256: forward 8192 x 32 heads 540 / - (550), 2 x 2048
+// x 16 heads - / 87 (82); with the backward pass 2127 / - (2089), - / 376 (315), 3 x 777 x 4 heads 65 / - (53).  A tile of the backward that is
+// not near costs what it costs without bias (8192 x 16 heads, far = 1: 822 us in the backward kernel, 823 without bias); a near one a third more,
+// for the read of the values and the travelling sums.
 constexpr int RPE_MAX_FAR = 1024;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 enum { RPE_NONE = 0, RPE_CAUSAL = 1, RPE_BOTH = 2 };
@@ -152,11 +153,10 @@ __device__ __forceinline__ uint64_t desc_mnmajor(uint32_t tile, int kk) {
 // (a single-CTA M = 128 product with both operands in shared memory uses the whole shared-memory bandwidth of the SM).
 // The price is an ordering constraint: the scores of block j+1 overwrite P(j), so S_t(j+1) is issued behind P_t(j) V(j)
 // on the (in-order) tensor pipe instead of during softmax j; the other query tile fills the gap.
-template <bool P_TMEM, int RPE>
+template <bool P_TMEM>
 __global__ void __launch_bounds__(FWD_THREADS, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                const __grid_constant__ CUtensorMap tmV, FwdParams p, const __grid_constant__ RpeParams rp) {
-  static_assert(!RPE || P_TMEM, "the bias by distance takes the shared memory of P");
+                const __grid_constant__ CUtensorMap tmV, FwdParams p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -316,19 +316,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     const uint32_t t_o = tmem_base + (uint32_t(quarter * 32) << 16) + 256 + t * 128;
     const uint32_t p_tile = sP + t * TILE_BYTES;
     const float sl2 = p.scale_log2;
-    float m = -INFINITY, l = 0.f;                    // RPE: m in units of log2, bias included
-    float lost_top = 0.f;                            // RPE: what the largest probability of each tile lost in rounding
+    float m = -INFINITY, l = 0.f;
     bool ok = true;
-    // near tiles reach distances of far + 253: 127 beyond their first column's
-    float* bias_s = reinterpret_cast<float*>(smem_gen + 5 * TILE_BYTES);
-    const int origin = RPE == RPE_BOTH ? rp.far + 256 : 128;
-    float beyond[2] = {0.f, 0.f};                    // of the tiles beyond +far, -far
-    if (RPE) {
-      for (int i = (int)threadIdx.x - 64; i < origin + rp.far + 256; i += 256) bias_s[i] = rpe_value(rp, RPE, p.H, h, i - origin);
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      beyond[0] = bias_s[origin + rp.far];
-      beyond[1] = bias_s[RPE == RPE_BOTH ? origin - rp.far : origin];
-    }
     for (int j = 0; j < nb[t] && ok; ++j) {
       const uint32_t par = uint32_t(j) & 1u;
       if (!mbar_wait(s_full(t), par, abort_flag, p.status, ST_ATTN + 7)) { ok = false; break; }
@@ -343,20 +332,6 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       tmem_wait_ld();
       tc_fence_before();
       mbar_arrive(s_free(t));
-      float mul = sl2, add = 0.f;                    // RPE: x = v * mul + add in units of log2
-      if (RPE) {
-        const int base = q0 + t * BQ - k0;           // distance of the tile's first row and column
-        if (base - 127 < rp.far && (RPE == RPE_CAUSAL || base + 127 > -rp.far)) {
-          const float* bt = bias_s + origin + base + r;
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[c][i] = __float_as_uint(fmaf(__uint_as_float(v[c][i]), sl2, bt[-(c * 32 + i)]));
-          mul = 1.f;
-        } else {
-          add = base > 0 ? beyond[0] : beyond[1];
-        }
-      }
       if (edge) {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
@@ -369,24 +344,15 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         bm4[c] = __uint_as_float(v[c][0]);
-        if (RPE) {
 #pragma unroll
-          for (int i = 1; i < 31; i += 2) bm4[c] = max3(bm4[c], __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
-          bm4[c] = fmaxf(bm4[c], __uint_as_float(v[c][31]));
-        } else {
-#pragma unroll
-          for (int i = 1; i < 32; ++i) bm4[c] = fmaxf(bm4[c], __uint_as_float(v[c][i]));
-        }
+        for (int i = 1; i < 32; ++i) bm4[c] = fmaxf(bm4[c], __uint_as_float(v[c][i]));
       }
-      float bm = fmaxf(fmaxf(bm4[0], bm4[1]), fmaxf(bm4[2], bm4[3]));
-      const float top = bm;
-      if (RPE) bm = fmaf(bm, mul, add);              // of the row, in the units of m
-      const float unit = RPE ? 1.f : sl2;
+      const float bm = fmaxf(fmaxf(bm4[0], bm4[1]), fmaxf(bm4[2], bm4[3]));
       // keep the old reference maximum unless the new one exceeds it by more than 2^8 (P stays below 256)
       float m_new = m;
-      if (bm > m && (m == -INFINITY || (bm - m) * unit > 8.f)) m_new = bm;
+      if (bm > m && (m == -INFINITY || (bm - m) * sl2 > 8.f)) m_new = bm;
       const float m_ref = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = (m == -INFINITY) ? 0.f : ex2((m - m_ref) * unit);
+      const float alpha = (m == -INFINITY) ? 0.f : ex2((m - m_ref) * sl2);
       const bool rescale = (j > 0) && (m_new != m);
       m = m_new;
       if (j > 0) {
@@ -405,9 +371,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         }
       }
       // P = exp2((S - m) * scale) as bf16 into the swizzled P tile; row sum in fp32
-      const float moff = RPE ? add - m_ref : -m_ref * sl2;
+      const float moff = -m_ref * sl2;
       float rs4[4] = {0.f, 0.f, 0.f, 0.f};
-      f2 rounded[2] = {0, 0};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
 #pragma unroll
@@ -415,15 +380,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           uint32_t w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float xa = fmaf(__uint_as_float(v[c][g * 8 + 2 * i]), RPE ? mul : sl2, moff);
-            const float xb = fmaf(__uint_as_float(v[c][g * 8 + 2 * i + 1]), RPE ? mul : sl2, moff);
+            const float xa = fmaf(__uint_as_float(v[c][g * 8 + 2 * i]), sl2, moff);
+            const float xb = fmaf(__uint_as_float(v[c][g * 8 + 2 * i + 1]), sl2, moff);
             const float ea = ex2(xa), eb = ex2(xb);        // exp2(-inf) = 0 for masked keys
+            rs4[i] += ea + eb;
             w[i] = pack_bf16(ea, eb);
-            if (RPE) {
-              rounded[i & 1] = f2_add(rounded[i & 1], f2_bf(w[i]));      // what enters the product
-            } else {
-              rs4[i] += ea + eb;
-            }
           }
           if (P_TMEM) {
             // the score registers of these 8 keys are dead: keep the packed probabilities in their place
@@ -442,16 +403,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       }
       if (P_TMEM) tmem_wait_st();
       if (p.pingpong) mbar_arrive(turn(t ^ 1));               // hand the unit to the other warpgroup
-      float rs = (rs4[0] + rs4[1]) + (rs4[2] + rs4[3]);
-      if (RPE) {
-        const float2 d = f2_unpack(f2_add(rounded[0], rounded[1]));
-        rs = d.x + d.y;
-      }
+      const float rs = (rs4[0] + rs4[1]) + (rs4[2] + rs4[3]);
       l = l * alpha + rs;
-      if (RPE) {
-        const float e = ex2(fmaf(top, mul, moff));
-        lost_top = lost_top * alpha + (e - __uint_as_float(pack_bf16(0.f, e) & 0xffff0000u));
-      }
       if (__any_sync(0xffffffffu, rescale)) {
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
@@ -488,7 +441,292 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
               o.z = pack_bf16(__uint_as_float(v[g * 8 + 4]) * inv, __uint_as_float(v[g * 8 + 5]) * inv);
               o.w = pack_bf16(__uint_as_float(v[g * 8 + 6]) * inv, __uint_as_float(v[g * 8 + 7]) * inv);
               *reinterpret_cast<uint4*>(orow + c * 32 + g * 8) = o;
-              if (RPE && rp.out_lo) {              // in place of these eight values
+            }
+          }
+        }
+        if (row < p.Lq)
+          p.lse[((long long)b * p.H + h) * p.Lq + row] = (m == -INFINITY ? 0.f : m) * p.scale + __logf(fmaxf(l, 1e-37f));
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// The forward with a bias by relative position.  Roles, tiles and tensor memory are those above, but the softmax goes by 64 keys, so that the two score
+// buffers of a tile (64 columns each, the probabilities packed over the first 32) take turns: the scores of the next 64 keys are there when a softmax
+// step ends, and the chain scores - softmax - P V - next scores, which bounds the kernel above, is cut.  The price is that a product of 64 key rows
+// reads its queries twice as often (1.5 times the time of the score products, by the shared memory's bandwidth).  Four slots for K and V, in the
+// shared memory that P does not need.  us, 128 keys a step in the kernel above / here: 8192 x 32 heads causal 559 / 540, 2 x 1333 x 16 35.6 / 31.7,
+// 3 x 777 x 4 22 / 21, 2 x 2048 x 16 both sides 91 / 87.  Without its exponentials it takes 537 at 8192, without most of its products 527, without
+// either 351: both sides are full.  Two threads a row, for the even and the odd steps, took 554 at 8192 and 85 for both sides; waits that spin
+// 549.
+template <int RPE>
+__global__ void __launch_bounds__(FWD_THREADS, 1)
+rpe_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+               const __grid_constant__ CUtensorMap tmV, FwdParams p, const __grid_constant__ RpeParams rp) {
+  constexpr int SUB = 64;                          // keys of a softmax step
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
+  const uint32_t sQ = smem_base, sKV = smem_base + 2 * TILE_BYTES;     // K(0) V(0) K(1) V(1) .. : tile i in slot i % 4
+  float* bias_s = reinterpret_cast<float*>(smem_gen + 6 * TILE_BYTES);
+  static_assert((2 * RPE_MAX_FAR + 512) * 4 <= TILE_BYTES, "values by distance");
+  constexpr uint32_t BAR_OFF = 7 * TILE_BYTES;
+  const uint32_t bar_base = smem_base + BAR_OFF;
+  const uint32_t q_full = bar_base;
+  auto kv_full = [&](int s) { return bar_base + 8u + 8u * s; };
+  auto kv_free = [&](int s) { return bar_base + 40u + 8u * s; };
+  // by tile and buffer (step number modulo 2)
+  auto s_full = [&](int t, int b) { return bar_base + 72u + 16u * t + 8u * b; };
+  auto p_ready = [&](int t, int b) { return bar_base + 104u + 16u * t + 8u * b; };
+  auto pv_done = [&](int t, int b) { return bar_base + 136u + 16u * t + 8u * b; };
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem_gen + BAR_OFF + 168);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_gen + BAR_OFF + 176);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // longest rows first: within a head, or (heads_fast) over all heads, which packs the blocks of a short grid better
+  const int qblk = (p.heads_fast ? gridDim.z : gridDim.x) - 1 - (p.heads_fast ? blockIdx.z : blockIdx.x);
+  const int h = p.heads_fast ? blockIdx.x : blockIdx.y, b = p.heads_fast ? blockIdx.y : blockIdx.z;
+  const int q0 = qblk * 2 * BQ;
+  int ns[2];                                       // softmax steps of each tile
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int r0 = q0 + t * BQ;
+    ns[t] = r0 >= p.Lq ? 0 : (min(p.Lk, p.causal ? r0 + BQ : p.Lk) + SUB - 1) / SUB;
+  }
+  const int n = (max(ns[0], ns[1]) + 1) / 2;       // blocks of 128 keys
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int s = 0; s < 4; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_free(s), 1); }
+    for (int t = 0; t < 2; ++t)
+      for (int b2 = 0; b2 < 2; ++b2) { mbar_init(s_full(t, b2), 1); mbar_init(p_ready(t, b2), 128); mbar_init(pv_done(t, b2), 1); }
+    *abort_flag = 0;
+    fence_barrier_init();
+    prefetch_tmap(&tmQ); prefetch_tmap(&tmK); prefetch_tmap(&tmV);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  wait_for_previous();
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    if (elect_one()) {
+      bool ok = true;
+      mbar_expect_tx(q_full, 2 * TILE_BYTES);
+      load_tile(sQ, &tmQ, q0, h, b, q_full);
+      load_tile(sQ + TILE_BYTES, &tmQ, q0 + BQ, h, b, q_full);
+      for (int i = 0; i < 2 * n && ok; ++i) {            // i even: K(i/2), i odd: V(i/2)
+        const int slot = i & 3;
+        const uint32_t use = uint32_t(i >> 2);
+        if (!mbar_wait(kv_free(slot), (use & 1u) ^ 1u, abort_flag, p.status, ST_ATTN + 1 + (i & 1))) { ok = false; break; }
+        mbar_expect_tx(kv_full(slot), TILE_BYTES);
+        load_tile(sKV + slot * TILE_BYTES, (i & 1) ? &tmV : &tmK, (i >> 1) * BK, h, b, kv_full(slot));
+      }
+      if (!ok) {
+        const unsigned long long t0 = globaltimer();
+        while (globaltimer() - t0 < 200000ull) { __nanosleep(1000); }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (elect_one() && n > 0) {
+      const uint32_t idesc_s = umma_idesc_bf16(128, SUB, 0, 0);     // S = Q K^T: both operands K-major
+      const uint32_t idesc_o = umma_idesc_bf16(128, 128, 0, 1);     // O += P V: P K-major (tensor memory), V MN-major
+      bool ok = mbar_wait(q_full, 0u, abort_flag, p.status, ST_ATTN + 3);
+      // Event loop over both tiles.  S_t(js) goes out as soon as its keys have landed and P_t(js-2) V, whose P lies in the same buffer, was issued
+      // (the pipe keeps the order); O_t += P_t(jp) V(jp) as soon as both are there.  Each tile's queue is served in order.
+      int s_idx[2] = {0, 0}, pv_idx[2] = {0, 0};
+      // a tile whose queue is at `done` of `all` steps needs block j no more
+      auto through = [](int done, int all, int j) { return all <= 2 * j || done >= min(2 * j + 2, all); };
+      unsigned long long t0 = globaltimer();       // time of the last progress
+      uint32_t spins = 0;
+      while (ok && (s_idx[0] < ns[0] || s_idx[1] < ns[1] || pv_idx[0] < ns[0] || pv_idx[1] < ns[1])) {
+        bool progress = false;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (pv_idx[t] < ns[t]) {
+            const int jp = pv_idx[t], j = jp >> 1, buf = jp & 1;
+            const int vslot = (2 * j + 1) & 3;
+            if (mbar_test(p_ready(t, buf), uint32_t(j) & 1u) && mbar_test(kv_full(vslot), uint32_t((2 * j + 1) >> 2) & 1u)) {
+              tc_fence_after();
+              const uint32_t sV = sKV + vslot * TILE_BYTES;
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)       // 16 keys = 8 packed columns of the step's score buffer
+                umma_bf16_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + buf * SUB + kk * 8, desc_mnmajor(sV, buf * 4 + kk), idesc_o,
+                             (jp | kk) ? 1u : 0u);
+              umma_commit(pv_done(t, buf));
+              pv_idx[t] = jp + 1;
+              if (through(jp + 1, ns[t], j) && through(pv_idx[t ^ 1], ns[t ^ 1], j)) umma_commit(kv_free(vslot));   // both tiles are through with V(j)
+              progress = true;
+            }
+          }
+          if (s_idx[t] < ns[t]) {
+            const int js = s_idx[t], j = js >> 1, buf = js & 1;
+            const int kslot = (2 * j) & 3;
+            if (mbar_test(kv_full(kslot), uint32_t((2 * j) >> 2) & 1u) && pv_idx[t] >= js - 1) {
+              tc_fence_after();
+              const uint32_t sK = sKV + kslot * TILE_BYTES + buf * (SUB * 128);          // 64 rows of 128 bytes in each box
+#pragma unroll
+              for (int kk = 0; kk < 8; ++kk)
+                umma_bf16(tmem_base + t * 128 + buf * SUB, desc_kmajor(sQ + t * TILE_BYTES, kk), desc_kmajor(sK, kk), idesc_s, kk ? 1u : 0u);
+              umma_commit(s_full(t, buf));
+              s_idx[t] = js + 1;
+              if (through(js + 1, ns[t], j) && through(s_idx[t ^ 1], ns[t ^ 1], j)) umma_commit(kv_free(kslot));    // both tiles are through with K(j)
+              progress = true;
+            }
+          }
+        }
+        if (progress) {
+          t0 = globaltimer();
+        } else {
+          if ((++spins & 255u) == 0u) {
+            if (*abort_flag) ok = false;
+            else if (globaltimer() - t0 > WAIT_BUDGET_NS) {
+              *abort_flag = 1;
+              if (p.status) atomicCAS(p.status, 0u, ((ST_ATTN + 6) << 24) | (blockIdx.x & 0xffffffu));
+              ok = false;
+            }
+          }
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax + epilogue: one thread per query row
+    const int t = (warp - 2) >> 2;
+    const int quarter = warp & 3;                    // TMEM lane quarter this warp may access
+    const int r = quarter * 32 + lane;               // row inside the tile
+    const int row = q0 + t * BQ + r;                 // query position
+    const uint32_t t_s = tmem_base + (uint32_t(quarter * 32) << 16) + t * 128;
+    const uint32_t t_o = tmem_base + (uint32_t(quarter * 32) << 16) + 256 + t * 128;
+    const float sl2 = p.scale_log2;
+    float m = -INFINITY, l = 0.f;                    // m in units of log2, bias included
+    float lost_top = 0.f;                            // what the largest probability of each step lost in rounding
+    bool ok = true;
+    // near steps reach distances from -127 (causal) or -far - 189 to far + 189
+    const int origin = RPE == RPE_BOTH ? rp.far + 256 : 128;
+    for (int i = (int)threadIdx.x - 64; i < origin + rp.far + 256; i += 256) bias_s[i] = rpe_value(rp, RPE, p.H, h, i - origin);
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    const float beyond[2] = {bias_s[origin + rp.far], bias_s[RPE == RPE_BOTH ? origin - rp.far : origin]};      // beyond +far, -far
+    for (int j = 0; j < ns[t] && ok; ++j) {
+      const int buf = j & 1, k0 = j * SUB;
+      if (!mbar_wait(s_full(t, buf), uint32_t(j >> 1) & 1u, abort_flag, p.status, ST_ATTN + 7)) { ok = false; break; }
+      tc_fence_after();
+      uint32_t v[2][32];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) tmem_ld_32x32(t_s + buf * SUB + c * 32, v[c]);
+      // P V of two steps before, which those scores came behind: there already, and seen so that no phase of its barrier is skipped
+      if (j > 1 && !mbar_wait(pv_done(t, buf), uint32_t((j - 2) >> 1) & 1u, abort_flag, p.status, ST_ATTN + 8)) { ok = false; break; }
+      tmem_wait_ld();
+      float mul = sl2, add = 0.f;                    // x = v * mul + add in units of log2
+      const int base = q0 + t * BQ - k0;             // distance of the first row and key
+      if (base - (SUB - 1) < rp.far && (RPE == RPE_CAUSAL || base + BQ - 1 > -rp.far)) {
+        const float* bt = bias_s + origin + base + r;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[c][i] = __float_as_uint(fmaf(__uint_as_float(v[c][i]), sl2, bt[-(c * 32 + i)]));
+        mul = 1.f;
+      } else {
+        add = base > 0 ? beyond[0] : beyond[1];
+      }
+      if ((p.causal && k0 + SUB - 1 > q0 + t * BQ) || k0 + SUB > p.Lk) {
+        const int limit = p.causal ? min(row, p.Lk - 1) : p.Lk - 1;      // last visible key of this row
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (k0 + c * 32 + i > limit) v[c][i] = 0xff800000u;      // -inf
+      }
+      // four independent chains keep the dependent-issue latency of the row maximum short
+      float bm4[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint32_t* w = v[c >> 1] + (c & 1) * 16;
+        bm4[c] = __uint_as_float(w[0]);
+#pragma unroll
+        for (int i = 1; i < 15; i += 2) bm4[c] = max3(bm4[c], __uint_as_float(w[i]), __uint_as_float(w[i + 1]));
+        bm4[c] = fmaxf(bm4[c], __uint_as_float(w[15]));
+      }
+      const float top = fmaxf(fmaxf(bm4[0], bm4[1]), fmaxf(bm4[2], bm4[3]));
+      const float bm = fmaf(top, mul, add);          // in the units of m
+      // keep the old reference maximum unless the new one exceeds it by more than 2^8 (P stays below 256)
+      float m_new = m;
+      if (bm > m && (m == -INFINITY || bm - m > 8.f)) m_new = bm;
+      const float m_ref = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = (m == -INFINITY) ? 0.f : ex2(m - m_ref);
+      const bool rescale = (j > 0) && (m_new != m);
+      m = m_new;
+      // P = exp2(x - m) as bf16 over the scores; the row sum is that of the rounded values
+      const float moff = add - m_ref;
+      f2 rounded[2] = {0, 0};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t pw[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float ea = ex2(fmaf(__uint_as_float(v[c][2 * i]), mul, moff));
+          const float eb = ex2(fmaf(__uint_as_float(v[c][2 * i + 1]), mul, moff));        // exp2(-inf) = 0 for masked keys
+          pw[i] = pack_bf16(ea, eb);
+          rounded[i & 1] = f2_add(rounded[i & 1], f2_bf(pw[i]));
+        }
+        tmem_st_32x16(t_s + buf * SUB + c * 16, pw);       // keys 32c .. 32c+31 -> packed columns 16c .. 16c+15
+      }
+      tmem_wait_st();
+      const float2 d = f2_unpack(f2_add(rounded[0], rounded[1]));
+      l = l * alpha + (d.x + d.y);
+      const float e = ex2(fmaf(top, mul, moff));
+      lost_top = lost_top * alpha + (e - __uint_as_float(pack_bf16(0.f, e) & 0xffff0000u));
+      if (__any_sync(0xffffffffu, rescale)) {
+        // the product of the step before must have left O
+        if (!mbar_wait(pv_done(t, buf ^ 1), uint32_t((j - 1) >> 1) & 1u, abort_flag, p.status, ST_ATTN + 8)) { ok = false; break; }
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t w[32];
+          tmem_ld_32x32(t_o + c * 32, w);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * alpha);
+          tmem_st_32x32(t_o + c * 32, w);
+        }
+        tmem_wait_st();
+      }
+      tc_fence_before();
+      mbar_arrive(p_ready(t, buf));
+    }
+    if (ok && ns[t] > 0) {
+      const int last = ns[t] - 1;
+      if (mbar_wait(pv_done(t, last & 1), uint32_t(last >> 1) & 1u, abort_flag, p.status, ST_ATTN + 9)) {
+        tc_fence_after();
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        __nv_bfloat16* orow = p.out + (long long)b * p.o_sb + (long long)row * p.o_sl + (long long)h * p.o_sh;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[32];
+          tmem_ld_32x32(t_o + c * 32, v);
+          tmem_wait_ld();
+          if (row < p.Lq) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              uint4 o;
+              o.x = pack_bf16(__uint_as_float(v[g * 8 + 0]) * inv, __uint_as_float(v[g * 8 + 1]) * inv);
+              o.y = pack_bf16(__uint_as_float(v[g * 8 + 2]) * inv, __uint_as_float(v[g * 8 + 3]) * inv);
+              o.z = pack_bf16(__uint_as_float(v[g * 8 + 4]) * inv, __uint_as_float(v[g * 8 + 5]) * inv);
+              o.w = pack_bf16(__uint_as_float(v[g * 8 + 6]) * inv, __uint_as_float(v[g * 8 + 7]) * inv);
+              *reinterpret_cast<uint4*>(orow + c * 32 + g * 8) = o;
+              if (rp.out_lo) {              // in place of these eight values
                 const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -497,7 +735,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 }
               }
             }
-            if (RPE && rp.out_lo) {
+            if (rp.out_lo) {
 #pragma unroll
               for (int g = 0; g < 2; ++g) {
                 uint32_t b[4];
@@ -512,7 +750,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           }
         }
         if (row < p.Lq)
-          p.lse[((long long)b * p.H + h) * p.Lq + row] = (m == -INFINITY ? 0.f : m) * (RPE ? LN2 : p.scale) + __logf(fmaxf(RPE ? l + lost_top : l, 1e-37f));
+          p.lse[((long long)b * p.H + h) * p.Lq + row] = (m == -INFINITY ? 0.f : m) * LN2 + __logf(fmaxf(l + lost_top, 1e-37f));
       }
     }
   }
@@ -1284,8 +1522,12 @@ static int attn_forward(const void* q, const void* k, const void* v, void* out, 
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -5;
   if (!(attr_set.load() >> dev & 1)) {
-    if (!RPE && cudaFuncSetAttribute(attn_fwd_kernel<false, RPE_NONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, FWD_SMEM) != cudaSuccess) return -5;
-    if (cudaFuncSetAttribute(attn_fwd_kernel<true, RPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, FWD_SMEM) != cudaSuccess) return -5;
+    if constexpr (RPE != RPE_NONE) {
+      if (cudaFuncSetAttribute(rpe_fwd_kernel<RPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, FWD_SMEM) != cudaSuccess) return -5;
+    } else {
+      if (cudaFuncSetAttribute(attn_fwd_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, FWD_SMEM) != cudaSuccess) return -5;
+      if (cudaFuncSetAttribute(attn_fwd_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, FWD_SMEM) != cudaSuccess) return -5;
+    }
     attr_set.fetch_or(1ull << dev);
   }
   FwdParams p{reinterpret_cast<__nv_bfloat16*>(out), lse, o_str[0], o_str[1], o_str[2], B, H, Lq, Lk, causal,
@@ -1299,8 +1541,8 @@ static int attn_forward(const void* q, const void* k, const void* v, void* out, 
   // measured gain at 128 MB, and nothing to gain at 256 MB.
   p.heads_fast = causal && (long long)B * H * Lk * HD * 4 <= (128LL << 20) && qblocks <= 65535 && B <= 65535;
   const dim3 grid = p.heads_fast ? dim3(H, B, qblocks) : dim3(qblocks, H, B);
-  auto* kernel = RPE || g_fwd_p_tmem ? attn_fwd_kernel<true, RPE> : attn_fwd_kernel<false, RPE_NONE>;
-  return launch_chained(false, kernel, grid, FWD_THREADS, FWD_SMEM, stream, tq, tk, tv, p, rp) ? -6 : 0;
+  if constexpr (RPE != RPE_NONE) return launch_chained(false, rpe_fwd_kernel<RPE>, grid, FWD_THREADS, FWD_SMEM, stream, tq, tk, tv, p, rp) ? -6 : 0;
+  else return launch_chained(false, g_fwd_p_tmem ? attn_fwd_kernel<true> : attn_fwd_kernel<false>, grid, FWD_THREADS, FWD_SMEM, stream, tq, tk, tv, p) ? -6 : 0;
 }
 
 
