@@ -66,8 +66,8 @@ struct FwdParams {
 //     order, with one sum per warp of the far tiles.
 //   - delta = sum(dO O) must be good to the rounding of dS itself: the forward divides by the sum of the ROUNDED probabilities, so that O is an
 //     exact average under slightly other weights, and hands on what O lost in rounding (out_lo).  The divisor in lse, which the backward's P
-//     has, gets back what the largest probability of each tile lost, which is most of it where a few keys have all the weight.  (A sum of
-//     the unrounded probabilities too cost the forward an eighth.)
+//     has, gets back what the largest probability of each tile lost, which is most of it where a few keys have all the weight.  Up to
+//     1024 tokens the probabilities enter in two parts instead (SPLIT below), and neither loses anything.
 //     What error e is left in a row's delta adds P e to each dS, and the sum of e over the rows is that of all dS, which should be zero: it is
 //     taken off the distances in proportion to their share of P, whose diagonals are summed up the same way.  (In a long causal row the far
 //     keys hold nearly all of P while their true sum is as small as that of the near ones: their error without this is a percent at 8192 keys.)
@@ -465,7 +465,13 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 // 3 x 777 x 4 22 / 21, 2 x 2048 x 16 both sides 91 / 87.  Without its exponentials it takes 537 at 8192, without most of its products 527, without
 // either 351: both sides are full.  Two threads a row, for the even and the odd steps, took 554 at 8192 and 85 for both sides; waits that spin
 // 549.
-template <int RPE>
+//
+// SPLIT: the probabilities enter the product as two bf16 values, the second what the first lost, in the other half of the step's buffer, and their
+// sum is that of the unrounded ones: the output is exact up to its own rounding, and so is delta.  The table's gradient then has an error of
+// 1e-5 to 3e-5 before its rounding, instead of 3e-4 to 2e-3, which counts most where few rows average it.  3 x 777 x 4 22 to 23
+// instead of 20 us; 2 x 2048 x 16 both sides 102 / 89, 8192 x 32 695 / 540: up to SPLIT_MAX tokens.
+constexpr int SPLIT_MAX = 1024;
+template <int RPE, bool SPLIT>
 __global__ void __launch_bounds__(FWD_THREADS, 1)
 rpe_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                const __grid_constant__ CUtensorMap tmV, FwdParams p, const __grid_constant__ RpeParams rp) {
@@ -563,8 +569,8 @@ rpe_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
               tc_fence_after();
               const uint32_t sV = sKV + vslot * TILE_BYTES;
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk)       // 16 keys = 8 packed columns of the step's score buffer
-                umma_bf16_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + buf * SUB + kk * 8, desc_mnmajor(sV, buf * 4 + kk), idesc_o,
+              for (int kk = 0; kk < (SPLIT ? 8 : 4); ++kk)       // 16 keys = 8 packed columns of the step's score buffer
+                umma_bf16_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + buf * SUB + kk * 8, desc_mnmajor(sV, buf * 4 + (kk & 3)), idesc_o,
                              (jp | kk) ? 1u : 0u);
               umma_commit(pv_done(t, buf));
               pv_idx[t] = jp + 1;
@@ -612,7 +618,7 @@ rpe_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     const uint32_t t_o = tmem_base + (uint32_t(quarter * 32) << 16) + 256 + t * 128;
     const float sl2 = p.scale_log2;
     float m = -INFINITY, l = 0.f;                    // m in units of log2, bias included
-    float lost_top = 0.f;                            // what the largest probability of each step lost in rounding
+    float lost_top = 0.f;                            // !SPLIT: what the largest probability of each step lost in rounding
     bool ok = true;
     // near steps reach distances from -127 (causal) or -far - 189 to far + 189
     const int origin = RPE == RPE_BOTH ? rp.far + 256 : 128;
@@ -668,26 +674,30 @@ rpe_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       const float alpha = (m == -INFINITY) ? 0.f : ex2(m - m_ref);
       const bool rescale = (j > 0) && (m_new != m);
       m = m_new;
-      // P = exp2(x - m) as bf16 over the scores; the row sum is that of the rounded values
+      // P = exp2(x - m) as bf16 over the scores; the row sum is that of what enters the product
       const float moff = add - m_ref;
-      f2 rounded[2] = {0, 0};
+      f2 sum[2] = {0, 0};
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        uint32_t pw[16];
+        uint32_t pw[16], lost_p[SPLIT ? 16 : 1];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const float ea = ex2(fmaf(__uint_as_float(v[c][2 * i]), mul, moff));
           const float eb = ex2(fmaf(__uint_as_float(v[c][2 * i + 1]), mul, moff));        // exp2(-inf) = 0 for masked keys
           pw[i] = pack_bf16(ea, eb);
-          rounded[i & 1] = f2_add(rounded[i & 1], f2_bf(pw[i]));
+          if constexpr (SPLIT) lost_p[i] = pack_bf16(ea - __uint_as_float(pw[i] << 16), eb - __uint_as_float(pw[i] & 0xffff0000u));
+          sum[i & 1] = f2_add(sum[i & 1], SPLIT ? f2_pack(ea, eb) : f2_bf(pw[i]));
         }
         tmem_st_32x16(t_s + buf * SUB + c * 16, pw);       // keys 32c .. 32c+31 -> packed columns 16c .. 16c+15
+        if constexpr (SPLIT) tmem_st_32x16(t_s + buf * SUB + 32 + c * 16, lost_p);
       }
       tmem_wait_st();
-      const float2 d = f2_unpack(f2_add(rounded[0], rounded[1]));
+      const float2 d = f2_unpack(f2_add(sum[0], sum[1]));
       l = l * alpha + (d.x + d.y);
-      const float e = ex2(fmaf(top, mul, moff));
-      lost_top = lost_top * alpha + (e - __uint_as_float(pack_bf16(0.f, e) & 0xffff0000u));
+      if (!SPLIT) {
+        const float e = ex2(fmaf(top, mul, moff));
+        lost_top = lost_top * alpha + (e - __uint_as_float(pack_bf16(0.f, e) & 0xffff0000u));
+      }
       if (__any_sync(0xffffffffu, rescale)) {
         // the product of the step before must have left O
         if (!mbar_wait(pv_done(t, buf ^ 1), uint32_t((j - 1) >> 1) & 1u, abort_flag, p.status, ST_ATTN + 8)) { ok = false; break; }
@@ -1523,7 +1533,8 @@ static int attn_forward(const void* q, const void* k, const void* v, void* out, 
   if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -5;
   if (!(attr_set.load() >> dev & 1)) {
     if constexpr (RPE != RPE_NONE) {
-      if (cudaFuncSetAttribute(rpe_fwd_kernel<RPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, FWD_SMEM) != cudaSuccess) return -5;
+      if (cudaFuncSetAttribute(rpe_fwd_kernel<RPE, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, FWD_SMEM) != cudaSuccess) return -5;
+      if (cudaFuncSetAttribute(rpe_fwd_kernel<RPE, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, FWD_SMEM) != cudaSuccess) return -5;
     } else {
       if (cudaFuncSetAttribute(attn_fwd_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, FWD_SMEM) != cudaSuccess) return -5;
       if (cudaFuncSetAttribute(attn_fwd_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, FWD_SMEM) != cudaSuccess) return -5;
@@ -1541,7 +1552,8 @@ static int attn_forward(const void* q, const void* k, const void* v, void* out, 
   // measured gain at 128 MB, and nothing to gain at 256 MB.
   p.heads_fast = causal && (long long)B * H * Lk * HD * 4 <= (128LL << 20) && qblocks <= 65535 && B <= 65535;
   const dim3 grid = p.heads_fast ? dim3(H, B, qblocks) : dim3(qblocks, H, B);
-  if constexpr (RPE != RPE_NONE) return launch_chained(false, rpe_fwd_kernel<RPE>, grid, FWD_THREADS, FWD_SMEM, stream, tq, tk, tv, p, rp) ? -6 : 0;
+  if constexpr (RPE != RPE_NONE) return launch_chained(false, Lk <= SPLIT_MAX ? rpe_fwd_kernel<RPE, true> : rpe_fwd_kernel<RPE, false>, grid, FWD_THREADS, FWD_SMEM,
+                                                       stream, tq, tk, tv, p, rp) ? -6 : 0;
   else return launch_chained(false, g_fwd_p_tmem ? attn_fwd_kernel<true> : attn_fwd_kernel<false>, grid, FWD_THREADS, FWD_SMEM, stream, tq, tk, tv, p) ? -6 : 0;
 }
 
