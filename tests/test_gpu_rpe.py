@@ -137,6 +137,18 @@ def test_maps_from_one_distance_to_the_longest(maxd, nb, causal):
         _inside(v, want, bound, name)
 
 
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "both"])
+@pytest.mark.parametrize("L", [1023, 1024, 1025])
+def test_where_the_probabilities_stop_entering_in_two_parts(L, causal):
+    c = _case(1, L, 2, 32, 128, causal, seed=L)
+    got = _run(*c[:3], math.sqrt(128), causal, c[3])
+    _status_ok()
+    for name, v, (want, bound) in zip(("o", "dqkv", "dtable"), got, _exact(*c[:3], math.sqrt(128), causal, c[3])):
+        _inside(v, want, bound, name)
+    with torch.no_grad():
+        assert torch.equal(ops.attention_rpe(*c[:3], math.sqrt(128), causal), got[0])
+
+
 def test_one_token_has_a_gradient_for_its_value_alone():
     for causal in (True, False):
         qkv, table, buckets, go = _case(3, 1, 5, 32, 128, causal)
