@@ -138,6 +138,12 @@ Tensor aligned(const Tensor& t) {
   return on16(c) ? c : c.clone();
 }
 Tensor aligned(const OptTensor& t) { return t.has_value() ? aligned(*t) : Tensor(); }
+// A saved tensor as it was saved: hooks may have given back other strides (made contiguous here) or another tensor altogether (refused).
+Tensor as_saved(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, at::Device device) {
+  TORCH_CHECK(t.defined() && t.sizes() == sizes && t.scalar_type() == type && t.device() == device, "a saved tensor's hooks gave back ",
+              t.defined() ? t.toString() : "nothing", " ", t.defined() ? t.sizes() : at::IntArrayRef(), ": ", type, " ", sizes, " on ", device, " was saved");
+  return aligned(t);
+}
 Tensor f32c(const Tensor& t) {
   Tensor d = t.detach();
   if (d.scalar_type() != F32) d = d.to(F32);
@@ -805,10 +811,9 @@ struct FlashRpe : Function<FlashRpe> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const variable_list s = ctx->get_saved_variables();
-    const Tensor &qkv = s[0], &buckets = s[2], &o = s[3], &lo = s[4], &lse = s[5];
     const bool causal = ctx->saved_data["causal"].toBool();
     if (at::GradMode::is_enabled()) {                    // create_graph
-      const Tensor again = rpe_statement(qkv, s[1], buckets, ctx->saved_data["bias_scale"].toDouble(), causal);
+      const Tensor again = rpe_statement(s[0], s[1], s[2], ctx->saved_data["bias_scale"].toDouble(), causal);
       variable_list wanted;
       for (const Tensor* t : {&s[0], &s[1]})
         if (t->requires_grad()) wanted.push_back(*t);
@@ -816,9 +821,14 @@ struct FlashRpe : Function<FlashRpe> {
       Tensor none;
       return {s[0].requires_grad() ? d.front() : none, s[1].requires_grad() ? d.back() : none, none, none, none};
     }
-    const Tensor table = contiguous(s[1]);
-    const int64_t B = qkv.size(0), Ln = qkv.size(1), H = qkv.size(2), far = causal ? buckets.size(0) - 1 : buckets.size(0) / 2;
-    const at::Device dev = qkv.device();
+    const int64_t B = g[0].size(0), Ln = g[0].size(1), H = g[0].size(2);
+    const at::Device dev = g[0].device();
+    const Tensor qkv = as_saved(s[0], {B, Ln, H, 384}, BF16, dev), o = as_saved(s[3], {B, Ln, H, 128}, BF16, dev),
+                 lo = as_saved(s[4], {B, Ln, H, 128}, at::kChar, dev), lse = as_saved(s[5], {B, H, Ln}, F32, dev),
+                 table = as_saved(s[1], {s[1].size(0), H}, s[1].scalar_type() == BF16 ? BF16 : F32, dev),
+                 buckets = as_saved(s[2], {s[2].numel()}, at::kInt, dev);
+    TORCH_CHECK(causal || buckets.size(0) % 2 == 1, "a saved tensor's hooks gave back a bucket map of ", buckets.size(0), " entries");
+    const int64_t far = causal ? buckets.size(0) - 1 : buckets.size(0) / 2;
     Tensor dqkv = alloc(qkv.sizes(), BF16, dev), dtable = alloc_like(table);
     if (Ln <= 1 || B * H == 0) {
       cleared(dqkv);
