@@ -142,7 +142,7 @@ Tensor aligned(const OptTensor& t) { return t.has_value() ? aligned(*t) : Tensor
 Tensor as_saved(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, at::Device device) {
   TORCH_CHECK(t.defined() && t.sizes() == sizes && t.scalar_type() == type && t.device() == device, "a saved tensor's hooks gave back ",
               t.defined() ? t.toString() : "nothing", " ", t.defined() ? t.sizes() : at::IntArrayRef(), ": ", type, " ", sizes, " on ", device, " was saved");
-  return aligned(t);
+  return contiguous(t);
 }
 Tensor f32c(const Tensor& t) {
   Tensor d = t.detach();
@@ -398,12 +398,14 @@ struct LayerNorm : Function<LayerNorm> {
       const Tensor dx = std::get<0>(d);
       return {gres.defined() ? dx + gres : dx, std::get<1>(d), std::get<2>(d), Tensor(), Tensor()};
     }
-    const Tensor xc = contiguous(x), w = contiguous(s[1]), gy = contiguous(g[0]), gr = gres.defined() ? contiguous(gres) : Tensor();
     const int64_t T = x.numel() / D;
-    const int type = type_code(x.scalar_type());
-    Tensor dx = alloc_like(x), dw = alloc({D}, x.scalar_type(), x.device()), db = alloc_like(dw),
-           partial = alloc({(int64_t)L.sb_layernorm_bwd_blocks(T, D, type) * 2 * D}, F32, x.device());
-    SB_CALL(sb_layernorm_bwd, T > 0 ? 2 : 1, ptr(xc), ptr(w), ptr(gy), f32(st), ptr(gr), out(dx), out(dw), out(db), f32o(partial), (int)T, (int)D,
+    const at::ScalarType xt = g[0].scalar_type();
+    const at::Device dev = g[0].device();
+    const Tensor xc = as_saved(x, g[0].sizes(), xt, dev), w = as_saved(s[1], {D}, xt, dev), sc = as_saved(st, {T, 2}, F32, dev), gy = contiguous(g[0]), gr = gres.defined() ? contiguous(gres) : Tensor();
+    const int type = type_code(xt);
+    Tensor dx = alloc_like(xc), dw = alloc({D}, xt, dev), db = alloc_like(dw),
+           partial = alloc({(int64_t)L.sb_layernorm_bwd_blocks(T, D, type) * 2 * D}, F32, dev);
+    SB_CALL(sb_layernorm_bwd, T > 0 ? 2 : 1, ptr(xc), ptr(w), ptr(gy), f32(sc), ptr(gr), out(dx), out(dw), out(db), f32o(partial), (int)T, (int)D,
             type, stream());
     return {dx, dw, db, Tensor(), Tensor()};
   }
@@ -823,8 +825,8 @@ struct FlashRpe : Function<FlashRpe> {
     }
     const int64_t B = g[0].size(0), Ln = g[0].size(1), H = g[0].size(2);
     const at::Device dev = g[0].device();
-    const Tensor qkv = as_saved(s[0], {B, Ln, H, 384}, BF16, dev), o = as_saved(s[3], {B, Ln, H, 128}, BF16, dev),
-                 lo = as_saved(s[4], {B, Ln, H, 128}, at::kChar, dev), lse = as_saved(s[5], {B, H, Ln}, F32, dev),
+    const Tensor qkv = aligned(as_saved(s[0], {B, Ln, H, 384}, BF16, dev)), o = aligned(as_saved(s[3], {B, Ln, H, 128}, BF16, dev)),
+                 lo = aligned(as_saved(s[4], {B, Ln, H, 128}, at::kChar, dev)), lse = as_saved(s[5], {B, H, Ln}, F32, dev),
                  table = as_saved(s[1], {s[1].size(0), H}, s[1].scalar_type() == BF16 ? BF16 : F32, dev),
                  buckets = as_saved(s[2], {s[2].numel()}, at::kInt, dev);
     TORCH_CHECK(causal || buckets.size(0) % 2 == 1, "a saved tensor's hooks gave back a bucket map of ", buckets.size(0), " entries");

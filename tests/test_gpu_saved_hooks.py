@@ -73,3 +73,31 @@ def test_attention_rpe_backward_refuses_other_tensors():
             o = ops.attention_rpe(qkv, table, buckets, 1.0, False)
         with pytest.raises(RuntimeError):
             torch.autograd.grad(o, (qkv, table), go)
+
+
+def _norm(T, D, dtype):
+    g = torch.Generator(device=DEV).manual_seed(T + D)
+    x, gy, gr = ((torch.randn(2, T, D, generator=g, device=DEV)).to(dtype) for _ in range(3))
+    w, b = ((1 + 0.1 * torch.randn(D, generator=g, device=DEV)).to(dtype) for _ in range(2))
+    return [t.requires_grad_(True) for t in (x, w, b)], gy, gr
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("T,D", [(40, 64), (33, 1000), (17, 331)])
+def test_layernorm_backward_of_other_strides(T, D, dtype):
+    leaves, gy, gr = _norm(T, D, dtype)
+    want = torch.autograd.grad(ops.layernorm_residual(*leaves, 1e-5), leaves, (gy, gr))
+    with _hooks(_other_strides):
+        y = ops.layernorm_residual(*leaves, 1e-5)
+    for got, w in zip(torch.autograd.grad(y, leaves, (gy, gr)), want):
+        assert torch.equal(got, w)
+
+
+def test_layernorm_backward_refuses_other_tensors():
+    leaves, gy, _ = _norm(20, 96, BF)
+    for change in (lambda t: t.cpu(), lambda t: t.float() if t.dtype == BF else t, lambda t: t[:, :10] if t.dim() == 3 else t,
+                   lambda t: t[:5] if t.dim() == 2 else t, lambda t: t[:40] if t.dim() == 1 else t):
+        with _hooks(change):
+            y = ops.layernorm(*leaves, 1e-5)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, leaves, gy)
