@@ -132,6 +132,7 @@ step_kernel(const Args a) {
       s[u] = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) s[u] = fmaf(q[i], f[i], s[u]);
+      if (!have) s[u] = 0.f;               // columns that this lane has not: 0 * inf of others' would be NaN
     }
 #pragma unroll
     for (int d = LPK / 2; d; d >>= 1)
