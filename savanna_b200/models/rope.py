@@ -17,18 +17,21 @@ from ..parallel import state
 
 def consecutive_positions(n: int, device=None) -> torch.Tensor:
     """0 .. n - 1, marked as such: operators that work by distance need not look at the values then."""
-    return mark_consecutive(torch.arange(n, device=device))
+    with torch.inference_mode(False):            # what is made in inference mode does not count the writes to it
+        return mark_consecutive(torch.arange(n, device=device))
 
 
 def mark_consecutive(positions: torch.Tensor) -> torch.Tensor:
-    positions._consecutive = 0 if positions.is_inference() else positions._version
+    """Marks positions that are 0 .. n - 1; a tensor made in inference mode, whose later writes nobody would see, stays without a mark."""
+    if not positions.is_inference():
+        positions._consecutive = positions._version
     return positions
 
 
 def are_consecutive(positions: torch.Tensor) -> bool:
     """Whether `positions` were made by `consecutive_positions` and not written to since; False says nothing about the values."""
     mark = getattr(positions, "_consecutive", None)
-    return mark is not None and mark == (0 if positions.is_inference() else positions._version)
+    return mark is not None and mark == positions._version
 
 
 class RotaryEmbedding(nn.Module):
