@@ -759,8 +759,10 @@ rpe_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
             }
           }
         }
-        if (row < p.Lq)
-          p.lse[((long long)b * p.H + h) * p.Lq + row] = (m == -INFINITY ? 0.f : m) * LN2 + __logf(fmaxf(l + lost_top, 1e-37f));
+        if (row < p.Lq) {
+          const float total = l + lost_top;          // NaN stays NaN, and makes the backward's P of the whole row NaN
+          p.lse[((long long)b * p.H + h) * p.Lq + row] = (m == -INFINITY ? 0.f : m) * LN2 + __logf(total < 1e-37f ? 1e-37f : total);
+        }
       }
     }
   }
