@@ -17,6 +17,7 @@
 #include <mutex>
 #include <sstream>
 
+#include <ATen/Context.h>
 #include <ATen/autocast_mode.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -969,9 +970,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     if (qkv.scalar_type() != BF16 || qkv.size(3) != 384 || !qkv.is_contiguous() || !on16(qkv) || qkv.size(0) >= 65535 || qkv.size(1) >= (1LL << 30) ||
         (causal ? buckets.size(0) - 1 : buckets.size(0) / 2) > max_far)
       return std::nullopt;
+    const bool train = wants_grad({&qkv, &table});
+    if (train && at::globalContext().deterministicAlgorithms()) return std::nullopt;       // the query gradient's order of addition varies
     const c10::cuda::CUDAGuard device(qkv.device());
     const Tensor t = table.scalar_type() == BF16 || table.scalar_type() == F32 ? table : table.to(F32);
-    if (!wants_grad({&qkv, &table})) return rpe_fwd(qkv, t, buckets, bias_scale, causal, false).o;
+    if (!train) return rpe_fwd(qkv, t, buckets, bias_scale, causal, false).o;
     return FlashRpe::apply(qkv, t, buckets, bias_scale, causal);
   });
   m.def("attention_rpe_step", [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& buckets, double bias_scale,

@@ -242,8 +242,8 @@ def _check_rpe(table, buckets, heads, device, causal):
 
 
 def attention_rpe_covers(qkv, far: int) -> bool:
-    """Whether `attention_rpe` runs the flash kernels: CUDA, contiguous bf16, heads of 128, `far` at most 1024.  It materialises the scores
-    otherwise."""
+    """Whether `attention_rpe` has flash kernels for the shape: CUDA, contiguous bf16, heads of 128, `far` at most 1024.  It materialises the
+    scores otherwise."""
     if not _k(qkv):
         return False
     from . import flash_sm100
@@ -257,7 +257,8 @@ def attention_rpe(qkv, table, buckets, scale: float = 1.0, causal: bool = True):
     table [nb, H]; buckets int32, the bucket of each distance query - key: [far + 1] for 0 .. far (causal) or [2 far + 1] for -far .. far,
     where what lies further away has the outermost entry's (`RelativePositionBias.bucket_map`).  An entry outside 0 .. nb - 1 has no bias on the
     kernel path.  The kernels form no [L, L] bias or scores; their query gradient is added up in an order that varies, as that of
-    `attention_packed` does, the table's in a fixed one."""
+    `attention_packed` does, the table's in a fixed one.  Under `torch.use_deterministic_algorithms` calls that want gradients therefore
+    materialise the scores, in fp32."""
     if _k(qkv):
         o = _CO.attention_rpe(qkv, table, buckets, scale, causal, RPE_MAX_FAR)
         if o is not None:
