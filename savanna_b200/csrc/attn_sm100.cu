@@ -93,9 +93,10 @@ struct RpeParams {
   int x_lo, x_hi;            // near tiles: query tile start - key block start, in units of 64
   float* acc;                // dq_acc, which the statistics kernel clears
 };
-// What fp32 bits x lost in being rounded to the bf16 bits hi (shifted up): their difference, of which the second byte is kept.  The integer
-// difference holds across an exponent's border too; 0x8000 (a tie that was rounded down) would come back as its negative.
-__device__ __forceinline__ uint32_t lost(float x, uint32_t hi) { return (uint32_t)min(int(__float_as_uint(x) - hi), 0x7fff); }
+// What fp32 bits x lost in being rounded to the bf16 bits hi (shifted up): their difference, of which the second byte is kept, rounded to its
+// nearest value (cut off, all outputs would come back half a 256th of a step too small; one that lost nothing comes back as it is).  The integer
+// difference holds across an exponent's border too; half a step up (0x7f80 on) would come back as its negative.
+__device__ __forceinline__ uint32_t lost(float x, uint32_t hi) { return (uint32_t)min(int(__float_as_uint(x) - hi) + 128, 0x7fff); }
 __device__ __forceinline__ float regained(uint32_t hi, int8_t lo) { return __uint_as_float(hi + (uint32_t)((int)lo * 256)); }
 // log2(e) * bias at distance d of head h; a bucket that does not exist has none
 __device__ __forceinline__ float rpe_value(const RpeParams& r, int mode, int H, int h, int d) {
