@@ -20,6 +20,7 @@ namespace act8 {
 
 typedef __nv_bfloat16 bf16;
 constexpr int BLOCK = 128;               // values that share a scale
+constexpr int MAX_D = 0x7fffffff - (BLOCK - 1);          // of a row: the number of its blocks is counted in 32 bits
 constexpr float TINY = 1e-30f;
 
 __device__ __forceinline__ float up(bf16 v) { return __bfloat162float(v); }
@@ -234,14 +235,14 @@ using namespace sb::act8;
 
 // x [rows, D] of type 0 (bf16), 1 (fp16) or 2 (fp32) -> q [rows, D] int8 and scale [rows, ceil(D / 128)] fp32.
 extern "C" int sb_act8_quantize(const void* x, void* q, float* scale, long long rows, int D, int type, cudaStream_t st) {
-  if (rows < 0 || D < 1 || type < 0 || type > 2) return -1;
+  if (rows < 0 || D < 1 || D > MAX_D || type < 0 || type > 2) return -1;
   if (rows == 0) return 0;
   const bool vec = by_vector(x, q, D);
   return type == 0 ? quantize<bf16>(x, q, scale, rows, D, vec, st) : type == 1 ? quantize<__half>(x, q, scale, rows, D, vec, st)
                                                                               : quantize<float>(x, q, scale, rows, D, vec, st);
 }
 extern "C" int sb_act8_dequantize(const void* q, const float* scale, void* x, long long rows, int D, int type, cudaStream_t st) {
-  if (rows < 0 || D < 1 || type < 0 || type > 2) return -1;
+  if (rows < 0 || D < 1 || D > MAX_D || type < 0 || type > 2) return -1;
   if (rows == 0) return 0;
   const bool vec = by_vector(x, q, D);
   return type == 0 ? dequantize<bf16>(q, scale, x, rows, D, vec, st) : type == 1 ? dequantize<__half>(q, scale, x, rows, D, vec, st)

@@ -865,6 +865,8 @@ void check_rpe(const Tensor& table, const Tensor& buckets, int64_t heads, at::De
                     "relative position table and bucket map belong on the device of the attention's inputs");
 }
 
+constexpr int64_t MAX_ACT_D = (1LL << 31) - 128;          // values of a row of act8.cu, whose columns have 32 bits
+
 // ------------------------------------------------------------------------------------ what Python calls
 bool fused(const py::handle& w) {          // the parameter's gradient lives in a persistent flat buffer (set by the ZeRO optimizers)
   PyObject* v = PyObject_GetAttrString(w.ptr(), "_fuse_grad_accum");
@@ -910,6 +912,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     const at::ScalarType type = x.scalar_type();
     TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && (type == BF16 || type == at::kHalf || type == F32),
                       "act_quantize takes bf16, fp16 or fp32 [..., D] with D >= 1, got ", type, " ", x.sizes());
+    TORCH_CHECK_VALUE(x.size(-1) <= MAX_ACT_D, "act_quantize takes rows of up to ", MAX_ACT_D, " values, got ", x.sizes());
     const c10::cuda::CUDAGuard device(x.device());
     const at::AutoDispatchBelowADInplaceOrView no_graph;
     const Tensor xc = contiguous(x);
@@ -924,6 +927,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
                       scale.sizes().vec() == with_last(q.sizes(), (q.size(-1) + 127) / 128),
                       "act_dequantize takes what act_quantize returned, got q ", q.scalar_type(), " ", q.sizes(), ", scale ", scale.scalar_type(), " ",
                       scale.sizes());
+    TORCH_CHECK_VALUE(q.size(-1) <= MAX_ACT_D, "act_dequantize takes rows of up to ", MAX_ACT_D, " values, got ", q.sizes());
     const c10::cuda::CUDAGuard device(q.device());
     const at::AutoDispatchBelowADInplaceOrView no_graph;
     const Tensor qc = contiguous(q), sc = contiguous(scale);

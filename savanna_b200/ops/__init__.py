@@ -293,8 +293,8 @@ def attention_rpe_step(q, k, v, table, buckets, scale: float = 1.0, lengths=None
 
 def act_quantize(x):
     """x [..., D] (bf16, fp16 or fp32) -> (q int8 of x's shape, scale fp32 [..., ceil(D / 128)]): 128 consecutive values of a row share
-    a scale of amax / 127, so that a value comes back within amax / 254 of itself and a rounding to its type.  A block that holds an infinity
-    or NaN comes back as NaN.  Not differentiated: the form in which a checkpointed activation waits for its recomputation."""
+    a scale of amax / 127, so that a value comes back within amax / 254 of itself and a rounding to its type (where amax is below 1e-30, as nearly
+    zero).  A block that holds an infinity or NaN comes back as NaN.  CUDA: rows of up to 2^31 - 128 values.  Not differentiated: the form in which a checkpointed activation waits for its recomputation."""
     if _k(x):
         return _CO.act_quantize(x)
     if x.dim() < 1 or x.shape[-1] < 1 or x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
