@@ -65,12 +65,16 @@ struct FwdParams {
 //     the diagonals from lane to lane.  Each warp writes its 64 sums to a place of its own, and rpe_finish_kernel adds them up in a fixed
 //     order, with one sum per warp of the far tiles.
 //   - delta = sum(dO O) must be good to the rounding of dS itself: the forward divides by the sum of the ROUNDED probabilities, so that O is an
-//     exact average under slightly other weights, and hands on what O lost in rounding (out_lo).  The divisor in lse, which the backward's P
-//     has, gets back what the largest probability of each tile lost, which is most of it where a few keys have all the weight.  Up to
-//     1024 tokens the probabilities enter in two parts instead (SPLIT below), and neither loses anything.
+//     exact average under slightly other weights, and hands on what O lost in rounding (out_lo, to half a 256th of a step).  The divisor in lse,
+//     which the backward's P has, gets back what the largest probability of each step lost, which is most of it where a few keys have all the
+//     weight (the sum of all unrounded ones would cost 85 us of 555).  Up to 1024 tokens the probabilities enter in two parts instead (SPLIT below),
+//     which leaves 2^-16 of them.
 //     What error e is left in a row's delta adds P e to each dS, and the sum of e over the rows is that of all dS, which should be zero: it is
-//     taken off the distances in proportion to their share of P, whose diagonals are summed up the same way.  (In a long causal row the far
-//     keys hold nearly all of P while their true sum is as small as that of the near ones: their error without this is a percent at 8192 keys.)
+//     taken off the distances in proportion to their share of P, whose diagonals are summed up the same way.  Error of the table's gradient before
+//     its rounding, 2-norm, random inputs, without that / with it: 1100 tokens causal 1.1e-3 / 8e-4, both sides 1.5e-3 / 1.0e-3; 8192 tokens 1.2e-3 /
+//     1.1e-3, both sides 2.7e-3 / 1.45e-3 (root mean squares; single heads up to 3.8e-3 with it); up to 1024 tokens, in two parts, 6e-6 either way.
+//   - P and dS enter the backward's three last products as bf16, at every length, as they do without a bias: each gradient is a sum of products with
+//     one factor off by 2^-8 at most.  As two values each they would double those three products (the tensor pipe is busy for 46 % of the kernel).
 //
 // Measured beside the kernels without bias, us, causal with far = 128 / both sides with far = 256: forward 8192 x 32 heads 540 / - (550), 2 x 2048
 // x 16 heads - / 87 (82); with the backward pass 2127 / - (2089), - / 376 (315), 3 x 777 x 4 heads 65 / - (53).  A tile of the backward that is
@@ -463,14 +467,15 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 // step ends, and the chain scores - softmax - P V - next scores, which bounds the kernel above, is cut.  The price is that a product of 64 key rows
 // reads its queries twice as often (1.5 times the time of the score products, by the shared memory's bandwidth).  Four slots for K and V, in the
 // shared memory that P does not need.  us, 128 keys a step in the kernel above / here: 8192 x 32 heads causal 559 / 540, 2 x 1333 x 16 35.6 / 31.7,
-// 3 x 777 x 4 22 / 21, 2 x 2048 x 16 both sides 91 / 87.  Without its exponentials it takes 537 at 8192, without most of its products 527, without
-// either 351: both sides are full.  Two threads a row, for the even and the odd steps, took 554 at 8192 and 85 for both sides; waits that spin
-// 549.
+// 3 x 777 x 4 22 / 21, 2 x 2048 x 16 both sides 91 / 87.  What bounds it is that a step's two sides wait for each other: no pipe is busy for more
+// than half of the time (tensor 48 %, exponentials 50 %), and without its exponentials it takes 537 at 8192, without most of its products 527, but
+// without either 351.  Two threads a row, for the even and the odd steps, took 554 at 8192 and 85 for both sides; waits that spin 549.
 //
-// SPLIT: the probabilities enter the product as two bf16 values, the second what the first lost, in the other half of the step's buffer, and their
-// sum is that of the unrounded ones: the output is exact up to its own rounding, and so is delta.  The table's gradient then has an error of
-// 1e-5 to 3e-5 before its rounding, instead of 3e-4 to 2e-3, which counts most where few rows average it.  3 x 777 x 4 22 to 23
-// instead of 20 us; 2 x 2048 x 16 both sides 102 / 89, 8192 x 32 695 / 540: up to SPLIT_MAX tokens.
+// SPLIT: the probabilities enter the product as two bf16 values, the second what the first lost, in the other half of the step's buffer, and are
+// divided by the sum of the unrounded ones.  The two hold P to 2^-16, so that the output before its rounding, and delta, are off by that and by the
+// 32-bit sums (2^-17).  The table's gradient then has an error of 1e-6 to 1.5e-5 before its rounding, instead of 1e-4 to 4e-3, which counts
+// most where few rows average it.  3 x 777 x 4 22 to 23 instead of 20 us; 2 x 2048 x 16 both sides 102 / 89, 8192 x 32 695 / 540: up to
+// SPLIT_MAX tokens.
 constexpr int SPLIT_MAX = 1024;
 template <int RPE, bool SPLIT>
 __global__ void __launch_bounds__(FWD_THREADS, 1)

@@ -291,6 +291,8 @@ static int launch(const Args& a, int B, cudaStream_t st) {
   // With long blocks on all SMs alike the reads of the far bias in every step cost more.  us, late / early: 8 sequences of 300, 32 heads of 128
   // 13.4 / 12.4; of up to 2000 28.9 / 25.4, of 2000 each 43.3 / 43.8; 12 of up to 1500, 16 heads of 64 15.7 / 14.1; one of 7000 28.4 / 25.2, of
   // 16000 44.1 / 44.9, of 32768 82.9 / 87.5; 8 of 16384, 16 heads of 64 82.8 / 93, of up to 16384 50.5 / 45.4.
+  // The lengths are on the device: a batch that passes them is taken for one of unequal sequences, and where they are equal and long it goes
+  // without the late form's gain.
   const bool early = (a.lengths && B > 1) || a.T <= 1024 * a.splits;
   auto* kernel = early ? a.hd <= 64 ? step_kernel<T, 8, true> : a.hd <= 128 ? step_kernel<T, 16, true> : step_kernel<T, 32, true>
                        : a.hd <= 64 ? step_kernel<T, 8, false> : a.hd <= 128 ? step_kernel<T, 16, false> : step_kernel<T, 32, false>;

@@ -62,8 +62,8 @@ class SelfAttention(nn.Module):
         self.score_bias = None
         if cfg.pos_emb in ("alibi", "rpe"):
             if operator_type != "global":
-                raise NotImplementedError(f"pos_emb={cfg.pos_emb!r} needs the `global` attention operator "
-                                          f"(got {operator_type!r}): the flash kernels take no score bias")
+                raise NotImplementedError(f"pos_emb={cfg.pos_emb!r} needs the `global` attention operator (got {operator_type!r}): "
+                                          "the others take no score bias")
             from .rope import AliBi, RelativePositionBias
             rank = state.get_model_parallel_rank()
             if cfg.pos_emb == "alibi":
