@@ -50,7 +50,8 @@ constexpr auto F32 = at::kFloat;
   X(sb_se_fwd) X(sb_se_fwd_taps) X(sb_se_bwd) X(sb_mr_fwd) X(sb_mr_bwd) X(sb_mr_tc_fwd) X(sb_mr_tc_bwd) X(sb_mr_umma_fwd) X(sb_mr_umma_bwd) \
   X(sb_li_fwd_tiled) \
   X(sb_li_bwd_tiled_chunk) X(sb_li_bwd_tiled) X(sb_attn_fwd) X(sb_attn_bwd) X(sb_attn_rope) \
-  X(sb_attn_step_splits) X(sb_attn_step) X(sb_attn_rpe_fwd) X(sb_attn_rpe_bwd_work) X(sb_attn_rpe_bwd) X(sb_layernorm_fwd) X(sb_layernorm_bwd_blocks) X(sb_layernorm_bwd) X(sb_act8_quantize) X(sb_act8_dequantize)
+  X(sb_attn_step_splits) X(sb_attn_step) X(sb_attn_rpe_fwd) X(sb_attn_rpe_bwd_work) X(sb_attn_rpe_bwd) X(sb_layernorm_fwd) X(sb_layernorm_bwd_blocks) X(sb_layernorm_bwd) X(sb_act8_quantize) X(sb_act8_dequantize) \
+  X(sb_fp8_block_quantize) X(sb_fp8_block_column_sums) X(sb_fp8_block_norm) X(sb_fp8_block_dequantize) X(sb_gemm_fp8_block)
 
 struct {
 #define SB_DECLARE(name) decltype(&::name) name = nullptr;
@@ -877,6 +878,8 @@ bool fused(const py::handle& w) {          // the parameter's gradient lives in 
 }
 OptTensor table(const OptTensor& t) { return t.has_value() ? OptTensor(aligned(t->to(F32))) : t; }
 
+#include "autograd_fp8_block.h"
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -937,6 +940,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     SB_CALL(sb_act8_dequantize, T > 0, ptr(qc), f32(sc), out(x), (long long)T, (int)D, (int)type, stream());
     return x;
   });
+  m.def("fp8_block_quantize", &fp8_block_quantize);
+  m.def("fp8_block_dequantize", &fp8_block_dequantize);
+  m.def("rmsnorm_fp8_block", &rmsnorm_fp8_block);
+  m.def("linear_fp8_block", &linear_fp8_block);
+  m.def("norm_linear_fp8_block", &norm_linear_fp8_block);
   m.def("norm_linear", [](const Tensor& x, const Tensor& wn, double eps, int64_t form, const py::object& w, const OptTensor& bias) {
     no_transforms();
     const Tensor wt = w.cast<Tensor>();

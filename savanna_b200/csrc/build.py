@@ -27,7 +27,7 @@ CUDA_LIB = os.path.join(PKG, "libsavanna_b200.so")
 DATA_LIB = os.path.join(PKG, "libsavanna_data.so")
 NATIVE_MODULE = os.path.join(PKG, "_native.so")
 NATIVE_SOURCES = ("autograd_native.cpp",)
-NATIVE_HEADERS = ("entries.h",)
+NATIVE_HEADERS = ("entries.h", "autograd_fp8_block.h")
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xptxas", "-v"]

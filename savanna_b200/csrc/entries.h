@@ -68,6 +68,18 @@ int sb_layernorm_bwd(const void* x, const void* w, const void* dy, const float* 
 // act8.cu
 int sb_act8_quantize(const void* x, void* q, float* scale, long long rows, int D, int type, cudaStream_t st);
 int sb_act8_dequantize(const void* q, const float* scale, void* x, long long rows, int D, int type, cudaStream_t st);
+// fp8_block.cu
+int sb_fp8_block_quantize(const void* x, long long ld, long long R, int C, int type, int form, void* q_rows, float* s_rows, void* q_cols,
+                          float* s_cols, long long ldq, const float* a, const void* g, float* sums, cudaStream_t st);
+int sb_fp8_block_column_sums(const float* sums, void* out, long long tiles, int C, int type, cudaStream_t st);
+int sb_fp8_block_norm(const void* x, long long ldx, const void* res, long long ldr, const void* g, void* sum, void* q, long long ldq,
+                      float* scale, float* a, long long T, int D, float eps, int form, int type, cudaStream_t st);
+int sb_fp8_block_dequantize(const void* q, long long ldq, const float* scale, long long s_row, long long s_col, int tiles, void* x,
+                            long long R, int C, int type, cudaStream_t st);
+// gemm_fp8_block.cu
+int sb_gemm_fp8_block(const void* A, const float* sa, long long sa_m, long long sa_k, const void* B, const float* sb, long long sb_n,
+                      long long sb_k, int sb_rows, void* C, const void* bias, const void* residual, int M, int N, int K, long long lda, long long ldb,
+                      long long ldc, long long ldr, int a_mn, int b_mn, int type, int beta, unsigned int* status, cudaStream_t stream);
 // attn_sm100.cu
 int sb_attn_fwd(const void* q, const void* k, const void* v, void* out, float* lse, int B, int H, int Lq, int Lk, const long long* q_str,
                 const long long* k_str, const long long* v_str, const long long* o_str, int causal, float scale, unsigned int* status,

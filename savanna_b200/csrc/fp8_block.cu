@@ -1,0 +1,390 @@
+// Operands of the block-scaled 8-bit products (gemm_fp8_block.cu) from 16- or 32-bit tensors, and back:
+//
+//   quantise   x [R, C] -> e4m3 with a scale for 128 values of a row, of a column, of both (two forms from one read), or of a 128 x 128 tile
+//   norm       s = x + residual;  y = s / rms(s) * g  -> e4m3 with a scale for 128 values of a row; y itself is never rounded to 16 bits
+//   dequantise
+//
+// Layouts.  Codes keep the shape of x; their rows are `ldq` bytes apart (a multiple of 16, what the tensor-core product's loads need).
+// Scales lie with the direction that the product does not contract contiguous: [C / 128][R] for rows, [R / 128][C] for columns (a warp of the
+// product reads those of 32 neighbouring rows at once), [R / 128][C / 128] for tiles.
+#include "device_info.h"
+#include "entries.h"
+#include "fp8_block.cuh"
+
+namespace sb {
+namespace blk8 {
+
+// ------------------------------------------------------------------------------------------------ tiles of 128 x 128
+// A block of 256 threads holds a tile in registers: sixteen threads eight columns each, eight rows a thread, all loads issued before the
+// first value is used.  From there a row's largest magnitude is four shuffles away and a column's one exchange through shared memory, so the
+// second form of the codes costs its writes alone.
+struct QuantArgs {
+  const void* x;
+  long long ld, R;
+  int C;
+  long long ldq;                   // of both forms
+  uint8_t* q_rows;                 // scales of rows, or of tiles
+  float* s_rows;
+  uint8_t* q_cols;
+  float* s_cols;
+  const float* a;                  // NORM: x * a[row] * g[column] is quantised
+  const void* g;
+  float* sums;                     // [R / 128][C] sums of x over a tile's rows (a bias gradient), or null
+  long long col_tiles;
+};
+
+enum { ROWS = 1, COLS = 2, TILE = 4 };
+
+template <class T, int FORM, bool NORM, bool VEC>
+__global__ void __launch_bounds__(256)
+quantize_kernel(QuantArgs p) {
+  __shared__ uint32_t part[8][BLOCK];                       // columns' largest magnitudes by warp
+  __shared__ float sum_part[8][BLOCK];
+  __shared__ float row_scale[BLOCK];
+  __shared__ uint32_t col_max[BLOCK];
+  const long long tile_r = blockIdx.x / p.col_tiles, tile_c = blockIdx.x - tile_r * p.col_tiles;
+  const int l = threadIdx.x & 15, h = threadIdx.x >> 4, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long r0 = tile_r * BLOCK;
+  const int c0 = int(tile_c) * BLOCK + l * 8;
+  const int n = min(8, p.C - c0);                           // of the thread's columns
+  const int rows = int(min((long long)BLOCK, p.R - r0));
+  const T* x = static_cast<const T*>(p.x) + r0 * p.ld + c0;
+  Eight<T> raw[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = h + 16 * i;
+    raw[i] = fetch<VEC, T>(x + r * p.ld, r < rows ? n : 0);
+  }
+  float g[8], a[8];
+  if (NORM) {
+    unpack(fetch<VEC, T>(static_cast<const T*>(p.g) + c0, n), g);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = h + 16 * i < rows ? p.a[r0 + h + 16 * i] : 0.f;
+  }
+  auto values = [&](int i, float (&f)[8]) {
+    unpack(raw[i], f);
+    if (NORM) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = f[j] * a[i] * g[j];
+    }
+  };
+  uint32_t cm[8];
+  float cs[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) { cm[j] = 0u; cs[j] = 0.f; }
+  uint32_t tile_max = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float f[8];
+    values(i, f);
+    if (FORM & COLS) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { cm[j] = max(cm[j], magnitude(f[j])); cs[j] += f[j]; }
+    }
+    if (FORM & TILE) tile_max = max(tile_max, largest(f));
+    if (FORM & ROWS) {
+      uint32_t m = largest(f);
+#pragma unroll
+      for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const Coder c(m);
+      const int r = h + 16 * i;
+      if (r < rows && n > 0) *reinterpret_cast<uint2*>(p.q_rows + (r0 + r) * p.ldq + c0) = encode(c, f);
+      if (l == 0) row_scale[r] = c.scale;
+    }
+  }
+  if (FORM & TILE) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) tile_max = max(tile_max, __shfl_xor_sync(0xffffffffu, tile_max, o));
+    if (lane == 0) col_max[warp] = tile_max;
+  }
+  if (FORM & COLS) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) cm[j] = max(cm[j], __shfl_xor_sync(0xffffffffu, cm[j], 16));
+    if (lane < 16) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) part[warp][l * 8 + j] = cm[j];
+    }
+    if (p.sums) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) cs[j] += __shfl_xor_sync(0xffffffffu, cs[j], 16);
+      if (lane < 16) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum_part[warp][l * 8 + j] = cs[j];
+      }
+    }
+  }
+  __syncthreads();
+  if ((FORM & ROWS) && threadIdx.x < rows) p.s_rows[tile_c * p.R + r0 + threadIdx.x] = row_scale[threadIdx.x];
+  if (FORM & TILE) {
+    uint32_t m = col_max[0];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) m = max(m, col_max[k]);
+    const Coder c(m);
+    if (threadIdx.x == 0) p.s_rows[blockIdx.x] = c.scale;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = h + 16 * i;
+      float f[8];
+      values(i, f);
+      if (r < rows && n > 0) *reinterpret_cast<uint2*>(p.q_rows + (r0 + r) * p.ldq + c0) = encode(c, f);
+    }
+  }
+  if (FORM & COLS) {
+    if (threadIdx.x < BLOCK) {
+      uint32_t m = part[0][threadIdx.x];
+#pragma unroll
+      for (int k = 1; k < 8; ++k) m = max(m, part[k][threadIdx.x]);
+      col_max[threadIdx.x] = m;
+      const long long c = tile_c * BLOCK + threadIdx.x;
+      if (c < p.C) {
+        p.s_cols[tile_r * p.C + c] = Coder(m).scale;
+        if (p.sums) {
+          float s = sum_part[0][threadIdx.x];
+#pragma unroll
+          for (int k = 1; k < 8; ++k) s += sum_part[k][threadIdx.x];
+          p.sums[tile_r * p.C + c] = s;
+        }
+      }
+    }
+    __syncthreads();
+    uint2 out[8];
+    // two columns at a time: a coder holds three values for each
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      const Coder c0_(col_max[l * 8 + j]), c1_(col_max[l * 8 + j + 1]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float f[8];
+        values(i, f);
+        const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(c0_(f[j]), c1_(f[j + 1])), __NV_SATFINITE, __NV_E4M3);
+        uint32_t& w = j < 4 ? out[i].x : out[i].y;
+        w = (j & 2) ? w | two << 16 : two;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = h + 16 * i;
+      if (r < rows && n > 0) *reinterpret_cast<uint2*>(p.q_cols + (r0 + r) * p.ldq + c0) = out[i];
+    }
+  }
+}
+
+// sums [tiles][C] -> out [C], in the order of the tiles
+template <class T>
+__global__ void __launch_bounds__(256)
+column_sum_kernel(const float* __restrict__ sums, T* __restrict__ out, long long tiles, int C) {
+  __shared__ float part[8][32];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
+  float s = 0.f;
+  if (c < C)
+    for (long long t = k; t < tiles; t += 8) s += sums[t * C + c];
+  part[k][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (k == 0 && c < C) {
+#pragma unroll
+    for (int j = 1; j < 8; ++j) s += part[j][threadIdx.x];
+    out[c] = down<T>(s);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ norm
+// One block a row, V times eight neighbouring columns a thread, held in registers between the sum of squares and the codes.  Sixteen threads
+// share a scale.
+struct NormArgs {
+  const void *x, *res, *g;
+  void* sum;                       // x + res, written where res is given
+  uint8_t* q;
+  float* scale;
+  float* a;                        // 1 / rms of each row, or null
+  long long ldx, ldr, ldq, T;
+  int D, form;
+  float eps;
+};
+
+template <class T, int V, bool VEC>
+__global__ void __launch_bounds__(512)
+norm_quantize_kernel(NormArgs p) {
+  __shared__ float red[16];
+  const long long row = blockIdx.x;
+  const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+  const T* res = p.res ? static_cast<const T*>(p.res) + row * p.ldr : nullptr;
+  Eight<T> s[V], r[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int c = (threadIdx.x + v * blockDim.x) * 8;
+    s[v] = fetch<VEC, T>(x + c, min(8, p.D - c));
+    if (res) r[v] = fetch<VEC, T>(res + c, min(8, p.D - c));
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    float f[8];
+    unpack(s[v], f);
+    if (res) {
+      float t[8];
+      unpack(r[v], t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] += t[j];
+      s[v] = pack<T>(f);                                  // the norm is that of the sum as it is kept
+      const int c = (threadIdx.x + v * blockDim.x) * 8;
+      put<VEC, T>(static_cast<T*>(p.sum) + row * p.D + c, s[v], min(8, p.D - c));
+      unpack(s[v], f);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss += f[j] * f[j];
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if (blockDim.x > 32) {
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
+    __syncthreads();
+    ss = 0.f;
+    for (int k = 0; k < int(blockDim.x >> 5); ++k) ss += red[k];
+  }
+  const float mean = ss / p.D;
+  const float a = p.form == 0 ? rsqrtf(mean + p.eps) : 1.f / (sqrtf(mean) + p.eps);
+  if (p.a && threadIdx.x == 0) p.a[row] = a;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int c = (threadIdx.x + v * blockDim.x) * 8;
+    float f[8], g[8];
+    unpack(s[v], f);
+    unpack(fetch<VEC, T>(static_cast<const T*>(p.g) + c, min(8, p.D - c)), g);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = f[j] * a * g[j];
+    uint32_t m = largest(f);
+#pragma unroll
+    for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const Coder k(m);
+    if (c < p.D) {
+      *reinterpret_cast<uint2*>(p.q + row * p.ldq + c) = encode(k, f);
+      if ((threadIdx.x & 15) == 0) p.scale[(long long)(c / BLOCK) * p.T + row] = k.scale;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ back
+template <class T, bool VEC>
+__global__ void __launch_bounds__(256)
+dequantize_kernel(const uint8_t* __restrict__ q, const float* __restrict__ scale, T* __restrict__ x, long long R, int C, long long ldq,
+                  long long s_row, long long s_col, int tiles) {
+  const int per_row = (C + 7) / 8;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const long long row = i / per_row;
+  if (row >= R) return;
+  const int c = int(i - row * per_row) * 8, n = min(8, C - c);
+  const float s = scale[(tiles ? row / BLOCK : row) * s_row + (c / BLOCK) * s_col];
+  uint32_t w[2] = {0u, 0u};
+  if (VEC) {
+    const uint2 t = *reinterpret_cast<const uint2*>(q + row * ldq + c);
+    w[0] = t.x; w[1] = t.y;
+  } else {
+    for (int j = 0; j < n; ++j) w[j >> 2] |= uint32_t(q[row * ldq + c + j]) << (8 * (j & 3));
+  }
+  float f[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 t = decode2(w[j >> 1] >> (16 * (j & 1)));
+    f[2 * j] = t.x * s; f[2 * j + 1] = t.y * s;
+  }
+  put<VEC, T>(x + row * C + c, pack<T>(f), n);
+}
+
+template <class T> bool aligned16(const void* p, long long ld) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * (long long)sizeof(T) % 16 == 0;
+}
+
+template <class T, int FORM, bool NORM>
+static int launch_quantize(const QuantArgs& p, cudaStream_t st) {
+  const long long tiles = (p.R + BLOCK - 1) / BLOCK * p.col_tiles;
+  if (tiles > 0x7fffffffLL) return -3;
+  const bool vec = p.C % 8 == 0 && aligned16<T>(p.x, p.ld) && (!NORM || aligned16<T>(p.g, 8));
+  if (vec) quantize_kernel<T, FORM, NORM, true><<<(unsigned)tiles, 256, 0, st>>>(p);
+  else quantize_kernel<T, FORM, NORM, false><<<(unsigned)tiles, 256, 0, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+}
+template <class T>
+static int launch_form(const QuantArgs& p, int form, cudaStream_t st) {
+  if (p.a) return form == COLS ? launch_quantize<T, COLS, true>(p, st) : -3;
+  switch (form) {
+    case ROWS: return launch_quantize<T, ROWS, false>(p, st);
+    case COLS: return launch_quantize<T, COLS, false>(p, st);
+    case ROWS | COLS: return launch_quantize<T, ROWS | COLS, false>(p, st);
+    case TILE: return launch_quantize<T, TILE, false>(p, st);
+  }
+  return -3;
+}
+
+template <class T, int V>
+static void launch_norm_v(const NormArgs& p, int threads, cudaStream_t st) {
+  const bool vec = p.D % 8 == 0 && aligned16<T>(p.x, p.ldx) && aligned16<T>(p.g, 8) && (!p.res || (aligned16<T>(p.res, p.ldr) && aligned16<T>(p.sum, 8)));
+  if (vec) norm_quantize_kernel<T, V, true><<<(unsigned)p.T, threads, 0, st>>>(p);
+  else norm_quantize_kernel<T, V, false><<<(unsigned)p.T, threads, 0, st>>>(p);
+}
+template <class T>
+static int launch_norm(const NormArgs& p, cudaStream_t st) {
+  const int groups = (p.D + 7) / 8;
+  auto threads = [&](int v) { return ((groups + v - 1) / v + 31) / 32 * 32; };
+  if (groups <= 128) launch_norm_v<T, 1>(p, threads(1), st);
+  else if (groups <= 512) launch_norm_v<T, 2>(p, threads(2), st);
+  else launch_norm_v<T, 4>(p, threads(4), st);
+  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+}
+
+template <class T>
+static int launch_dequantize(const void* q, const float* scale, void* x, long long R, int C, long long ldq, long long s_row, long long s_col,
+                             int tiles, cudaStream_t st) {
+  const long long blocks = (R * ((C + 7) / 8) + 255) / 256;
+  if (blocks > 0x7fffffffLL) return -3;
+  const bool vec = C % 8 == 0 && ldq % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  if (vec) dequantize_kernel<T, true><<<(unsigned)blocks, 256, 0, st>>>((const uint8_t*)q, scale, (T*)x, R, C, ldq, s_row, s_col, tiles);
+  else dequantize_kernel<T, false><<<(unsigned)blocks, 256, 0, st>>>((const uint8_t*)q, scale, (T*)x, R, C, ldq, s_row, s_col, tiles);
+  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+}
+
+}  // namespace blk8
+}  // namespace sb
+
+// x [R, C] of type 0 bf16, 1 fp16, 2 fp32, rows `ld` apart.  form: 1 rows, 2 columns, 3 both, 4 tiles (codes and scales in q_rows, s_rows).
+// a, g: form 2 of x * a[row] * g[column].  sums: column sums of each 128 rows (forms 2 and 3), or null.
+extern "C" int sb_fp8_block_quantize(const void* x, long long ld, long long R, int C, int type, int form, void* q_rows, float* s_rows,
+                                     void* q_cols, float* s_cols, long long ldq, const float* a, const void* g, float* sums,
+                                     cudaStream_t st) {
+  using namespace sb::blk8;
+  if (R <= 0 || C <= 0) return 0;
+  if (ldq % 16 || ldq < C) return -4;
+  QuantArgs p{x, ld, R, C, ldq, (uint8_t*)q_rows, s_rows, (uint8_t*)q_cols, s_cols, a, g, sums, (C + BLOCK - 1) / BLOCK};
+  return type == 0 ? launch_form<bf16>(p, form, st) : type == 1 ? launch_form<__half>(p, form, st) : launch_form<float>(p, form, st);
+}
+
+// sums [tiles][C] of sb_fp8_block_quantize -> out [C]
+extern "C" int sb_fp8_block_column_sums(const float* sums, void* out, long long tiles, int C, int type, cudaStream_t st) {
+  using namespace sb::blk8;
+  if (C <= 0) return 0;
+  const int grid = (C + 31) / 32;
+  if (type == 0) column_sum_kernel<bf16><<<grid, 256, 0, st>>>(sums, (bf16*)out, tiles, C);
+  else if (type == 1) column_sum_kernel<__half><<<grid, 256, 0, st>>>(sums, (__half*)out, tiles, C);
+  else column_sum_kernel<float><<<grid, 256, 0, st>>>(sums, (float*)out, tiles, C);
+  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+}
+
+// D up to 16384.  res and sum: both or neither.  form 0: eps under the root, 1: beside it.  a: 1 / rms [T], or null.
+extern "C" int sb_fp8_block_norm(const void* x, long long ldx, const void* res, long long ldr, const void* g, void* sum, void* q, long long ldq,
+                                 float* scale, float* a, long long T, int D, float eps, int form, int type, cudaStream_t st) {
+  using namespace sb::blk8;
+  if (T <= 0 || D <= 0) return 0;
+  if (D > 16384 || T > 0x7fffffffLL) return -3;
+  if (ldq % 16 || ldq < D || !res != !sum) return -4;
+  NormArgs p{x, res, g, sum, (uint8_t*)q, scale, a, ldx, ldr, ldq, T, D, form, eps};
+  return type == 0 ? launch_norm<bf16>(p, st) : type == 1 ? launch_norm<__half>(p, st) : launch_norm<float>(p, st);
+}
+
+// q [R, C], rows ldq apart, times scale[row * s_row + (column / 128) * s_col] (tiles: row / 128) -> x [R, C] of `type`
+extern "C" int sb_fp8_block_dequantize(const void* q, long long ldq, const float* scale, long long s_row, long long s_col, int tiles, void* x,
+                                       long long R, int C, int type, cudaStream_t st) {
+  using namespace sb::blk8;
+  if (R <= 0 || C <= 0) return 0;
+  return type == 0   ? launch_dequantize<bf16>(q, scale, x, R, C, ldq, s_row, s_col, tiles, st)
+         : type == 1 ? launch_dequantize<__half>(q, scale, x, R, C, ldq, s_row, s_col, tiles, st)
+                     : launch_dequantize<float>(q, scale, x, R, C, ldq, s_row, s_col, tiles, st);
+}

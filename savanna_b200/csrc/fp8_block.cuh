@@ -1,0 +1,122 @@
+// What 8-bit operands with a scale for each block of 128 values have in common (fp8_block.cu, gemm_fp8_block.cu, gemv_fp8_block.cu).
+//
+//   scale = max(amax, 2^-100) / 448,  q = e4m3(x * 448 / amax),  x' = q * scale
+//
+// 448 is the largest e4m3 value.  Values of 16-bit types often lie exactly halfway between two codes: there the quotient has to be exact for
+// the half to go to the even code, so the product with the reciprocal is corrected by its remainder (one step of Newton's method with a fused
+// multiply-add).  A block that holds an infinity or NaN has the scale NaN, so that an overflow stays visible.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace sb {
+namespace blk8 {
+
+typedef __nv_bfloat16 bf16;
+constexpr int BLOCK = 128;
+
+__device__ __forceinline__ uint32_t magnitude(float f) { return __float_as_uint(f) & 0x7fffffffu; }
+
+struct Coder {
+  float scale, amax, inv, top;             // amax and 448 in units in which x * 448 cannot overflow, and 1 / amax
+  __device__ __forceinline__ explicit Coder(uint32_t m) {                // m: bits of the block's largest magnitude
+    const float a = fmaxf(__uint_as_float(m), 7.8886090522101181e-31f);  // 2^-100
+    scale = m < 0x7f800000u ? __fmul_rn(a, 1.f / 448.f) : __uint_as_float(0x7fffffffu);
+    const float unit = a > 1.2676506002282294e30f ? 2.3283064365386963e-10f : 1.f;     // above 2^100: units of 2^32
+    amax = a * unit;
+    top = 448.f * unit;
+    inv = __frcp_rn(amax);
+  }
+  __device__ __forceinline__ float operator()(float x) const {
+    const float n = __fmul_rn(x, top), q = __fmul_rn(n, inv);
+    return __fmaf_rn(__fmaf_rn(-q, amax, n), inv, q);
+  }
+};
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  return uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3)) |
+         (uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3)) << 16);
+}
+__device__ __forceinline__ uint2 encode(const Coder& c, const float (&f)[8]) {
+  return make_uint2(e4m3x4(c(f[0]), c(f[1]), c(f[2]), c(f[3])), e4m3x4(c(f[4]), c(f[5]), c(f[6]), c(f[7])));
+}
+__device__ __forceinline__ float2 decode2(uint32_t two) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(two & 0xffffu), __NV_E4M3);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+__device__ __forceinline__ uint32_t largest(const float (&f)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = max(m, magnitude(f[j]));
+  return m;
+}
+
+__device__ __forceinline__ float up(bf16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float up(__half v) { return __half2float(v); }
+__device__ __forceinline__ float up(float v) { return v; }
+template <class T> __device__ __forceinline__ T down(float f);
+template <> __device__ __forceinline__ bf16 down<bf16>(float f) { return __float2bfloat16_rn(f); }
+template <> __device__ __forceinline__ __half down<__half>(float f) { return __float2half_rn(f); }
+template <> __device__ __forceinline__ float down<float>(float f) { return f; }
+
+// Eight consecutive values as they lie in memory.
+template <class T> struct alignas(16) Eight { uint4 v[sizeof(T) / 2]; };
+template <class T> __device__ __forceinline__ Eight<T> none() {
+  Eight<T> e;
+#pragma unroll
+  for (int i = 0; i < int(sizeof(T)) / 2; ++i) e.v[i] = make_uint4(0, 0, 0, 0);
+  return e;
+}
+// n: how many of them there are (the others come as zero); VEC: on 16-byte boundaries, all or none of them
+template <bool VEC, class T> __device__ __forceinline__ Eight<T> fetch(const T* p, int n) {
+  Eight<T> e = none<T>();
+  if (VEC) {
+    if (n > 0) e = *reinterpret_cast<const Eight<T>*>(p);
+  } else {
+    T* d = reinterpret_cast<T*>(&e);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) d[j] = p[j];
+  }
+  return e;
+}
+template <bool VEC, class T> __device__ __forceinline__ void put(T* p, const Eight<T>& e, int n) {
+  if (VEC) {
+    if (n > 0) *reinterpret_cast<Eight<T>*>(p) = e;
+  } else {
+    const T* s = reinterpret_cast<const T*>(&e);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) p[j] = s[j];
+  }
+}
+__device__ __forceinline__ void unpack(const Eight<bf16>& e, float (&f)[8]) {
+  const uint32_t w[4] = {e.v[0].x, e.v[0].y, e.v[0].z, e.v[0].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+__device__ __forceinline__ void unpack(const Eight<__half>& e, float (&f)[8]) {
+  const uint32_t w[4] = {e.v[0].x, e.v[0].y, e.v[0].z, e.v[0].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    f[2 * i] = t.x; f[2 * i + 1] = t.y;
+  }
+}
+__device__ __forceinline__ void unpack(const Eight<float>& e, float (&f)[8]) {
+  const uint32_t w[8] = {e.v[0].x, e.v[0].y, e.v[0].z, e.v[0].w, e.v[1].x, e.v[1].y, e.v[1].z, e.v[1].w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
+}
+template <class T> __device__ __forceinline__ Eight<T> pack(const float (&f)[8]) {
+  Eight<T> e;
+  T* d = reinterpret_cast<T*>(&e);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) d[j] = down<T>(f[j]);
+  return e;
+}
+
+}  // namespace blk8
+}  // namespace sb

@@ -151,6 +151,146 @@ def linear_reducescatter(x, w, seq_dim: int = 1, fp8: bool = False):
     return mappings.reduce_scatter_to_sequence_parallel_region(linear(x, w, None, fp8), seq_dim)
 
 
+# ----------------------------------------------------------------------------- 8-bit operands with a scale for each block of 128
+
+_FP8_BLOCK_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _check_fp8_block_input(what, x):
+    if x.dim() < 1 or x.shape[-1] < 1 or x.dtype not in _FP8_BLOCK_TYPES:
+        raise ValueError(f"{what} takes bf16, fp16 or fp32 [..., D] with D >= 1, got {x.dtype} {tuple(x.shape)}")
+
+
+def _check_fp8_block_pair(what, pair, tiles):
+    q, s = pair if len(pair) == 2 else (None, None)
+    ok = q is not None and q.dtype == torch.float8_e4m3fn and s.dtype == torch.float32 and s.device == q.device and q.dim() >= 1 and q.shape[-1] >= 1
+    if ok and tiles:
+        ok = q.dim() == 2 and tuple(s.shape) == tuple(-(-n // ref.FP8_BLOCK) for n in q.shape)
+    elif ok:
+        ok = tuple(s.shape) == tuple(q.shape[:-1]) + (-(-q.shape[-1] // ref.FP8_BLOCK),)
+    if not ok:
+        raise ValueError(f"{what}: float8_e4m3fn {'[N, K] with fp32 scales [N / 128, K / 128]' if tiles else '[..., K] with fp32 scales [..., K / 128]'} "
+                         f"on one device, got {[(t.dtype, tuple(t.shape)) for t in pair]}")
+
+
+def _check_fp8_block_norm(what, x, weight, residual):
+    _check_fp8_block_input(what, x)
+    if tuple(weight.shape) != (x.shape[-1],) or weight.dtype != x.dtype or weight.device != x.device:
+        raise ValueError(f"{what}: weight {weight.dtype} {tuple(weight.shape)} for {x.dtype} rows of {x.shape[-1]} values")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+        raise ValueError(f"{what}: residual of x's shape, type and device expected")
+
+
+def _check_fp8_block_projection(what, x, w, bias, residual, dtype):
+    wt = w
+    if isinstance(w, tuple):
+        _check_fp8_block_pair(what, w, True)
+        wt = w[0]
+    if wt.dim() != 2 or wt.shape[1] != x.shape[-1] or wt.shape[0] < 1 or wt.device != x.device or (wt is w and w.dtype != dtype):
+        raise ValueError(f"{what}: weight {wt.dtype} {tuple(wt.shape)} for rows of {x.shape[-1]} values of {dtype}")
+    for name, t, shape in (("bias", bias, (wt.shape[0],)), ("residual", residual, tuple(x.shape[:-1]) + (wt.shape[0],))):
+        if t is not None and (tuple(t.shape) != shape or t.dtype != dtype or t.device != x.device):
+            raise ValueError(f"{what}: {name} of {dtype} {shape} expected")
+
+
+def _check_norm_form(what, form):
+    if form not in ("te", "classic"):
+        raise ValueError(f"{what}: norm form {form!r} is 'te' (eps under the root) or 'classic' (eps added to it)")
+
+
+def fp8_block_quantize(x):
+    """x [..., D] (bf16, fp16 or fp32) -> (q float8_e4m3fn of x's shape, scale fp32 [..., ceil(D / 128)]): 128 consecutive values of a row share
+    the scale max(amax, 2^-100) / 448, q = x * 448 / amax rounded to e4m3, halves to the even code.  A block that holds an infinity or NaN has the
+    scale NaN.  CUDA: the scales of neighbouring rows lie together (`scale` is a view of [D / 128, rows]), and rows of codes begin on 16-byte
+    boundaries, so that q is no contiguous tensor where D % 16 != 0.  Not differentiated."""
+    if _k(x):
+        return _CO.fp8_block_quantize(x)
+    _check_fp8_block_input("fp8_block_quantize", x)
+    return ref.fp8_block_quantize(x)
+
+
+def fp8_block_quantize_weight(w):
+    """w [N, K] -> (q float8_e4m3fn [N, K], scale fp32 [ceil(N / 128), ceil(K / 128)]): as `fp8_block_quantize`, a scale for 128 x 128 values.  One
+    form of a weight for forward, input gradient and serving."""
+    if _k(w):
+        return _CO.fp8_block_quantize(w, True)
+    _check_fp8_block_input("fp8_block_quantize_weight", w)
+    if w.dim() != 2:
+        raise ValueError(f"fp8_block_quantize_weight takes [N, K], got {tuple(w.shape)}")
+    return ref.fp8_block_quantize_weight(w)
+
+
+def fp8_block_dequantize(q, scale, dtype=torch.bfloat16):
+    """q * scale as `dtype`, of rows or of a weight."""
+    if dtype not in _FP8_BLOCK_TYPES:
+        raise ValueError(f"fp8_block_dequantize gives bf16, fp16 or fp32, not {dtype}")
+    if _k(q):
+        return _CO.fp8_block_dequantize(q, scale, dtype)
+    _check_fp8_block_pair("fp8_block_dequantize", (q, scale), q.dim() == 2 and scale.dim() == 2 and scale.shape[0] != q.shape[0])
+    return ref.fp8_block_dequantize(q, scale, dtype)
+
+
+def rmsnorm_fp8_block(x, weight, eps: float, form: str = "te", residual=None):
+    """(q, scale, s): `fp8_block_quantize` of rmsnorm(s), which is not rounded to x's type in between; s = x + residual, rounded to x's type
+    (without a residual: x).  x, weight and residual are of one type.  CUDA: rows of up to 16384 values of any width.  Not differentiated:
+    `norm_linear_fp8_block` is."""
+    _check_norm_form("rmsnorm_fp8_block", form)
+    if _k(x):
+        r = _CO.rmsnorm_fp8_block(x, weight, eps, form, residual)
+        if r is not None:
+            return r
+    _check_fp8_block_norm("rmsnorm_fp8_block", x, weight, residual)
+    with torch.no_grad():
+        return ref.rmsnorm_fp8_block(x, weight, eps, form, residual)
+
+
+def linear_fp8_block(x, w, bias=None, residual=None, dtype=None):
+    """x w^T (+ bias) (+ residual) on e4m3 operands with a scale for each block of 128, fp32 sums, one rounding.
+
+    x [..., K]: a tensor, or the pair that `fp8_block_quantize` or `rmsnorm_fp8_block` returned (then `dtype` is the type of the result, bf16 if
+    not given).  w [N, K]: a tensor of x's type, quantised in every call, or the pair of `fp8_block_quantize_weight`, kept by the caller.  bias
+    [N] and residual [..., N] are of the result's type.
+
+    Gradients: dx = rows(dy) tiles(w), dw = columns(dy)^T columns(x), each operand in 8 bits with scales for 128 values along the contraction;
+    the rounding to 8 bits itself passes them on unchanged.  x is kept for them in 8 bits.  A weight given as a pair gets none, an x given as a pair
+    wants none (ValueError).  No second derivatives.  Products whose two scales multiply to more than fp32 holds are infinite or NaN."""
+    pair = isinstance(x, tuple)
+    if pair:
+        dtype = torch.bfloat16 if dtype is None else dtype
+    elif dtype is not None and dtype != x.dtype:
+        raise ValueError(f"linear_fp8_block: the result of a {x.dtype} tensor has its type, not {dtype}")
+    else:
+        dtype = x.dtype
+    if dtype not in _FP8_BLOCK_TYPES:
+        raise ValueError(f"linear_fp8_block gives bf16, fp16 or fp32, not {dtype}")
+    if _k(x[0] if pair else x):
+        return _CO.linear_fp8_block(x, w, bias, residual, dtype)
+    if pair:
+        _check_fp8_block_pair("linear_fp8_block", x, False)
+    else:
+        _check_fp8_block_input("linear_fp8_block", x)
+    _check_fp8_block_projection("linear_fp8_block", x[0] if pair else x, w, bias, residual, dtype)
+    if pair and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (None if isinstance(w, tuple) else w, bias, residual)):
+        raise ValueError("linear_fp8_block: inputs in 8 bits carry no gradient; call it under torch.no_grad, or with the tensor itself")
+    return ref.linear_fp8_block(x, w, bias, residual, dtype)
+
+
+def norm_linear_fp8_block(x, norm_weight, eps: float, form: str, w, bias=None, residual=None):
+    """(`linear_fp8_block` of rmsnorm(s), s), s = x + residual (without a residual: x): the norm's kernel adds the residual and writes the 8-bit
+    operand.  One autograd node: the gradient that reaches s down the residual branch is added inside the norm's backward kernel.  CUDA: rows
+    of up to 16384 values; with gradients bf16 rows of 64 or more in eights, other types and widths run PyTorch's norm in fp32 before the projection."""
+    _check_norm_form("norm_linear_fp8_block", form)
+    if _k(x):
+        r = _CO.norm_linear_fp8_block(x, norm_weight, eps, form, w, bias, residual)
+        if r is not None:
+            return r
+        s = x if residual is None else x + residual
+        return _CO.linear_fp8_block(ref.rmsnorm_f32(s, norm_weight, eps, form), w, bias, None, x.dtype), s
+    _check_fp8_block_norm("norm_linear_fp8_block", x, norm_weight, residual)
+    _check_fp8_block_projection("norm_linear_fp8_block", x, w, bias, None, x.dtype)
+    return ref.norm_linear_fp8_block(x, norm_weight, eps, form, w, bias, residual)
+
+
 def glu_act(a, b, act: str = "silu"):
     return _co().glu_act(a, b, act) if _k(a) else ref.glu_act(a, b, act)
 

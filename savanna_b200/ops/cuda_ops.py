@@ -1088,6 +1088,33 @@ def act_dequantize(q, scale, dtype):
     return _native("act_dequantize", q, scale, _TYPES[dtype])
 
 
+# ----------------------------------------------------------------------------- 8-bit operands with a scale for each block of 128
+
+
+def fp8_block_quantize(x, tiles=False):
+    return _native("fp8_block_quantize", x, tiles)
+
+
+def fp8_block_dequantize(q, scale, dtype):
+    return _native("fp8_block_dequantize", q, scale, _TYPES[dtype])
+
+
+def rmsnorm_fp8_block(x, weight, eps, form, residual):
+    """None where rows are wider than the kernel's 16384."""
+    return _native("rmsnorm_fp8_block", x, weight, float(eps), 0 if form == "te" else 1, residual)
+
+
+def linear_fp8_block(x, w, bias, residual, dtype):
+    (x, xs), (w, ws) = (t if isinstance(t, tuple) else (t, None) for t in (x, w))
+    return _native("linear_fp8_block", x, xs, w, ws, bias, residual, _TYPES[dtype])
+
+
+def norm_linear_fp8_block(x, norm_weight, eps, form, w, bias, residual):
+    """None where the kernels do not cover type or width."""
+    w, ws = w if isinstance(w, tuple) else (w, None)
+    return _native("norm_linear_fp8_block", x, norm_weight, float(eps), 0 if form == "te" else 1, w, ws, bias, residual)
+
+
 # ----------------------------------------------------------------------------- gated activation
 
 

@@ -59,6 +59,103 @@ def act_dequantize(q, scale, dtype):
     return (qf * scale.unsqueeze(-1)).view(*q.shape[:-1], n * ACT_BLOCK)[..., :D].to(dtype)
 
 
+# ----------------------------------------------------------------------------- 8-bit operands with a scale for each block of 128
+
+FP8_BLOCK = 128          # values that share a scale
+FP8_TOP = 448.0          # largest e4m3 value
+FP8_TINY = 2.0 ** -100   # least magnitude that a scale is made for
+
+
+def _fp8_codes(v, amax):
+    """(e4m3 codes of v, their scale): q = v * 448 / amax, halves to the even code.  Infinity or NaN among the values: scale NaN."""
+    a = amax.clamp(min=FP8_TINY)
+    unit = torch.where(a > 2.0 ** 100, 2.0 ** -32, 1.0)          # v * 448 must not overflow
+    q = (v * (FP8_TOP * unit) / (a * unit)).clamp(-FP8_TOP, FP8_TOP).to(torch.float8_e4m3fn)
+    return q, torch.where(amax.isfinite(), a * (1.0 / FP8_TOP), torch.nan)
+
+
+def fp8_block_quantize(x):
+    """(q e4m3 [..., D], scale fp32 [..., ceil(D / 128)])"""
+    D = x.shape[-1]
+    n = -(-D // FP8_BLOCK)
+    v = F.pad(x.detach().float(), (0, n * FP8_BLOCK - D)).view(*x.shape[:-1], n, FP8_BLOCK)
+    q, scale = _fp8_codes(v, v.abs().amax(-1, keepdim=True))
+    return q.view(*x.shape[:-1], n * FP8_BLOCK)[..., :D].contiguous(), scale.squeeze(-1)
+
+
+def fp8_block_quantize_weight(w):
+    """(q e4m3 [N, K], scale fp32 [ceil(N / 128), ceil(K / 128)])"""
+    N, K = w.shape
+    n, k = -(-N // FP8_BLOCK), -(-K // FP8_BLOCK)
+    v = F.pad(w.detach().float(), (0, k * FP8_BLOCK - K, 0, n * FP8_BLOCK - N)).view(n, FP8_BLOCK, k, FP8_BLOCK)
+    q, scale = _fp8_codes(v, v.abs().amax((1, 3), keepdim=True))
+    return q.view(n * FP8_BLOCK, k * FP8_BLOCK)[:N, :K].contiguous(), scale.view(n, k)
+
+
+def fp8_block_dequantize(q, scale, dtype=torch.float32):
+    s = scale.float()
+    if q.dim() == 2 and scale.shape[0] != q.shape[0]:
+        s = s.repeat_interleave(FP8_BLOCK, 0)[: q.shape[0]]
+    return (q.float() * s.repeat_interleave(FP8_BLOCK, -1)[..., : q.shape[-1]]).to(dtype)
+
+
+def _fp8_rows(x2):
+    return fp8_block_dequantize(*fp8_block_quantize(x2))
+
+
+def _fp8_columns(x2):
+    return _fp8_rows(x2.t()).t()
+
+
+def rmsnorm_f32(x, weight, eps, form="te"):
+    """`rmsnorm` without its last rounding."""
+    return rmsnorm(x.float(), weight.float(), eps, form)
+
+
+def rmsnorm_fp8_block(x, weight, eps, form="te", residual=None):
+    s = x if residual is None else x + residual
+    return fp8_block_quantize(rmsnorm_f32(s, weight, eps, form)) + (s,)
+
+
+class _Fp8BlockLinear(torch.autograd.Function):
+    """y = rows(x) tiles(w)^T, dx = rows(dy) tiles(w), dw = columns(dy)^T columns(x): every operand in 8 bits along its product's
+    contraction; what rounding to 8 bits does is not differentiated."""
+
+    @staticmethod
+    def forward(ctx, x, w, wd):
+        x2 = x.detach().reshape(-1, x.shape[-1]).float()
+        ctx.save_for_backward(_fp8_columns(x2) if w is not None and w.requires_grad else None, wd)
+        ctx.shape, ctx.types = x.shape, (x.dtype, None if w is None else w.dtype)
+        return (_fp8_rows(x2) @ wd.t()).view(*x.shape[:-1], wd.shape[0])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        xc, wd = ctx.saved_tensors
+        g2 = gy.reshape(-1, gy.shape[-1]).float()
+        gx = (_fp8_rows(g2) @ wd).view(ctx.shape).to(ctx.types[0]) if ctx.needs_input_grad[0] else None
+        gw = (_fp8_columns(g2).t() @ xc).to(ctx.types[1]) if ctx.needs_input_grad[1] else None
+        return gx, gw, None
+
+
+def linear_fp8_block(x, w, bias=None, residual=None, dtype=None):
+    wd = fp8_block_dequantize(*(w if isinstance(w, tuple) else fp8_block_quantize_weight(w)))
+    if isinstance(x, tuple):
+        y = fp8_block_dequantize(*x) @ wd.t()
+    else:
+        y = _Fp8BlockLinear.apply(x, None if isinstance(w, tuple) else w, wd)
+    if bias is not None:
+        y = y + bias.float()
+    if residual is not None:
+        y = y + residual.float()
+    return y.to(dtype)
+
+
+def norm_linear_fp8_block(x, norm_weight, eps, form, w, bias=None, residual=None):
+    s = x if residual is None else x + residual
+    return linear_fp8_block(rmsnorm_f32(s, norm_weight, eps, form), w, bias, None, x.dtype), s
+
+
 # ----------------------------------------------------------------------------- linear
 
 
