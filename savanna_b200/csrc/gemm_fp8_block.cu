@@ -8,8 +8,9 @@
 //
 //   warp 0     TMA producer: a k-block's operands, 32 KB a CTA and stage
 //   warp 1     MMA issuer: four products of 32 k a k-block, each k-block into the next of the TMEM buffers
+//   warp 2     the scales into a ring in shared memory (4-byte asynchronous copies: any strides), eight k-blocks deep, handed over by fours
 //   warps 4-11 a lane owns a row and half of the tile's columns: tcgen05.ld of 16 columns, eight packed multiply-adds, while the next 16 are on
-//              their way; after the last k-block the sums leave through shared memory in whole sectors
+//              their way; after the last k-block the sums leave in whole sectors
 //
 // Two tiles: 256 x 256 on a CTA pair (cta_group::2; two buffers of 256 columns, 128 sums a thread) and 128 x 128 on one CTA (four buffers of
 // 128, 64 sums), for outputs that leave the chip idle in the larger one.
@@ -33,19 +34,20 @@ struct GemmArgs {
   const float *sa, *sb;
   long long sa_m, sa_k, sb_n, sb_k;      // strides; sb_n counts blocks of 128 n where the scale is theirs
   long long ldc, ldr;
-  int M, N, K, type, beta, vec;          // vec: rows of C and residual on 16-byte boundaries
+  int M, N, K, type, beta, align;        // align: of the rows of C and residual and of the bias, 32 or 16 bytes or less
   uint32_t* status;
 };
 
 constexpr int EPI_WARPS = 8, NUM_THREADS = 128 + 32 * EPI_WARPS;
-// Registers: 168 a thread at launch (384 threads), of which the first four warps keep 40 and each of the other eight gets 232:
-// 128 * 40 + 256 * 232 = 384 * 168.
-constexpr int REGS_FEW = 40, REGS_MANY = 232;
+// Registers: 168 a thread at launch (384 threads), of which the first four warps keep 56 and each of the other eight gets 224:
+// 128 * 56 + 256 * 224 = 384 * 168.
+constexpr int REGS_FEW = 56, REGS_MANY = 224;
 static_assert(128 * REGS_FEW + 32 * EPI_WARPS * REGS_MANY <= NUM_THREADS * 168, "registers of a block");
 constexpr int STAGES = 6, OPERAND = 128 * 128, STAGE_BYTES = 2 * OPERAND;
-constexpr int BAR_OFF = STAGES * STAGE_BYTES, OUT_OFF = BAR_OFF + 256, OUT_BYTES = 32 * 64;      // a warp's 32 rows x 16 fp32 on their way out
-constexpr int SB_OFF = OUT_OFF + EPI_WARPS * OUT_BYTES, SB_BYTES = 2 * 128 * 4;                  // a warp's column scales of two k-blocks
-constexpr int SMEM_BYTES = SB_OFF + EPI_WARPS * SB_BYTES + 1024;
+constexpr int BAR_OFF = STAGES * STAGE_BYTES, OUT_OFF = BAR_OFF + 256, OUT_BYTES = 32 * 64;      // 16 sums of each of a warp's rows (store_row)
+// Scales of a k-block, rows and columns.  They change hands by GROUP k-blocks: a barrier for each cost the epilogue 200 cycles of 1000.
+constexpr int GROUP = 4, SLOTS = 2 * GROUP, SLOT_OFF = OUT_OFF + EPI_WARPS * OUT_BYTES, SLOT_BYTES = (128 + 256) * 4;
+constexpr int SMEM_BYTES = SLOT_OFF + SLOTS * SLOT_BYTES + 1024;
 static_assert(SMEM_BYTES <= 232448, "shared memory of a block");
 constexpr int GROUP_M = 8;               // raster: m-tiles that share the concurrently running n-tiles
 
@@ -55,23 +57,10 @@ __device__ __forceinline__ void raster(int tile, int m_tiles, int n_tiles, int& 
   nt = r / size;
 }
 
-__device__ __forceinline__ void load16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
+// acc += (a, b) * s.  Volatile, as the loads and their wait are: it stays behind the wait for a and b.
+__device__ __forceinline__ void add_scaled(f2& acc, uint32_t a, uint32_t b, f2 s) {
+  asm volatile("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tfma.rn.f32x2 %0, t, %3, %0;\n\t}" : "+l"(acc) : "r"(a), "r"(b), "l"(s));
 }
-// the registers pass through the wait: nothing that uses them can move ahead of it
-__device__ __forceinline__ void arrived(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
-                 "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-               :
-               : "memory");
-}
-__device__ __forceinline__ f2 pair_of(uint32_t a, uint32_t b) { return f2_pack(__uint_as_float(a), __uint_as_float(b)); }
 __device__ __forceinline__ void put4(uint32_t at, float a, float b, float c, float d) {
   asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
@@ -81,46 +70,124 @@ __device__ __forceinline__ float4 get4(uint32_t at) {
   return v;
 }
 
-template <class T>
-__device__ __forceinline__ void add8(const T* p, int n, bool vec, float (&f)[8]) {
-  float t[8];
-  unpack(vec && n == 8 ? fetch<true, T>(p, 8) : fetch<false, T>(p, n), t);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] += t[j];
-}
-// n of the eight sums of one row from column col on
-template <class T>
-__device__ __forceinline__ void finish8(const GemmArgs& p, int row, int col, int n, float (&f)[8]) {
-  T* c = static_cast<T*>(p.C) + row * p.ldc + col;
-  if (p.bias) add8(static_cast<const T*>(p.bias) + col, n, false, f);
-  if (p.residual) add8(static_cast<const T*>(p.residual) + row * p.ldr + col, n, p.vec, f);
-  if (p.beta) add8(c, n, p.vec, f);
-  if (p.vec && n == 8) put<true, T>(c, pack<T>(f), 8);
-  else put<false, T>(c, pack<T>(f), n);
-}
-// 16 sums of each of the warp's 32 rows, a lane a row, to memory.  Chunks of 16 bytes are permuted so that neither side meets a bank twice.
-__device__ __forceinline__ void store16(const GemmArgs& p, uint32_t stage, const f2* acc, int row0, int col0, int lane) {
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const float2 a = f2_unpack(acc[2 * c]), b = f2_unpack(acc[2 * c + 1]);
-    put4(stage + lane * 64 + ((c ^ (lane >> 1 & 3)) << 4), a.x, a.y, b.x, b.y);
-  }
-  __syncwarp();
-  const int g = lane & 1, col = col0 + 8 * g, n = min(8, p.N - col);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = 16 * i + (lane >> 1), x = r >> 1 & 3;
-    const float4 a = get4(stage + r * 64 + ((2 * g ^ x) << 4)), b = get4(stage + r * 64 + (((2 * g + 1) ^ x) << 4));
-    float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    if (row0 + r < p.M && n > 0) {
-      if (p.type == 0) finish8<bf16>(p, row0 + r, col, n, f);
-      else if (p.type == 1) finish8<__half>(p, row0 + r, col, n, f);
-      else finish8<float>(p, row0 + r, col, n, f);
-    }
-  }
-  __syncwarp();
+// The arrival that frees a TMEM buffer hands over no memory (what was read is in registers), so it orders none: a releasing one would wait for
+// the loads of the next scales too, and took four fifths of a k-block's time.
+__device__ __forceinline__ void arrive_relaxed(uint32_t cluster_addr, bool one) {
+  asm volatile("{\n\t.reg .pred P;\n\tsetp.ne.b32 P, %1, 0;\n\t@P mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n\t}"
+               ::"r"(cluster_addr), "r"(uint32_t(one)) : "memory");
 }
 
+// four bytes to shared memory, or zeros
+__device__ __forceinline__ void copy4(uint32_t dst, const float* src, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(__cvta_generic_to_global(src)), "r"(there ? 4 : 0) : "memory");
+}
+// the thread's copies so far arrive once they have landed
+__device__ __forceinline__ void copies_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ float get1(uint32_t at) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+
+// The way out.  A lane holds a row: it stores 16 columns at once, whole 32-byte sectors, so nothing has to be turned round in shared memory
+// first.  Rows that begin on 32-byte boundaries (WIDE) take one instruction for 8 words, others on 16 two, the rest one value after the other.
+struct Words { uint32_t w[8]; };
+template <bool WIDE> __device__ __forceinline__ Words read_words(const void* p) {
+  Words v;
+  if (WIDE) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7])
+                 : "l"(__cvta_generic_to_global(p)) : "memory");
+  } else {
+    reinterpret_cast<uint4*>(&v)[0] = static_cast<const uint4*>(p)[0];
+    reinterpret_cast<uint4*>(&v)[1] = static_cast<const uint4*>(p)[1];
+  }
+  return v;
+}
+template <bool WIDE> __device__ __forceinline__ void write_words(void* p, const Words& v) {
+  if (WIDE) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(__cvta_generic_to_global(p)), "r"(v.w[0]), "r"(v.w[1]), "r"(v.w[2]),
+                 "r"(v.w[3]), "r"(v.w[4]), "r"(v.w[5]), "r"(v.w[6]), "r"(v.w[7]) : "memory");
+  } else {
+    static_cast<uint4*>(p)[0] = reinterpret_cast<const uint4*>(&v)[0];
+    static_cast<uint4*>(p)[1] = reinterpret_cast<const uint4*>(&v)[1];
+  }
+}
+__device__ __forceinline__ float2 two(uint32_t w, bf16) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ float2 two(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ uint32_t word(float a, float b, bf16) { return pack_bf2(a, b); }
+__device__ __forceinline__ uint32_t word(float a, float b, __half) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// f += 16 values at p
+template <bool WIDE, class T> __device__ __forceinline__ void add16(const T* p, float (&f)[16]) {
+  if constexpr (sizeof(T) == 2) {
+    const Words v = read_words<WIDE>(p);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { const float2 t = two(v.w[j], T()); f[2 * j] += t.x; f[2 * j + 1] += t.y; }
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const Words v = read_words<WIDE>(p + 8 * h);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[8 * h + j] += __uint_as_float(v.w[j]);
+    }
+  }
+}
+template <bool WIDE, class T> __device__ __forceinline__ void store16(const GemmArgs& p, long long at_c, long long at_r, int col, float (&f)[16]) {
+  T* c = static_cast<T*>(p.C) + at_c + col;
+  if (p.bias) add16<WIDE, T>(static_cast<const T*>(p.bias) + col, f);
+  if (p.residual) add16<WIDE, T>(static_cast<const T*>(p.residual) + at_r + col, f);
+  if (p.beta) add16<WIDE, T>(c, f);
+  Words v;
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v.w[j] = word(f[2 * j], f[2 * j + 1], T());
+    write_words<WIDE>(c, v);
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v.w[j] = __float_as_uint(f[8 * h + j]);
+      write_words<WIDE>(c + 8 * h, v);
+    }
+  }
+}
+template <class T> __device__ __forceinline__ void store_one(const GemmArgs& p, long long at_c, long long at_r, int col, float f) {
+  T* c = static_cast<T*>(p.C) + at_c + col;
+  if (p.bias) f += up(static_cast<const T*>(p.bias)[col]);
+  if (p.residual) f += up(static_cast<const T*>(p.residual)[at_r + col]);
+  if (p.beta) f += up(*c);
+  *c = down<T>(f);
+}
+template <int COLS, class T>
+__device__ __forceinline__ void store_row(const GemmArgs& p, uint32_t own, const f2* acc, int row, int col0) {
+  const long long at_c = row * p.ldc, at_r = row * p.ldr;
+#pragma unroll
+  for (int c = 0; c < COLS / 16; ++c) {
+    const int col = col0 + c * 16;
+    float f[16];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { const float2 t = f2_unpack(acc[c * 8 + j]); f[2 * j] = t.x; f[2 * j + 1] = t.y; }
+    if (p.align == 32 && col + 16 <= p.N) store16<true, T>(p, at_c, at_r, col, f);
+    else if (p.align == 16 && col + 16 <= p.N) store16<false, T>(p, at_c, at_r, col, f);
+    else if (col < p.N) {                  // through the lane's own 64 bytes of shared memory: a short loop instead of 16 copies of it
+#pragma unroll
+      for (int j = 0; j < 4; ++j) put4(own + 16 * j, f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+#pragma unroll 1
+      for (int j = 0; j < min(16, p.N - col); ++j) store_one<T>(p, at_c, at_r, col + j, get1(own + 4 * j));
+    }
+  }
+}
+
+__device__ __forceinline__ bool spin_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t* status, uint32_t code) {
+  for (int i = 0; i < 64; ++i)
+    if (mbar_test(bar, parity)) return true;
+  return mbar_wait(bar, parity, abort_flag, status, code);
+}
 template <bool PAIR, int A_MN, int B_MN, bool SB_ROWS>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, GemmArgs p) {
@@ -133,8 +200,11 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   auto empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
   auto tfull_bar = [&](int b) { return bar_base + 8u * (2 * STAGES + b); };
   auto tempty_bar = [&](int b) { return bar_base + 8u * (2 * STAGES + 4 + b); };
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem_gen + BAR_OFF + 8 * (2 * STAGES + 8));
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_gen + BAR_OFF + 8 * (2 * STAGES + 8) + 8);
+  auto sfull_bar = [&](int g) { return bar_base + 8u * (2 * STAGES + 8 + g); };
+  auto sempty_bar = [&](int g) { return bar_base + 8u * (2 * STAGES + 10 + g); };
+  constexpr int FLAGS = BAR_OFF + 8 * (2 * STAGES + 12);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem_gen + FLAGS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_gen + FLAGS + 8);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0u;             // 0 issues the products, 1 is its partner
@@ -145,6 +215,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
     for (int b = 0; b < BUFS; ++b) { mbar_init(tfull_bar(b), 1); mbar_init(tempty_bar(b), (PAIR ? 2 : 1) * EPI_WARPS); }
+    for (int g = 0; g < 2; ++g) { mbar_init(sfull_bar(g), 32); mbar_init(sempty_bar(g), EPI_WARPS); }
     *abort_flag = 0;
     fence_barrier_init();
     prefetch_tmap(&tmA);
@@ -199,111 +270,123 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       bool ok = true;
       for (int tile = worker; tile < num_tiles && ok; tile += workers)
         for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(tempty_bar(buf), buf_phase ^ 1u, abort_flag, p.status, ST_FP8_BLOCK + 2) ||
-              !mbar_wait(full_bar(stage), phase, abort_flag, p.status, ST_FP8_BLOCK + 3)) { ok = false; break; }
-          tc_fence_after();
+          if (!spin_wait(full_bar(stage), phase, abort_flag, p.status, ST_FP8_BLOCK + 3)) { ok = false; break; }
           const uint32_t a_addr = smem_base + stage * STAGE_BYTES;
           const uint64_t adesc = umma_smem_desc(a_addr, a_lbo, 1024u), bdesc = umma_smem_desc(a_addr + OPERAND, b_lbo, 1024u);
+          if (!spin_wait(tempty_bar(buf), buf_phase ^ 1u, abort_flag, p.status, ST_FP8_BLOCK + 2)) { ok = false; break; }
+          tc_fence_after();
           const uint32_t d = tmem_base + buf * TN;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             if (PAIR) umma_fp8_pair(d, adesc + k * a_step, bdesc + k * b_step, idesc, k != 0);
             else umma_fp8(d, adesc + k * a_step, bdesc + k * b_step, idesc, k != 0);
           }
-          if (PAIR) { umma_commit_pair(empty_bar(stage)); umma_commit_pair(tfull_bar(buf)); }
-          else { umma_commit(empty_bar(stage)); umma_commit(tfull_bar(buf)); }
+          if (PAIR) { umma_commit_pair(tfull_bar(buf)); umma_commit_pair(empty_bar(stage)); }
+          else { umma_commit(tfull_bar(buf)); umma_commit(empty_bar(stage)); }
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
           if (++buf == BUFS) { buf = 0; buf_phase ^= 1u; }
         }
     }
+    if (warp == 2) {
+      int n = 0;                                                   // k-blocks so far, over all tiles
+      bool ok = true;
+      for (int tile = worker; tile < num_tiles && ok; tile += workers) {
+        int mt, nt; raster(tile, m_tiles, n_tiles, mt, nt);
+        const int m0 = mt * TM + int(rank) * 128 + lane, n0 = nt * TN;
+        for (int kb = 0; kb < num_kb; ++kb, ++n) {
+          const int group = n / GROUP & 1;
+          if (n % GROUP == 0 && !mbar_wait(sempty_bar(group), (n / SLOTS & 1) ^ 1, abort_flag, p.status, ST_FP8_BLOCK + 5)) { ok = false; break; }
+          const uint32_t at = smem_base + SLOT_OFF + (n % SLOTS) * SLOT_BYTES;
+          const float *sa = p.sa + kb * p.sa_k, *sb = p.sb + kb * p.sb_k;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int m = m0 + 32 * j;
+            copy4(at + (32 * j + lane) * 4, m < p.M ? sa + m * p.sa_m : sa, m < p.M);
+          }
+          if (SB_ROWS) {
+#pragma unroll
+            for (int j = 0; j < TN / 32; ++j) {
+              const int c = n0 + 32 * j + lane;
+              copy4(at + (128 + 32 * j + lane) * 4, c < p.N ? sb + c * p.sb_n : sb, c < p.N);
+            }
+          } else if (lane < TN / 128) {
+            const int c = n0 + 128 * lane;
+            copy4(at + (128 + lane) * 4, c < p.N ? sb + (c / BLOCK) * p.sb_n : sb, c < p.N);
+          }
+          if (n % GROUP == GROUP - 1) copies_arrive(sfull_bar(group));
+        }
+      }
+      if (n % GROUP) copies_arrive(sfull_bar(n / GROUP & 1));      // the last group may be a short one
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_MANY));
     const int q = warp & 3, half = (warp - 4) >> 2;
-    const uint32_t stage_w = smem_base + OUT_OFF + (warp - 4) * OUT_BYTES, sb_w = smem_base + SB_OFF + (warp - 4) * SB_BYTES;
-    int buf = 0; uint32_t buf_phase = 0;
+    const uint32_t own = smem_base + OUT_OFF + (warp - 4) * OUT_BYTES + lane * 64;
+    const uint32_t t_warp = tmem_base + (uint32_t(q * 32) << 16) + half * COLS;
+    const uint32_t tempty_0 = map_to_cta(tempty_bar(0), 0);        // the even CTA's
+    int buf = 0, n = 0; uint32_t buf_phase = 0;                    // n: k-blocks so far, over all tiles
+    const uint32_t slot_0 = smem_base + SLOT_OFF;
     bool ok = true;
     for (int tile = worker; tile < num_tiles && ok; tile += workers) {
       int mt, nt; raster(tile, m_tiles, n_tiles, mt, nt);
       const int row0 = mt * TM + int(rank) * 128 + q * 32, col0 = nt * TN + half * COLS;
-      const float* sa = p.sa + (long long)min(row0 + lane, p.M - 1) * p.sa_m;
-      const float* sb = SB_ROWS ? p.sb : p.sb + (min(col0, p.N - 1) / BLOCK) * p.sb_n;
-      // the scales of a k-block are fetched two k-blocks ahead
-      float a_next[2], b_next[2];
-      float c_next[COLS / 32];
-      auto columns = [&](int kb) {
-#pragma unroll
-        for (int j = 0; j < COLS / 32; ++j) {
-          const int c = col0 + lane + 32 * j;
-          c_next[j] = c < p.N && kb < num_kb ? sb[c * p.sb_n + kb * p.sb_k] : 0.f;
-        }
-      };
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        a_next[k] = k < num_kb ? sa[k * p.sa_k] : 0.f;
-        b_next[k] = !SB_ROWS && k < num_kb ? sb[k * p.sb_k] : 0.f;
-      }
-      if (SB_ROWS) columns(0);
       f2 acc[COLS / 2];
 #pragma unroll
       for (int j = 0; j < COLS / 2; ++j) acc[j] = 0ull;
       for (int kb = 0; kb < num_kb; ++kb) {
-        float s = a_next[0];
-        const uint32_t sb_k = sb_w + (kb & 1) * (SB_BYTES / 2);
-        if (SB_ROWS) {
-#pragma unroll
-          for (int j = 0; j < COLS / 32; ++j) asm volatile("st.shared.f32 [%0], %1;" ::"r"(sb_k + (lane + 32 * j) * 4), "f"(c_next[j]) : "memory");
-          __syncwarp();
-          columns(kb + 1);
-        } else {
-          s *= b_next[0];
-        }
-        a_next[0] = a_next[1]; b_next[0] = b_next[1];
-        if (kb + 2 < num_kb) {
-          a_next[1] = sa[(kb + 2) * p.sa_k];
-          if (!SB_ROWS) b_next[1] = sb[(kb + 2) * p.sb_k];
-        }
+        const int group = n / GROUP & 1;
+        if (n % GROUP == 0 && !spin_wait(sfull_bar(group), n / SLOTS & 1, abort_flag, p.status, ST_FP8_BLOCK + 6)) { ok = false; break; }
+        const uint32_t at = slot_0 + (n % SLOTS) * SLOT_BYTES, sb_k = at + (128 + half * COLS) * 4;
+        float s = get1(at + (q * 32 + lane) * 4);
+        if (!SB_ROWS) s *= get1(at + (128 + (PAIR ? half : 0)) * 4);
         const f2 s2 = f2_pack(s, s);
-        if (!mbar_wait(tfull_bar(buf), buf_phase, abort_flag, p.status, ST_FP8_BLOCK + 4)) { ok = false; break; }
-        tc_fence_after();
-        const uint32_t t = tmem_base + (uint32_t(q * 32) << 16) + buf * TN + half * COLS;
-        auto add = [&](int c, const uint32_t (&r)[16]) {
+        const uint32_t t = t_warp + buf * TN;
+        uint32_t r0[32], r1[32];
+        auto add = [&](int c, const uint32_t (&r)[32]) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < 8; ++j) {
+            f2 lo = s2, hi = s2;
             if (SB_ROWS) {
-              const float4 b = get4(sb_k + (c * 16 + 4 * j) * 4);
-              acc[c * 8 + 2 * j] = f2_fma(pair_of(r[4 * j], r[4 * j + 1]), f2_mul(f2_pack(b.x, b.y), s2), acc[c * 8 + 2 * j]);
-              acc[c * 8 + 2 * j + 1] = f2_fma(pair_of(r[4 * j + 2], r[4 * j + 3]), f2_mul(f2_pack(b.z, b.w), s2), acc[c * 8 + 2 * j + 1]);
-            } else {
-              acc[c * 8 + 2 * j] = f2_fma(pair_of(r[4 * j], r[4 * j + 1]), s2, acc[c * 8 + 2 * j]);
-              acc[c * 8 + 2 * j + 1] = f2_fma(pair_of(r[4 * j + 2], r[4 * j + 3]), s2, acc[c * 8 + 2 * j + 1]);
+              const float4 b = get4(sb_k + (c * 32 + 4 * j) * 4);
+              lo = f2_mul(f2_pack(b.x, b.y), s2); hi = f2_mul(f2_pack(b.z, b.w), s2);
             }
+            add_scaled(acc[c * 16 + 2 * j], r[4 * j], r[4 * j + 1], lo);
+            add_scaled(acc[c * 16 + 2 * j + 1], r[4 * j + 2], r[4 * j + 3], hi);
           }
         };
-        uint32_t r0[16], r1[16];
-        load16(t, r0);
-#pragma unroll
-        for (int c = 0; c < COLS / 16; c += 2) {
-          arrived(r0);
-          load16(t + (c + 1) * 16, r1);
-          add(c, r0);
-          arrived(r1);
-          if (c + 2 < COLS / 16) load16(t + (c + 2) * 16, r0);
-          else {                                                   // all read: the buffer is free again
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-              if (PAIR) mbar_arrive_cluster(map_to_cta(tempty_bar(buf), 0));
-              else mbar_arrive(tempty_bar(buf));
-            }
-          }
-          add(c + 1, r1);
+        if (!spin_wait(tfull_bar(buf), buf_phase, abort_flag, p.status, ST_FP8_BLOCK + 4)) { ok = false; break; }
+        __syncwarp();
+        tc_fence_after();
+        tmem_ld_32x32(t, r0);
+        tmem_ld_32x32(t + 32, r1);
+        tmem_wait_ld();
+        if (COLS == 128) {
+          add(0, r0);
+          tmem_ld_32x32(t + 64, r0);
+          add(1, r1);
+          tmem_ld_32x32(t + 96, r1);
+          tmem_wait_ld();
+        }
+        tc_fence_before();
+        __syncwarp();
+        arrive_relaxed(tempty_0 + 8u * buf, lane == 0);            // all read: the buffer is free again
+        add(COLS / 32 - 2, r0);
+        add(COLS / 32 - 1, r1);
+        if (n % GROUP == GROUP - 1) {                              // this group's scales have been read by the whole warp
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sempty_bar(group));
         }
         if (++buf == BUFS) { buf = 0; buf_phase ^= 1u; }
+        ++n;
       }
       if (!ok) break;
-#pragma unroll
-      for (int c = 0; c < COLS / 16; ++c)
-        if (col0 + c * 16 < p.N) store16(p, stage_w, acc + c * 8, row0, col0 + c * 16, lane);
+      const int row = row0 + lane;
+      if (row < p.M) {
+        if (p.type == 0) store_row<COLS, bf16>(p, own, acc, row, col0);
+        else if (p.type == 1) store_row<COLS, __half>(p, own, acc, row, col0);
+        else store_row<COLS, float>(p, own, acc, row, col0);
+      }
     }
   }
   tc_fence_before();
@@ -376,9 +459,10 @@ extern "C" int sb_gemm_fp8_block(const void* A, const float* sa, long long sa_m,
   if ((rc = a_mn ? make_tmap_2d_u8(&tmA, A, M, K, lda, 128, 128) : make_tmap_2d_u8(&tmA, A, K, M, lda, 128, 128))) return rc;
   if ((rc = b_mn ? make_tmap_2d_u8(&tmB, B, N, K, ldb, 128, 128) : make_tmap_2d_u8(&tmB, B, K, N, ldb, 128, 128))) return rc;
   const int size = type == 2 ? 4 : 2;
-  const bool vec = reinterpret_cast<uintptr_t>(C) % 16 == 0 && ldc * size % 16 == 0 &&
-                   (!residual || (reinterpret_cast<uintptr_t>(residual) % 16 == 0 && ldr * size % 16 == 0));
-  GemmArgs p{C, bias, residual, sa, sb, sa_m, sa_k, sb_n, sb_k, ldc, ldr, M, N, K, type, beta, vec, status};
+  const long long step = (reinterpret_cast<uintptr_t>(C) | ldc * size | reinterpret_cast<uintptr_t>(bias) |
+                          (residual ? reinterpret_cast<uintptr_t>(residual) | ldr * size : 0)) & 31;
+  const int align = step == 0 ? 32 : step == 16 ? 16 : 0;
+  GemmArgs p{C, bias, residual, sa, sb, sa_m, sa_k, sb_n, sb_k, ldc, ldr, M, N, K, type, beta, align, status};
   const bool pair = goes_by_pairs(M, N, num_sms());
   if (!a_mn && !b_mn && !sb_rows) return pair ? launch<true, 0, 0, false>(tmA, tmB, p, stream) : launch<false, 0, 0, false>(tmA, tmB, p, stream);
   if (!a_mn && b_mn && !sb_rows) return pair ? launch<true, 0, 1, false>(tmA, tmB, p, stream) : launch<false, 0, 1, false>(tmA, tmB, p, stream);
