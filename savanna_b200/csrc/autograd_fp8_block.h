@@ -33,15 +33,22 @@ Tensor flat(const Tensor& x) {
   return D == 1 || r.stride(1) == 1 ? r : r.contiguous();
 }
 
+// Scales [blocks, n] as the kernels write them: rows a multiple of four apart
+Tensor scale_rows(int64_t blocks, int64_t n, at::Device device) {
+  const int64_t ld = (n + 3) / 4 * 4;
+  Tensor s = alloc({blocks, ld}, F32, device);
+  return ld == n ? s : s.narrow(1, 0, n);
+}
+
 struct Coded { Tensor q, s; };                  // codes [R, C], scales as fp8_block.cu lays them out
 struct Quantized { Coded rows, cols; Tensor sums; };
 Quantized quantize(const Tensor& x2, int form, bool sums = false, const Tensor& a = Tensor(), const Tensor& g = Tensor()) {
   const int64_t R = x2.size(0), C = x2.size(1);
   const at::Device dev = x2.device();
   Quantized r;
-  if (form & BY_ROWS) r.rows = {codes(R, C, dev), alloc({blocks(C), R}, F32, dev)};
+  if (form & BY_ROWS) r.rows = {codes(R, C, dev), scale_rows(blocks(C), R, dev)};
   if (form & BY_TILES) r.rows = {codes(R, C, dev), alloc({blocks(R), blocks(C)}, F32, dev)};
-  if (form & BY_COLUMNS) r.cols = {codes(R, C, dev), alloc({blocks(R), C}, F32, dev)};
+  if (form & BY_COLUMNS) r.cols = {codes(R, C, dev), scale_rows(blocks(R), C, dev)};
   if (sums) r.sums = alloc({blocks(R), C}, F32, dev);
   SB_CALL(sb_fp8_block_quantize, R > 0, ptr(x2), (long long)(R > 1 ? x2.stride(0) : C), (long long)R, (int)C, type_code(x2.scalar_type()), form, out(r.rows.q), f32o(r.rows.s),
           out(r.cols.q), f32o(r.cols.s), (long long)((C + 15) / 16 * 16), f32(a), ptr(g), f32o(r.sums), stream());
@@ -78,13 +85,13 @@ Tensor block_forward(const Tensor& xq, const Tensor& xs, const Coded& w, at::Sca
 }
 Tensor block_input_grad(const Coded& g, const Coded& w, at::ScalarType type) {
   Tensor dx = alloc({g.q.size(0), w.q.size(1)}, type, g.q.device());
-  block_gemm({g.q, g.s, 1, g.s.size(1), false}, {w.q, w.s, w.s.stride(1), w.s.stride(0), true}, false, dx);
+  block_gemm({g.q, g.s, 1, g.s.stride(0), false}, {w.q, w.s, w.s.stride(1), w.s.stride(0), true}, false, dx);
   return dx;
 }
 // dw [N, K]; added by the product's epilogue straight into the parameter's gradient where that lives in a persistent flat buffer
 Tensor block_weight_grad(const Coded& g, const Coded& x, at::ScalarType type, const Tensor& sink) {
   const int64_t N = g.q.size(1), K = x.q.size(1);
-  const Factor a{g.q, g.s, 1, N, true}, b{x.q, x.s, 1, K, true};
+  const Factor a{g.q, g.s, 1, g.s.stride(0), true}, b{x.q, x.s, 1, x.s.stride(0), true};
   if (sink.defined()) {
     const Tensor& tgt = sink.grad();
     if (tgt.defined() && tgt.scalar_type() == type && tgt.is_contiguous() && tgt.dim() == 2 && tgt.size(0) == N && tgt.size(1) == K) {
@@ -166,7 +173,7 @@ BlockNorm block_norm(const Tensor& x, const OptTensor& residual, const Tensor& g
   BlockNorm n;
   n.s = residual.has_value() ? alloc({T, D}, x.scalar_type(), dev) : x2;
   n.q = codes(T, D, dev);
-  n.scale = alloc({blocks(D), T}, F32, dev);
+  n.scale = scale_rows(blocks(D), T, dev);
   if (want_a) n.a = alloc({T}, F32, dev);
   SB_CALL(sb_fp8_block_norm, T > 0, ptr(x2), (long long)(T > 1 ? x2.stride(0) : D), ptr(r2), (long long)(r2.defined() && T > 1 ? r2.stride(0) : D), ptr(gc),
           residual.has_value() ? out(n.s) : nullptr, out(n.q), (long long)((D + 15) / 16 * 16), f32o(n.scale), f32o(n.a), (long long)T, (int)D, (float)eps, (int)form,

@@ -5,14 +5,16 @@
 //   dequantise
 //
 // Layouts.  Codes keep the shape of x; their rows are `ldq` bytes apart (a multiple of 16, what the tensor-core product's loads need).
-// Scales lie with the direction that the product does not contract contiguous: [C / 128][R] for rows, [R / 128][C] for columns (a warp of the
-// product reads those of 32 neighbouring rows at once), [R / 128][C / 128] for tiles.
+// Scales lie with the direction that the product does not contract contiguous: [C / 128][R] for rows, [R / 128][C] for columns, both with the inner
+// dimension rounded up to fours (the product fetches those of 128 neighbouring rows in copies of 16 bytes), [R / 128][C / 128] for tiles.
 #include "device_info.h"
 #include "entries.h"
 #include "fp8_block.cuh"
 
 namespace sb {
 namespace blk8 {
+
+__host__ __device__ inline long long fours(long long n) { return (n + 3) / 4 * 4; }
 
 // ------------------------------------------------------------------------------------------------ tiles of 128 x 128
 // A block of 256 threads holds a tile in registers: sixteen threads eight columns each, eight rows a thread, all loads issued before the
@@ -114,7 +116,7 @@ quantize_kernel(QuantArgs p) {
     }
   }
   __syncthreads();
-  if ((FORM & ROWS) && threadIdx.x < rows) p.s_rows[tile_c * p.R + r0 + threadIdx.x] = row_scale[threadIdx.x];
+  if ((FORM & ROWS) && threadIdx.x < rows) p.s_rows[tile_c * fours(p.R) + r0 + threadIdx.x] = row_scale[threadIdx.x];
   if (FORM & TILE) {
     uint32_t m = col_max[0];
 #pragma unroll
@@ -137,7 +139,7 @@ quantize_kernel(QuantArgs p) {
       col_max[threadIdx.x] = m;
       const long long c = tile_c * BLOCK + threadIdx.x;
       if (c < p.C) {
-        p.s_cols[tile_r * p.C + c] = Coder(m).scale;
+        p.s_cols[tile_r * fours(p.C) + c] = Coder(m).scale;
         if (p.sums) {
           float s = sum_part[0][threadIdx.x];
 #pragma unroll
@@ -258,7 +260,7 @@ norm_quantize_kernel(NormArgs p) {
     const Coder k(m);
     if (c < p.D) {
       *reinterpret_cast<uint2*>(p.q + row * p.ldq + c) = encode(k, f);
-      if ((threadIdx.x & 15) == 0) p.scale[(long long)(c / BLOCK) * p.T + row] = k.scale;
+      if ((threadIdx.x & 15) == 0) p.scale[(c / BLOCK) * fours(p.T) + row] = k.scale;
     }
   }
 }

@@ -8,7 +8,7 @@
 //
 //   warp 0     TMA producer: a k-block's operands, 32 KB a CTA and stage
 //   warp 1     MMA issuer: four products of 32 k a k-block, each k-block into the next of the TMEM buffers
-//   warp 2     the scales into a ring in shared memory (4-byte asynchronous copies: any strides), eight k-blocks deep, handed over by fours
+//   warp 2     the scales into a ring in shared memory (asynchronous copies of 16 bytes, or of 4 for any strides), eight k-blocks deep, handed over by fours
 //   warps 4-11 a lane owns a row and half of the tile's columns: tcgen05.ld of 16 columns, eight packed multiply-adds, while the next 16 are on
 //              their way; after the last k-block the sums leave in whole sectors
 //
@@ -24,6 +24,7 @@
 
 namespace sb {
 
+int make_tmap_2d_bf16(CUtensorMap* out, const void* base, uint64_t inner, uint64_t outer, uint64_t ld, uint32_t box_inner, uint32_t box_outer);
 int make_tmap_2d_u8(CUtensorMap* out, const void* base, uint64_t inner, uint64_t outer, uint64_t ld, uint32_t box_inner, uint32_t box_outer);
 
 namespace blk8 {
@@ -34,7 +35,9 @@ struct GemmArgs {
   const float *sa, *sb;
   long long sa_m, sa_k, sb_n, sb_k;      // strides; sb_n counts blocks of 128 n where the scale is theirs
   long long ldc, ldr;
-  int M, N, K, type, beta, align;        // align: of the rows of C and residual and of the bias, 32 or 16 bytes or less
+  int M, N, K, type, beta;
+  bool boxes;                            // 16-bit results, and what is added, on 16-byte boundaries: stored by store_boxes
+  bool runs;                             // scales of neighbouring rows (and columns, where those have their own) lie together, on 16-byte boundaries
   uint32_t* status;
 };
 
@@ -43,12 +46,15 @@ constexpr int EPI_WARPS = 8, NUM_THREADS = 128 + 32 * EPI_WARPS;
 // 128 * 56 + 256 * 224 = 384 * 168.
 constexpr int REGS_FEW = 56, REGS_MANY = 224;
 static_assert(128 * REGS_FEW + 32 * EPI_WARPS * REGS_MANY <= NUM_THREADS * 168, "registers of a block");
-constexpr int STAGES = 6, OPERAND = 128 * 128, STAGE_BYTES = 2 * OPERAND;
-constexpr int BAR_OFF = STAGES * STAGE_BYTES, OUT_OFF = BAR_OFF + 256, OUT_BYTES = 32 * 64;      // 16 sums of each of a warp's rows (store_row)
+constexpr int OPERAND = 128 * 128, STAGE_BYTES = 2 * OPERAND;
 // Scales of a k-block, rows and columns.  They change hands by GROUP k-blocks: a barrier for each cost the epilogue 200 cycles of 1000.
-constexpr int GROUP = 4, SLOTS = 2 * GROUP, SLOT_OFF = OUT_OFF + EPI_WARPS * OUT_BYTES, SLOT_BYTES = (128 + 256) * 4;
-constexpr int SMEM_BYTES = SLOT_OFF + SLOTS * SLOT_BYTES + 1024;
-static_assert(SMEM_BYTES <= 232448, "shared memory of a block");
+constexpr int GROUP = 4, SLOTS = 2 * GROUP, SLOT_BYTES = (128 + 256) * 4;
+// Shared memory: operand stages; the tile on its way out, 32 rows x 64 columns of 16 bits a box, a box or two a warp; scales; barriers.
+template <bool PAIR> struct Space {
+  static constexpr int STAGES = PAIR ? 4 : 5, BOXES = PAIR ? 2 : 1, BOX = 32 * 128;
+  static constexpr int OUT = STAGES * STAGE_BYTES, SLOT = OUT + EPI_WARPS * BOXES * BOX, BAR = SLOT + SLOTS * SLOT_BYTES, BYTES = BAR + 256 + 1024;
+  static_assert(BYTES <= 232448, "shared memory of a block");
+};
 constexpr int GROUP_M = 8;               // raster: m-tiles that share the concurrently running n-tiles
 
 __device__ __forceinline__ void raster(int tile, int m_tiles, int n_tiles, int& mt, int& nt) {
@@ -61,15 +67,32 @@ __device__ __forceinline__ void raster(int tile, int m_tiles, int n_tiles, int& 
 __device__ __forceinline__ void add_scaled(f2& acc, uint32_t a, uint32_t b, f2 s) {
   asm volatile("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tfma.rn.f32x2 %0, t, %3, %0;\n\t}" : "+l"(acc) : "r"(a), "r"(b), "l"(s));
 }
-__device__ __forceinline__ void put4(uint32_t at, float a, float b, float c, float d) {
-  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
-}
-__device__ __forceinline__ float4 get4(uint32_t at) {
-  float4 v;
-  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+__device__ __forceinline__ f2 scaled(uint32_t a, uint32_t b, f2 s) {
+  f2 v;
+  asm volatile("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tmul.rn.f32x2 %0, t, %3;\n\t}" : "=l"(v) : "r"(a), "r"(b), "l"(s));
   return v;
 }
-
+// 32 rows x 32 columns of TMEM, spread as the tensor cores spread a fragment: of each 8 columns a lane has two neighbouring ones,
+// 2 (lane % 4), of rows lane / 4, + 8 (r[4 i ..]), + 16, + 24 (r[16 + 4 i ..])
+__device__ __forceinline__ void load_fragments(uint32_t taddr, uint32_t (&r)[32]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[16 * h]), "=r"(r[16 * h + 1]), "=r"(r[16 * h + 2]), "=r"(r[16 * h + 3]), "=r"(r[16 * h + 4]), "=r"(r[16 * h + 5]), "=r"(r[16 * h + 6]),
+          "=r"(r[16 * h + 7]), "=r"(r[16 * h + 8]), "=r"(r[16 * h + 9]), "=r"(r[16 * h + 10]), "=r"(r[16 * h + 11]), "=r"(r[16 * h + 12]),
+          "=r"(r[16 * h + 13]), "=r"(r[16 * h + 14]), "=r"(r[16 * h + 15])
+        : "r"(taddr + (uint32_t(16 * h) << 16))
+        : "memory");
+}
+__device__ __forceinline__ void put2(uint32_t at, float2 v) {
+  asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(v.x), "f"(v.y) : "memory");
+}
+__device__ __forceinline__ f2 get2(uint32_t at) {
+  f2 v;
+  asm volatile("ld.shared.b64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
+  return v;
+}
 // The arrival that frees a TMEM buffer hands over no memory (what was read is in registers), so it orders none: a releasing one would wait for
 // the loads of the next scales too, and took four fifths of a k-block's time.
 __device__ __forceinline__ void arrive_relaxed(uint32_t cluster_addr, bool one) {
@@ -81,6 +104,10 @@ __device__ __forceinline__ void arrive_relaxed(uint32_t cluster_addr, bool one) 
 __device__ __forceinline__ void copy4(uint32_t dst, const float* src, bool there) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(__cvta_generic_to_global(src)), "r"(there ? 4 : 0) : "memory");
 }
+// up to four values there are, zeros for the others
+__device__ __forceinline__ void copy16(uint32_t dst, const float* src, int there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(__cvta_generic_to_global(src)), "r"(min(max(there, 0), 4) * 4) : "memory");
+}
 // the thread's copies so far arrive once they have landed
 __device__ __forceinline__ void copies_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
@@ -91,30 +118,6 @@ __device__ __forceinline__ float get1(uint32_t at) {
   return v;
 }
 
-// The way out.  A lane holds a row: it stores 16 columns at once, whole 32-byte sectors, so nothing has to be turned round in shared memory
-// first.  Rows that begin on 32-byte boundaries (WIDE) take one instruction for 8 words, others on 16 two, the rest one value after the other.
-struct Words { uint32_t w[8]; };
-template <bool WIDE> __device__ __forceinline__ Words read_words(const void* p) {
-  Words v;
-  if (WIDE) {
-    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7])
-                 : "l"(__cvta_generic_to_global(p)) : "memory");
-  } else {
-    reinterpret_cast<uint4*>(&v)[0] = static_cast<const uint4*>(p)[0];
-    reinterpret_cast<uint4*>(&v)[1] = static_cast<const uint4*>(p)[1];
-  }
-  return v;
-}
-template <bool WIDE> __device__ __forceinline__ void write_words(void* p, const Words& v) {
-  if (WIDE) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(__cvta_generic_to_global(p)), "r"(v.w[0]), "r"(v.w[1]), "r"(v.w[2]),
-                 "r"(v.w[3]), "r"(v.w[4]), "r"(v.w[5]), "r"(v.w[6]), "r"(v.w[7]) : "memory");
-  } else {
-    static_cast<uint4*>(p)[0] = reinterpret_cast<const uint4*>(&v)[0];
-    static_cast<uint4*>(p)[1] = reinterpret_cast<const uint4*>(&v)[1];
-  }
-}
 __device__ __forceinline__ float2 two(uint32_t w, bf16) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 __device__ __forceinline__ float2 two(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 __device__ __forceinline__ uint32_t word(float a, float b, bf16) { return pack_bf2(a, b); }
@@ -122,65 +125,112 @@ __device__ __forceinline__ uint32_t word(float a, float b, __half) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// f += 16 values at p
-template <bool WIDE, class T> __device__ __forceinline__ void add16(const T* p, float (&f)[16]) {
-  if constexpr (sizeof(T) == 2) {
-    const Words v = read_words<WIDE>(p);
+__device__ __forceinline__ void tma_store_2d(const void* tmap, uint32_t src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(src) : "memory");
+}
+template <class T> __device__ __forceinline__ void add8(const T* p, float (&f)[16], int at) {
+  float t[8];
+  unpack(*reinterpret_cast<const Eight<T>*>(p), t);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) { const float2 t = two(v.w[j], T()); f[2 * j] += t.x; f[2 * j + 1] += t.y; }
+  for (int j = 0; j < 8; ++j) f[at + j] += t[j];
+}
+// A warp's 32 rows of 16-bit results by way of shared memory (128-byte rows, 128-byte swizzle) and a bulk store that runs beside the next
+// tile.  Stored from the registers a tile of 256 x 256 held its warps up for 2 us.  FRAGMENTS: the sums are spread as load_fragments leaves
+// them.  The sum of what is added to the product is formed in fp32.
+template <int COLS, class T, bool FRAGMENTS>
+__device__ __forceinline__ void store_boxes(const GemmArgs& p, const CUtensorMap* tmC, uint32_t space, const f2* acc, int row0, int col0, int lane) {
+  if (lane == 0) bulk_wait_read<0>();              // the last tile has left
+  __syncwarp();
+  if (FRAGMENTS) {
+#pragma unroll
+    for (int c = 0; c < COLS / 8; ++c)             // 8 columns each
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {                // rows lane / 4 + 8 k
+        const int r = (lane >> 2) + 8 * k, row = row0 + r, col = col0 + 8 * c + 2 * (lane & 3);
+        float2 f = f2_unpack(acc[(c >> 2) * 16 + (k >> 1) * 8 + (c & 3) * 2 + (k & 1)]);
+        if (p.beta && row < p.M && col < p.N) {
+          const float2 o = two(*reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.C) + row * p.ldc + col), T());
+          f.x += o.x; f.y += o.y;
+        }
+        const uint32_t at = space + (c >> 3) * (32 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4) + (lane & 3) * 4;
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(word(f.x, f.y, T())) : "memory");
+      }
   } else {
+    const int row = row0 + lane;
+    const bool extra = (p.bias || p.residual || p.beta) && row < p.M;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const Words v = read_words<WIDE>(p + 8 * h);
+    for (int c = 0; c < COLS / 16; ++c) {
+      float f[16];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[8 * h + j] += __uint_as_float(v.w[j]);
+      for (int j = 0; j < 8; ++j) { const float2 t = f2_unpack(acc[c * 8 + j]); f[2 * j] = t.x; f[2 * j + 1] = t.y; }
+      if (extra) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int col = col0 + c * 16 + 8 * h;
+          if (col < p.N) {
+            if (p.bias) add8(static_cast<const T*>(p.bias) + col, f, 8 * h);
+            if (p.residual) add8(static_cast<const T*>(p.residual) + row * p.ldr + col, f, 8 * h);
+            if (p.beta) add8(static_cast<const T*>(p.C) + row * p.ldc + col, f, 8 * h);
+          }
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t at = space + (c >> 2) * (32 * 128) + lane * 128 + (((2 * (c & 3) + h) ^ (lane & 7)) << 4);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(word(f[8 * h], f[8 * h + 1], T())), "r"(word(f[8 * h + 2], f[8 * h + 3], T())),
+                     "r"(word(f[8 * h + 4], f[8 * h + 5], T())), "r"(word(f[8 * h + 6], f[8 * h + 7], T())) : "memory");
+      }
     }
   }
-}
-template <bool WIDE, class T> __device__ __forceinline__ void store16(const GemmArgs& p, long long at_c, long long at_r, int col, float (&f)[16]) {
-  T* c = static_cast<T*>(p.C) + at_c + col;
-  if (p.bias) add16<WIDE, T>(static_cast<const T*>(p.bias) + col, f);
-  if (p.residual) add16<WIDE, T>(static_cast<const T*>(p.residual) + at_r + col, f);
-  if (p.beta) add16<WIDE, T>(c, f);
-  Words v;
-  if constexpr (sizeof(T) == 2) {
+  fence_proxy_async();
+  __syncwarp();
+  if (lane == 0 && row0 < p.M) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v.w[j] = word(f[2 * j], f[2 * j + 1], T());
-    write_words<WIDE>(c, v);
-  } else {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v.w[j] = __float_as_uint(f[8 * h + j]);
-      write_words<WIDE>(c + 8 * h, v);
-    }
+    for (int b = 0; b < COLS / 64; ++b)
+      if (col0 + 64 * b < p.N) tma_store_2d(tmC, space + b * (32 * 128), col0 + 64 * b, row0);
+    bulk_commit();
   }
 }
-template <class T> __device__ __forceinline__ void store_one(const GemmArgs& p, long long at_c, long long at_r, int col, float f) {
-  T* c = static_cast<T*>(p.C) + at_c + col;
+template <class T> __device__ __forceinline__ void store_one(const GemmArgs& p, int row, int col, float f) {
+  T* c = static_cast<T*>(p.C) + row * p.ldc + col;
   if (p.bias) f += up(static_cast<const T*>(p.bias)[col]);
-  if (p.residual) f += up(static_cast<const T*>(p.residual)[at_r + col]);
+  if (p.residual) f += up(static_cast<const T*>(p.residual)[row * p.ldr + col]);
   if (p.beta) f += up(*c);
   *c = down<T>(f);
 }
-template <int COLS, class T>
-__device__ __forceinline__ void store_row(const GemmArgs& p, uint32_t own, const f2* acc, int row, int col0) {
-  const long long at_c = row * p.ldc, at_r = row * p.ldr;
+// Everything else (fp32 results, rows off 16-byte boundaries): 16 columns at a time, a half-warp a row.
+template <int COLS, class T, bool FRAGMENTS>
+__device__ __forceinline__ void store_values(const GemmArgs& p, uint32_t space, const f2* acc, int row0, int col0, int lane) {
 #pragma unroll
   for (int c = 0; c < COLS / 16; ++c) {
-    const int col = col0 + c * 16;
-    float f[16];
+    __syncwarp();
+    if (FRAGMENTS) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) { const float2 t = f2_unpack(acc[c * 8 + j]); f[2 * j] = t.x; f[2 * j + 1] = t.y; }
-    if (p.align == 32 && col + 16 <= p.N) store16<true, T>(p, at_c, at_r, col, f);
-    else if (p.align == 16 && col + 16 <= p.N) store16<false, T>(p, at_c, at_r, col, f);
-    else if (col < p.N) {                  // through the lane's own 64 bytes of shared memory: a short loop instead of 16 copies of it
+      for (int k = 0; k < 4; ++k)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) put4(own + 16 * j, f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
-#pragma unroll 1
-      for (int j = 0; j < min(16, p.N - col); ++j) store_one<T>(p, at_c, at_r, col + j, get1(own + 4 * j));
+        for (int i = 0; i < 2; ++i) {
+          const int r = (lane >> 2) + 8 * k;
+          put2(space + r * 64 + (8 * i + 2 * (lane & 3)) * 4, f2_unpack(acc[(c >> 1) * 16 + (k >> 1) * 8 + (2 * (c & 1) + i) * 2 + (k & 1)]));
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) put2(space + lane * 64 + 8 * j, f2_unpack(acc[c * 8 + j]));
     }
+    __syncwarp();
+    const int col = col0 + c * 16 + (lane & 15);
+#pragma unroll 4
+    for (int r = lane >> 4; r < 32; r += 2)
+      if (col < p.N && row0 + r < p.M) store_one<T>(p, row0 + r, col, get1(space + r * 64 + (lane & 15) * 4));
   }
+  __syncwarp();
+}
+template <int COLS, bool FRAGMENTS>
+__device__ __forceinline__ void store_tile(const GemmArgs& p, const CUtensorMap* tmC, uint32_t space, const f2* acc, int row0, int col0, int lane) {
+  if (p.boxes && p.type == 0) store_boxes<COLS, bf16, FRAGMENTS>(p, tmC, space, acc, row0, col0, lane);
+  else if (p.boxes) store_boxes<COLS, __half, FRAGMENTS>(p, tmC, space, acc, row0, col0, lane);
+  else if (p.type == 0) store_values<COLS, bf16, FRAGMENTS>(p, space, acc, row0, col0, lane);
+  else if (p.type == 1) store_values<COLS, __half, FRAGMENTS>(p, space, acc, row0, col0, lane);
+  else store_values<COLS, float, FRAGMENTS>(p, space, acc, row0, col0, lane);
 }
 
 __device__ __forceinline__ bool spin_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t* status, uint32_t code) {
@@ -190,19 +240,21 @@ __device__ __forceinline__ bool spin_wait(uint32_t bar, uint32_t parity, volatil
 }
 template <bool PAIR, int A_MN, int B_MN, bool SB_ROWS>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
-gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, GemmArgs p) {
+gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC, GemmArgs p) {
+  typedef Space<PAIR> S;
+  constexpr int STAGES = S::STAGES;
   constexpr int TM = PAIR ? 256 : 128, TN = PAIR ? 256 : 128, BUFS = 512 / TN, COLS = TN / 2;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
-  const uint32_t bar_base = smem_base + BAR_OFF;
+  const uint32_t bar_base = smem_base + S::BAR;
   auto full_bar = [&](int s) { return bar_base + 8u * s; };
   auto empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
   auto tfull_bar = [&](int b) { return bar_base + 8u * (2 * STAGES + b); };
   auto tempty_bar = [&](int b) { return bar_base + 8u * (2 * STAGES + 4 + b); };
   auto sfull_bar = [&](int g) { return bar_base + 8u * (2 * STAGES + 8 + g); };
   auto sempty_bar = [&](int g) { return bar_base + 8u * (2 * STAGES + 10 + g); };
-  constexpr int FLAGS = BAR_OFF + 8 * (2 * STAGES + 12);
+  constexpr int FLAGS = S::BAR + 8 * (2 * STAGES + 12);
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem_gen + FLAGS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_gen + FLAGS + 8);
 
@@ -220,6 +272,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     fence_barrier_init();
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
+    if (p.boxes) prefetch_tmap(&tmC);
   }
   if (warp == 1) {
     if (PAIR) { tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512); tmem_relinquish_pair(); }
@@ -292,24 +345,37 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       bool ok = true;
       for (int tile = worker; tile < num_tiles && ok; tile += workers) {
         int mt, nt; raster(tile, m_tiles, n_tiles, mt, nt);
-        const int m0 = mt * TM + int(rank) * 128 + lane, n0 = nt * TN;
+        const int m0 = mt * TM + int(rank) * 128, n0 = nt * TN;
         for (int kb = 0; kb < num_kb; ++kb, ++n) {
           const int group = n / GROUP & 1;
           if (n % GROUP == 0 && !mbar_wait(sempty_bar(group), (n / SLOTS & 1) ^ 1, abort_flag, p.status, ST_FP8_BLOCK + 5)) { ok = false; break; }
-          const uint32_t at = smem_base + SLOT_OFF + (n % SLOTS) * SLOT_BYTES;
+          const uint32_t at = smem_base + S::SLOT + (n % SLOTS) * SLOT_BYTES;
           const float *sa = p.sa + kb * p.sa_k, *sb = p.sb + kb * p.sb_k;
+          if (p.runs) {
+            const int m = m0 + 4 * lane;
+            copy16(at + 16 * lane, m < p.M ? sa + m : sa, p.M - m);
+            if (SB_ROWS) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int m = m0 + 32 * j;
-            copy4(at + (32 * j + lane) * 4, m < p.M ? sa + m * p.sa_m : sa, m < p.M);
-          }
-          if (SB_ROWS) {
-#pragma unroll
-            for (int j = 0; j < TN / 32; ++j) {
-              const int c = n0 + 32 * j + lane;
-              copy4(at + (128 + 32 * j + lane) * 4, c < p.N ? sb + c * p.sb_n : sb, c < p.N);
+              for (int j = 0; j < TN / 128; ++j) {
+                const int c = n0 + 128 * j + 4 * lane;
+                copy16(at + (128 + 128 * j) * 4 + 16 * lane, c < p.N ? sb + c : sb, p.N - c);
+              }
             }
-          } else if (lane < TN / 128) {
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int m = m0 + 32 * j + lane;
+              copy4(at + (32 * j + lane) * 4, m < p.M ? sa + m * p.sa_m : sa, m < p.M);
+            }
+            if (SB_ROWS) {
+#pragma unroll
+              for (int j = 0; j < TN / 32; ++j) {
+                const int c = n0 + 32 * j + lane;
+                copy4(at + (128 + 32 * j + lane) * 4, c < p.N ? sb + c * p.sb_n : sb, c < p.N);
+              }
+            }
+          }
+          if (!SB_ROWS && lane < TN / 128) {
             const int c = n0 + 128 * lane;
             copy4(at + (128 + lane) * 4, c < p.N ? sb + (c / BLOCK) * p.sb_n : sb, c < p.N);
           }
@@ -322,11 +388,11 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_MANY));
     const int q = warp & 3, half = (warp - 4) >> 2;
-    const uint32_t own = smem_base + OUT_OFF + (warp - 4) * OUT_BYTES + lane * 64;
+    const uint32_t space = smem_base + S::OUT + (warp - 4) * (S::BOXES * S::BOX);
     const uint32_t t_warp = tmem_base + (uint32_t(q * 32) << 16) + half * COLS;
     const uint32_t tempty_0 = map_to_cta(tempty_bar(0), 0);        // the even CTA's
     int buf = 0, n = 0; uint32_t buf_phase = 0;                    // n: k-blocks so far, over all tiles
-    const uint32_t slot_0 = smem_base + SLOT_OFF;
+    const uint32_t slot_0 = smem_base + S::SLOT;
     bool ok = true;
     for (int tile = worker; tile < num_tiles && ok; tile += workers) {
       int mt, nt; raster(tile, m_tiles, n_tiles, mt, nt);
@@ -338,34 +404,57 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         const int group = n / GROUP & 1;
         if (n % GROUP == 0 && !spin_wait(sfull_bar(group), n / SLOTS & 1, abort_flag, p.status, ST_FP8_BLOCK + 6)) { ok = false; break; }
         const uint32_t at = slot_0 + (n % SLOTS) * SLOT_BYTES, sb_k = at + (128 + half * COLS) * 4;
-        float s = get1(at + (q * 32 + lane) * 4);
-        if (!SB_ROWS) s *= get1(at + (128 + (PAIR ? half : 0)) * 4);
-        const f2 s2 = f2_pack(s, s);
+        f2 s[SB_ROWS ? 4 : 1];                                     // scales of the lane's rows
+        if (SB_ROWS) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) { const float v = get1(at + (q * 32 + (lane >> 2) + 8 * k) * 4); s[k] = f2_pack(v, v); }
+        } else {
+          const float v = get1(at + (q * 32 + lane) * 4) * get1(at + (128 + (PAIR ? half : 0)) * 4);
+          s[0] = f2_pack(v, v);
+        }
         const uint32_t t = t_warp + buf * TN;
         uint32_t r0[32], r1[32];
-        auto add = [&](int c, const uint32_t (&r)[32]) {
+        auto load = [&](int c, uint32_t (&r)[32]) {
+          if (SB_ROWS) load_fragments(t + 32 * c, r);
+          else tmem_ld_32x32(t + 32 * c, r);
+        };
+        f2 b0[2], b1[2];                                           // scales of the lane's columns of a quarter
+        auto columns = [&](int c) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            f2 lo = s2, hi = s2;
-            if (SB_ROWS) {
-              const float4 b = get4(sb_k + (c * 32 + 4 * j) * 4);
-              lo = f2_mul(f2_pack(b.x, b.y), s2); hi = f2_mul(f2_pack(b.z, b.w), s2);
+          for (int i = 0; i < 2; ++i) {
+            b0[i] = get2(sb_k + (c * 32 + 8 * i + 2 * (lane & 3)) * 4);
+            b1[i] = get2(sb_k + (c * 32 + 16 + 8 * i + 2 * (lane & 3)) * 4);
+          }
+        };
+        if (SB_ROWS) columns(0);
+        auto add = [&](int c, const uint32_t (&r)[32]) {
+          if (SB_ROWS) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const f2 b = i < 2 ? b0[i] : b1[i - 2];
+              f2 v[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[k] = scaled(r[(k >> 1) * 16 + i * 4 + (k & 1) * 2], r[(k >> 1) * 16 + i * 4 + (k & 1) * 2 + 1], b);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) acc[c * 16 + (k >> 1) * 8 + i * 2 + (k & 1)] = f2_fma(v[k], s[SB_ROWS ? k : 0], acc[c * 16 + (k >> 1) * 8 + i * 2 + (k & 1)]);
             }
-            add_scaled(acc[c * 16 + 2 * j], r[4 * j], r[4 * j + 1], lo);
-            add_scaled(acc[c * 16 + 2 * j + 1], r[4 * j + 2], r[4 * j + 3], hi);
+            if (c + 1 < COLS / 32) columns(c + 1);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) add_scaled(acc[c * 16 + j], r[2 * j], r[2 * j + 1], s[0]);
           }
         };
         if (!spin_wait(tfull_bar(buf), buf_phase, abort_flag, p.status, ST_FP8_BLOCK + 4)) { ok = false; break; }
         __syncwarp();
         tc_fence_after();
-        tmem_ld_32x32(t, r0);
-        tmem_ld_32x32(t + 32, r1);
+        load(0, r0);
+        load(1, r1);
         tmem_wait_ld();
         if (COLS == 128) {
           add(0, r0);
-          tmem_ld_32x32(t + 64, r0);
+          load(2, r0);
           add(1, r1);
-          tmem_ld_32x32(t + 96, r1);
+          load(3, r1);
           tmem_wait_ld();
         }
         tc_fence_before();
@@ -381,13 +470,9 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         ++n;
       }
       if (!ok) break;
-      const int row = row0 + lane;
-      if (row < p.M) {
-        if (p.type == 0) store_row<COLS, bf16>(p, own, acc, row, col0);
-        else if (p.type == 1) store_row<COLS, __half>(p, own, acc, row, col0);
-        else store_row<COLS, float>(p, own, acc, row, col0);
-      }
+      store_tile<COLS, SB_ROWS>(p, &tmC, space, acc, row0, col0, lane);
     }
+    if (lane == 0) bulk_wait<0>();
   }
   tc_fence_before();
   __syncthreads();
@@ -408,9 +493,9 @@ static bool goes_by_pairs(int M, int N, int sms) {
 }
 
 template <bool PAIR, int A_MN, int B_MN, bool SB_ROWS>
-static int launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const GemmArgs& p, cudaStream_t stream) {
+static int launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmC, const GemmArgs& p, cudaStream_t stream) {
   auto kern = gemm_fp8_block_kernel<PAIR, A_MN, B_MN, SB_ROWS>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) return -5;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Space<PAIR>::BYTES) != cudaSuccess) return -5;
   // the split of the registers waits for good where a block has fewer of them than it deals out
   static const int regs = [] {
     cudaFuncAttributes a;
@@ -427,11 +512,11 @@ static int launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const GemmArgs
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned((tiles < slots ? tiles : slots) * (PAIR ? 2 : 1)));
   cfg.blockDim = dim3(NUM_THREADS);
-  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.dynamicSmemBytes = Space<PAIR>::BYTES;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = PAIR ? 2 : 1;
-  if (cudaLaunchKernelEx(&cfg, kern, tmA, tmB, p) == cudaSuccess) return 0;
+  if (cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmC, p) == cudaSuccess) return 0;
   (void)cudaGetLastError();
   return -6;
 }
@@ -454,18 +539,19 @@ extern "C" int sb_gemm_fp8_block(const void* A, const float* sa, long long sa_m,
   if (!ctx_bound) { cudaFree(0); ctx_bound = true; }
   if ((lda % 16) || (ldb % 16) || ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(B)) & 15)) return -4;
   if ((long long)((M + 127) / 128) * ((N + 127) / 128) > 0x7fffffffLL) return -3;
-  CUtensorMap tmA, tmB;
+  CUtensorMap tmA, tmB, tmC = {};
   int rc;
   if ((rc = a_mn ? make_tmap_2d_u8(&tmA, A, M, K, lda, 128, 128) : make_tmap_2d_u8(&tmA, A, K, M, lda, 128, 128))) return rc;
   if ((rc = b_mn ? make_tmap_2d_u8(&tmB, B, N, K, ldb, 128, 128) : make_tmap_2d_u8(&tmB, B, K, N, ldb, 128, 128))) return rc;
   const int size = type == 2 ? 4 : 2;
-  const long long step = (reinterpret_cast<uintptr_t>(C) | ldc * size | reinterpret_cast<uintptr_t>(bias) |
-                          (residual ? reinterpret_cast<uintptr_t>(residual) | ldr * size : 0)) & 31;
-  const int align = step == 0 ? 32 : step == 16 ? 16 : 0;
-  GemmArgs p{C, bias, residual, sa, sb, sa_m, sa_k, sb_n, sb_k, ldc, ldr, M, N, K, type, beta, align, status};
+  const auto on16 = [](const void* at, long long row_bytes) { return !((reinterpret_cast<uintptr_t>(at) | row_bytes) & 15); };
+  const bool boxes = type != 2 && N % 8 == 0 && on16(C, ldc * size) && on16(bias, 0) && (!residual || on16(residual, ldr * size));
+  const bool runs = sa_m == 1 && on16(sa, sa_k * 4) && (!sb_rows || (sb_n == 1 && on16(sb, sb_k * 4)));
+  if (boxes && (rc = make_tmap_2d_bf16(&tmC, C, N, M, ldc, 64, 32))) return rc;      // two-byte elements: fp16 alike
+  GemmArgs p{C, bias, residual, sa, sb, sa_m, sa_k, sb_n, sb_k, ldc, ldr, M, N, K, type, beta, boxes, runs, status};
   const bool pair = goes_by_pairs(M, N, num_sms());
-  if (!a_mn && !b_mn && !sb_rows) return pair ? launch<true, 0, 0, false>(tmA, tmB, p, stream) : launch<false, 0, 0, false>(tmA, tmB, p, stream);
-  if (!a_mn && b_mn && !sb_rows) return pair ? launch<true, 0, 1, false>(tmA, tmB, p, stream) : launch<false, 0, 1, false>(tmA, tmB, p, stream);
-  if (a_mn && b_mn && sb_rows) return pair ? launch<true, 1, 1, true>(tmA, tmB, p, stream) : launch<false, 1, 1, true>(tmA, tmB, p, stream);
+  if (!a_mn && !b_mn && !sb_rows) return pair ? launch<true, 0, 0, false>(tmA, tmB, tmC, p, stream) : launch<false, 0, 0, false>(tmA, tmB, tmC, p, stream);
+  if (!a_mn && b_mn && !sb_rows) return pair ? launch<true, 0, 1, false>(tmA, tmB, tmC, p, stream) : launch<false, 0, 1, false>(tmA, tmB, tmC, p, stream);
+  if (a_mn && b_mn && sb_rows) return pair ? launch<true, 1, 1, true>(tmA, tmB, tmC, p, stream) : launch<false, 1, 1, true>(tmA, tmB, tmC, p, stream);
   return -3;
 }
