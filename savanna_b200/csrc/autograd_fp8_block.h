@@ -77,10 +77,17 @@ void block_gemm(const Factor& a, const Factor& b, bool b_rows, const Tensor& o, 
   TORCH_CHECK(rc == 0, "gemm_fp8_block failed (code ", rc, "): M=", M, " N=", N, " K=", K, " ",
               layouts({{"a", &a.q}, {"b", &b.q}, {"out", &o}, {"bias", &bias}, {"residual", &residual}}));
 }
-// y [T, N] = rows (xs [T, K / 128] in any strides) * tiles^T
-Tensor block_forward(const Tensor& xq, const Tensor& xs, const Coded& w, at::ScalarType type, const Tensor& bias, const Tensor& residual) {
-  Tensor y = alloc({xq.size(0), w.q.size(0)}, type, xq.device());
-  block_gemm({xq, xs, xs.stride(0), xs.stride(1), false}, {w.q, w.s, w.s.stride(0), w.s.stride(1), false}, false, y, bias, residual);
+// y [T, N] = rows (xs [T, K / 128] in any strides) * tiles^T.  behind: the last launch on the stream wrote xq and xs.
+Tensor block_forward(const Tensor& xq, const Tensor& xs, const Coded& w, at::ScalarType type, const Tensor& bias, const Tensor& residual, bool behind) {
+  const int64_t T = xq.size(0), N = w.q.size(0);
+  Tensor y = alloc({T, N}, type, xq.device());
+  if (!L.sb_gemm_fp8_block_takes_few((int)T, (int)N)) {
+    block_gemm({xq, xs, xs.stride(0), xs.stride(1), false}, {w.q, w.s, w.s.stride(0), w.s.stride(1), false}, false, y, bias, residual);
+    return y;
+  }
+  SB_CALL(sb_gemm_fp8_block_few, T > 0, ptr(xq), f32(xs), (long long)xs.stride(0), (long long)xs.stride(1), ptr(w.q), f32(w.s), (long long)w.s.stride(0),
+          (long long)w.s.stride(1), out(y), ptr(bias), ptr(residual), (int)T, (int)N, (int)xq.size(1), (long long)row_stride(xq), (long long)row_stride(w.q), (long long)N,
+          (long long)(residual.defined() && T > 1 ? residual.stride(0) : N), type_code(type), (int)behind, status_word(xq.device()), stream());
   return y;
 }
 Tensor block_input_grad(const Coded& g, const Coded& w, at::ScalarType type) {
@@ -127,7 +134,7 @@ struct BlockLinear : Function<BlockLinear> {
     const Tensor x2 = flat(x);
     const int64_t N = wq.size(0);
     Quantized xq = quantize(x2, BY_ROWS | (train_w ? BY_COLUMNS : 0));
-    Tensor y = block_forward(xq.rows.q, xq.rows.s.t(), {wq, ws}, type, opt(bias), residual.has_value() ? flat(*residual) : Tensor());
+    Tensor y = block_forward(xq.rows.q, xq.rows.s.t(), {wq, ws}, type, opt(bias), residual.has_value() ? flat(*residual) : Tensor(), true);
     ctx->save_for_backward({train_w ? xq.cols.q : Tensor(), train_w ? xq.cols.s : Tensor(), wq, ws});
     ctx->saved_data["shape"] = x.sizes().vec();
     ctx->saved_data["w"] = w.has_value();
@@ -186,7 +193,7 @@ struct BlockNormLinear : Function<BlockNormLinear> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual, const Tensor& wn, const OptTensor& w, const OptTensor& bias,
                                const Tensor& wq, const Tensor& ws, double eps, int64_t form, bool fuse) {
     const BlockNorm n = block_norm(x, residual, wn, eps, form, true);
-    Tensor y = block_forward(n.q, n.scale.t(), {wq, ws}, x.scalar_type(), opt(bias), Tensor());
+    Tensor y = block_forward(n.q, n.scale.t(), {wq, ws}, x.scalar_type(), opt(bias), Tensor(), true);
     Tensor s = residual.has_value() ? n.s.view(x.sizes()) : x.view_as(x);
     ctx->save_for_backward({residual.has_value() ? s : x, wn, n.a, wq, ws});
     save_norm(ctx, x, eps, form);
@@ -339,10 +346,10 @@ Tensor linear_fp8_block(const Tensor& x, const OptTensor& xs, const py::object& 
   Tensor y;
   if (xs.has_value()) {
     const Tensor q2 = readable_codes(x.dim() == 2 ? x : x.reshape({T, K}));
-    y = block_forward(q2, xs->dim() == 2 ? *xs : xs->reshape({T, blocks(K)}), wc, type, opt(b), r2);
+    y = block_forward(q2, xs->dim() == 2 ? *xs : xs->reshape({T, blocks(K)}), wc, type, opt(b), r2, false);
   } else {
     const Coded xq = quantize(flat(x), BY_ROWS).rows;
-    y = block_forward(xq.q, xq.s.t(), wc, type, opt(b), r2);
+    y = block_forward(xq.q, xq.s.t(), wc, type, opt(b), r2, true);
   }
   return y.view(with_last(x.sizes(), w.size(0)));
 }
@@ -368,6 +375,6 @@ std::optional<std::tuple<Tensor, Tensor>> norm_linear_fp8_block(const Tensor& x,
   }
   const at::AutoDispatchBelowADInplaceOrView no_graph;
   const BlockNorm n = block_norm(x, residual, g, eps, form, false);
-  const Tensor y = block_forward(n.q, n.scale.t(), wc, x.scalar_type(), opt(b), Tensor());
+  const Tensor y = block_forward(n.q, n.scale.t(), wc, x.scalar_type(), opt(b), Tensor(), true);
   return std::make_tuple(y.view(with_last(x.sizes(), w.size(0))), residual.has_value() ? n.s.view(x.sizes()) : x);
 }

@@ -10,6 +10,7 @@
 #include "device_info.h"
 #include "entries.h"
 #include "fp8_block.cuh"
+#include "pdl.cuh"
 
 namespace sb {
 namespace blk8 {
@@ -44,6 +45,7 @@ quantize_kernel(QuantArgs p) {
   __shared__ float sum_part[8][BLOCK];
   __shared__ float row_scale[BLOCK];
   __shared__ uint32_t col_max[BLOCK];
+  let_next_start();                                         // first of a chain (pdl.cuh), or before a kernel that waits for all of it
   const long long tile_r = blockIdx.x / p.col_tiles, tile_c = blockIdx.x - tile_r * p.col_tiles;
   const int l = threadIdx.x & 15, h = threadIdx.x >> 4, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long r0 = tile_r * BLOCK;
@@ -207,6 +209,7 @@ template <class T, int V, bool VEC>
 __global__ void __launch_bounds__(512)
 norm_quantize_kernel(NormArgs p) {
   __shared__ float red[16];
+  let_next_start();
   const long long row = blockIdx.x;
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
   const T* res = p.res ? static_cast<const T*>(p.res) + row * p.ldr : nullptr;
