@@ -9,106 +9,116 @@
 constexpr auto E4M3 = at::kFloat8_e4m3fn;
 constexpr int64_t MAX_BLOCK_SIZE = (1LL << 31) - 256;       // of a product's dimensions, which have 32 bits
 int64_t blocks(int64_t n) { return (n + 127) / 128; }
+int64_t up_to(int64_t n, int64_t step) { return (n + step - 1) / step * step; }
 enum { BY_ROWS = 1, BY_COLUMNS = 2, BY_TILES = 4 };
 
 bool block_type(at::ScalarType t) { return t == BF16 || t == at::kHalf || t == F32; }
 
-// Codes [R, C] whose rows begin 16 bytes apart or a multiple of it, as the product's loads want them
+// A product's operand: codes [R, C], rows `ld` bytes apart; the scale of row r (BY_COLUMNS: column) and block b at s[r * s_row + b * s_block]; for
+// tiles r counts blocks of rows too.  Whose memory it is, is somebody else's business.
+struct Operand {
+  const void* q = nullptr;
+  const float* s = nullptr;
+  int64_t R = 0, C = 0, ld = 0, s_row = 0, s_block = 0;
+};
+// Codes and scales of one form in one buffer, as fp8_block.cu lays them out: rows of codes 16 bytes apart or a multiple of it, then the scales.
+struct Packed {
+  int64_t R, C, ld, codes, s_ld, bytes;
+  int form;
+  Packed(int64_t R_, int64_t C_, int form_) : R(R_), C(C_), ld(up_to(C_, 16)), codes(up_to(R_ * ld, 256)), form(form_) {
+    s_ld = form == BY_TILES ? blocks(C) : up_to(form == BY_ROWS ? R : C, 4);
+    bytes = codes + (form == BY_ROWS ? blocks(C) : blocks(R)) * s_ld * 4;
+  }
+  Tensor make(at::Device device) const { return alloc({bytes}, at::kByte, device); }
+  Operand in(const Tensor& buf) const {
+    const char* p = static_cast<const char*>(ptr(buf));
+    return {p, reinterpret_cast<const float*>(p + codes), R, C, ld, form == BY_TILES ? s_ld : 1, form == BY_TILES ? 1 : s_ld};
+  }
+};
+
+// Codes and scales as tensors (what fp8_block_quantize returns and linear_fp8_block takes)
+struct Coded { Tensor q, s; };
+int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : up_to(t.size(1), 16); }
 Tensor codes(int64_t R, int64_t C, at::Device device) {
-  const int64_t ld = (C + 15) / 16 * 16;
+  const int64_t ld = up_to(C, 16);
   Tensor q = alloc({R, ld}, at::kByte, device).view(E4M3);
   return ld == C ? q : q.narrow(1, 0, C);
 }
-int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : (t.size(1) + 15) / 16 * 16; }
 Tensor readable_codes(const Tensor& q) {
   if ((q.size(1) == 1 || q.stride(1) == 1) && row_stride(q) % 16 == 0 && row_stride(q) >= q.size(1) && on16(q)) return q;
   Tensor c = codes(q.size(0), q.size(1), q.device());
   c.view(at::kByte).copy_(q.view(at::kByte));
   return c;
 }
+Tensor scale_rows(int64_t blocks, int64_t n, at::Device device) {
+  const int64_t ld = up_to(n, 4);
+  Tensor s = alloc({blocks, ld}, F32, device);
+  return ld == n ? s : s.narrow(1, 0, n);
+}
+Operand operand(const Coded& c) { return {ptr(c.q), f32(c.s), c.q.size(0), c.q.size(1), row_stride(c.q), c.s.stride(0), c.s.stride(1)}; }
+
 // [.., D] -> [rows, D] with unit inner stride; any distance between rows
 Tensor flat(const Tensor& x) {
   const int64_t D = x.size(-1);
   Tensor r = x.dim() == 2 ? x : x.reshape({D ? x.numel() / D : 0, D});
   return D == 1 || r.stride(1) == 1 ? r : r.contiguous();
 }
+long long rows_apart(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
-// Scales [blocks, n] as the kernels write them: rows a multiple of four apart
-Tensor scale_rows(int64_t blocks, int64_t n, at::Device device) {
-  const int64_t ld = (n + 3) / 4 * 4;
-  Tensor s = alloc({blocks, ld}, F32, device);
-  return ld == n ? s : s.narrow(1, 0, n);
-}
-
-struct Coded { Tensor q, s; };                  // codes [R, C], scales as fp8_block.cu lays them out
-struct Quantized { Coded rows, cols; Tensor sums; };
-Quantized quantize(const Tensor& x2, int form, bool sums = false, const Tensor& a = Tensor(), const Tensor& g = Tensor()) {
+// x2 in the forms of `form`: rows (or tiles) to `r`, columns to `c`; sums: column sums of each 128 rows; a, g: of x2 * a[row] * g[column]
+void quantize(const Tensor& x2, int form, const Operand& r, const Operand& c, float* sums = nullptr, const Tensor& a = Tensor(), const Tensor& g = Tensor()) {
   const int64_t R = x2.size(0), C = x2.size(1);
-  const at::Device dev = x2.device();
-  Quantized r;
-  if (form & BY_ROWS) r.rows = {codes(R, C, dev), scale_rows(blocks(C), R, dev)};
-  if (form & BY_TILES) r.rows = {codes(R, C, dev), alloc({blocks(R), blocks(C)}, F32, dev)};
-  if (form & BY_COLUMNS) r.cols = {codes(R, C, dev), scale_rows(blocks(R), C, dev)};
-  if (sums) r.sums = alloc({blocks(R), C}, F32, dev);
-  SB_CALL(sb_fp8_block_quantize, R > 0, ptr(x2), (long long)(R > 1 ? x2.stride(0) : C), (long long)R, (int)C, type_code(x2.scalar_type()), form, out(r.rows.q), f32o(r.rows.s),
-          out(r.cols.q), f32o(r.cols.s), (long long)((C + 15) / 16 * 16), f32(a), ptr(g), f32o(r.sums), stream());
-  return r;
+  SB_CALL(sb_fp8_block_quantize, R > 0, ptr(x2), rows_apart(x2), (long long)R, (int)C, type_code(x2.scalar_type()), form, const_cast<void*>(r.q), const_cast<float*>(r.s),
+          const_cast<void*>(c.q), const_cast<float*>(c.s), (long long)up_to(C, 16), f32(a), ptr(g), sums, stream());
 }
-Tensor column_sums(const Tensor& sums, at::ScalarType type) {
-  Tensor o = alloc({sums.size(1)}, type, sums.device());
-  SB_CALL(sb_fp8_block_column_sums, 1, f32(sums), out(o), (long long)sums.size(0), (int)sums.size(1), type_code(type), stream());
+Tensor column_sums(const float* sums, int64_t tiles, int64_t C, at::ScalarType type, at::Device device) {
+  Tensor o = alloc({C}, type, device);
+  SB_CALL(sb_fp8_block_column_sums, 1, sums, out(o), (long long)tiles, (int)C, type_code(type), stream());
   return o;
 }
 
-// A product's operand: codes as they are stored, and where its scales lie
-struct Factor {
-  const Tensor& q;
-  const Tensor& s;
-  int64_t per_row, per_block;                   // strides of the scale
-  bool transposed;                              // stored with the contraction first
-};
-void block_gemm(const Factor& a, const Factor& b, bool b_rows, const Tensor& o, const Tensor& bias = Tensor(), const Tensor& residual = Tensor(),
-                bool accumulate = false) {
-  const int M = o.size(0), N = o.size(1), K = a.transposed ? a.q.size(0) : a.q.size(1);
-  const int rc = SB_RUN(sb_gemm_fp8_block, M > 0 && N > 0, ptr(a.q), f32(a.s), (long long)a.per_row, (long long)a.per_block, ptr(b.q), f32(b.s), (long long)b.per_row,
-                        (long long)b.per_block, (int)b_rows, out(o), ptr(bias), ptr(residual), M, N, K, (long long)row_stride(a.q), (long long)row_stride(b.q),
-                        (long long)(M > 1 ? o.stride(0) : N), (long long)(residual.defined() && M > 1 ? residual.stride(0) : N), (int)a.transposed,
-                        (int)b.transposed, type_code(o.scalar_type()), (int)accumulate, status_word(o.device()), stream());
-  TORCH_CHECK(rc == 0, "gemm_fp8_block failed (code ", rc, "): M=", M, " N=", N, " K=", K, " ",
-              layouts({{"a", &a.q}, {"b", &b.q}, {"out", &o}, {"bias", &bias}, {"residual", &residual}}));
+// o (+)= a b^T (+ bias) (+ residual); a_mn, b_mn: stored with the contraction first; b_rows: b has a scale for each of its rows
+void block_gemm(const Operand& a, bool a_mn, const Operand& b, bool b_mn, bool b_rows, int64_t K, const Tensor& o, const Tensor& bias = Tensor(),
+                const Tensor& residual = Tensor(), bool accumulate = false) {
+  const int M = o.size(0), N = o.size(1);
+  const int rc = SB_RUN(sb_gemm_fp8_block, M > 0 && N > 0, a.q, a.s, (long long)a.s_row, (long long)a.s_block, b.q, b.s, (long long)b.s_row, (long long)b.s_block, (int)b_rows,
+                        out(o), ptr(bias), ptr(residual), M, N, (int)K, (long long)a.ld, (long long)b.ld, rows_apart(o), residual.defined() ? rows_apart(residual) : 0LL,
+                        (int)a_mn, (int)b_mn, type_code(o.scalar_type()), (int)accumulate, status_word(o.device()), stream());
+  TORCH_CHECK(rc == 0, "gemm_fp8_block failed (code ", rc, "): M=", M, " N=", N, " K=", K, " lda=", a.ld, " ldb=", b.ld, " ",
+              layouts({{"out", &o}, {"bias", &bias}, {"residual", &residual}}));
 }
-// y [T, N] = rows (xs [T, K / 128] in any strides) * tiles^T.  behind: the last launch on the stream wrote xq and xs.
-Tensor block_forward(const Tensor& xq, const Tensor& xs, const Coded& w, at::ScalarType type, const Tensor& bias, const Tensor& residual, bool behind) {
-  const int64_t T = xq.size(0), N = w.q.size(0);
-  Tensor y = alloc({T, N}, type, xq.device());
+// y [T, N] = rows * tiles^T.  behind: the last launch on the stream wrote x.
+Tensor block_forward(const Operand& x, const Operand& w, at::ScalarType type, at::Device device, const Tensor& bias, const Tensor& residual, bool behind) {
+  const int64_t T = x.R, N = w.R;
+  Tensor y = alloc({T, N}, type, device);
   if (!L.sb_gemm_fp8_block_takes_few((int)T, (int)N)) {
-    block_gemm({xq, xs, xs.stride(0), xs.stride(1), false}, {w.q, w.s, w.s.stride(0), w.s.stride(1), false}, false, y, bias, residual);
+    block_gemm(x, false, w, false, false, x.C, y, bias, residual);
     return y;
   }
-  SB_CALL(sb_gemm_fp8_block_few, T > 0, ptr(xq), f32(xs), (long long)xs.stride(0), (long long)xs.stride(1), ptr(w.q), f32(w.s), (long long)w.s.stride(0),
-          (long long)w.s.stride(1), out(y), ptr(bias), ptr(residual), (int)T, (int)N, (int)xq.size(1), (long long)row_stride(xq), (long long)row_stride(w.q), (long long)N,
-          (long long)(residual.defined() && T > 1 ? residual.stride(0) : N), type_code(type), (int)behind, status_word(xq.device()), stream());
+  SB_CALL(sb_gemm_fp8_block_few, T > 0, x.q, x.s, (long long)x.s_row, (long long)x.s_block, w.q, w.s, (long long)w.s_row, (long long)w.s_block, out(y), ptr(bias), ptr(residual),
+          (int)T, (int)N, (int)x.C, (long long)x.ld, (long long)w.ld, (long long)N, residual.defined() ? rows_apart(residual) : 0LL, type_code(type), (int)behind,
+          status_word(device), stream());
   return y;
 }
-Tensor block_input_grad(const Coded& g, const Coded& w, at::ScalarType type) {
-  Tensor dx = alloc({g.q.size(0), w.q.size(1)}, type, g.q.device());
-  block_gemm({g.q, g.s, 1, g.s.stride(0), false}, {w.q, w.s, w.s.stride(1), w.s.stride(0), true}, false, dx);
+Tensor block_input_grad(const Operand& g, Operand w, at::ScalarType type, at::Device device) {
+  Tensor dx = alloc({g.R, w.C}, type, device);
+  std::swap(w.s_row, w.s_block);                            // the contraction goes over the weight's rows
+  block_gemm(g, false, w, true, false, g.C, dx);
   return dx;
 }
 // dw [N, K]; added by the product's epilogue straight into the parameter's gradient where that lives in a persistent flat buffer
-Tensor block_weight_grad(const Coded& g, const Coded& x, at::ScalarType type, const Tensor& sink) {
-  const int64_t N = g.q.size(1), K = x.q.size(1);
-  const Factor a{g.q, g.s, 1, g.s.stride(0), true}, b{x.q, x.s, 1, x.s.stride(0), true};
+Tensor block_weight_grad(const Operand& g, const Operand& x, at::ScalarType type, at::Device device, const Tensor& sink) {
+  const int64_t N = g.C, K = x.C, T = g.R;
   if (sink.defined()) {
     const Tensor& tgt = sink.grad();
     if (tgt.defined() && tgt.scalar_type() == type && tgt.is_contiguous() && tgt.dim() == 2 && tgt.size(0) == N && tgt.size(1) == K) {
-      if (g.q.size(0) > 0) block_gemm(a, b, true, tgt, Tensor(), Tensor(), true);
+      if (T > 0) block_gemm(g, true, x, true, true, T, tgt, Tensor(), Tensor(), true);
       return Tensor();
     }
   }
-  if (g.q.size(0) == 0) return zeros({N, K}, type, g.q.device());
-  Tensor dw = alloc({N, K}, type, g.q.device());
-  block_gemm(a, b, true, dw);
+  if (T == 0) return zeros({N, K}, type, device);
+  Tensor dw = alloc({N, K}, type, device);
+  block_gemm(g, true, x, true, true, T, dw);
   return dw;
 }
 
@@ -116,100 +126,124 @@ void no_second_derivative() {
   TORCH_CHECK(!at::GradMode::is_enabled(), "projections on 8-bit operands with a scale for each block have no second derivative (create_graph)");
 }
 // The output gradient in the forms that the wanted gradients need, and the bias gradient
-struct OutGrad { Quantized q; Tensor bias; };
+struct OutGrad {
+  Tensor buf_rows, buf_cols, bias;
+  Operand rows, cols;
+};
 OutGrad out_grad(const Tensor& g2, bool x, bool w, bool bias) {
   OutGrad r;
-  const int form = (x ? BY_ROWS : 0) | (w ? BY_COLUMNS : 0);
-  const bool sums = bias && w && g2.size(0) > 0;
-  if (form) r.q = quantize(g2, form, sums);
-  if (sums) r.bias = column_sums(r.q.sums, g2.scalar_type());
+  const int64_t T = g2.size(0), N = g2.size(1);
+  const at::Device dev = g2.device();
+  if (x) { const Packed p(T, N, BY_ROWS); r.buf_rows = p.make(dev); r.rows = p.in(r.buf_rows); }
+  if (w) { const Packed p(T, N, BY_COLUMNS); r.buf_cols = p.make(dev); r.cols = p.in(r.buf_cols); }
+  const bool sums = bias && w && T > 0;
+  const Tensor part = sums ? alloc({blocks(T), N}, F32, dev) : Tensor();
+  if (x || w) quantize(g2, (x ? BY_ROWS : 0) | (w ? BY_COLUMNS : 0), r.rows, r.cols, f32o(part));
+  if (sums) r.bias = column_sums(f32(part), blocks(T), N, g2.scalar_type(), dev);
   else if (bias) r.bias = g2.to(F32).sum(0).to(g2.scalar_type());
   return r;
 }
+// A weight that a node kept: packed codes (s absent), or the caller's pair
+Operand saved_weight(const Tensor& q, const Tensor& s, int64_t N, int64_t K, at::Device dev, Coded& hold) {
+  if (!s.defined()) {
+    const Packed p(N, K, BY_TILES);
+    hold.q = as_saved(q, {p.bytes}, at::kByte, dev);
+    return p.in(hold.q);
+  }
+  hold = {readable_codes(as_saved(q, {N, K}, E4M3, dev)), as_saved(s, {blocks(N), blocks(K)}, F32, dev)};
+  return operand(hold);
+}
 
-// y = x w^T (+ bias) (+ residual).  Edges: x, w where it is a tensor that training changes, bias, residual.  xs: x holds codes with these scales.
+// y = x w^T (+ bias) (+ residual).  Edges: x, w where it is a tensor that training changes, bias, residual.
 struct BlockLinear : Function<BlockLinear> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& w, const OptTensor& bias, const OptTensor& residual, const Tensor& wq,
-                        const Tensor& ws, bool fuse, bool train_w, at::ScalarType type) {
+                        const OptTensor& ws, bool fuse, bool train_w, at::ScalarType type, const Operand& wo) {
     const Tensor x2 = flat(x);
-    const int64_t N = wq.size(0);
-    Quantized xq = quantize(x2, BY_ROWS | (train_w ? BY_COLUMNS : 0));
-    Tensor y = block_forward(xq.rows.q, xq.rows.s.t(), {wq, ws}, type, opt(bias), residual.has_value() ? flat(*residual) : Tensor(), true);
-    ctx->save_for_backward({train_w ? xq.cols.q : Tensor(), train_w ? xq.cols.s : Tensor(), wq, ws});
+    const at::Device dev = x.device();
+    const int64_t N = wo.R;
+    const Packed rows(x2.size(0), x2.size(1), BY_ROWS), cols(x2.size(0), x2.size(1), BY_COLUMNS);
+    const Tensor kept = train_w ? cols.make(dev) : Tensor();
+    Tensor y;
+    {
+      const Tensor buf = rows.make(dev), r2 = residual.has_value() ? flat(*residual) : Tensor();
+      quantize(x2, BY_ROWS | (train_w ? BY_COLUMNS : 0), rows.in(buf), train_w ? cols.in(kept) : Operand());
+      y = block_forward(rows.in(buf), wo, type, dev, opt(bias), r2, true);
+    }
+    ctx->save_for_backward({kept, wq, opt(ws)});
     ctx->saved_data["shape"] = x.sizes().vec();
-    ctx->saved_data["w"] = w.has_value();
-    ctx->saved_data["train_w"] = train_w;
-    ctx->saved_data["bias"] = bias.has_value();
-    ctx->saved_data["res"] = residual.has_value();
+    ctx->saved_data["flags"] = int64_t(w.has_value()) | int64_t(train_w) << 1 | int64_t(bias.has_value()) << 2 | int64_t(residual.has_value()) << 3;
     ctx->saved_data["N"] = N;
     ctx->saved_data["xtype"] = (int64_t)x.scalar_type();
     if (fuse) ctx->saved_data["sink"] = *w;
-    return y.view(with_last(x.sizes(), N));
+    return x.dim() == 2 ? y : y.view(with_last(x.sizes(), N));
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     no_second_derivative();
     const variable_list s = ctx->get_saved_variables();
     const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
-    const int64_t N = ctx->saved_data["N"].toInt(), K = shape.back(), T = g[0].numel() / N;
-    const bool has_w = ctx->saved_data["w"].toBool(), has_b = ctx->saved_data["bias"].toBool();
-    const bool need_x = ctx->needs_input_grad(0), need_w = has_w && ctx->needs_input_grad(1) && ctx->saved_data["train_w"].toBool(),
-               need_b = has_b && ctx->needs_input_grad(1 + has_w);
+    const int64_t N = ctx->saved_data["N"].toInt(), K = shape.back(), T = g[0].numel() / N, flags = ctx->saved_data["flags"].toInt();
+    const bool has_w = flags & 1, has_b = flags & 4;
+    const bool need_x = ctx->needs_input_grad(0), need_w = has_w && (flags & 2) && ctx->needs_input_grad(1), need_b = has_b && ctx->needs_input_grad(1 + has_w);
     const at::Device dev = g[0].device();
-    const at::ScalarType xtype = (at::ScalarType)ctx->saved_data["xtype"].toInt();
     const OutGrad go = out_grad(flat(g[0]), need_x, need_w, need_b);
     Tensor gx, gw, gr;
     if (need_x) {
-      const Coded w{readable_codes(as_saved(s[2], {N, K}, E4M3, dev)), as_saved(s[3], {blocks(N), blocks(K)}, F32, dev)};
-      gx = block_input_grad(go.q.rows, w, xtype).view(shape);
+      Coded hold;
+      const Operand w = saved_weight(s[1], s[2], N, K, dev, hold);
+      gx = block_input_grad(go.rows, w, (at::ScalarType)ctx->saved_data["xtype"].toInt(), dev);
+      if (shape.size() != 2) gx = gx.view(shape);
     }
     if (need_w) {
-      const Coded x{readable_codes(as_saved(s[0], {T, K}, E4M3, dev)), as_saved(s[1], {blocks(T), K}, F32, dev)};
-      gw = block_weight_grad(go.q.cols, x, g[0].scalar_type(), sink(ctx, "sink"));
+      const Packed p(T, K, BY_COLUMNS);
+      const Tensor x = as_saved(s[0], {p.bytes}, at::kByte, dev);
+      gw = block_weight_grad(go.cols, p.in(x), g[0].scalar_type(), dev, sink(ctx, "sink"));
     }
-    if (ctx->saved_data["res"].toBool() && ctx->needs_input_grad(1 + has_w + has_b)) gr = g[0];
-    return {gx, gw, go.bias, gr, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    if ((flags & 8) && ctx->needs_input_grad(1 + has_w + has_b)) gr = g[0];
+    return {gx, gw, go.bias, gr, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
-// s = x + residual, codes of norm(s) * g by rows, 1 / rms
-struct BlockNorm { Tensor s, q, scale, a; };
-BlockNorm block_norm(const Tensor& x, const OptTensor& residual, const Tensor& g, double eps, int64_t form, bool want_a) {
+// s = x + residual, codes of norm(s) * g by rows to `q`, 1 / rms
+struct BlockNorm { Tensor s, a; };
+BlockNorm block_norm(const Tensor& x, const OptTensor& residual, const Tensor& g, double eps, int64_t form, bool want_a, const Operand& q) {
   const Tensor x2 = flat(x), r2 = residual.has_value() ? flat(*residual) : Tensor(), gc = contiguous(g);
   const int64_t T = x2.size(0), D = x2.size(1);
-  const at::Device dev = x.device();
   BlockNorm n;
-  n.s = residual.has_value() ? alloc({T, D}, x.scalar_type(), dev) : x2;
-  n.q = codes(T, D, dev);
-  n.scale = scale_rows(blocks(D), T, dev);
-  if (want_a) n.a = alloc({T}, F32, dev);
-  SB_CALL(sb_fp8_block_norm, T > 0, ptr(x2), (long long)(T > 1 ? x2.stride(0) : D), ptr(r2), (long long)(r2.defined() && T > 1 ? r2.stride(0) : D), ptr(gc),
-          residual.has_value() ? out(n.s) : nullptr, out(n.q), (long long)((D + 15) / 16 * 16), f32o(n.scale), f32o(n.a), (long long)T, (int)D, (float)eps, (int)form,
-          type_code(x.scalar_type()), stream());
+  n.s = residual.has_value() ? alloc(x.sizes(), x.scalar_type(), x.device()) : x;
+  if (want_a) n.a = alloc({T}, F32, x.device());
+  SB_CALL(sb_fp8_block_norm, T > 0, ptr(x2), rows_apart(x2), ptr(r2), r2.defined() ? rows_apart(r2) : 0LL, ptr(gc), residual.has_value() ? out(n.s) : nullptr,
+          const_cast<void*>(q.q), (long long)q.ld, const_cast<float*>(q.s), f32o(n.a), (long long)T, (int)D, (float)eps, (int)form, type_code(x.scalar_type()), stream());
   return n;
 }
 
 // (w norm(s)^T (+ bias), s), s = x + residual.  Edges: x, residual, norm weight, w, bias.
 struct BlockNormLinear : Function<BlockNormLinear> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual, const Tensor& wn, const OptTensor& w, const OptTensor& bias,
-                               const Tensor& wq, const Tensor& ws, double eps, int64_t form, bool fuse) {
-    const BlockNorm n = block_norm(x, residual, wn, eps, form, true);
-    Tensor y = block_forward(n.q, n.scale.t(), {wq, ws}, x.scalar_type(), opt(bias), Tensor(), true);
-    Tensor s = residual.has_value() ? n.s.view(x.sizes()) : x.view_as(x);
-    ctx->save_for_backward({residual.has_value() ? s : x, wn, n.a, wq, ws});
+                               const Tensor& wq, const OptTensor& ws, double eps, int64_t form, bool fuse, const Operand& wo) {
+    const at::Device dev = x.device();
+    const int64_t D = x.size(-1);
+    BlockNorm n;
+    Tensor y;
+    {
+      const Packed p(x.numel() / D, D, BY_ROWS);
+      const Tensor buf = p.make(dev);
+      n = block_norm(x, residual, wn, eps, form, true, p.in(buf));
+      y = block_forward(p.in(buf), wo, x.scalar_type(), dev, opt(bias), Tensor(), true);
+    }
+    ctx->save_for_backward({n.s, wn, n.a, wq, opt(ws)});
     save_norm(ctx, x, eps, form);
-    ctx->saved_data["res"] = residual.has_value();
-    ctx->saved_data["w"] = w.has_value();
-    ctx->saved_data["bias"] = bias.has_value();
-    ctx->saved_data["N"] = wq.size(0);
+    ctx->saved_data["flags"] = int64_t(residual.has_value()) | int64_t(w.has_value()) << 1 | int64_t(bias.has_value()) << 2;
+    ctx->saved_data["N"] = wo.R;
     if (fuse) ctx->saved_data["sink"] = *w;
     ctx->set_materialize_grads(false);
-    return {y.view(with_last(x.sizes(), wq.size(0))), s};
+    return {x.dim() == 2 ? y : y.view(with_last(x.sizes(), wo.R)), residual.has_value() ? n.s : x.view_as(x)};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     no_second_derivative();
-    const bool has_r = ctx->saved_data["res"].toBool(), has_w = ctx->saved_data["w"].toBool(), has_b = ctx->saved_data["bias"].toBool();
+    const int64_t flags = ctx->saved_data["flags"].toInt();
+    const bool has_r = flags & 1, has_w = flags & 2, has_b = flags & 4;
     const auto result = [&](const Tensor& dx, const Tensor& dwn, const Tensor& dw, const Tensor& db) -> variable_list {
-      return {dx, has_r ? dx : Tensor(), dwn, dw, db, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+      return {dx, has_r ? dx : Tensor(), dwn, dw, db, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     };
     if (!g[0].defined()) return result(g[1], Tensor(), Tensor(), Tensor());
     const variable_list s = ctx->get_saved_variables();
@@ -222,15 +256,20 @@ struct BlockNormLinear : Function<BlockNormLinear> {
     const Tensor s2 = aligned(as_saved(s[0], shape, type, dev)).view({T, D}), wn = aligned(as_saved(s[1], {D}, type, dev)), a = as_saved(s[2], {T}, F32, dev);
     const OutGrad go = out_grad(flat(g[0]), need_n, need_w, need_b);
     Tensor dx, dwn, dw;
-    if (need_w)
-      dw = block_weight_grad(go.q.cols, quantize(s2, BY_COLUMNS, false, a, wn).cols, type, sink(ctx, "sink"));
+    if (need_w) {
+      const Packed p(T, D, BY_COLUMNS);
+      const Tensor x = p.make(dev);
+      quantize(s2, BY_COLUMNS, Operand(), p.in(x), nullptr, a, wn);
+      dw = block_weight_grad(go.cols, p.in(x), type, dev, sink(ctx, "sink"));
+    }
     if (need_n) {
       if (T == 0) {
         dx = zeros(shape, type, dev);
         dwn = zeros({D}, type, dev);
       } else {
-        const Coded w{readable_codes(as_saved(s[3], {N, D}, E4M3, dev)), as_saved(s[4], {blocks(N), blocks(D)}, F32, dev)};
-        std::tie(dx, dwn) = norm_bwd(s2, wn, a, block_input_grad(go.q.rows, w, type), g[1].defined() ? aligned(g[1]) : g[1],
+        Coded hold;
+        const Operand w = saved_weight(s[3], s[4], N, D, dev, hold);
+        std::tie(dx, dwn) = norm_bwd(s2, wn, a, block_input_grad(go.rows, w, type, dev), g[1].defined() ? aligned(g[1]) : g[1],
                                      ctx->saved_data["eps"].toDouble(), ctx->saved_data["form"].toInt());
         dx = dx.view(shape);
       }
@@ -259,11 +298,22 @@ void check_coded(const char* what, const Tensor& q, const Tensor& s, bool tiles)
                     what, ": float8_e4m3fn ", tiles ? "[N, K] with fp32 scales [N / 128, K / 128]" : "[..., K] with fp32 scales [..., K / 128]", " on one device, got ",
                     q.scalar_type(), " ", q.sizes(), ", ", s.scalar_type(), " ", s.sizes());
 }
-// A weight as the product reads it: kept codes, or those of a tensor
-Coded block_weight(const Tensor& w, const OptTensor& ws) {
-  if (ws.has_value()) return {readable_codes(w), *ws};
+// A weight as the product reads it: the caller's codes, or packed ones of a tensor
+struct BlockWeight {
+  Tensor q;
+  OptTensor s;
+  Operand operand;
+};
+BlockWeight block_weight(const Tensor& w, const OptTensor& ws) {
+  if (ws.has_value()) {
+    const Coded c{readable_codes(w), *ws};
+    return {c.q, c.s, operand(c)};
+  }
   const at::AutoDispatchBelowADInplaceOrView no_graph;
-  return quantize(flat(w), BY_TILES).rows;
+  const Packed p(w.size(0), w.size(1), BY_TILES);
+  const Tensor buf = p.make(w.device());
+  quantize(flat(w), BY_TILES, p.in(buf), Operand());
+  return {buf, std::nullopt, p.in(buf)};
 }
 void check_projection(const char* what, const Tensor& x, int64_t K, const Tensor& w, const OptTensor& ws, const OptTensor& bias, const OptTensor& residual,
                       at::ScalarType type, at::IntArrayRef y) {
@@ -285,9 +335,12 @@ std::tuple<Tensor, Tensor> fp8_block_quantize(const Tensor& x, bool tiles) {
   TORCH_CHECK_VALUE(!tiles || x.dim() == 2, what, " takes [N, K], got ", x.sizes());
   const c10::cuda::CUDAGuard device(x.device());
   const at::AutoDispatchBelowADInplaceOrView no_graph;
-  const Quantized r = quantize(flat(x), tiles ? BY_TILES : BY_ROWS);
-  if (tiles) return {r.rows.q, r.rows.s};
-  return {r.rows.q.view(x.sizes()), r.rows.s.t().view(with_last(x.sizes(), blocks(x.size(-1))))};
+  const Tensor x2 = flat(x);
+  const int64_t R = x2.size(0), C = x2.size(1);
+  const Coded c{codes(R, C, x.device()), tiles ? alloc({blocks(R), blocks(C)}, F32, x.device()) : scale_rows(blocks(C), R, x.device())};
+  quantize(x2, tiles ? BY_TILES : BY_ROWS, operand(c), Operand());
+  if (tiles) return {c.q, c.s};
+  return {c.q.view(x.sizes()), c.s.t().view(with_last(x.sizes(), blocks(C)))};
 }
 Tensor fp8_block_dequantize(const Tensor& q, const Tensor& s, int64_t type) {
   no_transforms();
@@ -318,8 +371,10 @@ std::optional<std::tuple<Tensor, Tensor, Tensor>> rmsnorm_fp8_block(const Tensor
   if (x.size(-1) > 16384) return std::nullopt;
   const c10::cuda::CUDAGuard device(x.device());
   const at::AutoDispatchBelowADInplaceOrView no_graph;
-  const BlockNorm n = block_norm(x, residual, g, eps, form, false);
-  return std::make_tuple(n.q.view(x.sizes()), n.scale.t().view(with_last(x.sizes(), blocks(x.size(-1)))), residual.has_value() ? n.s.view(x.sizes()) : x);
+  const int64_t D = x.size(-1), T = x.numel() / D;
+  const Coded c{codes(T, D, x.device()), scale_rows(blocks(D), T, x.device())};
+  const BlockNorm n = block_norm(x, residual, g, eps, form, false, operand(c));
+  return std::make_tuple(x.dim() == 2 ? c.q : c.q.view(x.sizes()), x.dim() == 2 ? c.s.t() : c.s.t().view(with_last(x.sizes(), blocks(D))), n.s);
 }
 // type: of the result
 Tensor linear_fp8_block(const Tensor& x, const OptTensor& xs, const py::object& weight, const OptTensor& ws, const OptTensor& bias, const OptTensor& residual,
@@ -334,24 +389,27 @@ Tensor linear_fp8_block(const Tensor& x, const OptTensor& xs, const py::object& 
   TORCH_CHECK_VALUE(K <= MAX_BLOCK_SIZE && T <= MAX_BLOCK_SIZE, what, " takes up to ", MAX_BLOCK_SIZE, " rows of as many values, got ", x.sizes());
   check_projection(what, x, K, w, ws, bias, residual, type, with_last(x.sizes(), w.size(0)));
   const c10::cuda::CUDAGuard device(x.device());
-  const Coded wc = block_weight(w, ws);
+  const BlockWeight wc = block_weight(w, ws);
   const OptTensor b = contiguous(bias);
   const OptTensor wt = ws.has_value() ? OptTensor() : OptTensor(w);
   if (wants_grad({&x, given(wt), given(bias), given(residual)})) {
     TORCH_CHECK_VALUE(!xs.has_value(), what, ": inputs in 8 bits carry no gradient; call it under torch.no_grad, or with the tensor itself");
-    return BlockLinear::apply(x, wt, b, residual, wc.q, wc.s, !ws.has_value() && fused(weight), wants_grad({given(wt)}), type);
+    return BlockLinear::apply(x, wt, b, residual, wc.q, wc.s, !ws.has_value() && fused(weight), wants_grad({given(wt)}), type, wc.operand);
   }
   const at::AutoDispatchBelowADInplaceOrView no_graph;
   const Tensor r2 = residual.has_value() ? flat(*residual) : Tensor();
   Tensor y;
   if (xs.has_value()) {
-    const Tensor q2 = readable_codes(x.dim() == 2 ? x : x.reshape({T, K}));
-    y = block_forward(q2, xs->dim() == 2 ? *xs : xs->reshape({T, blocks(K)}), wc, type, opt(b), r2, false);
+    const Coded c{readable_codes(x.dim() == 2 ? x : x.reshape({T, K})), xs->dim() == 2 ? *xs : xs->reshape({T, blocks(K)})};
+    y = block_forward(operand(c), wc.operand, type, x.device(), opt(b), r2, false);
   } else {
-    const Coded xq = quantize(flat(x), BY_ROWS).rows;
-    y = block_forward(xq.q, xq.s.t(), wc, type, opt(b), r2, true);
+    const Tensor x2 = flat(x);
+    const Packed p(T, K, BY_ROWS);
+    const Tensor buf = p.make(x.device());
+    quantize(x2, BY_ROWS, p.in(buf), Operand());
+    y = block_forward(p.in(buf), wc.operand, type, x.device(), opt(b), r2, true);
   }
-  return y.view(with_last(x.sizes(), w.size(0)));
+  return x.dim() == 2 ? y : y.view(with_last(x.sizes(), w.size(0)));
 }
 // nothing where the kernels do not cover type or width
 std::optional<std::tuple<Tensor, Tensor>> norm_linear_fp8_block(const Tensor& x, const Tensor& g, double eps, int64_t form, const py::object& weight, const OptTensor& ws,
@@ -367,14 +425,16 @@ std::optional<std::tuple<Tensor, Tensor>> norm_linear_fp8_block(const Tensor& x,
   // the norm's backward kernel: bf16, rows of eights
   if (K > 16384 || (train && (x.scalar_type() != BF16 || K % 8 || K < 64))) return std::nullopt;
   const c10::cuda::CUDAGuard device(x.device());
-  const Coded wc = block_weight(w, ws);
+  const BlockWeight wc = block_weight(w, ws);
   const OptTensor b = contiguous(bias);
   if (train) {
-    variable_list r = BlockNormLinear::apply(x, residual, g, wt, b, wc.q, wc.s, eps, form, !ws.has_value() && fused(weight));
+    variable_list r = BlockNormLinear::apply(x, residual, g, wt, b, wc.q, wc.s, eps, form, !ws.has_value() && fused(weight), wc.operand);
     return std::make_tuple(r[0], r[1]);
   }
   const at::AutoDispatchBelowADInplaceOrView no_graph;
-  const BlockNorm n = block_norm(x, residual, g, eps, form, false);
-  const Tensor y = block_forward(n.q, n.scale.t(), wc, x.scalar_type(), opt(b), Tensor(), true);
-  return std::make_tuple(y.view(with_last(x.sizes(), w.size(0))), residual.has_value() ? n.s.view(x.sizes()) : x);
+  const Packed p(x.numel() / K, K, BY_ROWS);
+  const Tensor buf = p.make(x.device());
+  const BlockNorm n = block_norm(x, residual, g, eps, form, false, p.in(buf));
+  const Tensor y = block_forward(p.in(buf), wc.operand, x.scalar_type(), x.device(), opt(b), Tensor(), true);
+  return std::make_tuple(x.dim() == 2 ? y : y.view(with_last(x.sizes(), w.size(0))), n.s);
 }

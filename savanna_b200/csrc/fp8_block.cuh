@@ -12,6 +12,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace sb {
 namespace blk8 {
 
@@ -62,6 +64,17 @@ template <> __device__ __forceinline__ __half down<__half>(float f) { return __f
 template <> __device__ __forceinline__ float down<float>(float f) { return f; }
 
 // Eight consecutive values as they lie in memory.
+// Lets a kernel have its dynamic shared memory, once on each device (the call takes half a microsecond).
+template <class F> static bool allow_shared(std::atomic<unsigned long long>& known, F kern, int bytes) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (dev < 64 && (known.load(std::memory_order_relaxed) & bit)) return true;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  if (dev < 64) known.fetch_or(bit);
+  return true;
+}
+
 template <class T> struct alignas(16) Eight { uint4 v[sizeof(T) / 2]; };
 template <class T> __device__ __forceinline__ Eight<T> none() {
   Eight<T> e;

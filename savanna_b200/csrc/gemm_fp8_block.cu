@@ -495,7 +495,8 @@ static bool goes_by_pairs(int M, int N, int sms) {
 template <bool PAIR, int A_MN, int B_MN, bool SB_ROWS>
 static int launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmC, const GemmArgs& p, cudaStream_t stream) {
   auto kern = gemm_fp8_block_kernel<PAIR, A_MN, B_MN, SB_ROWS>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Space<PAIR>::BYTES) != cudaSuccess) return -5;
+  static std::atomic<unsigned long long> allowed{0};       // devices that know the kernel's shared memory
+  if (!allow_shared(allowed, kern, Space<PAIR>::BYTES)) return -5;
   // the split of the registers waits for good where a block has fewer of them than it deals out
   static const int regs = [] {
     cudaFuncAttributes a;

@@ -225,7 +225,8 @@ gemm_fp8_block_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_
 template <int TOK>
 static int launch_few(const CUtensorMap& tmW, const CUtensorMap& tmX, const FewArgs& p, bool chained, cudaStream_t stream) {
   auto kern = gemm_fp8_block_few_kernel<TOK>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FewSpace<TOK>::BYTES) != cudaSuccess) return -5;
+  static std::atomic<unsigned long long> allowed{0};       // devices that know the kernel's shared memory
+  if (!allow_shared(allowed, kern, FewSpace<TOK>::BYTES)) return -5;
   const int tiles = (p.N + 127) / 128, kbs = (p.K + 127) / 128;
   // as many parts of the contraction as give every SM a CTA, and two k-blocks each
   int parts = 1;
