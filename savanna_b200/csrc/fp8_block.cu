@@ -17,6 +17,13 @@ namespace blk8 {
 
 __host__ __device__ inline long long fours(long long n) { return (n + 3) / 4 * 4; }
 
+// These kernels are programmatic dependents of whatever is before them (pdl.cuh, the second kind) and let the next one start once all that is
+// complete: the product for few tokens, which follows, may then read weights ahead as the link of a chain behind an ordinary launch.
+__device__ __forceinline__ void begin() {
+  wait_for_previous();
+  let_next_start();
+}
+
 // ------------------------------------------------------------------------------------------------ tiles of 128 x 128
 // A block of 256 threads holds a tile in registers: sixteen threads eight columns each, eight rows a thread, all loads issued before the
 // first value is used.  From there a row's largest magnitude is four shuffles away and a column's one exchange through shared memory, so the
@@ -45,7 +52,7 @@ quantize_kernel(QuantArgs p) {
   __shared__ float sum_part[8][BLOCK];
   __shared__ float row_scale[BLOCK];
   __shared__ uint32_t col_max[BLOCK];
-  let_next_start();                                         // first of a chain (pdl.cuh), or before a kernel that waits for all of it
+  begin();
   const long long tile_r = blockIdx.x / p.col_tiles, tile_c = blockIdx.x - tile_r * p.col_tiles;
   const int l = threadIdx.x & 15, h = threadIdx.x >> 4, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long r0 = tile_r * BLOCK;
@@ -209,7 +216,7 @@ template <class T, int V, bool VEC>
 __global__ void __launch_bounds__(512)
 norm_quantize_kernel(NormArgs p) {
   __shared__ float red[16];
-  let_next_start();
+  begin();
   const long long row = blockIdx.x;
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
   const T* res = p.res ? static_cast<const T*>(p.res) + row * p.ldr : nullptr;
@@ -304,9 +311,7 @@ static int launch_quantize(const QuantArgs& p, cudaStream_t st) {
   const long long tiles = (p.R + BLOCK - 1) / BLOCK * p.col_tiles;
   if (tiles > 0x7fffffffLL) return -3;
   const bool vec = p.C % 8 == 0 && aligned16<T>(p.x, p.ld) && (!NORM || aligned16<T>(p.g, 8));
-  if (vec) quantize_kernel<T, FORM, NORM, true><<<(unsigned)tiles, 256, 0, st>>>(p);
-  else quantize_kernel<T, FORM, NORM, false><<<(unsigned)tiles, 256, 0, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+  return launch_chained(false, vec ? quantize_kernel<T, FORM, NORM, true> : quantize_kernel<T, FORM, NORM, false>, dim3((unsigned)tiles), 256, 0, st, p);
 }
 template <class T>
 static int launch_form(const QuantArgs& p, int form, cudaStream_t st) {
@@ -321,19 +326,17 @@ static int launch_form(const QuantArgs& p, int form, cudaStream_t st) {
 }
 
 template <class T, int V>
-static void launch_norm_v(const NormArgs& p, int threads, cudaStream_t st) {
+static int launch_norm_v(const NormArgs& p, int threads, cudaStream_t st) {
   const bool vec = p.D % 8 == 0 && aligned16<T>(p.x, p.ldx) && aligned16<T>(p.g, 8) && (!p.res || (aligned16<T>(p.res, p.ldr) && aligned16<T>(p.sum, 8)));
-  if (vec) norm_quantize_kernel<T, V, true><<<(unsigned)p.T, threads, 0, st>>>(p);
-  else norm_quantize_kernel<T, V, false><<<(unsigned)p.T, threads, 0, st>>>(p);
+  return launch_chained(false, vec ? norm_quantize_kernel<T, V, true> : norm_quantize_kernel<T, V, false>, dim3((unsigned)p.T), threads, 0, st, p);
 }
 template <class T>
 static int launch_norm(const NormArgs& p, cudaStream_t st) {
   const int groups = (p.D + 7) / 8;
   auto threads = [&](int v) { return ((groups + v - 1) / v + 31) / 32 * 32; };
-  if (groups <= 128) launch_norm_v<T, 1>(p, threads(1), st);
-  else if (groups <= 512) launch_norm_v<T, 2>(p, threads(2), st);
-  else launch_norm_v<T, 4>(p, threads(4), st);
-  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+  if (groups <= 128) return launch_norm_v<T, 1>(p, threads(1), st);
+  if (groups <= 512) return launch_norm_v<T, 2>(p, threads(2), st);
+  return launch_norm_v<T, 4>(p, threads(4), st);
 }
 
 template <class T>

@@ -8,8 +8,8 @@
 // 80 to 100 KB of operands on their way.  A k-block's product is read from TMEM and added, scaled, in fp32; the CTAs' sums are joined through
 // distributed shared memory in a fixed order.
 //
-// A link of a chain (pdl.cuh, the first kind) behind the kernel that quantises X: the first stages' weights, which do not depend on it, are on their
-// way before it has ended.  All waits are bounded (sm100.cuh).
+// A link of a chain (pdl.cuh, the first kind) behind the kernel that quantises X, which lets it start when all before itself is complete: the first
+// stages' weights, which do not depend on that kernel, are on their way before it has ended.  All waits are bounded (sm100.cuh).
 #include "entries.h"
 #include "fp8_block.cuh"
 #include "pdl.cuh"
@@ -196,6 +196,7 @@ gemm_fp8_block_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_
 #pragma unroll
     for (int t = 0; t < TOK; ++t) sums[t * 128 + n] = acc[t];
   }
+  let_next_start();
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -264,7 +265,7 @@ static int launch_few(const CUtensorMap& tmW, const CUtensorMap& tmX, const FewA
 extern "C" int sb_gemm_fp8_block_takes_few(int M, int N) { return M <= 16 || (M <= 64 && (N + 127) / 128 * 3 <= 2 * sb::num_sms()); }
 
 // As sb_gemm_fp8_block with neither operand transposed and tiles of 128 x 128 in W; up to 64 rows of X.  chained: the launch before it on the
-// stream was the ordinary one of the kernel that wrote X and sx, and did not write W or sw.
+// stream was that of sb_fp8_block_quantize or sb_fp8_block_norm, which wrote X and sx and not W or sw.
 extern "C" int sb_gemm_fp8_block_few(const void* X, const float* sx, long long sx_m, long long sx_k, const void* W, const float* sw, long long sw_n,
                                      long long sw_k, void* y, const void* bias, const void* residual, int M, int N, int K, long long ldx,
                                      long long ldw, long long ldc, long long ldr, int type, int chained, unsigned int* status, cudaStream_t stream) {
