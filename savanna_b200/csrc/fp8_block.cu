@@ -7,6 +7,8 @@
 // Layouts.  Codes keep the shape of x; their rows are `ldq` bytes apart (a multiple of 16, what the tensor-core product's loads need).
 // Scales lie with the direction that the product does not contract contiguous: [C / 128][R] for rows, [R / 128][C] for columns, both with the inner
 // dimension rounded up to fours (the product fetches those of 128 neighbouring rows in copies of 16 bytes), [R / 128][C / 128] for tiles.
+#include <type_traits>
+
 #include "device_info.h"
 #include "entries.h"
 #include "fp8_block.cuh"
@@ -48,7 +50,9 @@ enum { ROWS = 1, COLS = 2, TILE = 4 };
 template <class T, int FORM, bool NORM, bool VEC>
 __global__ void __launch_bounds__(256)
 quantize_kernel(QuantArgs p) {
-  __shared__ uint32_t part[8][BLOCK];                       // columns' largest magnitudes by warp
+  typedef typename std::conditional<NORM, float, T>::type M;          // what magnitudes are compared in
+  constexpr int MW = sizeof(M) == 2 ? 4 : 8;
+  __shared__ uint32_t part[8][16][MW];                      // columns' largest magnitudes by warp
   __shared__ float sum_part[8][BLOCK];
   __shared__ float row_scale[BLOCK];
   __shared__ uint32_t col_max[BLOCK];
@@ -66,89 +70,112 @@ quantize_kernel(QuantArgs p) {
     const int r = h + 16 * i;
     raw[i] = fetch<VEC, T>(x + r * p.ld, r < rows ? n : 0);
   }
-  float g[8], a[8];
+  f2 g[4];
+  float a[8];
   if (NORM) {
-    unpack(fetch<VEC, T>(static_cast<const T*>(p.g) + c0, n), g);
+    pairs(fetch<VEC, T>(static_cast<const T*>(p.g) + c0, n), g);
 #pragma unroll
     for (int i = 0; i < 8; ++i) a[i] = h + 16 * i < rows ? p.a[r0 + h + 16 * i] : 0.f;
   }
-  auto values = [&](int i, float (&f)[8]) {
-    unpack(raw[i], f);
+  auto values = [&](int i, f2 (&v)[4]) {
+    pairs(raw[i], v);
     if (NORM) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = f[j] * a[i] * g[j];
+      for (int j = 0; j < 4; ++j) v[j] = f2_mul(f2_mul(v[j], f2_pack(a[i], a[i])), g[j]);
     }
   };
-  uint32_t cm[8];
-  float cs[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) { cm[j] = 0u; cs[j] = 0.f; }
-  uint32_t tile_max = 0;
+  auto sizes = [&](int i) {
+    if constexpr (NORM) {
+      f2 v[4];
+      values(i, v);
+      return magnitudes(v);
+    } else {
+      return magnitudes(raw[i]);
+    }
+  };
+  Magnitudes<M> most = {};                                  // of the thread's columns
+  f2 cs[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float f[8];
-    values(i, f);
-    if (FORM & COLS) {
+    const Magnitudes<M> m = sizes(i);
+    if (FORM & (COLS | TILE)) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) { cm[j] = max(cm[j], magnitude(f[j])); cs[j] += f[j]; }
+      for (int j = 0; j < MW; ++j) most.w[j] = max_of<M>(most.w[j], m.w[j]);
     }
-    if (FORM & TILE) tile_max = max(tile_max, largest(f));
-    if (FORM & ROWS) {
-      uint32_t m = largest(f);
+    if ((FORM & COLS) && p.sums) {
+      f2 v[4];
+      values(i, v);
 #pragma unroll
-      for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const Coder c(m);
+      for (int j = 0; j < 4; ++j) cs[j] = f2_add(cs[j], v[j]);
+    }
+    if (FORM & ROWS) {
+      uint32_t top = largest(m);
+#pragma unroll
+      for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const Coder c(top);
       const int r = h + 16 * i;
-      if (r < rows && n > 0) *reinterpret_cast<uint2*>(p.q_rows + (r0 + r) * p.ldq + c0) = encode(c, f);
+      f2 v[4];
+      values(i, v);
+      if (r < rows && n > 0) *reinterpret_cast<uint2*>(p.q_rows + (r0 + r) * p.ldq + c0) = encode(c, v);
       if (l == 0) row_scale[r] = c.scale;
     }
   }
   if (FORM & TILE) {
+    uint32_t top = largest(most);
 #pragma unroll
-    for (int o = 16; o; o >>= 1) tile_max = max(tile_max, __shfl_xor_sync(0xffffffffu, tile_max, o));
-    if (lane == 0) col_max[warp] = tile_max;
+    for (int o = 16; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) col_max[warp] = top;
   }
   if (FORM & COLS) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) cm[j] = max(cm[j], __shfl_xor_sync(0xffffffffu, cm[j], 16));
+    for (int j = 0; j < MW; ++j) most.w[j] = max_of<M>(most.w[j], __shfl_xor_sync(0xffffffffu, most.w[j], 16));
     if (lane < 16) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) part[warp][l * 8 + j] = cm[j];
+      for (int j = 0; j < MW; ++j) part[warp][l][j] = most.w[j];
     }
     if (p.sums) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) cs[j] += __shfl_xor_sync(0xffffffffu, cs[j], 16);
-      if (lane < 16) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum_part[warp][l * 8 + j] = cs[j];
+      for (int j = 0; j < 4; ++j) {
+        const float2 t = f2_unpack(cs[j]);
+        const float u = t.x + __shfl_xor_sync(0xffffffffu, t.x, 16), v = t.y + __shfl_xor_sync(0xffffffffu, t.y, 16);
+        if (lane < 16) { sum_part[warp][l * 8 + 2 * j] = u; sum_part[warp][l * 8 + 2 * j + 1] = v; }
       }
     }
   }
   __syncthreads();
   if ((FORM & ROWS) && threadIdx.x < rows) p.s_rows[tile_c * fours(p.R) + r0 + threadIdx.x] = row_scale[threadIdx.x];
   if (FORM & TILE) {
-    uint32_t m = col_max[0];
+    uint32_t top = col_max[0];
 #pragma unroll
-    for (int k = 1; k < 8; ++k) m = max(m, col_max[k]);
-    const Coder c(m);
+    for (int k = 1; k < 8; ++k) top = max(top, col_max[k]);
+    const Coder c(top);
     if (threadIdx.x == 0) p.s_rows[blockIdx.x] = c.scale;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int r = h + 16 * i;
-      float f[8];
-      values(i, f);
-      if (r < rows && n > 0) *reinterpret_cast<uint2*>(p.q_rows + (r0 + r) * p.ldq + c0) = encode(c, f);
+      f2 v[4];
+      values(i, v);
+      if (r < rows && n > 0) *reinterpret_cast<uint2*>(p.q_rows + (r0 + r) * p.ldq + c0) = encode(c, v);
     }
   }
   if (FORM & COLS) {
-    if (threadIdx.x < BLOCK) {
-      uint32_t m = part[0][threadIdx.x];
+    if (threadIdx.x < 16 * MW) {                            // a word of magnitudes a thread: one column's or two neighbours'
+      const int who = threadIdx.x / MW, j = threadIdx.x % MW;
+      uint32_t top = part[0][who][j];
 #pragma unroll
-      for (int k = 1; k < 8; ++k) m = max(m, part[k][threadIdx.x]);
-      col_max[threadIdx.x] = m;
+      for (int k = 1; k < 8; ++k) top = max_of<M>(top, part[k][who][j]);
+      if (sizeof(M) == 2) {
+        col_max[who * 8 + 2 * j] = widen<M>(top & 0xffffu);
+        col_max[who * 8 + 2 * j + 1] = widen<M>(top >> 16);
+      } else {
+        col_max[who * 8 + j] = top;
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x < BLOCK) {
       const long long c = tile_c * BLOCK + threadIdx.x;
       if (c < p.C) {
-        p.s_cols[tile_r * fours(p.C) + c] = Coder(m).scale;
+        p.s_cols[tile_r * fours(p.C) + c] = Coder(col_max[threadIdx.x]).scale;
         if (p.sums) {
           float s = sum_part[0][threadIdx.x];
 #pragma unroll
@@ -157,25 +184,21 @@ quantize_kernel(QuantArgs p) {
         }
       }
     }
-    __syncthreads();
-    uint2 out[8];
-    // two columns at a time: a coder holds three values for each
+    f2 inv[4], minus[4];
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      const Coder c0_(col_max[l * 8 + j]), c1_(col_max[l * 8 + j + 1]);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float f[8];
-        values(i, f);
-        const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(c0_(f[j]), c1_(f[j + 1])), __NV_SATFINITE, __NV_E4M3);
-        uint32_t& w = j < 4 ? out[i].x : out[i].y;
-        w = (j & 2) ? w | two << 16 : two;
-      }
+    for (int j = 0; j < 4; ++j) {
+      const Coder a_(col_max[l * 8 + 2 * j]), b_(col_max[l * 8 + 2 * j + 1]);
+      inv[j] = f2_pack(a_.inv, b_.inv);
+      minus[j] = f2_pack(a_.minus_amax, b_.minus_amax);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int r = h + 16 * i;
-      if (r < rows && n > 0) *reinterpret_cast<uint2*>(p.q_cols + (r0 + r) * p.ldq + c0) = out[i];
+      f2 v[4];
+      values(i, v);
+      if (r < rows && n > 0)
+        *reinterpret_cast<uint2*>(p.q_cols + (r0 + r) * p.ldq + c0) =
+            make_uint2(code2(v[0], inv[0], minus[0]) | code2(v[1], inv[1], minus[1]) << 16, code2(v[2], inv[2], minus[2]) | code2(v[3], inv[3], minus[3]) << 16);
     }
   }
 }
@@ -227,24 +250,26 @@ norm_quantize_kernel(NormArgs p) {
     s[v] = fetch<VEC, T>(x + c, min(8, p.D - c));
     if (res) r[v] = fetch<VEC, T>(res + c, min(8, p.D - c));
   }
-  float ss = 0.f;
+  f2 ss2 = 0ull;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    float f[8];
-    unpack(s[v], f);
+    f2 f[4];
+    pairs(s[v], f);
     if (res) {
-      float t[8];
-      unpack(r[v], t);
+      f2 t[4];
+      pairs(r[v], t);
+      float sum[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] += t[j];
-      s[v] = pack<T>(f);                                  // the norm is that of the sum as it is kept
+      for (int j = 0; j < 4; ++j) { const float2 u = f2_unpack(f2_add(f[j], t[j])); sum[2 * j] = u.x; sum[2 * j + 1] = u.y; }
+      s[v] = pack<T>(sum);                                // the norm is that of the sum as it is kept
       const int c = (threadIdx.x + v * blockDim.x) * 8;
       put<VEC, T>(static_cast<T*>(p.sum) + row * p.D + c, s[v], min(8, p.D - c));
-      unpack(s[v], f);
+      pairs(s[v], f);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss += f[j] * f[j];
+    for (int j = 0; j < 4; ++j) ss2 = f2_fma(f[j], f[j], ss2);
   }
+  float ss = f2_unpack(ss2).x + f2_unpack(ss2).y;
 #pragma unroll
   for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   if (blockDim.x > 32) {
@@ -256,15 +281,16 @@ norm_quantize_kernel(NormArgs p) {
   const float mean = ss / p.D;
   const float a = p.form == 0 ? rsqrtf(mean + p.eps) : 1.f / (sqrtf(mean) + p.eps);
   if (p.a && threadIdx.x == 0) p.a[row] = a;
+  const f2 a2 = f2_pack(a, a);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int c = (threadIdx.x + v * blockDim.x) * 8;
-    float f[8], g[8];
-    unpack(s[v], f);
-    unpack(fetch<VEC, T>(static_cast<const T*>(p.g) + c, min(8, p.D - c)), g);
+    f2 f[4], g[4];
+    pairs(s[v], f);
+    pairs(fetch<VEC, T>(static_cast<const T*>(p.g) + c, min(8, p.D - c)), g);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = f[j] * a * g[j];
-    uint32_t m = largest(f);
+    for (int j = 0; j < 4; ++j) f[j] = f2_mul(f2_mul(f[j], a2), g[j]);
+    uint32_t m = largest(magnitudes(f));
 #pragma unroll
     for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     const Coder k(m);

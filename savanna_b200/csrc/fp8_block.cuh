@@ -14,6 +14,8 @@
 
 #include <atomic>
 
+#include "f32x2.cuh"
+
 namespace sb {
 namespace blk8 {
 
@@ -22,37 +24,47 @@ constexpr int BLOCK = 128;
 
 __device__ __forceinline__ uint32_t magnitude(float f) { return __float_as_uint(f) & 0x7fffffffu; }
 
+// The quotient in units of 2^20, in which x * 448 cannot overflow and a magnitude of 2^-100 is still far from the subnormal numbers.
 struct Coder {
-  float scale, amax, inv, top;             // amax and 448 in units in which x * 448 cannot overflow, and 1 / amax
+  float scale, minus_amax, inv;
   __device__ __forceinline__ explicit Coder(uint32_t m) {                // m: bits of the block's largest magnitude
     const float a = fmaxf(__uint_as_float(m), 7.8886090522101181e-31f);  // 2^-100
     scale = m < 0x7f800000u ? __fmul_rn(a, 1.f / 448.f) : __uint_as_float(0x7fffffffu);
-    const float unit = a > 1.2676506002282294e30f ? 2.3283064365386963e-10f : 1.f;     // above 2^100: units of 2^32
-    amax = a * unit;
-    top = 448.f * unit;
+    const float amax = a * 9.5367431640625e-07f;
+    minus_amax = -amax;
     inv = __frcp_rn(amax);
   }
-  __device__ __forceinline__ float operator()(float x) const {
-    const float n = __fmul_rn(x, top), q = __fmul_rn(n, inv);
-    return __fmaf_rn(__fmaf_rn(-q, amax, n), inv, q);
-  }
 };
-__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
-  return uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3)) |
-         (uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3)) << 16);
+// Two values as two codes: of one block, or of two (columns)
+__device__ __forceinline__ uint32_t code2(f2 x, f2 inv, f2 minus_amax) {
+  const float top = 448.f * 9.5367431640625e-07f;
+  const f2 n = f2_mul(x, f2_pack(top, top)), q = f2_mul(n, inv);
+  return __nv_cvt_float2_to_fp8x2(f2_unpack(f2_fma(f2_fma(q, minus_amax, n), inv, q)), __NV_SATFINITE, __NV_E4M3);
 }
-__device__ __forceinline__ uint2 encode(const Coder& c, const float (&f)[8]) {
-  return make_uint2(e4m3x4(c(f[0]), c(f[1]), c(f[2]), c(f[3])), e4m3x4(c(f[4]), c(f[5]), c(f[6]), c(f[7])));
+__device__ __forceinline__ uint2 encode(const Coder& c, const f2 (&v)[4]) {
+  const f2 inv = f2_pack(c.inv, c.inv), m = f2_pack(c.minus_amax, c.minus_amax);
+  return make_uint2(code2(v[0], inv, m) | code2(v[1], inv, m) << 16, code2(v[2], inv, m) | code2(v[3], inv, m) << 16);
 }
 __device__ __forceinline__ float2 decode2(uint32_t two) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(two & 0xffffu), __NV_E4M3);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
-__device__ __forceinline__ uint32_t largest(const float (&f)[8]) {
-  uint32_t m = 0;
+// Magnitudes of eight values in columns of their own, their element-wise maximum, the largest of all and one of them (as fp32 bits).  Those of
+// 16-bit types order as integers, two in a word.
+template <class T> struct Magnitudes {
+  uint32_t w[sizeof(T) == 2 ? 4 : 8];
+};
+template <class T> __device__ __forceinline__ uint32_t widen(uint32_t m16);
+template <> __device__ __forceinline__ uint32_t widen<__nv_bfloat16>(uint32_t m) { return m << 16; }
+template <> __device__ __forceinline__ uint32_t widen<__half>(uint32_t m) { return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m))); }
+template <> __device__ __forceinline__ uint32_t widen<float>(uint32_t m) { return m; }
+template <class T> __device__ __forceinline__ uint32_t max_of(uint32_t a, uint32_t b) { return sizeof(T) == 2 ? __vmaxu2(a, b) : max(a, b); }
+template <class T> __device__ __forceinline__ uint32_t largest(const Magnitudes<T>& m) {
+  constexpr int N = sizeof(T) == 2 ? 4 : 8;
+  uint32_t r = m.w[0];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) m = max(m, magnitude(f[j]));
-  return m;
+  for (int i = 1; i < N; ++i) r = max_of<T>(r, m.w[i]);
+  return sizeof(T) == 2 ? widen<T>(max(r & 0xffffu, r >> 16)) : r;
 }
 
 __device__ __forceinline__ float up(bf16 v) { return __bfloat162float(v); }
@@ -122,6 +134,28 @@ __device__ __forceinline__ void unpack(const Eight<float>& e, float (&f)[8]) {
   const uint32_t w[8] = {e.v[0].x, e.v[0].y, e.v[0].z, e.v[0].w, e.v[1].x, e.v[1].y, e.v[1].z, e.v[1].w};
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
+}
+__device__ __forceinline__ void pairs(const Eight<bf16>& e, f2 (&v)[4]) {
+  v[0] = f2_bf(e.v[0].x); v[1] = f2_bf(e.v[0].y); v[2] = f2_bf(e.v[0].z); v[3] = f2_bf(e.v[0].w);
+}
+template <class T> __device__ __forceinline__ void pairs(const Eight<T>& e, f2 (&v)[4]) {
+  float f[8];
+  unpack(e, f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = f2_pack(f[2 * i], f[2 * i + 1]);
+}
+template <class T> __device__ __forceinline__ Magnitudes<T> magnitudes(const Eight<T>& e) {
+  Magnitudes<T> m;
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&e);
+#pragma unroll
+  for (int i = 0; i < (sizeof(T) == 2 ? 4 : 8); ++i) m.w[i] = w[i] & (sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu);
+  return m;
+}
+__device__ __forceinline__ Magnitudes<float> magnitudes(const f2 (&v)[4]) {
+  Magnitudes<float> m;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { const float2 t = f2_unpack(v[i]); m.w[2 * i] = magnitude(t.x); m.w[2 * i + 1] = magnitude(t.y); }
+  return m;
 }
 template <class T> __device__ __forceinline__ Eight<T> pack(const float (&f)[8]) {
   Eight<T> e;
