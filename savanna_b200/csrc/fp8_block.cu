@@ -27,8 +27,8 @@ __device__ __forceinline__ void begin() {
 }
 
 // ------------------------------------------------------------------------------------------------ tiles of 128 x 128
-// A block of 256 threads holds a tile in registers: sixteen threads eight columns each, eight rows a thread, all loads issued before the
-// first value is used.  From there a row's largest magnitude is four shuffles away and a column's one exchange through shared memory, so the
+// A block holds a tile in registers: sixteen threads eight columns each, eight rows a thread (four where both forms are written), all loads issued before
+// the first value is used.  From there a row's largest magnitude is four shuffles away and a column's one exchange through shared memory, so the
 // second form of the codes costs its writes alone.
 struct QuantArgs {
   const void* x;
@@ -47,13 +47,19 @@ struct QuantArgs {
 
 enum { ROWS = 1, COLS = 2, TILE = 4 };
 
+// Threads of a block: with both forms, or a norm in front, half as many rows a thread, whose values and codes would otherwise leave room for two
+// blocks on an SM.
+__host__ __device__ constexpr int quant_threads(int form, bool norm) { return form == (ROWS | COLS) || norm ? 512 : 256; }
+// Blocks of an SM that the registers are cut for: 64 a thread where one form is written, 80 for columns.
+__host__ __device__ constexpr int quant_blocks(int form, bool norm) { return quant_threads(form, norm) == 512 ? 2 : form == COLS ? 3 : 4; }
 template <class T, int FORM, bool NORM, bool VEC>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(quant_threads(FORM, NORM), quant_blocks(FORM, NORM))
 quantize_kernel(QuantArgs p) {
+  constexpr int THREADS = quant_threads(FORM, NORM), HALVES = THREADS / 16, WARPS = THREADS / 32, RPT = BLOCK / HALVES;
   typedef typename std::conditional<NORM, float, T>::type M;          // what magnitudes are compared in
   constexpr int MW = sizeof(M) == 2 ? 4 : 8;
-  __shared__ uint32_t part[8][16][MW];                      // columns' largest magnitudes by warp
-  __shared__ float sum_part[8][BLOCK];
+  __shared__ uint32_t part[WARPS][16][MW];                      // columns' largest magnitudes by warp
+  __shared__ float sum_part[WARPS][BLOCK];
   __shared__ float row_scale[BLOCK];
   __shared__ uint32_t col_max[BLOCK];
   begin();
@@ -64,18 +70,18 @@ quantize_kernel(QuantArgs p) {
   const int n = min(8, p.C - c0);                           // of the thread's columns
   const int rows = int(min((long long)BLOCK, p.R - r0));
   const T* x = static_cast<const T*>(p.x) + r0 * p.ld + c0;
-  Eight<T> raw[8];
+  Eight<T> raw[RPT];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = h + 16 * i;
+  for (int i = 0; i < RPT; ++i) {
+    const int r = h + HALVES * i;
     raw[i] = fetch<VEC, T>(x + r * p.ld, r < rows ? n : 0);
   }
   f2 g[4];
-  float a[8];
+  float a[RPT];
   if (NORM) {
     pairs(fetch<VEC, T>(static_cast<const T*>(p.g) + c0, n), g);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = h + 16 * i < rows ? p.a[r0 + h + 16 * i] : 0.f;
+    for (int i = 0; i < RPT; ++i) a[i] = h + HALVES * i < rows ? p.a[r0 + h + HALVES * i] : 0.f;
   }
   auto values = [&](int i, f2 (&v)[4]) {
     pairs(raw[i], v);
@@ -96,7 +102,7 @@ quantize_kernel(QuantArgs p) {
   Magnitudes<M> most = {};                                  // of the thread's columns
   f2 cs[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < RPT; ++i) {
     const Magnitudes<M> m = sizes(i);
     if (FORM & (COLS | TILE)) {
 #pragma unroll
@@ -113,7 +119,7 @@ quantize_kernel(QuantArgs p) {
 #pragma unroll
       for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
       const Coder c(top);
-      const int r = h + 16 * i;
+      const int r = h + HALVES * i;
       f2 v[4];
       values(i, v);
       if (r < rows && n > 0) *reinterpret_cast<uint2*>(p.q_rows + (r0 + r) * p.ldq + c0) = encode(c, v);
@@ -147,12 +153,12 @@ quantize_kernel(QuantArgs p) {
   if (FORM & TILE) {
     uint32_t top = col_max[0];
 #pragma unroll
-    for (int k = 1; k < 8; ++k) top = max(top, col_max[k]);
+    for (int k = 1; k < WARPS; ++k) top = max(top, col_max[k]);
     const Coder c(top);
     if (threadIdx.x == 0) p.s_rows[blockIdx.x] = c.scale;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = h + 16 * i;
+    for (int i = 0; i < RPT; ++i) {
+      const int r = h + HALVES * i;
       f2 v[4];
       values(i, v);
       if (r < rows && n > 0) *reinterpret_cast<uint2*>(p.q_rows + (r0 + r) * p.ldq + c0) = encode(c, v);
@@ -163,7 +169,7 @@ quantize_kernel(QuantArgs p) {
       const int who = threadIdx.x / MW, j = threadIdx.x % MW;
       uint32_t top = part[0][who][j];
 #pragma unroll
-      for (int k = 1; k < 8; ++k) top = max_of<M>(top, part[k][who][j]);
+      for (int k = 1; k < WARPS; ++k) top = max_of<M>(top, part[k][who][j]);
       if (sizeof(M) == 2) {
         col_max[who * 8 + 2 * j] = widen<M>(top & 0xffffu);
         col_max[who * 8 + 2 * j + 1] = widen<M>(top >> 16);
@@ -179,7 +185,7 @@ quantize_kernel(QuantArgs p) {
         if (p.sums) {
           float s = sum_part[0][threadIdx.x];
 #pragma unroll
-          for (int k = 1; k < 8; ++k) s += sum_part[k][threadIdx.x];
+          for (int k = 1; k < WARPS; ++k) s += sum_part[k][threadIdx.x];
           p.sums[tile_r * p.C + c] = s;
         }
       }
@@ -192,8 +198,8 @@ quantize_kernel(QuantArgs p) {
       minus[j] = f2_pack(a_.minus_amax, b_.minus_amax);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = h + 16 * i;
+    for (int i = 0; i < RPT; ++i) {
+      const int r = h + HALVES * i;
       f2 v[4];
       values(i, v);
       if (r < rows && n > 0)
@@ -337,7 +343,7 @@ static int launch_quantize(const QuantArgs& p, cudaStream_t st) {
   const long long tiles = (p.R + BLOCK - 1) / BLOCK * p.col_tiles;
   if (tiles > 0x7fffffffLL) return -3;
   const bool vec = p.C % 8 == 0 && aligned16<T>(p.x, p.ld) && (!NORM || aligned16<T>(p.g, 8));
-  return launch_chained(false, vec ? quantize_kernel<T, FORM, NORM, true> : quantize_kernel<T, FORM, NORM, false>, dim3((unsigned)tiles), 256, 0, st, p);
+  return launch_chained(false, vec ? quantize_kernel<T, FORM, NORM, true> : quantize_kernel<T, FORM, NORM, false>, dim3((unsigned)tiles), quant_threads(FORM, NORM), 0, st, p);
 }
 template <class T>
 static int launch_form(const QuantArgs& p, int form, cudaStream_t st) {
