@@ -269,8 +269,13 @@ struct BlockNormLinear : Function<BlockNormLinear> {
       } else {
         Coded hold;
         const Operand w = saved_weight(s[3], s[4], N, D, dev, hold);
-        std::tie(dx, dwn) = norm_bwd(s2, wn, a, block_input_grad(go.rows, w, type, dev), g[1].defined() ? aligned(g[1]) : g[1],
-                                     ctx->saved_data["eps"].toDouble(), ctx->saved_data["form"].toInt());
+        const Tensor dn = block_input_grad(go.rows, w, F32, dev), ds = g[1].defined() ? contiguous(g[1]) : g[1];
+        const int64_t parts = L.sb_fp8_block_norm_back_blocks((long long)T, (int)D);
+        const Tensor dg = alloc({parts, D}, F32, dev);
+        dx = alloc({T, D}, type, dev);
+        SB_CALL(sb_fp8_block_norm_back, 1, ptr(s2), ptr(wn), f32(a), f32(dn), ptr(ds), out(dx), f32o(dg), (long long)T, (int)D, (float)ctx->saved_data["eps"].toDouble(),
+                (int)ctx->saved_data["form"].toInt(), type_code(type), stream());
+        dwn = column_sums(f32(dg), parts, D, type, dev);
         dx = dx.view(shape);
       }
     }
@@ -411,7 +416,7 @@ Tensor linear_fp8_block(const Tensor& x, const OptTensor& xs, const py::object& 
   }
   return x.dim() == 2 ? y : y.view(with_last(x.sizes(), w.size(0)));
 }
-// nothing where the kernels do not cover type or width
+// nothing where the kernels do not cover the width
 std::optional<std::tuple<Tensor, Tensor>> norm_linear_fp8_block(const Tensor& x, const Tensor& g, double eps, int64_t form, const py::object& weight, const OptTensor& ws,
                                                                 const OptTensor& bias, const OptTensor& residual) {
   const char* what = "norm_linear_fp8_block";
@@ -422,8 +427,7 @@ std::optional<std::tuple<Tensor, Tensor>> norm_linear_fp8_block(const Tensor& x,
   check_projection(what, x, K, w, ws, bias, OptTensor(), x.scalar_type(), {});
   const OptTensor wt = ws.has_value() ? OptTensor() : OptTensor(w);
   const bool train = wants_grad({&x, &g, given(wt), given(bias), given(residual)});
-  // the norm's backward kernel: bf16, rows of eights
-  if (K > 16384 || (train && (x.scalar_type() != BF16 || K % 8 || K < 64))) return std::nullopt;
+  if (K > 16384) return std::nullopt;
   const c10::cuda::CUDAGuard device(x.device());
   const BlockWeight wc = block_weight(w, ws);
   const OptTensor b = contiguous(bias);

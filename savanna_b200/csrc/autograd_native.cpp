@@ -51,7 +51,7 @@ constexpr auto F32 = at::kFloat;
   X(sb_li_fwd_tiled) \
   X(sb_li_bwd_tiled_chunk) X(sb_li_bwd_tiled) X(sb_attn_fwd) X(sb_attn_bwd) X(sb_attn_rope) \
   X(sb_attn_step_splits) X(sb_attn_step) X(sb_attn_rpe_fwd) X(sb_attn_rpe_bwd_work) X(sb_attn_rpe_bwd) X(sb_layernorm_fwd) X(sb_layernorm_bwd_blocks) X(sb_layernorm_bwd) X(sb_act8_quantize) X(sb_act8_dequantize) \
-  X(sb_fp8_block_quantize) X(sb_fp8_block_column_sums) X(sb_fp8_block_norm) X(sb_fp8_block_dequantize) X(sb_gemm_fp8_block) X(sb_gemm_fp8_block_takes_few) X(sb_gemm_fp8_block_few)
+  X(sb_fp8_block_quantize) X(sb_fp8_block_column_sums) X(sb_fp8_block_norm) X(sb_fp8_block_norm_back_blocks) X(sb_fp8_block_norm_back) X(sb_fp8_block_dequantize) X(sb_gemm_fp8_block) X(sb_gemm_fp8_block_takes_few) X(sb_gemm_fp8_block_few)
 
 struct {
 #define SB_DECLARE(name) decltype(&::name) name = nullptr;

@@ -74,6 +74,9 @@ int sb_fp8_block_quantize(const void* x, long long ld, long long R, int C, int t
 int sb_fp8_block_column_sums(const float* sums, void* out, long long tiles, int C, int type, cudaStream_t st);
 int sb_fp8_block_norm(const void* x, long long ldx, const void* res, long long ldr, const void* g, void* sum, void* q, long long ldq,
                       float* scale, float* a, long long T, int D, float eps, int form, int type, cudaStream_t st);
+int sb_fp8_block_norm_back_blocks(long long T, int D);
+int sb_fp8_block_norm_back(const void* x, const void* g, const float* a, const float* dn, const void* ds, void* dx, float* dg, long long T, int D,
+                           float eps, int form, int type, cudaStream_t st);
 int sb_fp8_block_dequantize(const void* q, long long ldq, const float* scale, long long s_row, long long s_col, int tiles, void* x,
                             long long R, int C, int type, cudaStream_t st);
 // gemm_fp8_block.cu

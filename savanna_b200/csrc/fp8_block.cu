@@ -307,6 +307,106 @@ norm_quantize_kernel(NormArgs p) {
   }
 }
 
+// ------------------------------------------------------------------------------------------------ norm, backward
+//   dx = a * (dn * g) - x * c * mean(dn * g * x) (+ ds),  dg = sum over the rows of dn * x * a
+// a = 1 / sqrt(mean(x^2) + eps) and c = a^3 (form 0), or a = 1 / (rms + eps) and c = a^2 / rms (form 1).  dn is the input gradient of the projection in
+// fp32, as its product leaves it: rounded to 16 bits it would cost dg, a sum over all rows, half as much again as its own rounding.  A block goes
+// through rows with a stride of the grid, its threads keep their columns and add up dg for them; the next row's loads are on their way while this
+// one's sum crosses the block.
+struct NormBackArgs {
+  const void *x, *g, *ds;
+  const float *a, *dn;
+  void* dx;
+  float* dg;                       // [blocks][D]
+  long long T;
+  int D, form;
+  float eps;
+};
+template <class T, int V, bool VEC>
+__global__ void __launch_bounds__(512, 1)
+norm_backward_kernel(NormBackArgs p) {
+  __shared__ float red[2][16];
+  begin();
+  f2 g[V][4], acc[V][4];
+  Eight<T> x[V], s[V];
+  Eight<float> dn[V];
+  auto column = [&](int v) { return int(threadIdx.x + v * blockDim.x) * 8; };
+  auto load = [&](long long row) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int c = column(v), n = row < p.T ? min(8, p.D - c) : 0;
+      x[v] = fetch<VEC, T>(static_cast<const T*>(p.x) + row * p.D + c, n);
+      dn[v] = fetch<VEC, float>(p.dn + row * p.D + c, n);
+      if (p.ds) s[v] = fetch<VEC, T>(static_cast<const T*>(p.ds) + row * p.D + c, n);
+    }
+  };
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    pairs(fetch<VEC, T>(static_cast<const T*>(p.g) + column(v), min(8, p.D - column(v))), g[v]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[v][j] = 0ull;
+  }
+  load(blockIdx.x);
+  int turn = 0;
+  for (long long row = blockIdx.x; row < p.T; row += gridDim.x, turn ^= 1) {
+    const float a = p.a[row];
+    const f2 a2 = f2_pack(a, a);
+    f2 xv[V][4], gv[V][4], sv[V][4], dot = 0ull;           // x, dn * g, ds
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      f2 d[4];
+      pairs(x[v], xv[v]);
+      pairs(dn[v], d);
+      if (p.ds) pairs(s[v], sv[v]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        gv[v][j] = f2_mul(d[j], g[v][j]);
+        dot = f2_fma(gv[v][j], xv[v][j], dot);
+        acc[v][j] = f2_fma(d[j], f2_mul(xv[v][j], a2), acc[v][j]);
+      }
+    }
+    load(row + gridDim.x);
+    float sum = f2_unpack(dot).x + f2_unpack(dot).y;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (blockDim.x > 32) {
+      if ((threadIdx.x & 31) == 0) red[turn][threadIdx.x >> 5] = sum;
+      __syncthreads();
+      sum = 0.f;
+      for (int k = 0; k < int(blockDim.x >> 5); ++k) sum += red[turn][k];
+    }
+    float c = a * a * a;
+    if (p.form == 1) {
+      const float rms = 1.f / a - p.eps;
+      c = rms > 0.f ? a * a / rms : 0.f;                   // a row of zeros
+    }
+    const float m = -c * (sum / p.D);
+    const f2 m2 = f2_pack(m, m);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f2 d = f2_fma(gv[v][j], a2, f2_mul(xv[v][j], m2));
+        if (p.ds) d = f2_add(d, sv[v][j]);
+        const float2 t = f2_unpack(d);
+        f[2 * j] = t.x; f[2 * j + 1] = t.y;
+      }
+      put<VEC, T>(static_cast<T*>(p.dx) + row * p.D + column(v), pack<T>(f), min(8, p.D - column(v)));
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int n = min(8, p.D - column(v));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 t = f2_unpack(acc[v][j]);
+      if (2 * j < n) p.dg[(long long)blockIdx.x * p.D + column(v) + 2 * j] = t.x;
+      if (2 * j + 1 < n) p.dg[(long long)blockIdx.x * p.D + column(v) + 2 * j + 1] = t.y;
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ back
 template <class T, bool VEC>
 __global__ void __launch_bounds__(256)
@@ -371,6 +471,24 @@ static int launch_norm(const NormArgs& p, cudaStream_t st) {
   return launch_norm_v<T, 4>(p, threads(4), st);
 }
 
+// threads of the backward kernel and its columns of eight a thread
+static int back_shape(int D, int& v) {
+  const int groups = (D + 7) / 8;
+  v = groups <= 256 ? 1 : groups <= 1024 ? 2 : 4;
+  return ((groups + v - 1) / v + 31) / 32 * 32;
+}
+template <class T, int V>
+static int launch_back_v(const NormBackArgs& p, int blocks, int threads, cudaStream_t st) {
+  const bool vec = p.D % 8 == 0 && aligned16<T>(p.x, 8) && aligned16<T>(p.g, 8) && aligned16<float>(p.dn, 8) && aligned16<T>(p.dx, 8) && aligned16<T>(p.ds, 8);
+  return launch_chained(false, vec ? norm_backward_kernel<T, V, true> : norm_backward_kernel<T, V, false>, dim3(blocks), threads, 0, st, p);
+}
+template <class T>
+static int launch_back(const NormBackArgs& p, int blocks, cudaStream_t st) {
+  int v;
+  const int threads = back_shape(p.D, v);
+  return v == 1 ? launch_back_v<T, 1>(p, blocks, threads, st) : v == 2 ? launch_back_v<T, 2>(p, blocks, threads, st) : launch_back_v<T, 4>(p, blocks, threads, st);
+}
+
 template <class T>
 static int launch_dequantize(const void* q, const float* scale, void* x, long long R, int C, long long ldq, long long s_row, long long s_col,
                              int tiles, cudaStream_t st) {
@@ -417,6 +535,25 @@ extern "C" int sb_fp8_block_norm(const void* x, long long ldx, const void* res, 
   if (ldq % 16 || ldq < D || !res != !sum) return -4;
   NormArgs p{x, res, g, sum, (uint8_t*)q, scale, a, ldx, ldr, ldq, T, D, form, eps};
   return type == 0 ? launch_norm<bf16>(p, st) : type == 1 ? launch_norm<__half>(p, st) : launch_norm<float>(p, st);
+}
+
+// Blocks of the backward kernel: rows of its dg.
+extern "C" int sb_fp8_block_norm_back_blocks(long long T, int D) {
+  int v;
+  const int threads = sb::blk8::back_shape(D, v), per_sm = 1024 / threads < 8 ? 1024 / threads : 8;
+  const long long most = (long long)sb::num_sms() * (per_sm < 1 ? 1 : per_sm);
+  return int(T < most ? T : most);
+}
+// x, dx, ds (or null) [T, D] and g [D] of `type`, dense; dn fp32 [T, D]; a [T] of sb_fp8_block_norm; dg fp32 [sb_fp8_block_norm_back_blocks][D], whose
+// column sums are the gain's gradient
+extern "C" int sb_fp8_block_norm_back(const void* x, const void* g, const float* a, const float* dn, const void* ds, void* dx, float* dg, long long T, int D,
+                                      float eps, int form, int type, cudaStream_t st) {
+  using namespace sb::blk8;
+  if (T <= 0 || D <= 0) return 0;
+  if (D > 16384) return -3;
+  const int blocks = sb_fp8_block_norm_back_blocks(T, D);
+  NormBackArgs p{x, g, ds, a, dn, dx, dg, T, D, form, eps};
+  return type == 0 ? launch_back<bf16>(p, blocks, st) : type == 1 ? launch_back<__half>(p, blocks, st) : launch_back<float>(p, blocks, st);
 }
 
 // q [R, C], rows ldq apart, times scale[row * s_row + (column / 128) * s_col] (tiles: row / 128) -> x [R, C] of `type`

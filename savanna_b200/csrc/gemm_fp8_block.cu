@@ -36,7 +36,7 @@ struct GemmArgs {
   long long sa_m, sa_k, sb_n, sb_k;      // strides; sb_n counts blocks of 128 n where the scale is theirs
   long long ldc, ldr;
   int M, N, K, type, beta;
-  bool boxes;                            // 16-bit results, and what is added, on 16-byte boundaries: stored by store_boxes
+  bool boxes;                            // results, and what is added, on 16-byte boundaries: stored in boxes
   bool runs;                             // scales of neighbouring rows (and columns, where those have their own) lie together, on 16-byte boundaries
   uint32_t* status;
 };
@@ -191,6 +191,45 @@ __device__ __forceinline__ void store_boxes(const GemmArgs& p, const CUtensorMap
     bulk_commit();
   }
 }
+// fp32 results: boxes of 32 columns, half of the warp's columns at a time
+template <int COLS>
+__device__ __forceinline__ void store_boxes_f32(const GemmArgs& p, const CUtensorMap* tmC, uint32_t space, const f2* acc, int row0, int col0, int lane) {
+  constexpr int BOXES = COLS / 64;
+  const int row = row0 + lane;
+  const bool extra = (p.bias || p.residual || p.beta) && row < p.M;
+#pragma unroll
+  for (int round = 0; round < 2; ++round) {
+    if (lane == 0) bulk_wait_read<0>();
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 4 * BOXES; ++c) {          // 8 columns each
+      const int first = round * 32 * BOXES + 8 * c, col = col0 + first;
+      float f[16];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { const float2 t = f2_unpack(acc[first / 2 + j]); f[2 * j] = t.x; f[2 * j + 1] = t.y; }
+      if (extra && col < p.N) {
+        if (p.bias) add8(static_cast<const float*>(p.bias) + col, f, 0);
+        if (p.residual) add8(static_cast<const float*>(p.residual) + row * p.ldr + col, f, 0);
+        if (p.beta) add8(static_cast<const float*>(p.C) + row * p.ldc + col, f, 0);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t at = space + (c >> 2) * (32 * 128) + lane * 128 + (((2 * (c & 3) + h) ^ (lane & 7)) << 4);
+        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(f[4 * h]), "f"(f[4 * h + 1]), "f"(f[4 * h + 2]), "f"(f[4 * h + 3]) : "memory");
+      }
+    }
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0 && row0 < p.M) {
+#pragma unroll
+      for (int b = 0; b < BOXES; ++b) {
+        const int col = col0 + round * 32 * BOXES + 32 * b;
+        if (col < p.N) tma_store_2d(tmC, space + b * (32 * 128), 2 * col, row0);      // the map counts 16-bit halves
+      }
+      bulk_commit();
+    }
+  }
+}
 template <class T> __device__ __forceinline__ void store_one(const GemmArgs& p, int row, int col, float f) {
   T* c = static_cast<T*>(p.C) + row * p.ldc + col;
   if (p.bias) f += up(static_cast<const T*>(p.bias)[col]);
@@ -198,7 +237,7 @@ template <class T> __device__ __forceinline__ void store_one(const GemmArgs& p, 
   if (p.beta) f += up(*c);
   *c = down<T>(f);
 }
-// Everything else (fp32 results, rows off 16-byte boundaries): 16 columns at a time, a half-warp a row.
+// Everything else (rows off 16-byte boundaries, fp32 sums in fragments): 16 columns at a time, a half-warp a row.
 template <int COLS, class T, bool FRAGMENTS>
 __device__ __forceinline__ void store_values(const GemmArgs& p, uint32_t space, const f2* acc, int row0, int col0, int lane) {
 #pragma unroll
@@ -226,6 +265,9 @@ __device__ __forceinline__ void store_values(const GemmArgs& p, uint32_t space, 
 }
 template <int COLS, bool FRAGMENTS>
 __device__ __forceinline__ void store_tile(const GemmArgs& p, const CUtensorMap* tmC, uint32_t space, const f2* acc, int row0, int col0, int lane) {
+  if constexpr (!FRAGMENTS) {
+    if (p.boxes && p.type == 2) return store_boxes_f32<COLS>(p, tmC, space, acc, row0, col0, lane);
+  }
   if (p.boxes && p.type == 0) store_boxes<COLS, bf16, FRAGMENTS>(p, tmC, space, acc, row0, col0, lane);
   else if (p.boxes) store_boxes<COLS, __half, FRAGMENTS>(p, tmC, space, acc, row0, col0, lane);
   else if (p.type == 0) store_values<COLS, bf16, FRAGMENTS>(p, space, acc, row0, col0, lane);
@@ -418,27 +460,21 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
           if (SB_ROWS) load_fragments(t + 32 * c, r);
           else tmem_ld_32x32(t + 32 * c, r);
         };
-        f2 b0[2], b1[2];                                           // scales of the lane's columns of a quarter
-        auto columns = [&](int c) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            b0[i] = get2(sb_k + (c * 32 + 8 * i + 2 * (lane & 3)) * 4);
-            b1[i] = get2(sb_k + (c * 32 + 16 + 8 * i + 2 * (lane & 3)) * 4);
-          }
-        };
-        if (SB_ROWS) columns(0);
+        // scales of the lane's two columns of eight, fetched one eight ahead
+        const uint32_t sb_lane = sb_k + 2 * (lane & 3) * 4;
+        f2 b_next = SB_ROWS ? get2(sb_lane) : 0ull;
         auto add = [&](int c, const uint32_t (&r)[32]) {
           if (SB_ROWS) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const f2 b = i < 2 ? b0[i] : b1[i - 2];
+              const f2 b = b_next;
+              if (c * 4 + i + 1 < COLS / 8) b_next = get2(sb_lane + (c * 4 + i + 1) * 32);
               f2 v[4];
 #pragma unroll
               for (int k = 0; k < 4; ++k) v[k] = scaled(r[(k >> 1) * 16 + i * 4 + (k & 1) * 2], r[(k >> 1) * 16 + i * 4 + (k & 1) * 2 + 1], b);
 #pragma unroll
               for (int k = 0; k < 4; ++k) acc[c * 16 + (k >> 1) * 8 + i * 2 + (k & 1)] = f2_fma(v[k], s[SB_ROWS ? k : 0], acc[c * 16 + (k >> 1) * 8 + i * 2 + (k & 1)]);
             }
-            if (c + 1 < COLS / 32) columns(c + 1);
           } else {
 #pragma unroll
             for (int j = 0; j < 16; ++j) add_scaled(acc[c * 16 + j], r[2 * j], r[2 * j + 1], s[0]);
@@ -546,9 +582,10 @@ extern "C" int sb_gemm_fp8_block(const void* A, const float* sa, long long sa_m,
   if ((rc = b_mn ? make_tmap_2d_u8(&tmB, B, N, K, ldb, 128, 128) : make_tmap_2d_u8(&tmB, B, K, N, ldb, 128, 128))) return rc;
   const int size = type == 2 ? 4 : 2;
   const auto on16 = [](const void* at, long long row_bytes) { return !((reinterpret_cast<uintptr_t>(at) | row_bytes) & 15); };
-  const bool boxes = type != 2 && N % 8 == 0 && on16(C, ldc * size) && on16(bias, 0) && (!residual || on16(residual, ldr * size));
+  const bool boxes = !(type == 2 && sb_rows) && N % 8 == 0 && N < (1 << 30) && on16(C, ldc * size) && on16(bias, 0) && (!residual || on16(residual, ldr * size));
   const bool runs = sa_m == 1 && on16(sa, sa_k * 4) && (!sb_rows || (sb_n == 1 && on16(sb, sb_k * 4)));
-  if (boxes && (rc = make_tmap_2d_bf16(&tmC, C, N, M, ldc, 64, 32))) return rc;      // two-byte elements: fp16 alike
+  const int halves = size / 2;                           // the map is in 16-bit units, whatever the type
+  if (boxes && (rc = make_tmap_2d_bf16(&tmC, C, (uint64_t)N * halves, M, ldc * halves, 64, 32))) return rc;
   GemmArgs p{C, bias, residual, sa, sb, sa_m, sa_k, sb_n, sb_k, ldc, ldr, M, N, K, type, beta, boxes, runs, status};
   const bool pair = goes_by_pairs(M, N, num_sms());
   if (!a_mn && !b_mn && !sb_rows) return pair ? launch<true, 0, 0, false>(tmA, tmB, tmC, p, stream) : launch<false, 0, 0, false>(tmA, tmB, tmC, p, stream);

@@ -278,7 +278,7 @@ def linear_fp8_block(x, w, bias=None, residual=None, dtype=None):
 def norm_linear_fp8_block(x, norm_weight, eps: float, form: str, w, bias=None, residual=None):
     """(`linear_fp8_block` of rmsnorm(s), s), s = x + residual (without a residual: x): the norm's kernel adds the residual and writes the 8-bit
     operand.  One autograd node: the gradient that reaches s down the residual branch is added inside the norm's backward kernel.  CUDA: rows
-    of up to 16384 values; with gradients bf16 rows of 64 or more in eights, other types and widths run PyTorch's norm in fp32 before the projection."""
+    of up to 16384 values; wider ones run PyTorch's norm in fp32 before the projection."""
     _check_norm_form("norm_linear_fp8_block", form)
     if _k(x):
         r = _CO.norm_linear_fp8_block(x, norm_weight, eps, form, w, bias, residual)

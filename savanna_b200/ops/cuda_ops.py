@@ -1110,7 +1110,7 @@ def linear_fp8_block(x, w, bias, residual, dtype):
 
 
 def norm_linear_fp8_block(x, norm_weight, eps, form, w, bias, residual):
-    """None where the kernels do not cover type or width."""
+    """None where rows are wider than the norm's kernels take."""
     w, ws = w if isinstance(w, tuple) else (w, None)
     return _native("norm_linear_fp8_block", x, norm_weight, float(eps), 0 if form == "te" else 1, w, ws, bias, residual)
 

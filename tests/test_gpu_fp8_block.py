@@ -218,8 +218,8 @@ def test_gradients_through_the_norm(T, K, N, residual, form):
         assert torch.equal(got["x"], got["r"])
 
 
-def test_norms_that_the_backward_kernel_does_not_cover():
-    for dtype, K in ((torch.float16, 256), (torch.bfloat16, 131), (torch.float32, 512)):
+def test_norms_of_other_types_and_widths():
+    for dtype, K in ((torch.float16, 256), (torch.bfloat16, 131), (torch.float32, 512), (torch.float32, 1), (torch.bfloat16, 20000)):
         x, g, w = _randn(20, K, dtype=dtype).requires_grad_(), _randn(K, seed=1, dtype=dtype).requires_grad_(), _randn(48, K, seed=2, dtype=dtype).requires_grad_()
         y, s = ops.norm_linear_fp8_block(x, g, 1e-5, "te", w)
         assert y.dtype == dtype and torch.equal(s, x)
