@@ -61,7 +61,8 @@ quantize_kernel(QuantArgs p) {
   __shared__ uint32_t part[WARPS][16][MW];                      // columns' largest magnitudes by warp
   __shared__ float sum_part[WARPS][BLOCK];
   __shared__ float row_scale[BLOCK];
-  __shared__ uint32_t col_max[BLOCK];
+  __shared__ uint32_t col_max[BLOCK];                       // tiles: by warp
+  __shared__ __align__(16) float col_inv[BLOCK], col_minus[BLOCK];
   begin();
   const long long tile_r = blockIdx.x / p.col_tiles, tile_c = blockIdx.x - tile_r * p.col_tiles;
   const int l = threadIdx.x & 15, h = threadIdx.x >> 4, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -165,23 +166,20 @@ quantize_kernel(QuantArgs p) {
     }
   }
   if (FORM & COLS) {
-    if (threadIdx.x < 16 * MW) {                            // a word of magnitudes a thread: one column's or two neighbours'
-      const int who = threadIdx.x / MW, j = threadIdx.x % MW;
-      uint32_t top = part[0][who][j];
+    if (threadIdx.x < BLOCK) {                              // a column a thread
+      const int who = threadIdx.x >> 3, j = threadIdx.x & 7;
+      uint32_t top = 0;
 #pragma unroll
-      for (int k = 1; k < WARPS; ++k) top = max_of<M>(top, part[k][who][j]);
-      if (sizeof(M) == 2) {
-        col_max[who * 8 + 2 * j] = widen<M>(top & 0xffffu);
-        col_max[who * 8 + 2 * j + 1] = widen<M>(top >> 16);
-      } else {
-        col_max[who * 8 + j] = top;
+      for (int k = 0; k < WARPS; ++k) {
+        const uint32_t w = part[k][who][sizeof(M) == 2 ? j >> 1 : j];
+        top = max(top, sizeof(M) == 2 ? (j & 1 ? w >> 16 : w & 0xffffu) : w);
       }
-    }
-    __syncthreads();
-    if (threadIdx.x < BLOCK) {
+      const Coder coder(widen<M>(top));
+      col_inv[threadIdx.x] = coder.inv;
+      col_minus[threadIdx.x] = coder.minus_amax;
       const long long c = tile_c * BLOCK + threadIdx.x;
       if (c < p.C) {
-        p.s_cols[tile_r * fours(p.C) + c] = Coder(col_max[threadIdx.x]).scale;
+        p.s_cols[tile_r * fours(p.C) + c] = coder.scale;
         if (p.sums) {
           float s = sum_part[0][threadIdx.x];
 #pragma unroll
@@ -190,12 +188,12 @@ quantize_kernel(QuantArgs p) {
         }
       }
     }
+    __syncthreads();
     f2 inv[4], minus[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const Coder a_(col_max[l * 8 + 2 * j]), b_(col_max[l * 8 + 2 * j + 1]);
-      inv[j] = f2_pack(a_.inv, b_.inv);
-      minus[j] = f2_pack(a_.minus_amax, b_.minus_amax);
+      inv[j] = *reinterpret_cast<const f2*>(&col_inv[l * 8 + 2 * j]);
+      minus[j] = *reinterpret_cast<const f2*>(&col_minus[l * 8 + 2 * j]);
     }
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
@@ -211,18 +209,21 @@ quantize_kernel(QuantArgs p) {
 
 // sums [tiles][C] -> out [C], in the order of the tiles
 template <class T>
-__global__ void __launch_bounds__(256)
-column_sum_kernel(const float* __restrict__ sums, T* __restrict__ out, long long tiles, int C) {
-  __shared__ float part[8][32];
+__global__ void __launch_bounds__(1024)
+column_sum_kernel(const float* sums, T* out, long long tiles, int C) {
+  __shared__ float part[32][33];
+  begin();
   const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
   float s = 0.f;
-  if (c < C)
-    for (long long t = k; t < tiles; t += 8) s += sums[t * C + c];
+  if (c < C) {
+#pragma unroll 8
+    for (long long t = k; t < tiles; t += 32) s += sums[t * C + c];
+  }
   part[k][threadIdx.x & 31] = s;
   __syncthreads();
   if (k == 0 && c < C) {
 #pragma unroll
-    for (int j = 1; j < 8; ++j) s += part[j][threadIdx.x];
+    for (int j = 1; j < 32; ++j) s += part[j][threadIdx.x];
     out[c] = down<T>(s);
   }
 }
@@ -327,45 +328,53 @@ __global__ void __launch_bounds__(512, 1)
 norm_backward_kernel(NormBackArgs p) {
   __shared__ float red[2][16];
   begin();
-  f2 g[V][4], acc[V][4];
-  Eight<T> x[V], s[V];
-  Eight<float> dn[V];
+  // with four times eight columns a thread, the gain is read again for each row and nothing is fetched ahead: the registers would not do
+  constexpr bool AHEAD = V < 4;
+  struct Row { Eight<T> x[V], s[V]; Eight<float> dn[V]; } now, next;
+  Eight<T> gain[AHEAD ? V : 1];
+  f2 acc[V][4];
   auto column = [&](int v) { return int(threadIdx.x + v * blockDim.x) * 8; };
-  auto load = [&](long long row) {
+  auto load = [&](Row& r, long long row) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int c = column(v), n = row < p.T ? min(8, p.D - c) : 0;
-      x[v] = fetch<VEC, T>(static_cast<const T*>(p.x) + row * p.D + c, n);
-      dn[v] = fetch<VEC, float>(p.dn + row * p.D + c, n);
-      if (p.ds) s[v] = fetch<VEC, T>(static_cast<const T*>(p.ds) + row * p.D + c, n);
+      r.x[v] = fetch<VEC, T>(static_cast<const T*>(p.x) + row * p.D + c, n);
+      r.dn[v] = fetch<VEC, float>(p.dn + row * p.D + c, n);
+      if (p.ds) r.s[v] = fetch<VEC, T>(static_cast<const T*>(p.ds) + row * p.D + c, n);
     }
   };
+  auto gains = [&](int v) { return fetch<VEC, T>(static_cast<const T*>(p.g) + column(v), min(8, p.D - column(v))); };
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    pairs(fetch<VEC, T>(static_cast<const T*>(p.g) + column(v), min(8, p.D - column(v))), g[v]);
+    if (AHEAD) gain[AHEAD ? v : 0] = gains(v);
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[v][j] = 0ull;
   }
-  load(blockIdx.x);
+  if (AHEAD) load(next, blockIdx.x);
   int turn = 0;
   for (long long row = blockIdx.x; row < p.T; row += gridDim.x, turn ^= 1) {
     const float a = p.a[row];
     const f2 a2 = f2_pack(a, a);
-    f2 xv[V][4], gv[V][4], sv[V][4], dot = 0ull;           // x, dn * g, ds
+    if (AHEAD) {
+      now = next;
+      load(next, row + gridDim.x);
+    } else {
+      load(now, row);
+    }
+    f2 gv[V][4], dot = 0ull;                               // dn * g
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      f2 d[4];
-      pairs(x[v], xv[v]);
-      pairs(dn[v], d);
-      if (p.ds) pairs(s[v], sv[v]);
+      f2 d[4], x[4], g[4];
+      pairs(now.x[v], x);
+      pairs(now.dn[v], d);
+      pairs(AHEAD ? gain[AHEAD ? v : 0] : gains(v), g);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        gv[v][j] = f2_mul(d[j], g[v][j]);
-        dot = f2_fma(gv[v][j], xv[v][j], dot);
-        acc[v][j] = f2_fma(d[j], f2_mul(xv[v][j], a2), acc[v][j]);
+        gv[v][j] = f2_mul(d[j], g[j]);
+        dot = f2_fma(gv[v][j], x[j], dot);
+        acc[v][j] = f2_fma(d[j], f2_mul(x[j], a2), acc[v][j]);
       }
     }
-    load(row + gridDim.x);
     float sum = f2_unpack(dot).x + f2_unpack(dot).y;
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -384,11 +393,14 @@ norm_backward_kernel(NormBackArgs p) {
     const f2 m2 = f2_pack(m, m);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
+      f2 x[4], s[4];
+      pairs(now.x[v], x);
+      if (p.ds) pairs(now.s[v], s);
       float f[8];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        f2 d = f2_fma(gv[v][j], a2, f2_mul(xv[v][j], m2));
-        if (p.ds) d = f2_add(d, sv[v][j]);
+        f2 d = f2_fma(gv[v][j], a2, f2_mul(x[j], m2));
+        if (p.ds) d = f2_add(d, s[j]);
         const float2 t = f2_unpack(d);
         f[2 * j] = t.x; f[2 * j + 1] = t.y;
       }
@@ -520,10 +532,9 @@ extern "C" int sb_fp8_block_column_sums(const float* sums, void* out, long long 
   using namespace sb::blk8;
   if (C <= 0) return 0;
   const int grid = (C + 31) / 32;
-  if (type == 0) column_sum_kernel<bf16><<<grid, 256, 0, st>>>(sums, (bf16*)out, tiles, C);
-  else if (type == 1) column_sum_kernel<__half><<<grid, 256, 0, st>>>(sums, (__half*)out, tiles, C);
-  else column_sum_kernel<float><<<grid, 256, 0, st>>>(sums, (float*)out, tiles, C);
-  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+  if (type == 0) return sb::launch_chained(false, column_sum_kernel<bf16>, dim3(grid), 1024, 0, st, sums, (bf16*)out, tiles, C);
+  if (type == 1) return sb::launch_chained(false, column_sum_kernel<__half>, dim3(grid), 1024, 0, st, sums, (__half*)out, tiles, C);
+  return sb::launch_chained(false, column_sum_kernel<float>, dim3(grid), 1024, 0, st, sums, (float*)out, tiles, C);
 }
 
 // D up to 16384.  res and sum: both or neither.  form 0: eps under the root, 1: beside it.  a: 1 / rms [T], or null.
@@ -540,8 +551,8 @@ extern "C" int sb_fp8_block_norm(const void* x, long long ldx, const void* res, 
 // Blocks of the backward kernel: rows of its dg.
 extern "C" int sb_fp8_block_norm_back_blocks(long long T, int D) {
   int v;
-  const int threads = sb::blk8::back_shape(D, v), per_sm = 1024 / threads < 8 ? 1024 / threads : 8;
-  const long long most = (long long)sb::num_sms() * (per_sm < 1 ? 1 : per_sm);
+  const int threads = sb::blk8::back_shape(D, v), per_sm = threads >= 512 ? 1 : 512 / threads < 4 ? 512 / threads : 4;
+  const long long most = (long long)sb::num_sms() * per_sm;
   return int(T < most ? T : most);
 }
 // x, dx, ds (or null) [T, D] and g [D] of `type`, dense; dn fp32 [T, D]; a [T] of sb_fp8_block_norm; dg fp32 [sb_fp8_block_norm_back_blocks][D], whose
