@@ -204,6 +204,8 @@ def describe_dtype(cfg, fused_tp_fp8) -> str:
         return "bf16"
     if getattr(cfg, "fp8_recipe", "delayed") == "mxfp8":
         d = "bf16 + block-scaled fp8 (MXFP8: e4m3, one E8M0 scale per 32 elements) projection GEMMs"
+    elif getattr(cfg, "fp8_recipe", "delayed") == "block128":
+        d = "bf16 + block-scaled fp8 (e4m3, fp32 scales for 128 elements, weights 128 x 128) projection GEMMs"
     else:
         d = "bf16 + fp8 (e4m3/e5m2, per-tensor delayed scaling) projection GEMMs"
     if fused_tp_fp8 is False:

@@ -382,8 +382,9 @@ std::optional<std::tuple<Tensor, Tensor, Tensor>> rmsnorm_fp8_block(const Tensor
   return std::make_tuple(x.dim() == 2 ? c.q : c.q.view(x.sizes()), x.dim() == 2 ? c.s.t() : c.s.t().view(with_last(x.sizes(), blocks(D))), n.s);
 }
 // type: of the result
+// kept: codes and scales of a weight tensor that its owner keeps between updates (quantised here otherwise)
 Tensor linear_fp8_block(const Tensor& x, const OptTensor& xs, const py::object& weight, const OptTensor& ws, const OptTensor& bias, const OptTensor& residual,
-                        int64_t type_) {
+                        int64_t type_, const OptTensor& kept_q, const OptTensor& kept_s) {
   const char* what = "linear_fp8_block";
   const at::ScalarType type = type_ == 0 ? BF16 : type_ == 1 ? at::kHalf : F32;
   const Tensor w = weight.cast<Tensor>();
@@ -392,9 +393,9 @@ Tensor linear_fp8_block(const Tensor& x, const OptTensor& xs, const py::object& 
   else check_block_input(what, x);
   const int64_t K = x.size(-1), T = x.numel() / K;
   TORCH_CHECK_VALUE(K <= MAX_BLOCK_SIZE && T <= MAX_BLOCK_SIZE, what, " takes up to ", MAX_BLOCK_SIZE, " rows of as many values, got ", x.sizes());
-  check_projection(what, x, K, w, ws, bias, residual, type, with_last(x.sizes(), w.size(0)));
+  check_projection(what, x, K, w, ws, bias, residual, type, w.dim() == 2 ? with_last(x.sizes(), w.size(0)) : x.sizes().vec());
   const c10::cuda::CUDAGuard device(x.device());
-  const BlockWeight wc = block_weight(w, ws);
+  const BlockWeight wc = kept_q.has_value() ? block_weight(*kept_q, kept_s) : block_weight(w, ws);
   const OptTensor b = contiguous(bias);
   const OptTensor wt = ws.has_value() ? OptTensor() : OptTensor(w);
   if (wants_grad({&x, given(wt), given(bias), given(residual)})) {
@@ -418,7 +419,8 @@ Tensor linear_fp8_block(const Tensor& x, const OptTensor& xs, const py::object& 
 }
 // nothing where the kernels do not cover the width
 std::optional<std::tuple<Tensor, Tensor>> norm_linear_fp8_block(const Tensor& x, const Tensor& g, double eps, int64_t form, const py::object& weight, const OptTensor& ws,
-                                                                const OptTensor& bias, const OptTensor& residual) {
+                                                                const OptTensor& bias, const OptTensor& residual, const OptTensor& kept_q,
+                                                                const OptTensor& kept_s) {
   const char* what = "norm_linear_fp8_block";
   const Tensor w = weight.cast<Tensor>();
   no_tangents({&x, &g, &w, given(bias), given(residual)});
@@ -429,7 +431,7 @@ std::optional<std::tuple<Tensor, Tensor>> norm_linear_fp8_block(const Tensor& x,
   const bool train = wants_grad({&x, &g, given(wt), given(bias), given(residual)});
   if (K > 16384) return std::nullopt;
   const c10::cuda::CUDAGuard device(x.device());
-  const BlockWeight wc = block_weight(w, ws);
+  const BlockWeight wc = kept_q.has_value() ? block_weight(*kept_q, kept_s) : block_weight(w, ws);
   const OptTensor b = contiguous(bias);
   if (train) {
     variable_list r = BlockNormLinear::apply(x, residual, g, wt, b, wc.q, wc.s, eps, form, !ws.has_value() && fused(weight), wc.operand);

@@ -608,12 +608,13 @@ class _LinearFP8(torch.autograd.Function):
 
 
 # ----------------------------------------------------------------------------- block-scaled fp8 (MXFP8)
-FP8_RECIPE = "delayed"      # "delayed": per-tensor scaling (default); "mxfp8": one E8M0 scale per 32 elements of the contraction
+FP8_RECIPE = "delayed"      # "delayed": per-tensor scaling (default); "mxfp8": one E8M0 scale per 32 elements of the contraction;
+                            # "block128": fp32 scales for 1 x 128 activations and gradients, 128 x 128 weights
 
 
 def set_fp8_recipe(name: str) -> None:
     global FP8_RECIPE
-    if name not in ("delayed", "mxfp8"):
+    if name not in ("delayed", "mxfp8", "block128"):
         raise ValueError(f"unknown fp8 recipe {name!r}")
     FP8_RECIPE = name
 
@@ -721,6 +722,8 @@ class _LinearMX(torch.autograd.Function):
 
 
 def linear(x, w, bias=None, fp8: bool = False, residual=None):
+    if fp8 and FP8_RECIPE == "block128" and _is_bf16(x, w, bias, residual):
+        return _native("linear_fp8_block", x, None, w, None, bias, residual, _TYPES[bf16], *_block_weight(w))
     if fp8 and FP8_RECIPE == "mxfp8" and _is_bf16(x, w, bias, residual) and w.shape[0] % 32 == 0 and w.shape[1] % 32 == 0 \
             and (x.numel() // x.shape[-1]) % 32 == 0:
         return _LinearMX.apply(x, w, bias, residual)
@@ -734,15 +737,15 @@ def linear(x, w, bias=None, fp8: bool = False, residual=None):
 
 def linear_allgather(x, w, bias, seq_dim, fp8):
     from ..parallel import fused_tp
-    if fp8 and FP8_RECIPE == "mxfp8":
-        return None                 # block-scaled operands: the caller gathers with NCCL and runs the MXFP8 projection
+    if fp8 and FP8_RECIPE != "delayed":
+        return None                 # block-scaled operands: the caller gathers with NCCL and runs the block-scaled projection
     return fused_tp.linear_allgather(x, w, bias, seq_dim, fp8=bool(fp8) and _is_bf16(x, w, bias))
 
 
 def linear_reducescatter(x, w, seq_dim, fp8):
     from ..parallel import fused_tp
-    if fp8 and FP8_RECIPE == "mxfp8":
-        return None                 # as above: MXFP8 projection, then an NCCL reduce-scatter
+    if fp8 and FP8_RECIPE != "delayed":
+        return None                 # as above: block-scaled projection, then an NCCL reduce-scatter
     return fused_tp.linear_reducescatter(x, w, seq_dim, fp8=bool(fp8) and _is_bf16(x, w))
 
 
@@ -1026,6 +1029,10 @@ def norm_linear(x, norm_weight, eps, form, w, bias, fp8):
     """(linear(rmsnorm(x)), x).  With fp8 projections and delayed scaling the norm emits the fp8 operand itself."""
     if fp8 and _fp8_fusable(x, w, norm_weight, bias) and 64 <= x.shape[-1] <= 16384:
         return _NormLinearFP8.apply(x, norm_weight, float(eps), 0 if form == "te" else 1, w, bias)
+    if fp8 and FP8_RECIPE == "block128" and _is_bf16(x, norm_weight, w, bias):
+        r = _native("norm_linear_fp8_block", x, norm_weight, float(eps), 0 if form == "te" else 1, w, None, bias, None, *_block_weight(w))
+        if r is not None:
+            return r
     if not fp8 and _norm_covers(x, norm_weight) and _is_bf16(w, bias) and _gemm_covers(w):
         return _native("norm_linear", x, norm_weight, float(eps), 0 if form == "te" else 1, w, bias)
     y, res = rmsnorm_residual(x, norm_weight, eps, form)
@@ -1105,14 +1112,28 @@ def rmsnorm_fp8_block(x, weight, eps, form, residual):
 
 
 def linear_fp8_block(x, w, bias, residual, dtype):
-    (x, xs), (w, ws) = (t if isinstance(t, tuple) else (t, None) for t in (x, w))
-    return _native("linear_fp8_block", x, xs, w, ws, bias, residual, _TYPES[dtype])
+    x, xs = x if isinstance(x, tuple) else (x, None)
+    w, ws = w if isinstance(w, tuple) else (w, None)
+    return _native("linear_fp8_block", x, xs, w, ws, bias, residual, _TYPES[dtype], None, None)
 
 
 def norm_linear_fp8_block(x, norm_weight, eps, form, w, bias, residual):
     """None where rows are wider than the norm's kernels take."""
     w, ws = w if isinstance(w, tuple) else (w, None)
-    return _native("norm_linear_fp8_block", x, norm_weight, float(eps), 0 if form == "te" else 1, w, ws, bias, residual)
+    return _native("norm_linear_fp8_block", x, norm_weight, float(eps), 0 if form == "te" else 1, w, ws, bias, residual, None, None)
+
+
+def _block_weight(w):
+    """Codes and scales of a parameter under the recipe `block128`, kept on it until an optimizer step (which may write through addresses) or
+    an operation of PyTorch (which counts versions) changes it.  (None, None), for the call to quantise by itself, while a graph is captured: what
+    a graph computes is there after its replays alone, and weights change between those."""
+    if w.is_inference() or torch.cuda.is_current_stream_capturing():
+        return None, None
+    state = (PARAM_EPOCH, w._version, w.data_ptr(), torch._C._cuda_getCurrentRawStream(w.get_device()))
+    cache = getattr(w, "_fp8_block_cache", None)
+    if cache is None or cache[0] != state:
+        cache = w._fp8_block_cache = (state, _native("fp8_block_quantize", w.detach(), True))
+    return cache[1]
 
 
 # ----------------------------------------------------------------------------- gated activation

@@ -173,3 +173,11 @@ def test_no_second_derivative():
     g, = torch.autograd.grad(y.sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+def test_recipe_key():
+    import os
+    from savanna_b200.config import GlobalConfig
+    tiny = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "configs", "baseline", "tiny_sh2_cpu.yml")
+    cfg = GlobalConfig.from_ymls([tiny], {"global_num_gpus": 1, "fp8_recipe": "block128", "use_fp8_linears": True})
+    assert cfg.fp8_recipe == "block128"

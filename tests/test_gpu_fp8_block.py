@@ -339,3 +339,103 @@ def test_nothing_is_written_outside_of_the_outputs(T, K, N):
 def test_refusals(i):
     with pytest.raises(ValueError):
         refusals("cuda")[i]()
+
+
+# ------------------------------------------------------------------------------------------------ as models use them
+
+
+@pytest.fixture
+def recipe():
+    from savanna_b200.ops import cuda_ops
+    cuda_ops.set_fp8_recipe("block128")
+    yield cuda_ops
+    cuda_ops.set_fp8_recipe("delayed")
+
+
+def test_norm_projection_gate_projection_in_a_row(recipe):
+    """A gated MLP by the operators one after the other, and by the model's entry point under the recipe: the same bits."""
+    T, D, F = 70, 256, 384
+    x, g, w12, w3, b = (_randn(*s, seed=i, std=v) for i, (s, v) in enumerate([((2, T // 2, D), 1.0), ((D,), 0.1), ((2 * F, D), 0.05), ((D, F), 0.05), ((D,), 0.1)]))
+    leaves = [t.requires_grad_() for t in (x, g, w12, w3, b)]
+    gy = _randn(2, T // 2, D, seed=9)
+    y = ops.mlp_gated(x, g, 1e-5, "te", w12, w3, b, "silu", fp8=True)
+    got = torch.autograd.grad(y, leaves, gy)
+    ab, s = ops.norm_linear_fp8_block(x, g, 1e-5, "te", w12)
+    z = ops.linear_fp8_block(ops.glu_act_packed(ab, "silu"), w3, b, s)
+    assert torch.equal(y, z)
+    for a, e in zip(got, torch.autograd.grad(z, leaves, gy)):
+        assert torch.equal(a, e)
+
+
+def test_recipe_sees_changed_weights(recipe):
+    x, w = _randn(20, 256), torch.nn.Parameter(_randn(64, 256, seed=1))
+    with torch.no_grad():
+        a = ops.linear(x, w, fp8=True)
+        w.mul_(2.0)
+        assert torch.equal(ops.linear(x, w, fp8=True).float(), 2.0 * a.float())
+        w.data.view(torch.int16).bitwise_xor_(-0x8000)            # the sign bits, past PyTorch's version counter, as a fused step writes
+        recipe.bump_param_epoch()
+        assert torch.equal(ops.linear(x, w, fp8=True).float(), -2.0 * a.float())
+
+
+def test_weight_gradient_added_in_place(recipe):
+    for T, K, N in ((77, 256, 264), (1000, 520, 300), (300, 129, 65)):
+        x, w, gy = _randn(T, K), torch.nn.Parameter(_randn(N, K, seed=1)), _randn(T, N, seed=2)
+        fresh, = torch.autograd.grad(ops.linear_fp8_block(x, w), w, gy)
+        w._fuse_grad_accum = True
+        start = _randn(N, K, seed=3)
+        w.grad = start.clone()
+        ops.linear(x, w, fp8=True).backward(gy)
+        gcol, xcol = (_whole(*ref.fp8_block_quantize(t.t().contiguous())).t() for t in (gy, x))
+        want = start.double() + gcol.t() @ xcol
+        close_sum(w.grad, want, gcol.abs().t() @ xcol.abs() + start.double().abs(), torch.bfloat16, "accumulated")
+        assert not torch.equal(w.grad, fresh)
+
+
+def test_training_under_the_recipe_tracks_bf16(recipe):
+    import os
+    from savanna_b200.config import GlobalConfig
+    from savanna_b200.data.synthetic import acgt_batch
+    from savanna_b200.parallel import state
+    from savanna_b200.train.trainer import Trainer
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    over = {"global_num_gpus": 1, "use_fp8_linears": True, "use_fp8_input_projections": True, "use_fp8_output_projections": True, "use_fp8_mlp_projections": True,
+            "fp8_recipe": "block128"}
+    cfg = GlobalConfig.from_ymls([os.path.join(root, "configs", "baseline", "tiny_sh2_gpu.yml")], over)
+    tr = Trainer(cfg, load=False)
+    batches = iter([{"text": acgt_batch(cfg.train_micro_batch_size_per_gpu, cfg.seq_length, seed=i).cuda()} for i in range(3)])
+    before = recipe.launch_count()
+    losses = [float(tr.train_step(batches)) for _ in range(3)]
+    state.destroy_model_parallel()
+    assert all(torch.isfinite(torch.tensor(losses))) and recipe.launch_count() > before
+    recipe.check_status()
+    assert any(getattr(p, "_fp8_block_cache", None) is not None for p in tr.model.parameters())
+
+
+def test_recipe_in_a_captured_graph_leaves_no_codes_behind(recipe):
+    x, w = _randn(20, 256), torch.nn.Parameter(_randn(64, 256, seed=1))
+    with torch.no_grad():
+        ops.linear(x, torch.nn.Parameter(_randn(64, 256, seed=5)), fp8=True)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = ops.linear(x, w, fp8=True)
+        eager = ops.linear(x, w, fp8=True).clone()                # before any replay
+        graph.replay()
+        assert torch.equal(y, eager)
+        w.mul_(2.0)
+        graph.replay()
+        assert torch.equal(y.float(), 2.0 * eager.float())
+
+
+def test_recipe_on_two_streams(recipe):
+    x, w = _randn(20, 256), torch.nn.Parameter(_randn(64, 256, seed=1))
+    with torch.no_grad():
+        want = ops.linear_fp8_block(x, w)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        got = [ops.linear(x, w, fp8=True)]
+        with torch.cuda.stream(side):
+            got.append(ops.linear(x, w, fp8=True))
+        torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
