@@ -302,6 +302,7 @@ void check_coded(const char* what, const Tensor& q, const Tensor& s, bool tiles)
                         (tiles ? s.dim() == 2 && s.size(0) == blocks(q.size(0)) && s.size(1) == blocks(q.size(1)) : s.sizes().vec() == with_last(q.sizes(), blocks(q.size(-1)))),
                     what, ": float8_e4m3fn ", tiles ? "[N, K] with fp32 scales [N / 128, K / 128]" : "[..., K] with fp32 scales [..., K / 128]", " on one device, got ",
                     q.scalar_type(), " ", q.sizes(), ", ", s.scalar_type(), " ", s.sizes());
+  TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !s.requires_grad(), what, ": scales carry no gradient");
 }
 // A weight as the product reads it: the caller's codes, or packed ones of a tensor
 struct BlockWeight {

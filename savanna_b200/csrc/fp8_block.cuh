@@ -76,6 +76,15 @@ template <> __device__ __forceinline__ __half down<__half>(float f) { return __f
 template <> __device__ __forceinline__ float down<float>(float f) { return f; }
 
 // Eight consecutive values as they lie in memory.
+// The calling thread's current device has its context bound; allowed while a stream is captured.
+static inline bool bind_context() {
+  static thread_local int bound = -1;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  if (dev != bound && cudaSetDevice(dev) != cudaSuccess) return false;
+  bound = dev;
+  return true;
+}
 // Lets a kernel have its dynamic shared memory, once on each device (the call takes half a microsecond).
 template <class F> static bool allow_shared(std::atomic<unsigned long long>& known, F kern, int bytes) {
   int dev = 0;

@@ -15,6 +15,11 @@
 // Two tiles: 256 x 256 on a CTA pair (cta_group::2; two buffers of 256 columns, 128 sums a thread) and 128 x 128 on one CTA (four buffers of
 // 128, 64 sums), for outputs that leave the chip idle in the larger one.
 //
+// 8192 x 4096 x 12288: 324 us forward, 313 input gradient, 526 weight gradient (2540, 2630, 1570 TFLOP/s; the per-tensor kernel 261 to 271).  A k-block
+// of a pair takes some 900 cycles where its products need 512: reading 256 columns of TMEM and a multiply-add for each value, in warps that also wait for
+// every accumulator; the weight gradient, whose values have a factor for their column too, 1300.  Without the multiply-adds the forward takes 250.
+// The single-CTA tile is bound by the 32 KB of operands that a k-block takes from L2.
+//
 // A programmatic dependent of the kernel before it (pdl.cuh, the second kind).  All waits are bounded (sm100.cuh).
 #include "entries.h"
 #include "f32x2.cuh"
@@ -521,6 +526,8 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
 }
 
 // Whether an [M, N] product goes by 256 x 256 tiles on CTA pairs: waves of either tile times what a k-block of it takes.
+// us back to back, pairs and single: 8192 x 4096 x 12288 340, 450; 300 x 2048 x 8192 13.2, 14.1; 1333 x 4096 x 4096 33.8, 34.3; 2000 x 768 x 2304 8.9, 8.7;
+// 512 x 4096 x 4096 20.5, 15.0; 777 x 1027 x 650 22.9, 13.3; the weight gradient of 2000 x 768 x 2304 17.4, 11.0.
 static bool goes_by_pairs(int M, int N, int sms) {
   auto waves = [](long long tiles, long long slots) { return (tiles + slots - 1) / slots; };
   const long long pair = waves((long long)((M + 255) / 256) * ((N + 255) / 256), sms / 2) * 512,
@@ -572,8 +579,7 @@ extern "C" int sb_gemm_fp8_block(const void* A, const float* sa, long long sa_m,
   using namespace sb::blk8;
   if (M <= 0 || N <= 0) return 0;
   if (K <= 0) return -3;
-  static thread_local bool ctx_bound = false;            // the tensor-map encoder needs a current context
-  if (!ctx_bound) { cudaFree(0); ctx_bound = true; }
+  if (!bind_context()) return -5;                        // the tensor-map encoder needs a current context
   if ((lda % 16) || (ldb % 16) || ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(B)) & 15)) return -4;
   if ((long long)((M + 127) / 128) * ((N + 127) / 128) > 0x7fffffffLL) return -3;
   CUtensorMap tmA, tmB, tmC = {};

@@ -171,6 +171,8 @@ def _check_fp8_block_pair(what, pair, tiles):
     if not ok:
         raise ValueError(f"{what}: float8_e4m3fn {'[N, K] with fp32 scales [N / 128, K / 128]' if tiles else '[..., K] with fp32 scales [..., K / 128]'} "
                          f"on one device, got {[(t.dtype, tuple(t.shape)) for t in pair]}")
+    if s.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: scales carry no gradient")
 
 
 def _check_fp8_block_norm(what, x, weight, residual):

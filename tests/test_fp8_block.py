@@ -154,6 +154,8 @@ def refusals(device):
         lambda: ops.linear_fp8_block(x, (wq, ws[:, :1])),
         lambda: ops.linear_fp8_block(x, (wq, s)),
         lambda: ops.linear_fp8_block((q, s), w.clone().requires_grad_()),
+        lambda: ops.linear_fp8_block((q, s.clone().requires_grad_()), (wq, ws)),
+        lambda: ops.fp8_block_dequantize(wq, ws.clone().requires_grad_()),
         lambda: ops.norm_linear_fp8_block(x, g, 1e-5, "te", w, b.float()),
         lambda: ops.norm_linear_fp8_block(x, g, 1e-5, "te", w[:, :100]),
         lambda: ops.norm_linear_fp8_block(x, g, 1e-5, "none", w),
