@@ -30,8 +30,8 @@ struct Packed {
     bytes = codes + (form == BY_ROWS ? blocks(C) : blocks(R)) * s_ld * 4;
   }
   Tensor make(at::Device device) const { return alloc({bytes}, at::kByte, device); }
-  Operand in(const Tensor& buf) const {
-    const char* p = static_cast<const char*>(ptr(buf));
+  Operand in(const Tensor& buf) const { return in(static_cast<const char*>(ptr(buf))); }
+  Operand in(const char* p) const {
     return {p, reinterpret_cast<const float*>(p + codes), R, C, ld, form == BY_TILES ? s_ld : 1, form == BY_TILES ? 1 : s_ld};
   }
 };
@@ -41,7 +41,7 @@ struct Coded { Tensor q, s; };
 int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : up_to(t.size(1), 16); }
 Tensor codes(int64_t R, int64_t C, at::Device device) {
   const int64_t ld = up_to(C, 16);
-  Tensor q = alloc({R, ld}, at::kByte, device).view(E4M3);
+  Tensor q = alloc({R, ld}, E4M3, device);
   return ld == C ? q : q.narrow(1, 0, C);
 }
 Tensor readable_codes(const Tensor& q) {
@@ -50,10 +50,13 @@ Tensor readable_codes(const Tensor& q) {
   c.view(at::kByte).copy_(q.view(at::kByte));
   return c;
 }
-Tensor scale_rows(int64_t blocks, int64_t n, at::Device device) {
-  const int64_t ld = up_to(n, 4);
-  Tensor s = alloc({blocks, ld}, F32, device);
-  return ld == n ? s : s.narrow(1, 0, n);
+// Scales of x's rows, [..., D / 128], as the kernels write them: those of neighbouring rows together, blocks a multiple of four rows apart
+Tensor row_scales(const Tensor& x, int64_t R, int64_t C) {
+  const int64_t ld = up_to(R, 4), last = x.dim() - 1;
+  std::vector<int64_t> sizes = with_last(x.sizes(), blocks(C)), strides(sizes.size(), ld);
+  int64_t step = 1;
+  for (int64_t i = last - 1; i >= 0; --i) { strides[i] = step; step *= sizes[i]; }
+  return alloc({blocks(C) * ld}, F32, x.device()).as_strided(sizes, strides);
 }
 Operand operand(const Coded& c) { return {ptr(c.q), f32(c.s), c.q.size(0), c.q.size(1), row_stride(c.q), c.s.stride(0), c.s.stride(1)}; }
 
@@ -127,19 +130,26 @@ void no_second_derivative() {
 }
 // The output gradient in the forms that the wanted gradients need, and the bias gradient
 struct OutGrad {
-  Tensor buf_rows, buf_cols, bias;
+  Tensor buf, bias;
   Operand rows, cols;
 };
 OutGrad out_grad(const Tensor& g2, bool x, bool w, bool bias) {
   OutGrad r;
   const int64_t T = g2.size(0), N = g2.size(1);
   const at::Device dev = g2.device();
-  if (x) { const Packed p(T, N, BY_ROWS); r.buf_rows = p.make(dev); r.rows = p.in(r.buf_rows); }
-  if (w) { const Packed p(T, N, BY_COLUMNS); r.buf_cols = p.make(dev); r.cols = p.in(r.buf_cols); }
   const bool sums = bias && w && T > 0;
-  const Tensor part = sums ? alloc({blocks(T), N}, F32, dev) : Tensor();
-  if (x || w) quantize(g2, (x ? BY_ROWS : 0) | (w ? BY_COLUMNS : 0), r.rows, r.cols, f32o(part));
-  if (sums) r.bias = column_sums(f32(part), blocks(T), N, g2.scalar_type(), dev);
+  const Packed rows(T, N, BY_ROWS), cols(T, N, BY_COLUMNS);
+  const int64_t at_cols = x ? up_to(rows.bytes, 256) : 0, at_sums = at_cols + (w ? up_to(cols.bytes, 256) : 0);
+  float* part = nullptr;
+  if (x || w) {
+    r.buf = alloc({at_sums + (sums ? blocks(T) * N * 4 : 0)}, at::kByte, dev);
+    char* p = static_cast<char*>(out(r.buf));
+    if (x) r.rows = rows.in(p);
+    if (w) r.cols = cols.in(p + at_cols);
+    if (sums) part = reinterpret_cast<float*>(p + at_sums);
+    quantize(g2, (x ? BY_ROWS : 0) | (w ? BY_COLUMNS : 0), r.rows, r.cols, part);
+  }
+  if (sums) r.bias = column_sums(part, blocks(T), N, g2.scalar_type(), dev);
   else if (bias) r.bias = g2.to(F32).sum(0).to(g2.scalar_type());
   return r;
 }
@@ -343,10 +353,9 @@ std::tuple<Tensor, Tensor> fp8_block_quantize(const Tensor& x, bool tiles) {
   const at::AutoDispatchBelowADInplaceOrView no_graph;
   const Tensor x2 = flat(x);
   const int64_t R = x2.size(0), C = x2.size(1);
-  const Coded c{codes(R, C, x.device()), tiles ? alloc({blocks(R), blocks(C)}, F32, x.device()) : scale_rows(blocks(C), R, x.device())};
-  quantize(x2, tiles ? BY_TILES : BY_ROWS, operand(c), Operand());
-  if (tiles) return {c.q, c.s};
-  return {c.q.view(x.sizes()), c.s.t().view(with_last(x.sizes(), blocks(C)))};
+  const Coded c{codes(R, C, x.device()), tiles ? alloc({blocks(R), blocks(C)}, F32, x.device()) : row_scales(x, R, C)};
+  quantize(x2, tiles ? BY_TILES : BY_ROWS, {ptr(c.q), f32(c.s), R, C}, Operand());
+  return {x.dim() == 2 ? c.q : c.q.view(x.sizes()), c.s};
 }
 Tensor fp8_block_dequantize(const Tensor& q, const Tensor& s, int64_t type) {
   no_transforms();
@@ -378,9 +387,9 @@ std::optional<std::tuple<Tensor, Tensor, Tensor>> rmsnorm_fp8_block(const Tensor
   const c10::cuda::CUDAGuard device(x.device());
   const at::AutoDispatchBelowADInplaceOrView no_graph;
   const int64_t D = x.size(-1), T = x.numel() / D;
-  const Coded c{codes(T, D, x.device()), scale_rows(blocks(D), T, x.device())};
-  const BlockNorm n = block_norm(x, residual, g, eps, form, false, operand(c));
-  return std::make_tuple(x.dim() == 2 ? c.q : c.q.view(x.sizes()), x.dim() == 2 ? c.s.t() : c.s.t().view(with_last(x.sizes(), blocks(D))), n.s);
+  const Coded c{codes(T, D, x.device()), row_scales(x, T, D)};
+  const BlockNorm n = block_norm(x, residual, g, eps, form, false, {ptr(c.q), f32(c.s), T, D, up_to(D, 16)});
+  return std::make_tuple(x.dim() == 2 ? c.q : c.q.view(x.sizes()), c.s, n.s);
 }
 // type: of the result
 // kept: codes and scales of a weight tensor that its owner keeps between updates (quantised here otherwise)

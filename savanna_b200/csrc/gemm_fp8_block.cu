@@ -9,8 +9,8 @@
 //   warp 0     TMA producer: a k-block's operands, 32 KB a CTA and stage
 //   warp 1     MMA issuer: four products of 32 k a k-block, each k-block into the next of the TMEM buffers
 //   warp 2     the scales into a ring in shared memory (asynchronous copies of 16 bytes, or of 4 for any strides), eight k-blocks deep, handed over by fours
-//   warps 4-11 a lane owns a row and half of the tile's columns: tcgen05.ld of 16 columns, eight packed multiply-adds, while the next 16 are on
-//              their way; after the last k-block the sums leave in whole sectors
+//   warps 4-11 a lane owns a row and half of the tile's columns: tcgen05.ld of 32 columns twice, packed multiply-adds on the one while the next of the
+//              other are on their way; after the last k-block the sums leave by bulk stores beside the next tile's products
 //
 // Two tiles: 256 x 256 on a CTA pair (cta_group::2; two buffers of 256 columns, 128 sums a thread) and 128 x 128 on one CTA (four buffers of
 // 128, 64 sums), for outputs that leave the chip idle in the larger one.

@@ -439,3 +439,47 @@ def test_recipe_on_two_streams(recipe):
             got.append(ops.linear(x, w, fp8=True))
         torch.cuda.synchronize()
     assert all(torch.equal(g, want) for g in got)
+
+
+# ------------------------------------------------------------------------------------------------ sizes
+
+
+def test_more_than_two_to_the_31_values():
+    """The last rows of tensors whose offsets pass 32 bits are those of the same rows by themselves."""
+    T, D, N = 270001, 8192, 128
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("wants 40 GB")
+    g = _randn(D, seed=1)
+    x = torch.empty(T, D, device="cuda", dtype=torch.bfloat16)
+    x[-1000:] = _randn(1000, D)
+    x[:-1000] = 1.0
+    tail = x[-300:].clone()
+    q, s, kept = ops.rmsnorm_fp8_block(x, g, 1e-5, "te", x)
+    q1, s1, kept1 = ops.rmsnorm_fp8_block(tail, g, 1e-5, "te", tail)
+    assert _same_bits(q[-300:], q1) and torch.equal(s[-300:], s1) and torch.equal(kept[-300:], kept1)
+    del kept
+    assert torch.equal(ops.fp8_block_dequantize(q, s)[-300:], ops.fp8_block_dequantize(q1, s1))
+    w = ops.fp8_block_quantize_weight(_randn(N, D, seed=2))
+    with torch.no_grad():
+        assert torch.equal(ops.linear_fp8_block((q, s), w)[-200:], ops.linear_fp8_block((q1[100:], s1[100:]), w))
+    del q, s
+    q, s = ops.fp8_block_quantize(x)
+    q1, s1 = ops.fp8_block_quantize(tail)
+    assert _same_bits(q[-300:], q1) and torch.equal(s[-300:], s1)
+    del q, s
+    # a wide result, its input gradient and the weight gradient over all tokens
+    h = torch.zeros(T, 128, device="cuda", dtype=torch.bfloat16)
+    h[-200:] = _randn(200, 128, seed=3)
+    h.requires_grad_()
+    w = _randn(D, 128, seed=4).requires_grad_()
+    gy = x
+    y = ops.linear_fp8_block(h, w)
+    short = h[-200:].detach().requires_grad_()
+    y1 = ops.linear_fp8_block(short, w)
+    assert torch.equal(y[-200:], y1)
+    gh, gw = torch.autograd.grad(y, (h, w), gy)
+    assert torch.equal(gh[-200:], torch.autograd.grad(y1, short, gy[-200:].contiguous())[0])
+    # columns of the last tokens alone: the others' activations are zero, and blocks of tokens begin where T - 200 is no multiple of 128
+    n0 = (T - 200) // 128 * 128
+    gcol, xcol = (_whole(*ref.fp8_block_quantize(t[n0:].detach().t().contiguous())).t() for t in (gy, h))
+    close_sum(gw, gcol.t() @ xcol, gcol.abs().t() @ xcol.abs(), torch.bfloat16, "dw")
