@@ -423,30 +423,45 @@ norm_backward_kernel(NormBackArgs p) {
 }
 
 // ------------------------------------------------------------------------------------------------ back
+// Eight values a thread and turn, two turns with both loads on their way before the first value is used.
 template <class T, bool VEC>
 __global__ void __launch_bounds__(256)
 dequantize_kernel(const uint8_t* __restrict__ q, const float* __restrict__ scale, T* __restrict__ x, long long R, int C, long long ldq,
                   long long s_row, long long s_col, int tiles) {
-  const int per_row = (C + 7) / 8;
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long row = i / per_row;
-  if (row >= R) return;
-  const int c = int(i - row * per_row) * 8, n = min(8, C - c);
-  const float s = scale[(tiles ? row / BLOCK : row) * s_row + (c / BLOCK) * s_col];
-  uint32_t w[2] = {0u, 0u};
-  if (VEC) {
-    const uint2 t = *reinterpret_cast<const uint2*>(q + row * ldq + c);
-    w[0] = t.x; w[1] = t.y;
-  } else {
-    for (int j = 0; j < n; ++j) w[j >> 2] |= uint32_t(q[row * ldq + c + j]) << (8 * (j & 3));
-  }
-  float f[8];
+  constexpr int TURNS = 2;
+  const uint32_t per_row = (uint32_t(C) + 7) / 8;
+  const long long total = R * per_row;
+  uint32_t w[TURNS][2];
+  float s[TURNS];
+  long long row[TURNS];
+  int c[TURNS];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 t = decode2(w[j >> 1] >> (16 * (j & 1)));
-    f[2 * j] = t.x * s; f[2 * j + 1] = t.y * s;
+  for (int u = 0; u < TURNS; ++u) {
+    const long long i = ((long long)blockIdx.x * TURNS + u) * 256 + threadIdx.x;
+    row[u] = i >= total ? -1 : total < 0x80000000LL ? (long long)(uint32_t(i) / per_row) : i / per_row;
+    w[u][0] = w[u][1] = 0u;
+    if (row[u] < 0) continue;
+    c[u] = int(i - row[u] * per_row) * 8;
+    s[u] = scale[(tiles ? row[u] / BLOCK : row[u]) * s_row + (c[u] / BLOCK) * s_col];
+    const uint8_t* from = q + row[u] * ldq + c[u];
+    if (VEC) {
+      const uint2 t = *reinterpret_cast<const uint2*>(from);
+      w[u][0] = t.x; w[u][1] = t.y;
+    } else {
+      for (int j = 0; j < min(8, C - c[u]); ++j) w[u][j >> 2] |= uint32_t(from[j]) << (8 * (j & 3));
+    }
   }
-  put<VEC, T>(x + row * C + c, pack<T>(f), n);
+#pragma unroll
+  for (int u = 0; u < TURNS; ++u) {
+    if (row[u] < 0) continue;
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 t = decode2(w[u][j >> 1] >> (16 * (j & 1)));
+      f[2 * j] = t.x * s[u]; f[2 * j + 1] = t.y * s[u];
+    }
+    put<VEC, T>(x + row[u] * C + c[u], pack<T>(f), min(8, C - c[u]));
+  }
 }
 
 template <class T> bool aligned16(const void* p, long long ld) {
@@ -507,7 +522,7 @@ static int launch_back(const NormBackArgs& p, int blocks, cudaStream_t st) {
 template <class T>
 static int launch_dequantize(const void* q, const float* scale, void* x, long long R, int C, long long ldq, long long s_row, long long s_col,
                              int tiles, cudaStream_t st) {
-  const long long blocks = (R * ((C + 7) / 8) + 255) / 256;
+  const long long blocks = (R * (((long long)C + 7) / 8) + 511) / 512;                // two turns of 256 threads
   if (blocks > 0x7fffffffLL) return -3;
   const bool vec = C % 8 == 0 && ldq % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
   if (vec) dequantize_kernel<T, true><<<(unsigned)blocks, 256, 0, st>>>((const uint8_t*)q, scale, (T*)x, R, C, ldq, s_row, s_col, tiles);
