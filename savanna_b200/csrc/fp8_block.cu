@@ -106,28 +106,33 @@ quantize_kernel(QuantArgs p) {
   Magnitudes<M> most = {};                                  // of the thread's columns
   f2 cs[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
-  for (int i = 0; i < RPT; ++i) {
-    const Magnitudes<M> m = sizes(i);
+  for (int i = 0; i < RPT; i += 2) {
+    const Magnitudes<M> m[2] = {sizes(i), sizes(i + 1)};
     if (FORM & (COLS | TILE)) {
 #pragma unroll
-      for (int j = 0; j < MW; ++j) most.w[j] = max_of<M>(most.w[j], m.w[j]);
+      for (int j = 0; j < MW; ++j) most.w[j] = max_of<M>(most.w[j], max_of<M>(m[0].w[j], m[1].w[j]));
     }
     if ((FORM & COLS) && p.sums) {
-      f2 v[4];
-      values(i, v);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) cs[j] = f2_add(cs[j], v[j]);
+      for (int k = 0; k < 2; ++k) {
+        f2 v[4];
+        values(i + k, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) cs[j] = f2_add(cs[j], v[j]);
+      }
     }
     if (FORM & ROWS) {
-      uint32_t top = largest(m);
+      uint32_t top[2];
+      largest_of_rows(m[0], m[1], top[0], top[1]);
 #pragma unroll
-      for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const Coder c(top);
-      const int r = h + HALVES * i;
-      f2 v[4];
-      values(i, v);
-      if (r < rows && n > 0) *reinterpret_cast<uint2*>(p.q_rows + (r0 + r) * p.ldq + c0) = encode(c, v);
-      if (l == 0) row_scale[r] = c.scale;
+      for (int k = 0; k < 2; ++k) {
+        const Coder c(top[k]);
+        const int r = h + HALVES * (i + k);
+        f2 v[4];
+        values(i + k, v);
+        if (r < rows && n > 0) *reinterpret_cast<uint2*>(p.q_rows + (r0 + r) * p.ldq + c0) = encode(c, v);
+        if (l == 0) row_scale[r] = c.scale;
+      }
     }
   }
   if (FORM & TILE) {

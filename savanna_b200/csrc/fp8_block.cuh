@@ -67,6 +67,26 @@ template <class T> __device__ __forceinline__ uint32_t largest(const Magnitudes<
   return sizeof(T) == 2 ? widen<T>(max(r & 0xffffu, r >> 16)) : r;
 }
 
+// The largest magnitudes of eight values of each of two rows, over the 16 threads that share the rows.  16-bit magnitudes travel two in a word.
+template <class T> __device__ __forceinline__ void largest_of_rows(const Magnitudes<T>& a, const Magnitudes<T>& b, uint32_t& ma, uint32_t& mb) {
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t x = __vmaxu2(__vmaxu2(a.w[0], a.w[1]), __vmaxu2(a.w[2], a.w[3])), y = __vmaxu2(__vmaxu2(b.w[0], b.w[1]), __vmaxu2(b.w[2], b.w[3]));
+    uint32_t m = __vmaxu2(__byte_perm(x, y, 0x5410), __byte_perm(x, y, 0x7632));
+#pragma unroll
+    for (int o = 8; o; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+    ma = widen<T>(m & 0xffffu);
+    mb = widen<T>(m >> 16);
+  } else {
+    ma = largest(a);
+    mb = largest(b);
+#pragma unroll
+    for (int o = 8; o; o >>= 1) {
+      ma = max(ma, __shfl_xor_sync(0xffffffffu, ma, o));
+      mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, o));
+    }
+  }
+}
+
 __device__ __forceinline__ float up(bf16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float up(__half v) { return __half2float(v); }
 __device__ __forceinline__ float up(float v) { return v; }
