@@ -27,12 +27,14 @@ __device__ __forceinline__ uint32_t magnitude(float f) { return __float_as_uint(
 // The reciprocal is CUDA's approximate one: the remainder makes good what it lacks.  The quotient is in units of 2^20, in which x * 448 cannot overflow and a magnitude of 2^-100 is still far from the subnormal numbers.
 struct Coder {
   float scale, minus_amax, inv;
-  __device__ __forceinline__ explicit Coder(uint32_t m) {                // m: bits of the block's largest magnitude
+  // m: bits of the block's largest magnitude.  rounded: CUDA's correctly rounded reciprocal instead
+  __device__ __forceinline__ explicit Coder(uint32_t m, bool rounded = false) {
     const float a = fmaxf(__uint_as_float(m), 7.8886090522101181e-31f);  // 2^-100
     scale = m < 0x7f800000u ? __fmul_rn(a, 1.f / 448.f) : __uint_as_float(0x7fffffffu);
     const float amax = a * 9.5367431640625e-07f;
     minus_amax = -amax;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(amax));
+    if (rounded) inv = __frcp_rn(amax);
+    else asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(amax));
   }
 };
 // Two values as two codes: of one block, or of two (columns)
