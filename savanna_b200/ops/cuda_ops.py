@@ -1126,8 +1126,9 @@ def norm_linear_fp8_block(x, norm_weight, eps, form, w, bias, residual):
 def _block_weight(w):
     """Codes and scales of a parameter under the recipe `block128`, kept on it until an optimizer step (which may write through addresses) or
     an operation of PyTorch (which counts versions) changes it.  (None, None), for the call to quantise by itself, while a graph is captured: what
-    a graph computes is there after its replays alone, and weights change between those."""
-    if w.is_inference() or torch.cuda.is_current_stream_capturing():
+    a graph computes is there after its replays alone, and weights change between those; and while one is traced, which would take kept codes
+    for constants."""
+    if w.is_inference() or torch.cuda.is_current_stream_capturing() or torch._C._get_tracing_state() is not None:
         return None, None
     state = (PARAM_EPOCH, w._version, w.data_ptr(), torch._C._cuda_getCurrentRawStream(w.get_device()))
     cache = getattr(w, "_fp8_block_cache", None)
