@@ -129,6 +129,17 @@ def linear(x, w, bias=None, fp8: bool = False, residual=None):
     return y if residual is None else y + residual
 
 
+# What the fp8 recipes keep on a weight (ops/cuda_ops.py): every recipe's attribute stands here.
+_WEIGHT_CODES = ("_fp8_cache", "_mx_cache", "_fp8_block_cache")
+
+
+def drop_weight_codes(w) -> None:
+    """Frees the 8-bit copies that the fp8 recipes keep on a weight."""
+    for name in _WEIGHT_CODES:
+        if getattr(w, name, None) is not None:
+            setattr(w, name, None)
+
+
 def linear_allgather(x, w, bias=None, seq_dim: int = 1, fp8: bool = False):
     """Sequence-parallel column projection: all-gather x along `seq_dim` over the tensor-parallel group,
     then x w^T.  CUDA: one fused peer-memory kernel when the symmetric workspace is up."""

@@ -171,10 +171,7 @@ class UnitFlat:
         self.full.untyped_storage().resize_(0)
         self.resident = False
         for p in self.params:                                  # quantised copies of the weights go with them
-            if getattr(p, "_fp8_cache", None) is not None:
-                p._fp8_cache = None
-            if getattr(p, "_mx_cache", None) is not None:
-                p._mx_cache = None
+            ops.drop_weight_codes(p)
 
     # -- gradients -----------------------------------------------------------------
     def alloc_grads(self) -> None:

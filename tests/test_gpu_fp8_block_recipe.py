@@ -42,5 +42,57 @@ def test_traced_graph_sees_changed_weights(recipe):
             assert torch.equal(a.float(), 2.0 * b.float())
 
 
+
 # ------------------------------------------------------------------------------------------------ optimizers
 
+_OVER = {"global_num_gpus": 1, "train_micro_batch_size_per_gpu": 1, "use_fp8_linears": True, "use_fp8_input_projections": True, "use_fp8_output_projections": True,
+         "use_fp8_mlp_projections": True}
+
+
+def _trainer(over):
+    import os
+    from savanna_b200.config import GlobalConfig
+    from savanna_b200.train.trainer import Trainer
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    return Trainer(GlobalConfig.from_ymls([os.path.join(root, "configs", "baseline", "tiny_sh2_gpu.yml")], dict(_OVER, **over)), load=False)
+
+
+def _batches(cfg, n, first=0):
+    from savanna_b200.data.synthetic import acgt_batch
+    return iter([{"text": acgt_batch(cfg.train_micro_batch_size_per_gpu, cfg.seq_length, seed=first + i, pin=True)} for i in range(n)])
+
+
+@pytest.fixture
+def trainers():
+    from savanna_b200.ops import cuda_ops
+    from savanna_b200.parallel import state
+    yield _trainer
+    state.destroy_model_parallel()
+    cuda_ops.set_fp8_recipe("delayed")
+
+
+def _trace(over, n=6):
+    from savanna_b200.parallel import state
+    tr = _trainer(over)
+    d = _batches(tr.cfg, n * tr.gas)
+    out = [float(tr.train_step(d)) for _ in range(n)]
+    state.destroy_model_parallel()
+    return out
+
+
+def test_released_units_keep_no_codes(trainers):
+    tr = trainers({"fp8_recipe": "block128", "zero_optimization": {"stage": 3}})
+    for i in range(2):
+        tr.train_step(_batches(tr.cfg, 1, i))
+    tr.evaluate(_batches(tr.cfg, 1, 9), iters=1)
+    flats = [f for u in tr.optimizer.units[1:] for f in u.flats]
+    assert flats and all(f.full.untyped_storage().size() == 0 for f in flats)
+    kept = [p for f in flats for p in f.params if getattr(p, "_fp8_block_cache", None) is not None]
+    assert not kept
+
+
+def test_partitioned_stage_3_matches_stage_1(trainers):
+    over = {"fp8_recipe": "block128", "gradient_accumulation_steps": 2}
+    want = _trace(dict(over, zero_optimization={"stage": 1}))
+    got = _trace(dict(over, zero_optimization={"stage": 3}, checkpoint_activations=True, checkpoint_num_layers=2))
+    assert max(abs(a - b) for a, b in zip(want, got)) < 2e-2 * max(want), (want, got)
