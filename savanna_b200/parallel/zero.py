@@ -217,13 +217,17 @@ class ZeroOptimizer:
         else:
             dist.all_gather_into_tensor(g.flat_param, shard, group=self.group)
 
+    def _weights_written(self) -> None:
+        """Flat buffers are written past the parameters' version counters: cached fp8 copies of the weights are stale from here on."""
+        if any(g.flat_param.is_cuda for g in self.groups):
+            from ..ops import cuda_ops
+            cuda_ops.bump_param_epoch()
+
     # ------------------------------------------------------------------ step
     @torch.no_grad()
     def step(self) -> torch.Tensor:
         """Runs one optimizer step; returns the global gradient norm (0-dim fp32 tensor, on device)."""
-        if self.groups and self.groups[0].flat_param.is_cuda:
-            from ..ops import cuda_ops
-            cuda_ops.bump_param_epoch()             # cached fp8 copies of the weights are stale after this step
+        self._weights_written()
         if self.fused is not None:
             return self.fused.step(self)
         self.step_count += 1
@@ -324,11 +328,13 @@ class ZeroOptimizer:
             self.loss_scaler.load_state_dict(sd["loss_scaler"])
 
     def refresh_master_from_params(self) -> None:
+        self._weights_written()                     # by whoever asks for this
         for g in self.groups:
             if not g.master_is_view:
                 g.master.copy_(g.shard_slice(g.flat_param))
 
     def sync_params_from_master(self) -> None:
+        self._weights_written()
         for g in self.groups:
             if not g.master_is_view:
                 g.shard_slice(g.flat_param).copy_(g.master)

@@ -414,11 +414,16 @@ class PartitionedZeroOptimizer:
             if f.grads_live:
                 f.gfull.zero_()
 
-    @torch.no_grad()
-    def step(self) -> torch.Tensor:
-        if self.groups and self.groups[0].master.is_cuda:
+    def _weights_written(self) -> None:
+        """Shards and flat buffers are written past the parameters' version counters (and masters may lie on the host while the parameters do not):
+        whatever was made of the old weights ends here."""
+        if any(f.full.is_cuda for f in self.groups):
             from ..ops import cuda_ops
             cuda_ops.bump_param_epoch()
+
+    @torch.no_grad()
+    def step(self) -> torch.Tensor:
+        self._weights_written()
         self.finish_backward()
         for f in self.units[0].flats:               # the resident root unit reduces once per step
             self._sync_replicated(f)
@@ -499,6 +504,7 @@ class PartitionedZeroOptimizer:
     def refresh_master_from_params(self) -> None:
         """Rebuild shards and fp32 masters from the parameters: from the full buffer where a unit is whole (inside
         `full_params`, and always for resident units), else from the low-precision shard."""
+        self._weights_written()
         with torch.no_grad():
             for f in self.groups:
                 if f.resident:
@@ -507,6 +513,7 @@ class PartitionedZeroOptimizer:
                     f.master.copy_(f.param_shard)
 
     def sync_params_from_master(self) -> None:
+        self._weights_written()
         with torch.no_grad():
             for f in self.groups:
                 if not f.master_is_view:
@@ -543,6 +550,7 @@ class PartitionedZeroOptimizer:
             raise ValueError("optimizer state has a different number of flat buffers: it was written by another ZeRO "
                              "stage or model cut; load the module only and rebuild the optimizer state")
         st = sd["base_optimizer_state"]["state"]
+        self._weights_written()
         with torch.no_grad():
             for i, f in enumerate(self.groups):
                 if masters[i].numel() != f.master.numel():
