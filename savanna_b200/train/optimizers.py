@@ -239,6 +239,9 @@ class DataParallelOptimizer:
             for p in params:
                 p.grad.mul_(coef.to(p.grad.dtype))
         self.inner.step()
+        if any(p.is_cuda for p in params):
+            from ..ops import cuda_ops
+            cuda_ops.bump_param_epoch()             # cached fp8 copies of the weights are stale after this step
         self.last_grad_norm = norm
         return norm
 

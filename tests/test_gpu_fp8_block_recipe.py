@@ -124,6 +124,20 @@ def test_weights_rewritten_from_optimizer_state(trainers, stage):
     assert cuda_ops.PARAM_EPOCH > epoch and loss() == want
 
 
+@pytest.mark.parametrize("fp8_recipe", ["delayed", "mxfp8", "block128"])
+def test_other_optimizers_are_followed(recipe, fp8_recipe):
+    """A step of SGD that doubles the weight doubles its projection."""
+    from savanna_b200.train.optimizers import DataParallelOptimizer
+    recipe.set_fp8_recipe(fp8_recipe)
+    x, w = _randn(32, 256), torch.nn.Parameter(_randn(64, 256, seed=1))
+    opt = DataParallelOptimizer(torch.optim.SGD([w], lr=1.0), 0.0, None, 1)
+    w.grad = -w.detach().clone()
+    with torch.no_grad():
+        before = [ops.linear(x, w, fp8=True).float() for _ in range(2)][1]
+        opt.step()
+        assert torch.equal(ops.linear(x, w, fp8=True).float(), 2.0 * before)
+
+
 def test_released_units_keep_no_codes(trainers):
     tr = trainers({"fp8_recipe": "block128", "zero_optimization": {"stage": 3}})
     for i in range(2):
