@@ -12,6 +12,7 @@ number of kernels the C entry point launches).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import importlib.util
 import os
@@ -1123,14 +1124,30 @@ def norm_linear_fp8_block(x, norm_weight, eps, form, w, bias, residual):
     return _native("norm_linear_fp8_block", x, norm_weight, float(eps), 0 if form == "te" else 1, w, ws, bias, residual, None, None)
 
 
+_UNCHANGED = None          # inside `weights_unchanged`: what marks the codes made there
+
+
+@contextlib.contextmanager
+def weights_unchanged():
+    """The caller's word that no parameter changes inside (the micro-batches of a training step, an evaluation): under the recipe `block128` each
+    weight is quantised once there.  Elsewhere every call quantises its weight: who writes it through `.data`, by its address or in a replayed
+    graph leaves no trace on it.  A program that keeps weights in 8 bits by itself hands their codes to `ops.linear_fp8_block`."""
+    global _UNCHANGED
+    outer = _UNCHANGED
+    _UNCHANGED = outer or object()
+    try:
+        yield
+    finally:
+        _UNCHANGED = outer
+
+
 def _block_weight(w):
-    """Codes and scales of a parameter under the recipe `block128`, kept on it until an optimizer step (which may write through addresses) or
-    an operation of PyTorch (which counts versions) changes it.  (None, None), for the call to quantise by itself, while a graph is captured: what
-    a graph computes is there after its replays alone, and weights change between those; and while one is traced, which would take kept codes
-    for constants."""
-    if w.is_inference() or torch.cuda.is_current_stream_capturing() or torch._C._get_tracing_state() is not None:
+    """Codes and scales of a parameter under the recipe `block128`, kept on it inside of one `weights_unchanged` (and there until its version or
+    address changes).  (None, None), for the call to quantise by itself, elsewhere; while a graph is captured: what a graph computes is there after
+    its replays alone, and weights change between those; and while one is traced, which would take kept codes for constants."""
+    if _UNCHANGED is None or w.is_inference() or torch.cuda.is_current_stream_capturing() or torch._C._get_tracing_state() is not None:
         return None, None
-    state = (PARAM_EPOCH, w._version, w.data_ptr(), torch._C._cuda_getCurrentRawStream(w.get_device()))
+    state = (_UNCHANGED, PARAM_EPOCH, w._version, w.data_ptr(), torch._C._cuda_getCurrentRawStream(w.get_device()))
     cache = getattr(w, "_fp8_block_cache", None)
     if cache is None or cache[0] != state:
         cache = w._fp8_block_cache = (state, _native("fp8_block_quantize", w.detach(), True))

@@ -183,24 +183,25 @@ def pipeline_train_step(trainer, data_iterator) -> torch.Tensor:
         return None if first else x_in.grad
 
     x_in = None
-    for _ in range(warmup):
-        x_in = _exchange(None, -1, act, prev)
-        out = forward(x_in)
-        _exchange(out.detach(), nxt, None, -1)
-    if steady > 0:
-        x_in = _exchange(None, -1, act, prev)
-    for i in range(steady):
-        out = forward(x_in)
-        g = _exchange(None if last else out.detach(), nxt, None if last else act, nxt)
-        dx = backward(g)
-        if i == steady - 1:
+    with trainer._weights_unchanged():
+        for _ in range(warmup):
+            x_in = _exchange(None, -1, act, prev)
+            out = forward(x_in)
+            _exchange(out.detach(), nxt, None, -1)
+        if steady > 0:
+            x_in = _exchange(None, -1, act, prev)
+        for i in range(steady):
+            out = forward(x_in)
+            g = _exchange(None if last else out.detach(), nxt, None if last else act, nxt)
+            dx = backward(g)
+            if i == steady - 1:
+                _exchange(dx, prev, None, -1)
+            else:
+                x_in = _exchange(dx, prev, act, prev)
+        for _ in range(warmup):
+            g = _exchange(None, -1, act, nxt)
+            dx = backward(g)
             _exchange(dx, prev, None, -1)
-        else:
-            x_in = _exchange(dx, prev, act, prev)
-    for _ in range(warmup):
-        g = _exchange(None, -1, act, nxt)
-        dx = backward(g)
-        _exchange(dx, prev, None, -1)
     _sync_tied_embedding_grads(model)
     trainer._sync_replicated_grads()
     trainer.grad_norm = trainer.optimizer.step()

@@ -315,6 +315,14 @@ class Trainer:
             stack.enter_context(det.section(name))
         return stack
 
+    def _weights_unchanged(self):
+        """Context between two updates: weights that run in 8 bits are quantised once inside."""
+        import contextlib
+        if self.device.type != "cuda":
+            return contextlib.nullcontext()
+        from ..ops import cuda_ops
+        return cuda_ops.weights_unchanged()
+
     def train_step(self, data_iterator: Iterator) -> torch.Tensor:
         """One optimizer step over `gradient_accumulation_steps` micro-batches.  Returns the mean loss
         (0-dim device tensor; no host synchronisation happens inside the step)."""
@@ -331,28 +339,29 @@ class Trainer:
             max_len = cfg.curriculum_seqlen = self.curriculum.update_difficulty(self.iteration + 1)
             if max_len >= cfg.seq_length:
                 max_len = None
-        for micro in range(self.gas):
-            # the last micro-batch's forward plants the hooks through which its backward reports finished blocks
-            overlap = self._zero_overlap if micro == self.gas - 1 else None
-            if overlap is not None:
-                opt = self.optimizer
-                self.model.grad_boundary_callback = lambda i: overlap.grads_final_from(opt, i)
-            try:
-                with self._mark("TRAIN_STEP_FORWARD"):
-                    b = batch_mod.get_batch(cfg, data_iterator, self.device, max_len)
-                    loss = self.forward_step(b)
-                with self._mark("TRAIN_STEP_BACKWARD"):
-                    if overlap is not None:
-                        overlap.begin_overlap(self.optimizer)
-                    if self.loss_scaler is not None:
-                        (loss * (self.loss_scaler.scale / self.gas)).backward()
-                    else:
-                        (loss / self.gas).backward()
-                    if self.partitioned:
-                        self.optimizer.finish_backward()
-            finally:
-                self.model.grad_boundary_callback = None
-            total = loss.detach() if total is None else total + loss.detach()
+        with self._weights_unchanged():
+            for micro in range(self.gas):
+                # the last micro-batch's forward plants the hooks through which its backward reports finished blocks
+                overlap = self._zero_overlap if micro == self.gas - 1 else None
+                if overlap is not None:
+                    opt = self.optimizer
+                    self.model.grad_boundary_callback = lambda i: overlap.grads_final_from(opt, i)
+                try:
+                    with self._mark("TRAIN_STEP_FORWARD"):
+                        b = batch_mod.get_batch(cfg, data_iterator, self.device, max_len)
+                        loss = self.forward_step(b)
+                    with self._mark("TRAIN_STEP_BACKWARD"):
+                        if overlap is not None:
+                            overlap.begin_overlap(self.optimizer)
+                        if self.loss_scaler is not None:
+                            (loss * (self.loss_scaler.scale / self.gas)).backward()
+                        else:
+                            (loss / self.gas).backward()
+                        if self.partitioned:
+                            self.optimizer.finish_backward()
+                finally:
+                    self.model.grad_boundary_callback = None
+                total = loss.detach() if total is None else total + loss.detach()
         if not self.partitioned:
             self._sync_replicated_grads()
         if self.noise_scale is not None:
@@ -410,9 +419,10 @@ class Trainer:
         self.model.eval()
         n = iters if iters is not None else cfg.eval_iters
         acc = torch.zeros((), device=self.device)
-        for _ in range(n):
-            b = batch_mod.get_batch(cfg, data_iterator, self.device)
-            acc += self.forward_step(b).float()
+        with self._weights_unchanged():
+            for _ in range(n):
+                b = batch_mod.get_batch(cfg, data_iterator, self.device)
+                acc += self.forward_step(b).float()
         self.model.train()
         acc = acc / max(1, n)
         if dist.is_initialized() and state.get_data_parallel_world_size() > 1:

@@ -42,6 +42,67 @@ def test_traced_graph_sees_changed_weights(recipe):
             assert torch.equal(a.float(), 2.0 * b.float())
 
 
+# ------------------------------------------------------------------------------------------------ written past PyTorch's counters
+
+
+def test_weights_written_through_their_data(recipe):
+    x, g, w = _randn(20, 256), _randn(256, seed=2), torch.nn.Parameter(_randn(64, 256, seed=1))
+    with torch.no_grad():
+        before = ops.linear(x, w, fp8=True), ops.norm_linear(x, g, 1e-5, "te", w, None, True)[0]
+        w.data.mul_(2.0)                                          # a version counter of its own
+        after = ops.linear(x, w, fp8=True), ops.norm_linear(x, g, 1e-5, "te", w, None, True)[0]
+    for a, b in zip(after, before):
+        assert torch.equal(a.float(), 2.0 * b.float())
+
+
+def test_weights_written_by_a_replayed_graph(recipe):
+    x, w = _randn(20, 256), torch.nn.Parameter(_randn(64, 256, seed=1))
+    with torch.no_grad():
+        ops.linear(x, torch.nn.Parameter(_randn(64, 256, seed=5)), fp8=True)
+        torch.cuda.synchronize()
+        update = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(update):
+            w.mul_(2.0)
+        before = ops.linear(x, w, fp8=True).float()
+        update.replay()
+        assert torch.equal(ops.linear(x, w, fp8=True).float(), 2.0 * before)
+
+
+def test_weights_are_quantised_once_where_they_do_not_change(recipe):
+    x, w = _randn(20, 256), torch.nn.Parameter(_randn(64, 256, seed=1))
+
+    def launches(call):
+        before = recipe.launch_count()
+        y = call()
+        return recipe.launch_count() - before, y
+    with torch.no_grad():
+        alone, want = launches(lambda: ops.linear(x, w, fp8=True))
+        with recipe.weights_unchanged():
+            first, a = launches(lambda: ops.linear(x, w, fp8=True))
+            with recipe.weights_unchanged():                      # the outer one's codes hold in it
+                again, b = launches(lambda: ops.linear(x, w, fp8=True))
+            after, c = launches(lambda: ops.linear(x, w, fp8=True))
+        assert first == alone and again == after == alone - 1
+        assert all(torch.equal(y, want) for y in (a, b, c))
+        w.data.mul_(2.0)
+        with recipe.weights_unchanged():
+            assert torch.equal(ops.linear(x, w, fp8=True).float(), 2.0 * want.float())
+        w.data.mul_(2.0)
+        assert torch.equal(ops.linear(x, w, fp8=True).float(), 4.0 * want.float())
+
+
+def test_traced_graph_from_between_two_updates(recipe):
+    x, m = _randn(20, 256, seed=7), _Projections()
+    with torch.no_grad():
+        m.b.zero_()
+        with recipe.weights_unchanged():
+            m(x)
+            f = torch.jit.trace(m, (x,), check_trace=False)
+            before = f(x)
+        m.w.data.mul_(2.0)
+        for a, b in zip(f(x), before):
+            assert torch.equal(a.float(), 2.0 * b.float())
+
 
 # ------------------------------------------------------------------------------------------------ optimizers
 
