@@ -75,18 +75,21 @@ class _Traced(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, name, *args):
-        ins = [a.detach().requires_grad_(a.requires_grad) if isinstance(a, torch.Tensor) else a for a in args]
-        with torch.enable_grad():
+        grad = len(ctx.next_functions) > 0       # the caller's grad mode, now and at each later run: no edges without it
+        ins = [a.detach().requires_grad_(grad and a.requires_grad) if isinstance(a, torch.Tensor) else a for a in args]
+        with torch.set_grad_enabled(grad):
             out = getattr(_N, name)(*ins)
-        ctx.graph = ins, out
         many = isinstance(out, tuple)
-        got = tuple(None if o is None else o.detach() for o in (out if many else (out,)))
+        outs = out if many else (out,)
+        ctx.graph = ins, outs
+        got = tuple(None if o is None else o.detach() for o in outs)
+        ctx.mark_non_differentiable(*(d for d, o in zip(got, outs) if o is not None and not o.requires_grad))
         return got if many else got[0]
 
     @staticmethod
     def backward(ctx, *grads):
         ins, out = ctx.graph
-        outs = [(o, g) for o, g in zip(out if isinstance(out, tuple) else (out,), grads) if o is not None and o.requires_grad]
+        outs = [(o, g) for o, g in zip(out, grads) if o is not None and o.requires_grad]
         want = [a for a in ins if isinstance(a, torch.Tensor) and a.requires_grad]
         got = iter(torch.autograd.grad([o for o, _ in outs], want, [g for _, g in outs], retain_graph=True, allow_unused=True))
         return (None,) + tuple(next(got) if isinstance(a, torch.Tensor) and a.requires_grad else None for a in ins)

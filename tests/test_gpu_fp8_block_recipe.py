@@ -215,3 +215,47 @@ def test_partitioned_stage_3_matches_stage_1(trainers):
     want = _trace(dict(over, zero_optimization={"stage": 1}))
     got = _trace(dict(over, zero_optimization={"stage": 3}, checkpoint_activations=True, checkpoint_num_layers=2))
     assert max(abs(a - b) for a, b in zip(want, got)) < 2e-2 * max(want), (want, got)
+
+
+# ------------------------------------------------------------------------------------------------ traced
+
+
+class _Codes(_Projections):
+    def forward(self, x):
+        q, s, _ = ops.rmsnorm_fp8_block(x, self.g, 1e-5)
+        return ops.linear_fp8_block((q, s), self.w, self.b), ops.norm_linear_fp8_block(x, self.g, 1e-5, "te", self.w, self.b)[0]
+
+
+def test_traced_calls_with_codes_under_no_grad(recipe):
+    """A parameter in the projection of an input given as codes is no reason to refuse it where no gradient is wanted."""
+    m = _Codes()
+    with torch.no_grad():
+        traced = torch.jit.trace(m, (_randn(20, 256, seed=7),), check_trace=False)
+        y = _randn(20, 256, seed=8)
+        for a, e in zip(traced(y), m(y)):
+            assert torch.equal(a, e) and not a.requires_grad
+
+
+def test_traced_without_gradients_and_run_with_them(recipe):
+    m, x = _Projections(), _randn(20, 256, seed=7)
+    with torch.no_grad():
+        f = torch.jit.trace(m, (x,), check_trace=False)
+    got, want = (torch.autograd.grad([y.float().square().sum() for y in g(x)], list(m.parameters())) for g in (f, m))
+    for a, e in zip(got, want):
+        assert torch.equal(a, e)
+
+
+class _KeptCodes(_Projections):
+    def __init__(self):
+        super().__init__()
+        self.q, self.s = ops.fp8_block_quantize_weight(self.w.detach())
+
+    def forward(self, x):
+        q, s, _ = ops.rmsnorm_fp8_block(x, self.g, 1e-5)
+        return ops.linear_fp8_block((q, s), (self.q, self.s))
+
+
+def test_traced_codes_want_no_gradient(recipe):
+    """Codes of an input that wants a gradient carry none, traced as otherwise."""
+    m, x = _KeptCodes(), _randn(20, 256, seed=7)
+    assert torch.equal(torch.jit.trace(m, (x,), check_trace=False)(x), m(x))
