@@ -4,7 +4,8 @@
     model, tokenizer, cfg = load_for_inference(ckpt_dir, config_files=["model.yml"])
 
 Only the model states are read (no optimizer shards); tensor-parallel shards are merged when the checkpoint was written
-with more than one model-parallel rank and this process runs alone.  Command line: prints completions for prompts.
+with more than one model-parallel rank and this process runs alone.  On a GPU the configuration's `fp8_recipe` becomes the process's,
+as under the trainer: prompts run their 8-bit projections by it, single steps of cached generation run in bf16.  Command line: prints completions for prompts.
 
     python -m savanna_b200.inference.load <save>/global_step100 --prompt ACGTTGCA --tokens 64 [--temperature 0.8]
 """
@@ -39,6 +40,9 @@ def load_for_inference(step_dir: str, config_files: Optional[List[str]] = None, 
     if not state.model_parallel_is_initialized():
         state.initialize_model_parallel(1, 1, 1)
     dev = torch.device(device or ("cuda" if torch.cuda.is_available() else "cpu"))
+    if dev.type == "cuda":
+        from ..ops import cuda_ops
+        cuda_ops.set_fp8_recipe(cfg.fp8_recipe)              # the process's, as the trainer sets it
     model = build_model(cfg, device=dev)
     shards = load_shards(step_dir)
     module = merge_module([s["module"] for s in shards]) if len(shards) > 1 else shards[0]["module"]

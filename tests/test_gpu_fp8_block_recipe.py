@@ -259,3 +259,28 @@ def test_traced_codes_want_no_gradient(recipe):
     """Codes of an input that wants a gradient carry none, traced as otherwise."""
     m, x = _KeptCodes(), _randn(20, 256, seed=7)
     assert torch.equal(torch.jit.trace(m, (x,), check_trace=False)(x), m(x))
+
+
+# ------------------------------------------------------------------------------------------------ loaded for generation
+
+
+@pytest.mark.parametrize("fp8_recipe", ["mxfp8", "block128"])
+def test_loaded_checkpoints_run_their_recipe(trainers, fp8_recipe, tmp_path):
+    import os
+    from savanna_b200.ckpt import save_checkpoint
+    from savanna_b200.inference.load import load_for_inference
+    from savanna_b200.ops import cuda_ops
+    tr = trainers({"fp8_recipe": fp8_recipe, "zero_optimization": {"stage": 1}, "save": str(tmp_path)})
+    tr.train_step(_batches(tr.cfg, 1))
+    save_checkpoint(tr, 1)
+    tokens = next(_batches(tr.cfg, 1, 5))["text"][:, :96].long().cuda()
+    tr.model.eval()
+    positions = torch.arange(96, device="cuda")
+    with torch.no_grad():
+        want = tr.model(tokens, positions)
+        cuda_ops.set_fp8_recipe("delayed")
+        root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+        model, _, cfg = load_for_inference(str(tmp_path), [os.path.join(root, "configs", "baseline", "tiny_sh2_gpu.yml")], overrides=dict(_OVER, fp8_recipe=fp8_recipe))
+        assert cfg.fp8_recipe == fp8_recipe and cuda_ops.FP8_RECIPE == fp8_recipe
+        if fp8_recipe == "block128":                             # the other's model has projections with an amax history too
+            assert torch.equal(model(tokens, positions), want)
