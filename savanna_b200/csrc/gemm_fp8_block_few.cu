@@ -262,10 +262,15 @@ static int launch_few(const CUtensorMap& tmW, const CUtensorMap& tmX, const FewA
 }  // namespace sb
 
 // Whether a product of M tokens goes by this kernel.  With more tokens their tiles weigh as much as the weights', which the 128 x 128 tiles of the
-// other kernel read once for 128 tokens; but those leave SMs idle where there are fewer than two tiles of weights for three SMs.  us back to back, this
-// kernel and the other: 1 x 4096 x 12288 12.7, 19.7; 16 x 11264 x 4096 12.6, 25.2; 32 x 4096 x 12288 15.1, 13.9; 32 x 11264 x 4096 13.6, 26.0;
-// 64 x 4096 x 12288 17.6, 14.4; 64 x 4096 x 4096 10.6, 12.0.
-extern "C" int sb_gemm_fp8_block_takes_few(int M, int N) { return M <= 16 || (M <= 64 && (N + 127) / 128 * 3 <= 2 * sb::num_sms()); }
+// other kernel read once for 128 tokens; but those leave SMs idle where there are fewer tiles of weights than 7 for 16 SMs, and take a quarter longer for
+// tokens that end inside of 32.  us, this kernel and the other, weights from memory:
+//   K = 4096    N = 4096      8192        9472        12288       22528
+//   T = 17       8.7, 12.6   11.0, 17.7  13.0, 18.2  15.2, 18.9  21.0, 29.6
+//   T = 31                   11.4, 17.3  13.2, 17.1  15.6, 18.5  21.9, 29.9
+//   T = 32       9.2, 12.7   11.5, 13.3  13.5, 13.4  15.7, 14.4  21.9, 25.9
+//   T = 64      11.2, 12.8   12.9, 13.3  15.2, 13.7  18.2, 14.8  25.4, 26.1
+// (K = 1024, N = 12288: T = 17 8.0, 7.8; T = 64 10.5, 7.5.  K = 11264: T = 17 28.7, 30.8; T = 64 32.0, 31.5.)
+extern "C" int sb_gemm_fp8_block_takes_few(int M, int N) { return M < 32 || (M <= 64 && (N + 127) / 128 * 16 <= 7 * sb::num_sms()); }
 
 // As sb_gemm_fp8_block with neither operand transposed and tiles of 128 x 128 in W; up to 64 rows of X.  chained: the launch before it on the
 // stream was that of sb_fp8_block_quantize or sb_fp8_block_norm, which wrote X and sx and not W or sw.
