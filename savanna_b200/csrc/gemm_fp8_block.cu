@@ -568,6 +568,9 @@ static int launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensor
 }  // namespace blk8
 }  // namespace sb
 
+// Whether an [M, N] product goes by 256 x 256 tiles on CTA pairs.
+extern "C" int sb_gemm_fp8_block_goes_by_pairs(int M, int N) { return sb::blk8::goes_by_pairs(M, N, sb::num_sms()); }
+
 // C [M, N] of type 0 bf16, 1 fp16, 2 fp32 (bias, residual and a C that is added to: of the same type).  A: [M, K], or stored as [K, M] (a_mn);
 // B: [N, K] or [K, N] (b_mn); bytes, rows lda / ldb apart, 16-byte boundaries.  Scale of A at sa[m * sa_m + (k / 128) * sa_k], of B at
 // sb[n * sb_n + (k / 128) * sb_k] (sb_rows) or sb[(n / 128) * sb_n + (k / 128) * sb_k].  Forms: neither operand transposed, B, or both with sb_rows.

@@ -226,15 +226,19 @@ gemm_fp8_block_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_
   if (parts > 1) { cluster_arrive(); cluster_wait(); }             // no part leaves while its sums are read
 }
 
+// As many parts of the contraction as give every SM a CTA, and two k-blocks each.
+static int few_parts(int N, int K) {
+  const int tiles = (N + 127) / 128, kbs = (K + 127) / 128;
+  int parts = 1;
+  while (parts < 8 && (long long)tiles * parts < num_sms() && 4 * parts <= kbs) parts *= 2;
+  return parts;
+}
 template <int TOK>
 static int launch_few(const CUtensorMap& tmW, const CUtensorMap& tmX, const FewArgs& p, bool chained, cudaStream_t stream) {
   auto kern = gemm_fp8_block_few_kernel<TOK>;
   static std::atomic<unsigned long long> allowed{0};       // devices that know the kernel's shared memory
   if (!allow_shared(allowed, kern, FewSpace<TOK>::BYTES)) return -5;
-  const int tiles = (p.N + 127) / 128, kbs = (p.K + 127) / 128;
-  // as many parts of the contraction as give every SM a CTA, and two k-blocks each
-  int parts = 1;
-  while (parts < 8 && (long long)tiles * parts < num_sms() && 4 * parts <= kbs) parts *= 2;
+  const int tiles = (p.N + 127) / 128, parts = few_parts(p.N, p.K);
   if ((long long)tiles * parts > 0x7fffffffLL) return -3;
   cudaLaunchAttribute attr[2];
   int n = 0;
@@ -271,6 +275,9 @@ static int launch_few(const CUtensorMap& tmW, const CUtensorMap& tmX, const FewA
 //   T = 64      11.2, 12.8   12.9, 13.3  15.2, 13.7  18.2, 14.8  25.4, 26.1
 // (K = 1024, N = 12288: T = 17 8.0, 7.8; T = 64 10.5, 7.5.  K = 11264: T = 17 28.7, 30.8; T = 64 32.0, 31.5.)
 extern "C" int sb_gemm_fp8_block_takes_few(int M, int N) { return M < 32 || (M <= 64 && (N + 127) / 128 * 16 <= 7 * sb::num_sms()); }
+
+// CTAs that share a tile's k-blocks.
+extern "C" int sb_gemm_fp8_block_few_parts(int N, int K) { return sb::blk8::few_parts(N, K); }
 
 // As sb_gemm_fp8_block with neither operand transposed and tiles of 128 x 128 in W; up to 64 rows of X.  chained: the launch before it on the
 // stream was that of sb_fp8_block_quantize or sb_fp8_block_norm, which wrote X and sx and not W or sw.
