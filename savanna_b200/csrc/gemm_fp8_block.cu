@@ -573,7 +573,8 @@ extern "C" int sb_gemm_fp8_block_goes_by_pairs(int M, int N) { return sb::blk8::
 
 // C [M, N] of type 0 bf16, 1 fp16, 2 fp32 (bias, residual and a C that is added to: of the same type).  A: [M, K], or stored as [K, M] (a_mn);
 // B: [N, K] or [K, N] (b_mn); bytes, rows lda / ldb apart, 16-byte boundaries.  Scale of A at sa[m * sa_m + (k / 128) * sa_k], of B at
-// sb[n * sb_n + (k / 128) * sb_k] (sb_rows) or sb[(n / 128) * sb_n + (k / 128) * sb_k].  Forms: neither operand transposed, B, or both with sb_rows.
+// sb[n * sb_n + (k / 128) * sb_k] (sb_rows) or sb[(n / 128) * sb_n + (k / 128) * sb_k].  Forms: neither operand transposed, B, or both with sb_rows
+// (a weight gradient's: without bias and residual).
 extern "C" int sb_gemm_fp8_block(const void* A, const float* sa, long long sa_m, long long sa_k, const void* B, const float* sb, long long sb_n,
                                  long long sb_k, int sb_rows, void* C, const void* bias, const void* residual, int M, int N, int K,
                                  long long lda, long long ldb, long long ldc, long long ldr, int a_mn, int b_mn, int type, int beta, unsigned int* status,
@@ -581,7 +582,7 @@ extern "C" int sb_gemm_fp8_block(const void* A, const float* sa, long long sa_m,
   using namespace sb;
   using namespace sb::blk8;
   if (M <= 0 || N <= 0) return 0;
-  if (K <= 0) return -3;
+  if (K <= 0 || (sb_rows && (bias || residual))) return -3;
   if (!bind_context()) return -5;                        // the tensor-map encoder needs a current context
   if ((lda % 16) || (ldb % 16) || ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(B)) & 15)) return -4;
   if ((long long)((M + 127) / 128) * ((N + 127) / 128) > 0x7fffffffLL) return -3;
