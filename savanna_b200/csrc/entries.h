@@ -84,6 +84,7 @@ int sb_gemm_fp8_block(const void* A, const float* sa, long long sa_m, long long 
                       long long sb_k, int sb_rows, void* C, const void* bias, const void* residual, int M, int N, int K, long long lda, long long ldb,
                       long long ldc, long long ldr, int a_mn, int b_mn, int type, int beta, unsigned int* status, cudaStream_t stream);
 int sb_gemm_fp8_block_goes_by_pairs(int M, int N);
+int sb_gemm_fp8_block_weight_goes_by_pairs(int M, int N);
 // gemm_fp8_block_few.cu
 int sb_gemm_fp8_block_few_parts(int N, int K);
 int sb_gemm_fp8_block_takes_few(int M, int N);

@@ -525,14 +525,18 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   }
 }
 
-// Whether an [M, N] product goes by 256 x 256 tiles on CTA pairs: waves of either tile times what a k-block of it takes.
-// us back to back, pairs and single: 8192 x 4096 x 12288 340, 450; 300 x 2048 x 8192 13.2, 14.1; 1333 x 4096 x 4096 33.8, 34.3; 2000 x 768 x 2304 8.9, 8.7;
-// 512 x 4096 x 4096 20.5, 15.0; 777 x 1027 x 650 22.9, 13.3; the weight gradient of 2000 x 768 x 2304 17.4, 11.0.
-static bool goes_by_pairs(int M, int N, int sms) {
+// Whether an [M, N] product goes by 256 x 256 tiles on CTA pairs: where 128 x 128 tiles need more than 1.4 times as many waves, for a weight gradient
+// (scales for single columns) 1.7 times.  Fitted to, us in a graph, pairs and single (waves):
+//   forward, K = 4096   2304 x 2304 32.8, 32.6 (2, 3)   3712 x 3712 59.4, 61.4 (4, 6)   4480 x 4224 74.8, 82.4 (5, 8)   4096 x 4096 63.3, 72.9 (4, 7)
+//                       512 x 4096 19.0, 14.0 (1, 1)    1100 x 2100 32.8, 35.1 (1, 2)   8192 x 12288 342, 435 (21, 42); input gradients alike
+//   weight, K = 8192    2304 x 2304 90.9, 80.5 (2, 3)   3712 x 3712 176, 158 (4, 6)     4480 x 4224 220, 208 (5, 8)     4096 x 4096 179, 182 (4, 7)
+//                       1024 x 1024 48.1, 29.0 (1, 1)   2048 x 2048 50.0, 55.9 (1, 2)   12288 x 4096 493, 581 (11, 21)
+// Short contractions would want the smaller tiles up to 1.75 times the waves (forward, K = 1024: 2304 x 2304 14.4, 12.0; 4096 x 4096 24.4, 24.5).
+static bool goes_by_pairs(int M, int N, bool columns, int sms) {
   auto waves = [](long long tiles, long long slots) { return (tiles + slots - 1) / slots; };
-  const long long pair = waves((long long)((M + 255) / 256) * ((N + 255) / 256), sms / 2) * 512,
-                  single = waves((long long)((M + 127) / 128) * ((N + 127) / 128), sms) * 320;
-  return 8 * single > 7 * pair;
+  const long long pair = waves((long long)((M + 255) / 256) * ((N + 255) / 256), sms / 2),
+                  single = waves((long long)((M + 127) / 128) * ((N + 127) / 128), sms);
+  return 10 * single > (columns ? 17 : 14) * pair;
 }
 
 template <bool PAIR, int A_MN, int B_MN, bool SB_ROWS>
@@ -568,8 +572,9 @@ static int launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensor
 }  // namespace blk8
 }  // namespace sb
 
-// Whether an [M, N] product goes by 256 x 256 tiles on CTA pairs.
-extern "C" int sb_gemm_fp8_block_goes_by_pairs(int M, int N) { return sb::blk8::goes_by_pairs(M, N, sb::num_sms()); }
+// Whether an [M, N] product, or a weight gradient, goes by 256 x 256 tiles on CTA pairs.
+extern "C" int sb_gemm_fp8_block_goes_by_pairs(int M, int N) { return sb::blk8::goes_by_pairs(M, N, false, sb::num_sms()); }
+extern "C" int sb_gemm_fp8_block_weight_goes_by_pairs(int M, int N) { return sb::blk8::goes_by_pairs(M, N, true, sb::num_sms()); }
 
 // C [M, N] of type 0 bf16, 1 fp16, 2 fp32 (bias, residual and a C that is added to: of the same type).  A: [M, K], or stored as [K, M] (a_mn);
 // B: [N, K] or [K, N] (b_mn); bytes, rows lda / ldb apart, 16-byte boundaries.  Scale of A at sa[m * sa_m + (k / 128) * sa_k], of B at
@@ -597,7 +602,7 @@ extern "C" int sb_gemm_fp8_block(const void* A, const float* sa, long long sa_m,
   const int halves = size / 2;                           // the map is in 16-bit units, whatever the type
   if (boxes && (rc = make_tmap_2d_bf16(&tmC, C, (uint64_t)N * halves, M, ldc * halves, 64, 32))) return rc;
   GemmArgs p{C, bias, residual, sa, sb, sa_m, sa_k, sb_n, sb_k, ldc, ldr, M, N, K, type, beta, boxes, runs, status};
-  const bool pair = goes_by_pairs(M, N, num_sms());
+  const bool pair = goes_by_pairs(M, N, sb_rows != 0, num_sms());
   if (!a_mn && !b_mn && !sb_rows) return pair ? launch<true, 0, 0, false>(tmA, tmB, tmC, p, stream) : launch<false, 0, 0, false>(tmA, tmB, tmC, p, stream);
   if (!a_mn && b_mn && !sb_rows) return pair ? launch<true, 0, 1, false>(tmA, tmB, tmC, p, stream) : launch<false, 0, 1, false>(tmA, tmB, tmC, p, stream);
   if (a_mn && b_mn && sb_rows) return pair ? launch<true, 1, 1, true>(tmA, tmB, tmC, p, stream) : launch<false, 1, 1, true>(tmA, tmB, tmC, p, stream);

@@ -33,6 +33,14 @@ def test_wide_products_of_more_than_31_tokens_go_by_tiles():
     assert all(_takes_few(T, 12288) for T in (1, 16, 17, 31)) and all(_takes_few(T, 8192) for T in (1, 32, 64))
 
 
+def test_weight_gradients_have_a_rule_of_their_own():
+    """128 x 128 tiles where they take half as many waves again: [2304, 2304] of 8192 tokens 81 us, by pairs 91."""
+    pairs = cuda_ops.require().sb_gemm_fp8_block_weight_goes_by_pairs
+    assert not any(pairs(*s) for s in ((2304, 2304), (1333, 4096), (3712, 3712), (4480, 4224), (1024, 1024)))
+    assert all(pairs(*s) for s in ((2048, 2048), (4096, 4096), (12288, 4096), (1096, 2104)))
+    assert all(_by_pairs(*s) for s in ((3712, 3712), (4480, 4224), (4096, 4096))) and not _by_pairs(512, 4096)
+
+
 # k-blocks of a CTA: fewer than its stages, more, more than twice as many, more than its accumulators and than a group of 16 scales, more than two groups
 FEW = [(T, K, N, kbs) for T in (1, 16, 17, 32, 33, 64) for K, N, kbs in ((2900, 130, 3), (6100, 130, 6), (10200, 261, 10), (17300, 100, 17), (33700, 130, 33))]
 FEW += [(3, 4100, 19000, 33), (31, 2100, 18990, 17), (64, 4100, 5000, 9)]
@@ -62,7 +70,7 @@ def test_gradients_by_pairs(T, K, N, dtype):
     """Input gradient [T, K] or weight gradient [N, K] (or both) by 256 x 256 tiles that end inside, fresh and added in place."""
     assert _by_pairs(T, K) or _by_pairs(N, K) or _by_pairs(T, N)
     if T < 2000:
-        assert _by_pairs(T, K) and _by_pairs(N, K)
+        assert _by_pairs(T, K) and cuda_ops.require().sb_gemm_fp8_block_weight_goes_by_pairs(N, K)
     x, b, gy = (_randn(*s, seed=i, dtype=dtype) for i, s in ((0, (T, K)), (2, (N,)), (4, (T, N))))
     w = torch.nn.Parameter(_randn(N, K, seed=1, dtype=dtype))
     x.requires_grad_(), b.requires_grad_()
