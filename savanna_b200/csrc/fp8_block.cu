@@ -9,7 +9,7 @@
 // dimension rounded up to fours (the product fetches those of 128 neighbouring rows in copies of 16 bytes), [R / 128][C / 128] for tiles.
 // Bound by memory, and where both forms are written by the instructions for them (some 20 a value).  us for bf16, in brackets those of a copy of as many
 // bytes: 8192 x 12288 rows 51 (46), columns 55 (46), both 89 (62), tiles 47 (46); norm with residual 8192 x 4096 39 (36), its backward 58 (51), back to
-// 16 bits 18 (15).
+// 16 bits 18 (15).  Of fp32, whose instances spill some 100 to 250 bytes: 8192 x 4096 rows 41 (27), columns 42 (27), both 50 (32), tiles 41 (27).
 #include <type_traits>
 
 #include "device_info.h"
@@ -323,7 +323,9 @@ norm_quantize_kernel(NormArgs p) {
 // a = 1 / sqrt(mean(x^2) + eps) and c = a^3 (form 0), or a = 1 / (rms + eps) and c = a^2 / rms (form 1).  dn is the input gradient of the projection in
 // fp32, as its product leaves it: rounded to 16 bits it would cost dg, a sum over all rows, half as much again as its own rounding.  A block goes
 // through rows with a stride of the grid, its threads keep their columns and add up dg for them; the next row's loads are on their way while this
-// one's sum crosses the block.
+// one's sum crosses the block.  us with ds, in brackets those of a copy of as many bytes: bf16 8192 x 4096 58 (53), 4096 x 8192 64 (53); above 8192 columns the
+// sums and one row fill the 128 registers of 512 threads and 112 to 272 bytes spill, 4096 x 8200 84 (53), 2048 x 16384 75 (53).  fp32 spills from 2049
+// columns on (128 to 360 bytes): 8192 x 2048 56 (43), 8192 x 4096 124 (83), 2048 x 16384 135 (83).
 struct NormBackArgs {
   const void *x, *g, *ds;
   const float *a, *dn;

@@ -1,4 +1,4 @@
-// What 8-bit operands with a scale for each block of 128 values have in common (fp8_block.cu, gemm_fp8_block.cu, gemv_fp8_block.cu).
+// What 8-bit operands with a scale for each block of 128 values have in common (fp8_block.cu, gemm_fp8_block.cu, gemm_fp8_block_few.cu).
 //
 //   scale = max(amax, 2^-100) / 448,  q = e4m3(x * 448 / amax),  x' = q * scale
 //
@@ -97,7 +97,6 @@ template <> __device__ __forceinline__ bf16 down<bf16>(float f) { return __float
 template <> __device__ __forceinline__ __half down<__half>(float f) { return __float2half_rn(f); }
 template <> __device__ __forceinline__ float down<float>(float f) { return f; }
 
-// Eight consecutive values as they lie in memory.
 // The calling thread's current device has its context bound; allowed while a stream is captured.
 static inline bool bind_context() {
   static thread_local int bound = -1;
@@ -118,6 +117,7 @@ template <class F> static bool allow_shared(std::atomic<unsigned long long>& kno
   return true;
 }
 
+// Eight consecutive values as they lie in memory.
 template <class T> struct alignas(16) Eight { uint4 v[sizeof(T) / 2]; };
 template <class T> __device__ __forceinline__ Eight<T> none() {
   Eight<T> e;

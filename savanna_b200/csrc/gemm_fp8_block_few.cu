@@ -8,8 +8,11 @@
 // 80 to 100 KB of operands on their way.  A k-block's product is read from TMEM and added, scaled, in fp32; the CTAs' sums are joined through
 // distributed shared memory in a fixed order.
 //
-// 1 x 4096 x 12288: 12.7 us back to back (the weights alone 7.7), 13.6 with the quantiser before it; what is left is a launch, barriers and tensor memory, the
-// first loads' way and the join.  More parts than it takes to reach every SM cost more than they give (2 parts 12.5 us, 3 17, 4 15.4, 8 19.0; one 13.0).
+// 1 x 4096 x 12288: 12.7 us back to back on the same weights, 14.4 with others each time (the bytes alone 7.7), 13.6 on the same with the quantiser before it.
+// What is left: an uneven share (with two parts 44 SMs have two CTAs and 104 one, so that the fullest reads 524 KB of weights where an even share is 340),
+// a launch, barriers and tensor memory, the first loads' way and the join.  More parts than it takes to reach every SM cost more than they give (2 parts
+// 12.5 us, 3 17, 4 15.4, 8 19.0; one 13.0); so do clusters that do not all find room at once (34 to 36 tiles in eight parts, 72 and 73 in four: T = 1, K = 4096,
+// 33 tiles 8.2 us, 34 11.4, 37 8.5; 71 10.6, 72 14.5, 74 11.9).
 //
 // A link of a chain (pdl.cuh, the first kind) behind the kernel that quantises X, which lets it start when all before itself is complete: the first
 // stages' weights, which do not depend on that kernel, are on their way before it has ended.  All waits are bounded (sm100.cuh).

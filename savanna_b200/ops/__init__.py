@@ -266,7 +266,8 @@ def linear_fp8_block(x, w, bias=None, residual=None, dtype=None):
 
     Gradients: dx = rows(dy) tiles(w), dw = columns(dy)^T columns(x), each operand in 8 bits with scales for 128 values along the contraction;
     the rounding to 8 bits itself passes them on unchanged.  x is kept for them in 8 bits.  A weight given as a pair gets none, an x given as a pair
-    wants none (ValueError).  No second derivatives.  Products whose two scales multiply to more than fp32 holds are infinite or NaN."""
+    wants none (ValueError).  No second derivatives.  Products whose two scales multiply to more than fp32 holds are infinite or NaN on the GPU; where
+    they multiply to less than 2^-126 they lose bits, up to 2^-125 of the result for every 128 products."""
     pair = isinstance(x, tuple)
     if pair:
         dtype = torch.bfloat16 if dtype is None else dtype
