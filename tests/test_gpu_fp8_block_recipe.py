@@ -210,11 +210,33 @@ def test_released_units_keep_no_codes(trainers):
     assert not kept
 
 
+def test_kept_codes_are_those_of_the_weights_they_stand_for(trainers):
+    """After steps and an evaluation: whatever is kept on a parameter is a fresh quantisation of it."""
+    tr = trainers({"fp8_recipe": "block128", "zero_optimization": {"stage": 1}, "gradient_accumulation_steps": 2})
+    for i in range(3):
+        tr.train_step(_batches(tr.cfg, 2, 2 * i))
+    tr.evaluate(_batches(tr.cfg, 1, 9), iters=1)
+    kept = [(p, p._fp8_block_cache[1]) for p in tr.model.parameters() if getattr(p, "_fp8_block_cache", None) is not None]
+    assert kept
+    for p, (q, s) in kept:
+        want_q, want_s = ops.fp8_block_quantize_weight(p.detach())
+        assert torch.equal(s, want_s) and torch.equal(q.view(torch.uint8), want_q.view(torch.uint8))
+
+
 def test_partitioned_stage_3_matches_stage_1(trainers):
     over = {"fp8_recipe": "block128", "gradient_accumulation_steps": 2}
     want = _trace(dict(over, zero_optimization={"stage": 1}))
     got = _trace(dict(over, zero_optimization={"stage": 3}, checkpoint_activations=True, checkpoint_num_layers=2))
     assert max(abs(a - b) for a, b in zip(want, got)) < 2e-2 * max(want), (want, got)
+
+
+def test_training_follows_bf16(trainers):
+    """The loss of 30 steps under the recipe stays beside that in bf16: as near as the block-scaled hardware format has to."""
+    plain = _trace({k: False for k in _OVER if k.startswith("use_fp8")} | {"train_micro_batch_size_per_gpu": 2}, 30)
+    block = _trace({"fp8_recipe": "block128", "train_micro_batch_size_per_gpu": 2}, 30)
+    assert abs(plain[-1] - block[-1]) < 0.06 * plain[-1], (plain[-1], block[-1])
+    assert max(abs(a - b) for a, b in zip(plain, block)) < 0.2, (plain, block)
+    assert plain != block
 
 
 # ------------------------------------------------------------------------------------------------ traced
