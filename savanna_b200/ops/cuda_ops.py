@@ -17,6 +17,7 @@ import ctypes
 import importlib.util
 import os
 import sys
+import threading
 from typing import Optional
 
 import torch
@@ -1127,30 +1128,41 @@ def norm_linear_fp8_block(x, norm_weight, eps, form, w, bias, residual):
     return _native("norm_linear_fp8_block", x, norm_weight, float(eps), 0 if form == "te" else 1, w, ws, bias, residual, None, None)
 
 
-_UNCHANGED = None          # inside `weights_unchanged`: what marks the codes made there
+_UNCHANGED = None          # the open `weights_unchanged`: (its thread, what marks the codes made there)
 
 
 @contextlib.contextmanager
 def weights_unchanged():
     """The caller's word that no parameter changes inside (the micro-batches of a training step, an evaluation): under the recipe `block128` each
     weight is quantised once there.  Elsewhere every call quantises its weight: who writes it through `.data`, by its address or in a replayed
-    graph leaves no trace on it.  A program that keeps weights in 8 bits by itself hands their codes to `ops.linear_fp8_block`."""
+    graph leaves no trace on it.  A program that keeps weights in 8 bits by itself hands their codes to `ops.linear_fp8_block`.
+
+    It holds for the calling thread, and for what its backward passes compute again.  While one thread is inside, others gain nothing by it."""
     global _UNCHANGED
-    outer = _UNCHANGED
-    _UNCHANGED = outer or object()
+    if _UNCHANGED is not None:
+        yield                                            # the outer one's; or another thread's, which this one's calls do not see
+        return
+    _UNCHANGED = (threading.get_ident(), object())
     try:
         yield
     finally:
-        _UNCHANGED = outer
+        _UNCHANGED = None
+
+
+def _unchanged():
+    """What marks codes that hold for this call, or None.  Within a backward pass the calls are the autograd engine's."""
+    u = _UNCHANGED
+    return u[1] if u is not None and (u[0] == threading.get_ident() or torch._C._current_graph_task_id() >= 0) else None
 
 
 def _block_weight(w):
     """Codes and scales of a parameter under the recipe `block128`, kept on it inside of one `weights_unchanged` (and there until its version or
     address changes).  (None, None), for the call to quantise by itself, elsewhere; while a graph is captured: what a graph computes is there after
     its replays alone, and weights change between those; and while one is traced, which would take kept codes for constants."""
-    if _UNCHANGED is None or w.is_inference() or torch.cuda.is_current_stream_capturing() or torch._C._get_tracing_state() is not None:
+    mark = _unchanged()
+    if mark is None or w.is_inference() or torch.cuda.is_current_stream_capturing() or torch._C._get_tracing_state() is not None:
         return None, None
-    state = (_UNCHANGED, PARAM_EPOCH, w._version, w.data_ptr(), torch._C._cuda_getCurrentRawStream(w.get_device()))
+    state = (mark, PARAM_EPOCH, w._version, w.data_ptr(), torch._C._cuda_getCurrentRawStream(w.get_device()))
     cache = getattr(w, "_fp8_block_cache", None)
     if cache is None or cache[0] != state:
         cache = w._fp8_block_cache = (state, _native("fp8_block_quantize", w.detach(), True))

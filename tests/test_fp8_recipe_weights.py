@@ -33,20 +33,77 @@ def test_block_scaled_recipes_leave_the_fused_tensor_parallel_projections_out():
         cuda_ops.set_fp8_recipe("delayed")
 
 
+def _in_thread(call):
+    import threading
+    out = []
+    t = threading.Thread(target=lambda: out.append(call()))
+    t.start()
+    t.join()
+    return out[0]
+
+
 def test_unchanged_weights_end_with_the_outer_context_and_with_an_error():
     from savanna_b200.ops import cuda_ops
-    assert cuda_ops._UNCHANGED is None
+    assert cuda_ops._unchanged() is None
     with cuda_ops.weights_unchanged():
-        outer = cuda_ops._UNCHANGED
+        outer = cuda_ops._unchanged()
+        assert outer is not None
         with cuda_ops.weights_unchanged():
-            assert cuda_ops._UNCHANGED is outer
-        assert cuda_ops._UNCHANGED is outer
-    assert cuda_ops._UNCHANGED is None
+            assert cuda_ops._unchanged() is outer
+        assert cuda_ops._unchanged() is outer
+    assert cuda_ops._unchanged() is None
     try:
         with cuda_ops.weights_unchanged():
             raise KeyError
     except KeyError:
         pass
-    assert cuda_ops._UNCHANGED is None
+    assert cuda_ops._unchanged() is None
     with cuda_ops.weights_unchanged():
-        assert cuda_ops._UNCHANGED is not outer
+        assert cuda_ops._unchanged() not in (None, outer)
+
+
+def test_unchanged_weights_of_one_thread_are_no_others():
+    """Contexts that overlap in two threads leave nothing open, and hold for one of them alone."""
+    import threading
+    from savanna_b200.ops import cuda_ops
+    inside, go = threading.Event(), threading.Event()
+    seen = []
+
+    def other():
+        with cuda_ops.weights_unchanged():
+            seen.append(cuda_ops._unchanged())
+            inside.set()
+            go.wait(30)
+            seen.append(cuda_ops._unchanged())
+    t = threading.Thread(target=other)
+    with cuda_ops.weights_unchanged():
+        assert cuda_ops._unchanged() is not None and _in_thread(cuda_ops._unchanged) is None
+        t.start()
+        assert inside.wait(30)
+    assert cuda_ops._unchanged() is None
+    go.set()
+    t.join()
+    assert seen == [None, None] and cuda_ops._unchanged() is None
+
+
+def test_unchanged_weights_hold_in_the_backward_pass():
+    """Checkpointed blocks run again there, by the autograd engine."""
+    from savanna_b200.ops import cuda_ops
+    seen = []
+
+    class Again(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return x * 2
+
+        @staticmethod
+        def backward(ctx, g):
+            seen.append(cuda_ops._unchanged())
+            return g * 2
+    x = torch.ones(3, requires_grad=True)
+    with cuda_ops.weights_unchanged():
+        mark = cuda_ops._unchanged()
+        Again.apply(x).sum().backward()
+        _in_thread(lambda: Again.apply(x).sum().backward())
+    Again.apply(x).sum().backward()
+    assert seen == [mark, mark, None]
