@@ -1157,11 +1157,15 @@ def _unchanged():
 
 def _block_weight(w):
     """Codes and scales of a parameter under the recipe `block128`, kept on it inside of one `weights_unchanged` (and there until its version or
-    address changes).  (None, None), for the call to quantise by itself, elsewhere; while a graph is captured: what a graph computes is there after
-    its replays alone, and weights change between those; and while one is traced, which would take kept codes for constants."""
-    mark = _unchanged()
-    if mark is None or w.is_inference() or torch.cuda.is_current_stream_capturing() or torch._C._get_tracing_state() is not None:
+    address changes); made for the call alone elsewhere, and while a graph is captured: what a graph computes is there after its replays alone, and
+    weights change between those.  What is saved for the backward pass is the same kind of pair either way, so that a forward pass and its
+    recomputation may stand on different sides.  (None, None), for the call to quantise by itself, while a graph is traced: a pair made here would
+    be a constant of it."""
+    if torch._C._get_tracing_state() is not None:
         return None, None
+    mark = _unchanged()
+    if mark is None or w.is_inference() or torch.cuda.is_current_stream_capturing():
+        return _native("fp8_block_quantize", w.detach(), True)
     state = (mark, PARAM_EPOCH, w._version, w.data_ptr(), torch._C._cuda_getCurrentRawStream(w.get_device()))
     cache = getattr(w, "_fp8_block_cache", None)
     if cache is None or cache[0] != state:

@@ -91,6 +91,25 @@ def test_weights_are_quantised_once_where_they_do_not_change(recipe):
         assert torch.equal(ops.linear(x, w, fp8=True).float(), 4.0 * want.float())
 
 
+@pytest.mark.parametrize("forward_inside", [False, True])
+def test_checkpointed_forward_and_its_recomputation_on_different_sides(recipe, forward_inside):
+    import contextlib
+    from torch.utils.checkpoint import checkpoint
+    m, x = _Projections(), _randn(20, 256, seed=7).requires_grad_()
+    leaves = [x] + list(m.parameters())
+
+    def loss(run):
+        return sum(y.float().square().sum() for y in run(x))
+    want = torch.autograd.grad(loss(m), leaves)
+    sides = [recipe.weights_unchanged, contextlib.nullcontext]
+    with sides[not forward_inside]():
+        y = loss(lambda t: checkpoint(m, t, use_reentrant=False))
+    with sides[forward_inside]():
+        got = torch.autograd.grad(y, leaves)
+    for a, e in zip(got, want):
+        assert torch.equal(a, e)
+
+
 def test_traced_graph_from_between_two_updates(recipe):
     x, m = _randn(20, 256, seed=7), _Projections()
     with torch.no_grad():
