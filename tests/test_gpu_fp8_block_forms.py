@@ -116,3 +116,18 @@ def test_norm_and_projection_of_rows_beyond_the_norms_kernel(form):
     assert torch.equal(s, x)
     # the result's rounding, and a few values beside a border that have the neighbouring code
     assert (y.double() - want).norm() <= (2 * half_step(torch.bfloat16) + 1e-3) * want.norm()
+
+
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("shape", [(0, 130), (2, 0, 256)])
+def test_norms_of_no_rows(shape, residual):
+    D = shape[-1]
+    x, g, w, b = torch.empty(shape, device="cuda", dtype=torch.bfloat16), _randn(D), _randn(9, D, seed=1), _randn(9, seed=2)
+    r = torch.empty_like(x) if residual else None
+    q, s, kept = ops.rmsnorm_fp8_block(x, g, 1e-5, "te", r)
+    assert q.shape == kept.shape == x.shape and s.shape == shape[:-1] + (-(-D // 128),)
+    leaves = [t.requires_grad_() for t in (x, r, g, w, b) if t is not None]
+    y, s = ops.norm_linear_fp8_block(x, g, 1e-5, "te", w, b, r)
+    assert y.shape == shape[:-1] + (9,) and s.shape == x.shape
+    grads = torch.autograd.grad((y, s), leaves, (torch.empty_like(y), torch.empty_like(s)))
+    assert all(a.shape == t.shape and (a == 0).all() for a, t in zip(grads, leaves))
