@@ -83,10 +83,7 @@ int sb_fp8_block_dequantize(const void* q, long long ldq, const float* scale, lo
 int sb_gemm_fp8_block(const void* A, const float* sa, long long sa_m, long long sa_k, const void* B, const float* sb, long long sb_n,
                       long long sb_k, int sb_rows, void* C, const void* bias, const void* residual, int M, int N, int K, long long lda, long long ldb,
                       long long ldc, long long ldr, int a_mn, int b_mn, int type, int beta, unsigned int* status, cudaStream_t stream);
-int sb_gemm_fp8_block_goes_by_pairs(int M, int N);
-int sb_gemm_fp8_block_weight_goes_by_pairs(int M, int N);
 // gemm_fp8_block_few.cu
-int sb_gemm_fp8_block_few_parts(int N, int K);
 int sb_gemm_fp8_block_takes_few(int M, int N);
 int sb_gemm_fp8_block_few(const void* X, const float* sx, long long sx_m, long long sx_k, const void* W, const float* sw, long long sw_n, long long sw_k,
                           void* y, const void* bias, const void* residual, int M, int N, int K, long long ldx, long long ldw, long long ldc,
